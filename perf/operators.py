@@ -235,8 +235,9 @@ def _own_attention(s):
 
 def _own_verify(s):
     h = _handles(s)
-    h["cri"].verify_drafts(s["target"], s["draft"], s["ids"], s["u"], s["offsets"], s["out_ids"], s["accepted"],
-                           h["ws"])
+    # one set of numbers decides and draws, as in the plain form (a sampler has independent ones)
+    h["cri"].verify_drafts(s["target"], s["draft"], s["ids"], s["u"], s["u"], s["offsets"], s["out_ids"],
+                           s["accepted"], h["ws"])
     return s["out_ids"], s["accepted"]
 
 
