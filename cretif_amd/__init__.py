@@ -53,6 +53,15 @@ __all__ = [
     "stream_read",
     "GGUFFile",
     "Decoder",
+    "Rotation",
+    "PagedKV",
+    "PagedBatch",
+    "qk_norm_rope",
+    "paged_append",
+    "paged_attention",
+    "paged_attention_workspace_bytes",
+    "verify_drafts",
+    "verify_drafts_workspace_bytes",
     "FORMAT_IDS",
     "ABI_SYMBOLS",
 ]
@@ -123,6 +132,12 @@ ABI_SYMBOLS = (
         "cri_decoder_kv_cache",
         "cri_decoder_weight_bytes",
         "cri_decoder_step_weight_bytes",
+        "cri_qk_norm_rope",
+        "cri_paged_append",
+        "cri_paged_attention",
+        "cri_paged_attention_workspace_bytes",
+        "cri_verify_drafts",
+        "cri_verify_drafts_workspace_bytes",
         "cri_stream_read",
         "cri_stream_read_ex",
         "cri_timestamp",
@@ -306,6 +321,7 @@ def lib():
     L.cri_block_elems.argtypes = [i32]
     L.cri_block_elems.restype = i32
     L.cri_version.restype = i32
+    serving.declare(L)
     _lib = L
     return L
 
@@ -803,3 +819,17 @@ class Decoder:
     def step_weight_bytes(self, M):
         """Weight bytes one step of M tokens reads (M token-table rows, not the whole table)."""
         return int(lib().cri_decoder_step_weight_bytes(self._h, M))
+
+
+from . import serving  # noqa: E402
+from .serving import (  # noqa: E402
+    PagedBatch,
+    PagedKV,
+    Rotation,
+    paged_append,
+    paged_attention,
+    paged_attention_workspace_bytes,
+    qk_norm_rope,
+    verify_drafts,
+    verify_drafts_workspace_bytes,
+)

@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "internal.hpp"
@@ -624,6 +625,265 @@ int cri_fused_decode_attention_noalloc(const float* Q, const float* K_cache, con
                                                               head_dim, kv_len, scale, ws,
                                                               cri::detail::kNoallocScratchBytes, s);
     if (rc != 0) return fail(CRI_ERR_UNSUPPORTED, fn, "no kernel for this shape");
+    return check_launch(fn);
+}
+
+// ---- serving a batch from a paged cache -------------------------------------
+
+namespace {
+
+// the kernels' numbering of a cache type, -1 for none
+int kv_type(int type) {
+    return type == CRI_FP32 ? cri::kKvF32 : type == CRI_FP16 ? cri::kKvF16 : type == CRI_BF16 ? cri::kKvBF16 : -1;
+}
+
+constexpr int kMaxPagedHeadDim = 256;
+constexpr long kMaxPositions = 1L << 30;
+
+int check_rotation(const cri_rotation* rot, int head_dim, cri::HeadRotation* out, const char* fn) {
+    if (!rot) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null rotation");
+    if (rot->pairs != CRI_ROPE_ADJACENT && rot->pairs != CRI_ROPE_HALVES)
+        return fail(CRI_ERR_UNSUPPORTED, fn, "unknown pairing of the rotation");
+    if (rot->rot_dim < 0 || rot->rot_dim > head_dim || rot->rot_dim % 8 != 0)
+        return fail(CRI_ERR_SHAPE, fn, "rot_dim=" + std::to_string(rot->rot_dim) +
+                                           " must be a multiple of 8 up to head_dim");
+    if (rot->rot_dim > 0 && !(rot->theta > 0.0f && std::isfinite(rot->theta)))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "theta must be positive and finite");
+    if ((rot->q_norm || rot->k_norm) && !(rot->eps >= 0.0f))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "eps must not be negative");
+    if (!aligned(rot->q_norm, 4) || !aligned(rot->k_norm, 4))
+        return fail(CRI_ERR_ALIGNMENT, fn, "norm weights must be 4-byte aligned");
+    *out = cri::HeadRotation{rot->q_norm, rot->k_norm, rot->eps, rot->rot_dim, rot->pairs == CRI_ROPE_HALVES,
+                             rot->rot_dim > 0 ? -2.0 * std::log2(static_cast<double>(rot->theta)) / rot->rot_dim : 0.0};
+    return CRI_OK;
+}
+
+int check_head_dim(int head_dim, const char* fn) {
+    if (head_dim < 8 || head_dim > kMaxPagedHeadDim || head_dim % 8 != 0)
+        return fail(CRI_ERR_UNSUPPORTED, fn, "head_dim=" + std::to_string(head_dim) +
+                                                 " must be a multiple of 8 in [8, " + std::to_string(kMaxPagedHeadDim) + "]");
+    return CRI_OK;
+}
+
+int check_paged(const cri_paged_kv* kv, const cri_paged_batch* batch, cri::PagePool* pool, cri::PageBatch* b, int* type,
+                const char* fn) {
+    if (!kv || !batch) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null descriptor");
+    if (batch->n_seqs < 0 || batch->n_rows < 0 || batch->max_pages < 0 || kv->n_pages < 0 || kv->page_size < 0 ||
+        kv->n_kv_heads < 0 || kv->head_dim < 0)
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "negative dimension");
+    *type = kv_type(kv->type);
+    if (*type < 0) return fail(CRI_ERR_UNSUPPORTED, fn, "the cache's type must be CRI_FP32, CRI_FP16 or CRI_BF16");
+    if (const int st = check_head_dim(kv->head_dim, fn)) return st;
+    if (kv->n_kv_heads < 1 || kv->page_size < 1 || kv->n_pages < 1)
+        return fail(CRI_ERR_SHAPE, fn, "n_kv_heads, page_size and n_pages must be at least 1");
+    const long page = static_cast<long>(kv->page_size) * kv->n_kv_heads;
+    if (page > kMaxElems / kv->head_dim || kv->page_stride > kMaxElems)
+        return fail(CRI_ERR_SHAPE, fn, "problem too large");
+    if (kv->page_stride < page * kv->head_dim || kv->page_stride % 8 != 0)
+        return fail(CRI_ERR_SHAPE, fn, "page_stride must be a multiple of 8 and hold page_size * n_kv_heads * head_dim elements");
+    if (static_cast<long>(batch->max_pages) * kv->page_size > kMaxPositions)
+        return fail(CRI_ERR_SHAPE, fn, "max_pages * page_size exceeds 2^30 positions");
+    int l = 0;
+    while ((1L << l) < kv->page_size) ++l;
+    *pool = cri::PagePool{kv->k, kv->v, static_cast<long>(kv->page_stride), kv->n_pages, kv->page_size, kv->n_kv_heads,
+                          kv->head_dim, static_cast<uint32_t>((1UL << (31 + l)) / kv->page_size + 1), 31 + l};
+    *b = cri::PageBatch{batch->offsets, batch->lens, batch->pages, batch->n_seqs, batch->n_rows, batch->max_pages};
+    return CRI_OK;
+}
+
+// pointers of a call that has rows
+int check_paged_pointers(const cri::PagePool& pool, const cri::PageBatch& b, const char* fn) {
+    if (!pool.k || !pool.v || !b.offsets || !b.lens || (!b.pages && b.max_pages > 0))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null pointer in a descriptor");
+    if (!aligned(pool.k, 16) || !aligned(pool.v, 16))
+        return fail(CRI_ERR_ALIGNMENT, fn, "the pool's k and v must be 16-byte aligned");
+    if (!aligned(b.offsets, 4) || !aligned(b.lens, 4) || !aligned(b.pages, 4))
+        return fail(CRI_ERR_ALIGNMENT, fn, "offsets, lens and pages must be 4-byte aligned");
+    return CRI_OK;
+}
+
+// bytes from the first to the last element of `rows` rows of `width` floats, ld apart
+long span_bytes(long rows, long width, long ld) { return rows <= 0 || width <= 0 ? 0 : ((rows - 1) * ld + width) * 4; }
+
+// whether rows of two buffers meet: columns of the same rows (equal ld, less than a row apart) do not
+bool rows_overlap(const float* a, long wa, long lda, const float* b, long wb, long ldb, long rows) {
+    if (!overlaps(a, span_bytes(rows, wa, lda), b, span_bytes(rows, wb, ldb))) return false;
+    if (lda == ldb) {
+        const long d = (reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / 4;
+        if ((d >= wa && d + wb <= lda) || (-d >= wb && -d + wa <= lda)) return false;
+    }
+    return true;
+}
+
+int check_rows(const float* p, int ld, long width, const char* name, const char* fn) {
+    if (!p) return fail(CRI_ERR_INVALID_ARGUMENT, fn, std::string("null ") + name);
+    if (!aligned(p, 4)) return fail(CRI_ERR_ALIGNMENT, fn, std::string(name) + " must be 4-byte aligned");
+    if (ld < width)
+        return fail(CRI_ERR_SHAPE, fn, std::string("ld of ") + name + " is " + std::to_string(ld) + ", below its width " +
+                                           std::to_string(width));
+    return CRI_OK;
+}
+
+}  // namespace
+
+int cri_qk_norm_rope(const cri_rotation* rot, const float* q, int ldq, const float* k, int ldk, float* q_out, int ldq_out,
+                     float* k_out, int ldk_out, const int* positions, int M, int n_heads, int n_kv_heads, int head_dim,
+                     hipStream_t s) {
+    const char* fn = "cri_qk_norm_rope";
+    if (M < 0 || n_heads < 0 || n_kv_heads < 0 || head_dim < 0)
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "negative dimension");
+    if (const int st = check_head_dim(head_dim, fn)) return st;
+    cri::HeadRotation R;
+    if (const int st = check_rotation(rot, head_dim, &R, fn)) return st;
+    if (M == 0 || (n_heads == 0 && n_kv_heads == 0)) return CRI_OK;
+    const long wq = static_cast<long>(n_heads) * head_dim, wk = static_cast<long>(n_kv_heads) * head_dim;
+    if (!positions) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null positions");
+    if (!aligned(positions, 4)) return fail(CRI_ERR_ALIGNMENT, fn, "positions must be 4-byte aligned");
+    int st = CRI_OK;
+    if (n_heads > 0 && ((st = check_rows(q, ldq, wq, "q", fn)) || (st = check_rows(q_out, ldq_out, wq, "q_out", fn)))) return st;
+    if (n_kv_heads > 0 && ((st = check_rows(k, ldk, wk, "k", fn)) || (st = check_rows(k_out, ldk_out, wk, "k_out", fn))))
+        return st;
+    if (static_cast<long>(M) * std::max({ldq, ldk, ldq_out, ldk_out}) > kMaxElems)
+        return fail(CRI_ERR_SHAPE, fn, "problem too large");
+    const bool same_q = q == q_out && ldq == ldq_out, same_k = k == k_out && ldk == ldk_out;
+    if ((n_heads > 0 && !same_q && rows_overlap(q, wq, ldq, q_out, wq, ldq_out, M)) ||
+        (n_kv_heads > 0 && !same_k && rows_overlap(k, wk, ldk, k_out, wk, ldk_out, M)) ||
+        (n_heads > 0 && n_kv_heads > 0 &&
+         (rows_overlap(q, wq, ldq, k_out, wk, ldk_out, M) || rows_overlap(k, wk, ldk, q_out, wq, ldq_out, M) ||
+          rows_overlap(q_out, wq, ldq_out, k_out, wk, ldk_out, M))))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "an output overlaps another buffer");
+    clear_pending_error();
+    if (cri::detail::launch_qk_norm_rope(R, q, ldq, k, ldk, q_out, ldq_out, k_out, ldk_out, positions, M, n_heads,
+                                         n_kv_heads, head_dim, s) != 0)
+        return fail(CRI_ERR_UNSUPPORTED, fn, "no kernel for this shape");
+    return check_launch(fn);
+}
+
+int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const cri_rotation* rot, const float* q, int ldq,
+                     float* q_out, int ldq_out, int n_heads, const float* k, int ldk, const float* v, int ldv,
+                     hipStream_t s) {
+    const char* fn = "cri_paged_append";
+    cri::PagePool pool;
+    cri::PageBatch b;
+    cri::HeadRotation R;
+    int type, st;
+    if ((st = check_paged(kv, batch, &pool, &b, &type, fn))) return st;
+    if ((st = check_rotation(rot, pool.head_dim, &R, fn))) return st;
+    if (n_heads < 0) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "negative dimension");
+    if (b.n_seqs == 0 || b.n_rows == 0) return CRI_OK;
+    if ((st = check_paged_pointers(pool, b, fn))) return st;
+    const long wk = static_cast<long>(pool.n_kv_heads) * pool.head_dim;
+    const long wq = q ? static_cast<long>(n_heads) * pool.head_dim : 0;
+    if ((st = check_rows(k, ldk, wk, "k", fn)) || (st = check_rows(v, ldv, wk, "v", fn))) return st;
+    if (wq > 0 && ((st = check_rows(q, ldq, wq, "q", fn)) || (st = check_rows(q_out, ldq_out, wq, "q_out", fn)))) return st;
+    if (static_cast<long>(b.n_rows) * std::max({wq > 0 ? std::max(ldq, ldq_out) : 0, ldk, ldv}) > kMaxElems)
+        return fail(CRI_ERR_SHAPE, fn, "problem too large");
+    if (wq > 0 && ((!(q == q_out && ldq == ldq_out) && rows_overlap(q, wq, ldq, q_out, wq, ldq_out, b.n_rows)) ||
+                   rows_overlap(k, wk, ldk, q_out, wq, ldq_out, b.n_rows) ||
+                   rows_overlap(v, wk, ldv, q_out, wq, ldq_out, b.n_rows)))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "q_out overlaps another buffer");
+    clear_pending_error();
+    if (cri::detail::launch_paged_append(pool, type, b, R, wq > 0 ? q : nullptr, ldq, q_out, ldq_out, n_heads, k, ldk, v,
+                                         ldv, s) != 0)
+        return fail(CRI_ERR_UNSUPPORTED, fn, "no kernel for this shape");
+    return check_launch(fn);
+}
+
+namespace {
+int check_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, int prefix_len, int n_heads,
+                          cri::PagePool* pool, cri::PageBatch* b, int* type, const char* fn) {
+    if (const int st = check_paged(kv, batch, pool, b, type, fn)) return st;
+    if (prefix_len < 0 || n_heads < 0) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "negative dimension");
+    if (n_heads % pool->n_kv_heads != 0)
+        return fail(CRI_ERR_SHAPE, fn, "n_heads=" + std::to_string(n_heads) + " is not a multiple of n_kv_heads=" +
+                                           std::to_string(pool->n_kv_heads));
+    if (prefix_len > kMaxPositions) return fail(CRI_ERR_SHAPE, fn, "prefix_len exceeds 2^30 positions");
+    if (b->max_pages < 1 && b->n_seqs > 0 && b->n_rows > 0) return fail(CRI_ERR_SHAPE, fn, "max_pages must be at least 1");
+    if (static_cast<long>(b->n_rows) * n_heads > (1L << 24))
+        return fail(CRI_ERR_SHAPE, fn, "problem too large (more than 2^24 rows x heads)");
+    return CRI_OK;
+}
+}  // namespace
+
+long long cri_paged_attention_workspace_bytes(const cri_paged_kv* kv, const cri_paged_batch* batch, int prefix_len,
+                                              int n_heads) {
+    const char* fn = "cri_paged_attention_workspace_bytes";
+    cri::PagePool pool;
+    cri::PageBatch b;
+    int type;
+    if (const int st = check_paged_attention(kv, batch, prefix_len, n_heads, &pool, &b, &type, fn)) return st;
+    if (b.n_seqs == 0 || b.n_rows == 0 || n_heads == 0) return 0;
+    return cri::detail::paged_attention_workspace_bytes(pool, type, b, n_heads, prefix_len);
+}
+
+int cri_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, const int* prefix_pages, int prefix_len,
+                        const float* q, int ldq, float* out, int ldo, int n_heads, float scale, void* workspace,
+                        long long workspace_bytes, hipStream_t s) {
+    const char* fn = "cri_paged_attention";
+    cri::PagePool pool;
+    cri::PageBatch b;
+    int type, st;
+    if ((st = check_paged_attention(kv, batch, prefix_len, n_heads, &pool, &b, &type, fn))) return st;
+    if (b.n_seqs == 0 || b.n_rows == 0 || n_heads == 0) return CRI_OK;
+    if ((st = check_paged_pointers(pool, b, fn))) return st;
+    if (prefix_len > 0 && !prefix_pages) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null prefix_pages");
+    if (!aligned(prefix_pages, 4)) return fail(CRI_ERR_ALIGNMENT, fn, "prefix_pages must be 4-byte aligned");
+    const long w = static_cast<long>(n_heads) * pool.head_dim;
+    if ((st = check_rows(q, ldq, w, "q", fn)) || (st = check_rows(out, ldo, w, "out", fn))) return st;
+    if (static_cast<long>(b.n_rows) * std::max(ldq, ldo) > kMaxElems) return fail(CRI_ERR_SHAPE, fn, "problem too large");
+    if (rows_overlap(q, w, ldq, out, w, ldo, b.n_rows))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out overlaps q (other workgroups still read it)");
+    const long need = cri::detail::paged_attention_workspace_bytes(pool, type, b, n_heads, prefix_len);
+    if (need > 0) {
+        if (!workspace) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null workspace");
+        if (!aligned(workspace, 16)) return fail(CRI_ERR_ALIGNMENT, fn, "workspace must be 16-byte aligned");
+        if (workspace_bytes < need)
+            return fail(CRI_ERR_SHAPE, fn, "workspace of " + std::to_string(workspace_bytes) + " bytes, " +
+                                               std::to_string(need) + " needed");
+    }
+    clear_pending_error();
+    if (cri::detail::launch_paged_attention(pool, type, b, prefix_pages, prefix_len, q, ldq, out, ldo, n_heads, scale,
+                                            static_cast<float*>(workspace), s) != 0)
+        return fail(CRI_ERR_UNSUPPORTED, fn, "no kernel for this shape");
+    return check_launch(fn);
+}
+
+long long cri_verify_drafts_workspace_bytes(int n_seqs, int vocab) {
+    if (n_seqs < 0 || vocab < 0)
+        return fail(CRI_ERR_INVALID_ARGUMENT, "cri_verify_drafts_workspace_bytes", "negative dimension");
+    if (n_seqs == 0 || vocab == 0) return 0;
+    return cri::detail::verify_workspace_bytes(n_seqs, vocab);
+}
+
+int cri_verify_drafts(const float* target, long long ldt, const float* draft, long long ldd, const int* draft_ids,
+                      const float* uniforms, const float* draws, const int* offsets, int n_seqs, int n_rows,
+                      int vocab, int* out_ids, int* n_accepted, void* workspace, long long workspace_bytes,
+                      hipStream_t s) {
+    const char* fn = "cri_verify_drafts";
+    if (n_seqs < 0 || n_rows < 0 || vocab < 0) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "negative dimension");
+    if (n_seqs == 0) return CRI_OK;
+    if (vocab == 0) return fail(CRI_ERR_SHAPE, fn, "vocab must be at least 1");
+    if (n_seqs > (1 << 20)) return fail(CRI_ERR_SHAPE, fn, "more than 2^20 sequences");
+    if (!offsets || !n_accepted || (n_rows > 0 && (!target || !draft_ids || !uniforms || !draws || !out_ids)))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null pointer");
+    if (!aligned(target, 4) || !aligned(draft, 4) || !aligned(draft_ids, 4) || !aligned(uniforms, 4) ||
+        !aligned(draws, 4) || !aligned(offsets, 4) || !aligned(out_ids, 4) || !aligned(n_accepted, 4))
+        return fail(CRI_ERR_ALIGNMENT, fn, "buffers must be 4-byte aligned");
+    if (ldt < vocab || (draft && ldd < vocab)) return fail(CRI_ERR_SHAPE, fn, "ldt and ldd must be at least vocab");
+    if (ldt > kMaxElems / std::max(n_rows, 1) || (draft && ldd > kMaxElems / std::max(n_rows, 1)))
+        return fail(CRI_ERR_SHAPE, fn, "problem too large");
+    const long ids = static_cast<long>(n_rows) * 4;
+    if (overlaps(out_ids, ids, draft_ids, ids)) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out_ids overlaps draft_ids");
+    const long need = cri::detail::verify_workspace_bytes(n_seqs, vocab);
+    if (!workspace) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null workspace");
+    if (!aligned(workspace, 8)) return fail(CRI_ERR_ALIGNMENT, fn, "workspace must be 8-byte aligned");
+    if (workspace_bytes < need)
+        return fail(CRI_ERR_SHAPE, fn, "workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) +
+                                           " needed");
+    clear_pending_error();
+    if (cri::detail::launch_verify_drafts(target, ldt, draft, ldd, draft_ids, uniforms, draws, offsets, n_seqs, n_rows, vocab,
+                                          out_ids, n_accepted, static_cast<double*>(workspace), s) != 0)
+        return fail(CRI_ERR_UNSUPPORTED, fn, "no kernel for this shape");
     return check_launch(fn);
 }
 

@@ -18,6 +18,7 @@
 #include "../../include/cuinfer/kernels/elementwise.h"
 #include "../../include/cuinfer/kernels/matmul_quant.h"
 #include "../../include/cuinfer/quantization.h"
+#include "../../include/cuinfer/serving.h"
 #include "../../include/cuinfer/tensor.h"
 
 namespace cuinfer {
@@ -80,6 +81,43 @@ void prefill_attention(const float* Q, int ldq, const float* K_cache, const floa
                                             scale, ws.data(), bytes, stream));
     // the workspace is released when this returns: wait for the kernels that use it
     CUINFER_CHECK_HIP(hipStreamSynchronize(stream));
+}
+
+// ---------------------------------------------------------------- serving
+namespace {
+long long checked_bytes(long long n) {
+    if (n < 0) CUINFER_CHECK_CRI(static_cast<int>(n));
+    return n;
+}
+}  // namespace
+
+void qk_norm_rope(const HeadRotation& rot, const float* q, int ldq, const float* k, int ldk, float* q_out, int ldq_out,
+                  float* k_out, int ldk_out, const int* positions, int M, int n_heads, int n_kv_heads, int head_dim,
+                  hipStream_t s) {
+    CUINFER_CHECK_CRI(cri_qk_norm_rope(&rot, q, ldq, k, ldk, q_out, ldq_out, k_out, ldk_out, positions, M, n_heads,
+                                       n_kv_heads, head_dim, s));
+}
+void paged_append(const PagedKV& kv, const PagedBatch& batch, const HeadRotation& rot, const float* q, int ldq, float* q_out,
+                  int ldq_out, int n_heads, const float* k, int ldk, const float* v, int ldv, hipStream_t s) {
+    CUINFER_CHECK_CRI(cri_paged_append(&kv, &batch, &rot, q, ldq, q_out, ldq_out, n_heads, k, ldk, v, ldv, s));
+}
+void paged_attention(const PagedKV& kv, const PagedBatch& batch, const int* prefix_pages, int prefix_len, const float* q,
+                     int ldq, float* out, int ldo, int n_heads, float scale, void* workspace, long long workspace_bytes,
+                     hipStream_t s) {
+    CUINFER_CHECK_CRI(cri_paged_attention(&kv, &batch, prefix_pages, prefix_len, q, ldq, out, ldo, n_heads, scale, workspace,
+                                          workspace_bytes, s));
+}
+long long paged_attention_workspace_bytes(const PagedKV& kv, const PagedBatch& batch, int prefix_len, int n_heads) {
+    return checked_bytes(cri_paged_attention_workspace_bytes(&kv, &batch, prefix_len, n_heads));
+}
+void verify_drafts(const float* target, long long ldt, const float* draft, long long ldd, const int* draft_ids,
+                   const float* uniforms, const float* draws, const int* offsets, int n_seqs, int n_rows, int vocab,
+                   int* out_ids, int* n_accepted, void* workspace, long long workspace_bytes, hipStream_t s) {
+    CUINFER_CHECK_CRI(cri_verify_drafts(target, ldt, draft, ldd, draft_ids, uniforms, draws, offsets, n_seqs, n_rows, vocab,
+                                        out_ids, n_accepted, workspace, workspace_bytes, s));
+}
+long long verify_drafts_workspace_bytes(int n_seqs, int vocab) {
+    return checked_bytes(cri_verify_drafts_workspace_bytes(n_seqs, vocab));
 }
 
 // ---------------------------------------------------------------- dispatch

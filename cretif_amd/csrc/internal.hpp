@@ -90,6 +90,32 @@ struct SplitSums {
     int nss = 0;  // sums of squares added for the row factor (0: S of them)
 };
 
+// ---- a paged cache and a ragged batch of sequences, as the kernels take them (paged.hpp) ----
+constexpr int kKvF32 = 0, kKvF16 = 1, kKvBF16 = 2;  // cache types
+struct PagePool {
+    void* k;
+    void* v;
+    long stride;  // elements from one page to the next
+    int n_pages, page_size, n_kv_heads, head_dim;
+    uint32_t magic;  // page_index()
+    int shift;
+};
+struct PageBatch {
+    const int* offsets;  // [n_seqs + 1]: sequence s has the rows offsets[s] .. offsets[s + 1] - 1
+    const int* lens;     // [n_seqs]: positions it holds, those rows' included
+    const int* pages;    // [n_seqs][max_pages]
+    int n_seqs, n_rows, max_pages;
+};
+// norms and rotation of query and key heads
+struct HeadRotation {
+    const float* q_norm;  // null: not normed
+    const float* k_norm;
+    float eps;
+    int rot_dim;
+    bool halves;    // pairs (i, i + rot_dim / 2) instead of (2 i, 2 i + 1)
+    double log2_step;  // -2 log2(theta) / rot_dim: pair i turns by 2^(i log2_step) radians per position
+};
+
 namespace detail {
 
 // Launcher status: 0 = enqueued; kDeclined = this kernel does not take the shape
@@ -308,6 +334,27 @@ int launch_pos_set(int* pos, int value, hipStream_t stream);
 int launch_prefill_attention(const float* q, long ldq, const float* kc, const float* vc, float* ctx, int m0, int M,
                              int H, int Hkv, int D, int T4, const int* pos, float scale, float* qh, float* kt,
                              float* vh, float* sc, float* oh, hipStream_t stream);
+// norms and rotates the heads of q and k rows (head_rows.hip); positions [M]
+int launch_qk_norm_rope(const HeadRotation& R, const float* q, long ldq, const float* k, long ldk, float* q_out,
+                        long ldqo, float* k_out, long ldko, const int* positions, int M, int n_heads, int n_kv_heads,
+                        int head_dim, hipStream_t stream);
+// the same with k and v going to the cache's pages and the positions from the batch; q may be null
+int launch_paged_append(const PagePool& P, int type, const PageBatch& B, const HeadRotation& R, const float* q,
+                        long ldq, float* q_out, long ldqo, int n_heads, const float* k, long ldk, const float* v,
+                        long ldv, hipStream_t stream);
+
+// attention of the batch's rows over the pages, positions below prefix_len through prefix_pages
+// (paged_attention.hip); ws: 16-byte aligned, paged_attention_workspace_bytes of it, written before it is read
+long paged_attention_workspace_bytes(const PagePool& P, int type, const PageBatch& B, int n_heads, int prefix_len);
+int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, const int* prefix_pages, int prefix_len,
+                           const float* q, long ldq, float* out, long ldo, int n_heads, float scale, float* ws,
+                           hipStream_t stream);
+// drafted tokens against the target's probabilities (verify.hip); ws: 8-byte aligned, written before it is read
+long verify_workspace_bytes(int n_seqs, int vocab);
+int launch_verify_drafts(const float* target, long ldt, const float* draft, long ldd, const int* ids, const float* u,
+                         const float* draws, const int* offsets, int n_seqs, int n_rows, int vocab, int* out, int* accepted, double* ws,
+                         hipStream_t stream);
+
 // rows per launch_prefill_attention call of the C ABI and the decode step (the scores workspace
 // holds n_heads x this many rows x the cache length)
 constexpr int kPromptRows = 512;

@@ -1,0 +1,129 @@
+// paged_attention.hip -- how a call of the paged attention is cut into workgroups, and the kernel that joins their
+// records.
+#include "paged_attention.hpp"
+
+namespace cri {
+namespace dev {
+namespace {
+
+// One wave per (row, head): the records' maxima and sums weigh the accumulators.  Bound by the records' bytes.
+__global__ __launch_bounds__(256) void paged_join_kernel(const float* __restrict__ rec, float* __restrict__ out, long ldo,
+                                                         const int* __restrict__ offsets, int n_seqs, int n_rows, int H,
+                                                         int D, int lg, int nrec) {
+    const int lane = threadIdx.x & 63;
+    const int id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const int t = id / H, h = id % H;
+    if (t >= n_rows || t < offsets[0] || t >= offsets[n_seqs]) return;  // rows of no sequence stay as they were
+    const float* r = rec + static_cast<long>(id) * nrec * (D + 4);
+    float m = -INFINITY, l = 0.0f;
+    if (lane < nrec) {
+        const f32x2 x = *reinterpret_cast<const f32x2*>(r + static_cast<long>(lane) * (D + 4));
+        m = x.x;
+        l = x.y;
+    }
+    const float mx = wave_max(m);
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+    const float total = group_sum(l * f, 6);
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    // 2^lg lanes hold a record's accumulators, the wave's 64 >> lg groups of them take the records in turn
+    const int c = lane & ((1 << lg) - 1), grp = lane >> lg, groups = 64 >> lg;
+    f32x4 x = {0, 0, 0, 0};
+    for (int k0 = 0; k0 < nrec; k0 += groups) {
+        const int k = k0 + grp;
+        const float w = __shfl(f, min(k, nrec - 1));  // every lane takes part
+        if (k < nrec && w != 0.0f && 4 * c < D)        // a record of weight 0 may hold nothing
+            x += *reinterpret_cast<const f32x4*>(r + static_cast<long>(k) * (D + 4) + 4 + 4 * c) * w;
+    }
+    for (int m = 1 << lg; m < 64; m <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], m);
+    if (grp == 0 && 4 * c < D)
+        *reinterpret_cast<f32x4_a4*>(out + t * ldo + static_cast<long>(h) * D + 4 * c) =
+            f32x4_a4{x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+}
+
+// the cut of a call, from what the host knows of it
+struct Cut {
+    bool even;
+    int nc, pre_wq, pre_tiles, pre_chunks, pre_blocks, own_wq, own_tiles, own_chunks, nrec;
+    long own_blocks;
+};
+
+constexpr int kMaxRecords = 64;  // the joining wave keeps one record's maximum per lane
+
+Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int prefix_len) {
+    Cut c{};
+    const int D = P.head_dim, G = n_heads / P.n_kv_heads;
+    c.even = (D == 64 || D == 128 || D == 256) && P.page_size % 16 == 0;
+    const long rows = static_cast<long>(B.n_rows) * G;         // of a KV head
+    const long mean = (rows + B.n_seqs - 1) / B.n_seqs;        // of a KV head and sequence
+    const int tile = type == kKvF32 ? 16 : 32;
+    c.nc = c.even && D <= 128 && (mean > 16 || (prefix_len > 0 && rows > 16)) ? 2 : 1;
+    const int block = 16 * c.nc;
+    auto waves_of = [&](long r) { return r <= block ? 1 : r <= 2 * block ? 2 : 4; };
+    c.pre_wq = waves_of(rows);
+    c.own_wq = waves_of(mean);
+    const int target = 512;  // workgroups of each kind: two per CU
+    if (prefix_len > 0) {
+        c.pre_tiles = static_cast<int>((rows + block * c.pre_wq - 1) / (block * c.pre_wq));
+        const long streams = static_cast<long>(P.n_kv_heads) * c.pre_tiles;
+        const int wk = kPagedWaves / c.pre_wq, tiles = (prefix_len + tile - 1) / tile;
+        long n = (target + streams - 1) / streams;
+        n = std::min<long>(n, (tiles + 2 * wk - 1) / (2 * wk));  // at least two tiles to a wave
+        c.pre_chunks = static_cast<int>(std::min<long>(std::max<long>(n, 1), kMaxRecords / 2));
+        const int groups = (P.n_kv_heads * c.pre_chunks + kPagedXcds - 1) / kPagedXcds;
+        c.pre_blocks = groups * kPagedXcds * c.pre_tiles;
+    }
+    const long cap = static_cast<long>(B.max_pages) * P.page_size, own = std::max(cap - prefix_len, 0L);
+    const int rt = block * c.own_wq;
+    c.own_tiles = static_cast<int>(rows / rt + std::min<long>(B.n_seqs, B.n_rows));
+    {
+        const long streams = static_cast<long>(P.n_kv_heads) * c.own_tiles;
+        const int wk = kPagedWaves / c.own_wq;
+        long n = (target + streams - 1) / streams;
+        n = std::min<long>(n, (own + 2 * wk * tile - 1) / (2 * wk * tile));
+        c.own_chunks = static_cast<int>(std::min<long>(std::max<long>(n, 1), kMaxRecords / 2));
+    }
+    c.own_blocks = static_cast<long>(c.own_tiles) * c.own_chunks * P.n_kv_heads;
+    c.nrec = c.pre_chunks + c.own_chunks;
+    return c;
+}
+
+}  // namespace
+}  // namespace dev
+
+namespace detail {
+
+long paged_attention_workspace_bytes(const PagePool& P, int type, const PageBatch& B, int n_heads, int prefix_len) {
+    const dev::Cut c = dev::cut_of(P, type, B, n_heads, prefix_len);
+    return c.nrec == 1 ? 0 : static_cast<long>(B.n_rows) * n_heads * c.nrec * (P.head_dim + 4) * 4;
+}
+
+int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, const int* prefix_pages, int prefix_len,
+                           const float* q, long ldq, float* out, long ldo, int n_heads, float scale, float* ws,
+                           hipStream_t stream) {
+    const dev::Cut c = dev::cut_of(P, type, B, n_heads, prefix_len);
+    dev::PagedAttnArgs a{};
+    a.q = q, a.out = out, a.rec = ws, a.ldq = ldq, a.ldo = ldo;
+    a.P = P, a.B = B;
+    a.prefix_pages = prefix_pages, a.prefix_len = prefix_len;
+    a.H = n_heads, a.G = n_heads / P.n_kv_heads, a.nrec = c.nrec;
+    a.pre_wq = c.pre_wq, a.pre_tiles = c.pre_tiles, a.pre_chunks = c.pre_chunks, a.pre_blocks = c.pre_blocks;
+    a.own_wq = c.own_wq, a.own_tiles = c.own_tiles, a.own_chunks = c.own_chunks;
+    a.qscale = scale * 1.44269504088896340736f;
+    const long blocks = c.pre_blocks + c.own_blocks;
+    if (blocks > 0x7FFFFFFFL) return kDeclined;
+    const auto run = type == kKvF32 ? dev::run_paged_attn_f32 : type == kKvF16 ? dev::run_paged_attn_f16 : dev::run_paged_attn_bf16;
+    run(a, c.even, c.nc, static_cast<int>(blocks), stream);
+    if (c.nrec > 1) {
+        const long waves = static_cast<long>(B.n_rows) * n_heads;
+        int lg = 0;
+        while ((4 << lg) < P.head_dim) ++lg;
+        hipLaunchKernelGGL(dev::paged_join_kernel, dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, stream, ws,
+                           out, ldo, B.offsets, B.n_seqs, B.n_rows, n_heads, P.head_dim, lg, c.nrec);
+    }
+    return 0;
+}
+
+}  // namespace detail
+}  // namespace cri

@@ -1,0 +1,12 @@
+// paged_attention_f32.hip -- paged attention over a cache of this type (a unit of its own: the three compile side by side).
+#include "paged_attention.hpp"
+
+namespace cri {
+namespace dev {
+
+void run_paged_attn_f32(const PagedAttnArgs& a, bool even, int nc, int blocks, hipStream_t stream) {
+    run_paged_attn_type<kKvF32>(a, even, nc, blocks, stream);
+}
+
+}  // namespace dev
+}  // namespace cri

@@ -45,7 +45,8 @@ typedef enum cri_format {
     CRI_Q4_K = 3,
     CRI_Q6_K = 4,
     CRI_FP16 = 5,
-    CRI_FP32 = 6 /* only for cri_embedding_rows and cri_gguf_tensor.format */
+    CRI_FP32 = 6, /* only for cri_embedding_rows, cri_gguf_tensor.format and cri_paged_kv.type */
+    CRI_BF16 = 7  /* only for cri_paged_kv.type */
 } cri_format;
 
 /* ---- fused dequant + matmul: C[M,N] = A[M,K] * dequant(B[N,K])^T ---------- */
@@ -338,6 +339,118 @@ long long cri_decoder_weight_bytes(const cri_decoder* dec);
 /* weight bytes one step of M tokens reads: every layer's matrices and norms, the final norm and
  * LM head, and M token-table rows (the whole table when the head is tied to it) */
 long long cri_decoder_step_weight_bytes(const cri_decoder* dec, int M);
+
+/* ---- serving a batch from a paged cache ------------------------------------
+ * No counterpart in the reference, which decodes one sequence over a contiguous cache.  A layer of a
+ * batched step is: the fused q/k/v product, cri_paged_append, cri_paged_attention, the o product; a
+ * step that checks drafted tokens ends with cri_verify_drafts.  Activations are fp32, as everywhere
+ * in this library; the cache is fp32, fp16 or bf16.
+ *
+ * All of these enqueue on `stream` without synchronising, allocate nothing and may be captured in a
+ * HIP graph (what a descriptor points to is read when the kernels run, the descriptor itself and
+ * every host number at the call).  Calls that share a workspace must be ordered on one stream.
+ *
+ * A pool of pages: page p holds the K rows of page_size positions at k + p * page_stride elements,
+ * [page_size, n_kv_heads, head_dim], and the V rows likewise at v.  head_dim a multiple of 8, up to
+ * 256; page_stride a multiple of 8 and at least page_size * n_kv_heads * head_dim; k and v 16-byte
+ * aligned. */
+typedef struct cri_paged_kv {
+    void* k;
+    void* v;
+    long long page_stride; /* elements */
+    int type;              /* CRI_FP32, CRI_FP16 or CRI_BF16 */
+    int n_pages, page_size, n_kv_heads, head_dim;
+} cri_paged_kv;
+/* A ragged batch: sequence s has the rows offsets[s] .. offsets[s + 1] - 1 of q, k, v and the
+ * outputs (n_s of them, 0 or more), and holds lens[s] positions, those rows' included: its i-th row
+ * is at position lens[s] - n_s + i.  Position p lies in page pages[s * max_pages + p / page_size], at
+ * p % page_size.  offsets must not decrease.  n_rows: rows that the buffers have; rows before
+ * offsets[0] and from offsets[n_seqs] on (a padded batch) are neither read nor written.
+ * max_pages * page_size at most 2^30. */
+typedef struct cri_paged_batch {
+    const int* offsets; /* device [n_seqs + 1] */
+    const int* lens;    /* device [n_seqs] */
+    const int* pages;   /* device [n_seqs, max_pages] */
+    int n_seqs, n_rows, max_pages;
+} cri_paged_batch;
+/* Norms and rotation of query and key heads.  A head x becomes x * w / sqrt(mean(x^2) + eps) with w
+ * the norm weights [head_dim] (null: x as it is), then each pair (a, b) of its first rot_dim elements
+ * becomes (a cos - b sin, b cos + a sin) at the angle p * theta^(-2 i / rot_dim) for position p and
+ * pair i; elements from rot_dim on are not turned.  rot_dim a multiple of 8, up to head_dim (0: no
+ * rotation).  Angles are computed in 64 bits. */
+typedef enum cri_rope_pairs {
+    CRI_ROPE_ADJACENT = 0, /* pair i: elements 2 i and 2 i + 1, the decoder's layout */
+    CRI_ROPE_HALVES = 1    /* pair i: elements i and i + rot_dim / 2 */
+} cri_rope_pairs;
+typedef struct cri_rotation {
+    const float* q_norm; /* device, or null */
+    const float* k_norm;
+    float eps;
+    float theta;
+    int rot_dim;
+    int pairs; /* cri_rope_pairs */
+} cri_rotation;
+
+/* q_out = the heads of q [M, n_heads, head_dim], k_out = the heads of k [M, n_kv_heads, head_dim],
+ * normed and rotated, row m at position positions[m] (device int32).  Rows are ldq, ldk, ldq_out and
+ * ldk_out floats apart (at least their heads' width).  q_out may be q with ldq_out == ldq, k_out k
+ * with ldk_out == ldk; no other overlap of an output with another buffer (outputs of columns of one
+ * row are fine).  q or k may be left out with 0 heads.  Pointers 4-byte aligned. */
+int cri_qk_norm_rope(const cri_rotation* rot, const float* q, int ldq, const float* k, int ldk, float* q_out, int ldq_out,
+                     float* k_out, int ldk_out, const int* positions, int M, int n_heads, int n_kv_heads, int head_dim,
+                     hipStream_t stream);
+/* The batch's k rows, normed and rotated at their positions, and v rows as they are, go to their
+ * pages, rounded to the cache's type (to nearest even); with q not null, its n_heads heads go to
+ * q_out, normed and rotated, as by cri_qk_norm_rope.  A row whose position has no page (below 0,
+ * past the table's max_pages, a page number outside the pool) is left out: its page and q_out row
+ * stay as they were.  Pages that are written must belong to one sequence. */
+int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const cri_rotation* rot, const float* q, int ldq,
+                     float* q_out, int ldq_out, int n_heads, const float* k, int ldk, const float* v, int ldv,
+                     hipStream_t stream);
+/* out[row, h] = sum_j softmax_j(scale q[row, h] . k[j, h / G]) v[j, h / G] over the positions j in
+ * [0, p] of the row's sequence, p the row's position, G = n_heads / n_kv_heads; one row per sequence
+ * is a decode step, more are drafted tokens or a prompt's piece.  Positions j < prefix_len are read
+ * through prefix_pages (device [ceil(prefix_len / page_size)]) instead of the sequence's own table:
+ * a prefix that all sequences share, whose K and V are read once for the batch (its last page may
+ * be partly filled; the sequences' own positions start at prefix_len of their own tables).
+ * prefix_len 0: every position through its sequence's table.  A row at a position below 0 sees
+ * nothing and gets zeros; positions past the table (max_pages * page_size) are not seen.  Nothing
+ * behind a row's last position reaches it, whatever its pages hold there.  Table entries of positions
+ * that rows see must be inside the pool (others give unspecified numbers in their sequence's rows).
+ *
+ * q rows are ldq floats apart, out rows ldo; out must not overlap q or the pool.  n_heads a multiple
+ * of n_kv_heads.  q, out 4-byte aligned, workspace 16-byte, cri_paged_attention_workspace_bytes of
+ * it (the same kv, batch and prefix_len; only their host numbers count, so the bytes of a batch's
+ * n_seqs, n_rows and max_pages serve every step of it).  Sums, maxima and products are in fp32
+ * accuracy for every cache type; the order of sums is fixed by the host numbers. */
+int cri_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, const int* prefix_pages, int prefix_len,
+                        const float* q, int ldq, float* out, int ldo, int n_heads, float scale, void* workspace,
+                        long long workspace_bytes, hipStream_t stream);
+long long cri_paged_attention_workspace_bytes(const cri_paged_kv* kv, const cri_paged_batch* batch, int prefix_len,
+                                              int n_heads);
+/* Drafted tokens checked by rejection sampling.  Sequence s has the rows offsets[s] ..
+ * offsets[s + 1] - 1 (n_s of them) of target (probabilities of the token that follows each row's
+ * token, [n_rows, vocab], rows ldt floats apart), draft (the draft's probabilities, rows ldd apart;
+ * null: the draft was sure of its tokens), draft_ids, uniforms and draws ([n_rows], random numbers in
+ * [0, 1)).  Row j < n_s - 1 holds the drafted token that follows it; the last row's draft and
+ * draft_ids are not read.  Draft j is accepted when uniforms[j] * draft[j][x] < target[j][x], x =
+ * draft_ids[j] (a token outside [0, vocab) never is).  The first that is not is replaced by a token
+ * drawn from max(target - draft, 0) of its row (of target where that leaves nothing; a sure draft:
+ * target without x); with all accepted one more is drawn from the last row's target.  Drawing takes
+ * the smallest token whose running sum of weights exceeds draws[that row] times their total (the last
+ * token with any weight where rounding or the number leaves none; -1 where no token has weight).
+ * The tokens follow the target's distribution when draws are independent of uniforms: a row's number
+ * that has decided about its draft must not draw its replacement too.
+ * out_ids [n_rows]: the accepted drafts, the drawn token, -1 in the sequence's remaining rows;
+ * n_accepted [n_seqs].  Rows outside [offsets[0], offsets[n_seqs]) are neither read nor written, a
+ * sequence of no rows gets n_accepted 0.  NaN and negative probabilities count as zero.  Comparisons
+ * and sums are in 64 bits and in a fixed order.
+ * out_ids must not overlap draft_ids.  workspace: 8-byte aligned, cri_verify_drafts_workspace_bytes. */
+int cri_verify_drafts(const float* target, long long ldt, const float* draft, long long ldd, const int* draft_ids,
+                      const float* uniforms, const float* draws, const int* offsets, int n_seqs, int n_rows,
+                      int vocab, int* out_ids, int* n_accepted, void* workspace, long long workspace_bytes,
+                      hipStream_t stream);
+long long cri_verify_drafts_workspace_bytes(int n_seqs, int vocab);
 
 /* ---- diagnostics ---------------------------------------------------------- */
 

@@ -1,0 +1,186 @@
+"""The batched serving entry points refuse bad arguments before touching the GPU (so this runs without one), and
+the definitions the GPU tests use agree with what they claim."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import cretif_amd as cri
+import serving_ref as ref
+from cretif_amd import serving
+
+FAKE = 1 << 20  # never dereferenced: every case below fails validation first
+
+
+def kv(**kw):
+    c = dict(k=FAKE, v=FAKE, page_stride=16 * 2 * 64, type=5, n_pages=4, page_size=16, n_kv_heads=2, head_dim=64)
+    c.update(kw)
+    return serving._PagedKV(**c)
+
+
+def batch(**kw):
+    c = dict(offsets=FAKE, lens=FAKE, pages=FAKE, n_seqs=2, n_rows=3, max_pages=5)
+    c.update(kw)
+    return serving._PagedBatch(**c)
+
+
+def rot(**kw):
+    c = dict(q_norm=0, k_norm=0, eps=1e-6, theta=1e4, rot_dim=64, pairs=0)
+    c.update(kw)
+    return serving._Rotation(**c)
+
+
+def ref_of(x):
+    return None if x is None else ctypes.addressof(x)
+
+
+def status(fn, *args):
+    return getattr(cri.lib(), fn)(*args)
+
+
+# rows of fake buffers are far apart
+Q, K, V, O, O2, WS = (FAKE << i for i in range(2, 8))
+
+
+def norm_rope(r=None, q=Q, ldq=256, k=K, ldk=128, qo=O, ldqo=256, ko=O2, ldko=128, pos=FAKE, M=3, H=4, Hkv=2, D=64):
+    r = rot() if r is None else r
+    return status("cri_qk_norm_rope", ref_of(r), q, ldq, k, ldk, qo, ldqo, ko, ldko, pos, M, H, Hkv, D, None)
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(M=-1), -1), (dict(H=-1), -1), (dict(D=-8), -1), (dict(D=0), -5), (dict(D=60), -5), (dict(D=264), -5),
+    (dict(r=rot(pairs=2)), -5), (dict(r=rot(rot_dim=12)), -2), (dict(r=rot(rot_dim=72)), -2), (dict(r=rot(rot_dim=-8)), -2),
+    (dict(r=rot(theta=0.0)), -1), (dict(r=rot(theta=float("nan"))), -1), (dict(r=rot(theta=float("inf"))), -1),
+    (dict(r=rot(q_norm=FAKE, eps=-1.0)), -1), (dict(r=rot(q_norm=FAKE + 2)), -3), (dict(pos=0), -1), (dict(pos=FAKE + 1), -3),
+    (dict(q=0), -1), (dict(qo=0), -1), (dict(k=0), -1), (dict(ko=0), -1), (dict(q=Q + 2), -3), (dict(ldq=255), -2),
+    (dict(ldk=127), -2), (dict(ldqo=8), -2), (dict(qo=Q + 16), -1), (dict(ko=Q), -1), (dict(qo=Q, ldqo=512), -1),
+    (dict(ko=O + 4 * 128, ldko=256), -1), (dict(M=1 << 30, ldq=1 << 20), -2),
+])
+def test_norm_rope_refuses(kw, want):
+    assert norm_rope(**kw) == want
+
+
+def test_norm_rope_null_rotation():
+    assert status("cri_qk_norm_rope", None, Q, 256, K, 128, O, 256, O2, 128, FAKE, 3, 4, 2, 64, None) == -1
+
+
+def test_norm_rope_empty():
+    assert norm_rope(M=0, q=0, k=0, qo=0, ko=0, pos=0) == 0
+    assert norm_rope(H=0, Hkv=0, q=0, k=0, qo=0, ko=0, pos=0) == 0
+
+
+def append(p=None, b=None, r=None, q=Q, ldq=256, qo=O, ldqo=256, H=4, k=K, ldk=128, v=V, ldv=128):
+    p, b, r = kv() if p is None else p, batch() if b is None else b, rot() if r is None else r
+    return status("cri_paged_append", ref_of(p), ref_of(b), ref_of(r), q, ldq, qo, ldqo, H, k, ldk, v, ldv, None)
+
+
+POOL = [
+    (dict(p=kv(type=3)), -5), (dict(p=kv(type=0)), -5), (dict(p=kv(head_dim=60)), -5), (dict(p=kv(head_dim=512)), -5),
+    (dict(p=kv(n_pages=-1)), -1), (dict(p=kv(n_pages=0)), -2), (dict(p=kv(page_size=0)), -2), (dict(p=kv(n_kv_heads=0)), -2),
+    (dict(p=kv(page_stride=16 * 2 * 64 - 8)), -2), (dict(p=kv(page_stride=16 * 2 * 64 + 4)), -2),
+    (dict(p=kv(page_stride=-1)), -2), (dict(p=kv(page_stride=1 << 50)), -2), (dict(p=kv(k=0)), -1), (dict(p=kv(v=0)), -1),
+    (dict(p=kv(k=FAKE + 8)), -3), (dict(p=kv(v=FAKE + 2)), -3), (dict(b=batch(n_seqs=-1)), -1), (dict(b=batch(n_rows=-1)), -1),
+    (dict(b=batch(max_pages=-1)), -1), (dict(b=batch(max_pages=1 << 27)), -2), (dict(b=batch(offsets=0)), -1),
+    (dict(b=batch(lens=0)), -1), (dict(b=batch(pages=0)), -1), (dict(b=batch(pages=FAKE + 2)), -3),
+]
+
+
+@pytest.mark.parametrize("kw,want", POOL + [
+    (dict(r=rot(rot_dim=4)), -2), (dict(H=-1), -1), (dict(k=0), -1), (dict(v=0), -1), (dict(v=V + 1), -3), (dict(ldv=127), -2),
+    (dict(qo=0), -1), (dict(ldq=255), -2), (dict(qo=K), -1), (dict(qo=V), -1), (dict(qo=Q, ldqo=257), -1),
+])
+def test_append_refuses(kw, want):
+    assert append(**kw) == want
+
+
+def test_append_empty():
+    assert append(b=batch(n_seqs=0, offsets=0, lens=0, pages=0), k=0, v=0) == 0
+    assert append(b=batch(n_rows=0), k=0, v=0, q=0, qo=0) == 0
+
+
+def attend(p=None, b=None, pp=FAKE, P=20, q=Q, ldq=256, o=O, ldo=256, H=4, ws=WS, wsb=1 << 40):
+    p, b = kv() if p is None else p, batch() if b is None else b
+    return status("cri_paged_attention", ref_of(p), ref_of(b), pp, P, q, ldq, o, ldo, H, 0.125, ws, wsb, None)
+
+
+@pytest.mark.parametrize("kw,want", POOL + [
+    (dict(H=3), -2), (dict(H=-2), -1), (dict(P=-1), -1), (dict(P=(1 << 30) + 1), -2), (dict(pp=0), -1), (dict(pp=FAKE + 2), -3),
+    (dict(q=0), -1), (dict(o=0), -1), (dict(ldq=255), -2), (dict(ldo=100), -2), (dict(o=Q), -1), (dict(o=Q + 1024), -1),
+    (dict(ws=0), -1), (dict(ws=WS + 8), -3), (dict(wsb=100), -2), (dict(b=batch(max_pages=0)), -2),
+    (dict(b=batch(n_rows=1 << 23)), -2),
+])
+def test_attention_refuses(kw, want):
+    assert attend(**kw) == want
+
+
+def test_attention_empty():
+    assert attend(b=batch(n_seqs=0), q=0, o=0, ws=0) == 0
+    assert attend(b=batch(n_rows=0), q=0, o=0, ws=0) == 0
+    assert attend(H=0, q=0, o=0, ws=0) == 0
+    f = cri.lib().cri_paged_attention_workspace_bytes
+    assert f(ref_of(kv()), ref_of(batch(n_seqs=0)), 20, 4) == 0
+    assert f(ref_of(kv()), ref_of(batch()), 20, 4) > 0
+    assert f(ref_of(kv()), ref_of(batch()), 20, 3) == -2
+    assert f(None, ref_of(batch()), 20, 4) == -1
+
+
+def verify(t=Q, ldt=100, d=K, ldd=100, ids=FAKE, u=V, dr=V, off=FAKE, B=2, n=5, vocab=100, out=O, acc=O2, ws=WS, wsb=1 << 40):
+    return status("cri_verify_drafts", t, ldt, d, ldd, ids, u, dr, off, B, n, vocab, out, acc, ws, wsb, None)
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(B=-1), -1), (dict(n=-1), -1), (dict(vocab=-1), -1), (dict(vocab=0), -2), (dict(t=0), -1), (dict(ids=0), -1),
+    (dict(u=0), -1), (dict(dr=0), -1), (dict(dr=V + 2), -3), (dict(off=0), -1), (dict(out=0), -1), (dict(acc=0), -1), (dict(t=Q + 2), -3), (dict(d=K + 1), -3),
+    (dict(ldt=99), -2), (dict(ldd=99), -2), (dict(ldt=1 << 50), -2), (dict(out=FAKE + 4), -1), (dict(ws=0), -1),
+    (dict(ws=WS + 4), -3), (dict(wsb=16), -2), (dict(B=(1 << 20) + 1), -2),
+])
+def test_verify_refuses(kw, want):
+    assert verify(**kw) == want
+
+
+def test_verify_empty():
+    assert verify(B=0, t=0, ids=0, u=0, off=0, out=0, acc=0, ws=0) == 0
+    f = cri.lib().cri_verify_drafts_workspace_bytes
+    assert f(0, 100) == 0 and f(2, 100) > 0 and f(-1, 100) == -1
+
+
+def test_messages_name_the_function():
+    attend(H=3)
+    assert cri.lib().cri_last_error_string().decode().startswith("cri_paged_attention: n_heads=3")
+
+
+def test_python_refuses_host_tensors():
+    torch = pytest.importorskip("torch")
+    x = torch.zeros(4, 16, 2, 64)
+    with pytest.raises(ValueError, match="device"):
+        cri.PagedKV(x, x)
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        cri.PagedKV(x.double(), x.double())
+    with pytest.raises(ValueError, match="n_pages"):
+        cri.PagedKV(x, x[0])
+    with pytest.raises(ValueError, match="int32"):
+        cri.PagedBatch(torch.zeros(3), torch.zeros(2), torch.zeros(2, 5))
+    with pytest.raises(ValueError, match="q_norm"):
+        cri.Rotation(1e4, 64, q_norm=torch.zeros(64, dtype=torch.float64))
+    with pytest.raises(KeyError):
+        cri.Rotation(1e4, 64, "sideways")
+    with pytest.raises(ValueError, match="device"):
+        cri.qk_norm_rope(cri.Rotation(1e4, 64), torch.zeros(2, 128), None, torch.zeros(2, 128), None,
+                         torch.zeros(2, dtype=torch.int32), 2, 0, 64)
+    with pytest.raises(ValueError, match="float32"):
+        cri.verify_drafts(torch.zeros(2, 8).half(), None, None, None, None, None, None, None)
+
+
+def test_definition_keeps_the_targets_distribution():
+    """Rejection sampling as defined draws from the target whatever the draft: over a fine grid of numbers, every
+    token's share of the first output is the target's (off by the grid's steps: one per accepted or drawn interval)."""
+    p, q = np.array([0.5, 0.2, 0.0, 0.3]), np.array([0.1, 0.6, 0.2, 0.1])
+    n = 40
+    share = np.zeros(4)
+    for x in range(4):  # the draft's token, with its probability
+        for i in range(n):
+            for j in range(n):
+                u, d = [(i + 0.5) / n, 0.5], [(j + 0.5) / n, 0.5]
+                out, _ = ref.verify(np.stack([p, p]), np.stack([q, q]), [x, 0], u, d, [0, 2], [0, 0], [0])
+                share[out[0]] += q[x] / n / n
+    assert np.abs(share - p).max() <= 1.0 / n
