@@ -852,6 +852,8 @@ long long cri_verify_drafts_workspace_bytes(int n_seqs, int vocab) {
     if (n_seqs < 0 || vocab < 0)
         return fail(CRI_ERR_INVALID_ARGUMENT, "cri_verify_drafts_workspace_bytes", "negative dimension");
     if (n_seqs == 0 || vocab == 0) return 0;
+    if (n_seqs > (1 << 20) || vocab > (1 << 28))
+        return fail(CRI_ERR_SHAPE, "cri_verify_drafts_workspace_bytes", "more than 2^20 sequences or 2^28 tokens");
     return cri::detail::verify_workspace_bytes(n_seqs, vocab);
 }
 
@@ -863,7 +865,7 @@ int cri_verify_drafts(const float* target, long long ldt, const float* draft, lo
     if (n_seqs < 0 || n_rows < 0 || vocab < 0) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "negative dimension");
     if (n_seqs == 0) return CRI_OK;
     if (vocab == 0) return fail(CRI_ERR_SHAPE, fn, "vocab must be at least 1");
-    if (n_seqs > (1 << 20)) return fail(CRI_ERR_SHAPE, fn, "more than 2^20 sequences");
+    if (n_seqs > (1 << 20) || vocab > (1 << 28)) return fail(CRI_ERR_SHAPE, fn, "more than 2^20 sequences or 2^28 tokens");
     if (!offsets || !n_accepted || (n_rows > 0 && (!target || !draft_ids || !uniforms || !draws || !out_ids)))
         return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null pointer");
     if (!aligned(target, 4) || !aligned(draft, 4) || !aligned(draft_ids, 4) || !aligned(uniforms, 4) ||

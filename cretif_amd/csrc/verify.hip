@@ -7,10 +7,11 @@
 // weights up to and with v exceeds d times the total.
 //
 //   * u q(x) < p(x) is decided in 64 bits, where the product of two 32-bit numbers is exact.
-//   * Weights are differences in 64 bits and so are their sums, whose order is fixed: per lane, wave, slice.
+//   * Weights are differences in 64 bits and so are their sums, whose order is fixed: thread, wave, slice.
 //   * Bound by memory: one row of p and of q per sequence (2 V floats), whatever the number of drafts.  A sequence's
-//     rows are cut into slices over workgroups, so that a single sequence, too, is read by many CUs; the second
-//     kernel finds the slice by the slices' sums and the token within it, re-reading that slice alone.
+//     rows are cut into slices over workgroups, so that a single sequence, too, is read by many CUs.  The second
+//     kernel finds the slice by the slices' sums and the token within it in one pass of 1024 threads, eight tokens
+//     each, over that slice alone, which the first kernel has left in the caches.
 #include <algorithm>
 
 #include "common.hpp"
@@ -21,6 +22,9 @@ namespace dev {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64;
+constexpr int kPer = 8;                          // tokens of a picking thread
+constexpr int kMaxSlice = kPer * kPickThreads;  // tokens of a slice
 
 struct VerifyArgs {
     const float* target;
@@ -33,6 +37,7 @@ struct VerifyArgs {
     int* out;
     int* accepted;
     double* sums;  // [n_seqs][slices]: sums of the weights, of p
+    int* counts;   // [n_seqs]: drafts accepted, -1 for a sequence of no rows
     int n_seqs, n_rows, V, slices, per;
 };
 
@@ -67,19 +72,35 @@ __device__ __forceinline__ void accept(const VerifyArgs& a, int s, int& first, i
     acc = n - 1;
 }
 
-// the weight of token v: what the draft leaves of p, or p itself
+// the weight of a token: what the draft leaves of p, or p itself
 struct Weight {
     const float* p;
     const float* q;  // null: none
     int sure;        // the token a draft without probabilities is sure of, or -1
-    __device__ __forceinline__ void at(int v, double& w, double& t) const {
-        t = p[v] > 0.0f ? static_cast<double>(p[v]) : 0.0;  // NaN counts as zero
+    __device__ __forceinline__ void of(int v, float pv, float qv, double& w, double& t) const {
+        t = pv > 0.0f ? static_cast<double>(pv) : 0.0;  // NaN counts as zero
         w = t;
         if (q != nullptr) {
-            w = t - static_cast<double>(q[v]);
+            w = t - static_cast<double>(qv);
             w = w > 0.0 ? w : 0.0;
         }
         if (v == sure) w = 0.0;
+    }
+    // tokens v .. v + 3, zeros from hi on
+    __device__ __forceinline__ void load4(int v, int hi, f32x4& pv, f32x4& qv) const {
+        pv = qv = f32x4{0, 0, 0, 0};
+        if (v + 4 <= hi) {
+            pv = ld_f32x4(p + v);
+            if (q != nullptr) qv = ld_f32x4(q + v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                if (v + i < hi) {
+                    pv[i] = p[v + i];
+                    if (q != nullptr) qv[i] = q[v + i];
+                }
+            }
+        }
     }
 };
 __device__ __forceinline__ Weight weight_of(const VerifyArgs& a, int first, int n, int acc) {
@@ -104,15 +125,25 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyArgs 
     const int s = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
     int first, n, acc;
     accept(a, s, first, n, acc);
+    if (slice == 0 && threadIdx.x == 0) a.counts[s] = n == 0 ? -1 : acc;
     if (n == 0) return;
     const Weight W = weight_of(a, first, n, acc);
     const int lo = slice * a.per, hi = min(lo + a.per, a.V);
     double w = 0.0, t = 0.0;
-    for (int v = lo + threadIdx.x; v < hi; v += kThreads) {
-        double x, y;
-        W.at(v, x, y);
-        w += x;
-        t += y;
+    constexpr int kAhead = 4;  // loads of p and of q in flight
+    for (int v0 = lo + 4 * threadIdx.x; v0 < hi; v0 += 4 * kThreads * kAhead) {
+        f32x4 p[kAhead], q[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) W.load4(v0 + 4 * kThreads * j, hi, p[j], q[j]);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                double x, y;
+                W.of(v0 + 4 * kThreads * j + i, p[j][i], q[j][i], x, y);
+                w += x;
+                t += y;
+            }
     }
     w = wave_sum(w);
     t = wave_sum(t);
@@ -132,24 +163,35 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyArgs 
     }
 }
 
+__device__ __forceinline__ double scan_up(double c, int lane) {  // inclusive sums over the wave
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const double o = __shfl_up(c, m);
+        if (lane >= m) c += o;
+    }
+    return c;
+}
+
 // grid (sequences): the token, the sequence's output rows
-__global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyArgs a) {
-    __shared__ double part[kWaves];
-    __shared__ int found[kWaves], last[kWaves];
+__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyArgs a) {
+    __shared__ double part[kPickWaves];
+    __shared__ int found[kPickWaves], last[kPickWaves];
     const int s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int first, n, acc;
-    accept(a, s, first, n, acc);
-    if (n == 0) {
+    const int acc = a.counts[s], first = a.offsets[s], n = a.offsets[s + 1] - first;
+    if (acc < 0) {
         if (threadIdx.x == 0) a.accepted[s] = 0;
         return;
     }
     Weight W = weight_of(a, first, n, acc);
+    // every wave: the totals, then the first slice whose running sum exceeds the wanted one, else the last with weight
     const double* sums = a.sums + static_cast<long>(s) * a.slices * 2;
     double total = 0.0, plain = 0.0;
-    for (int i = 0; i < a.slices; ++i) {
+    for (int i = lane; i < a.slices; i += 64) {
         total += sums[2 * i];
         plain += sums[2 * i + 1];
     }
+    total = wave_sum(total);
+    plain = wave_sum(plain);
     const int which = total > 0.0 ? 0 : 1;  // the draft leaves nothing: from p itself
     if (which) {
         W.q = nullptr;
@@ -157,72 +199,77 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyArgs 
         total = plain;
     }
     const double want = a.draws[first + acc] * total;
-    // the slice: the first whose running sum exceeds the wanted one, else the last with any weight
     double before = 0.0, run = 0.0;
-    int slice = -1, heavy = -1;
-    double heavy_before = 0.0;
-    for (int i = 0; i < a.slices; ++i) {
-        const double x = sums[2 * i + which];
-        if (x > 0.0) {
-            heavy = i;
-            heavy_before = run;
+    int slice = -1;
+    for (int base = 0; base < a.slices; base += 64) {
+        const int i = base + lane;
+        const double x = i < a.slices ? sums[2 * i + which] : 0.0;
+        const double c = scan_up(x, lane), prev = __shfl_up(c, 1);
+        const double at = lane ? run + prev : run;
+        const unsigned long hit = __ballot(x > 0.0 && run + c > want), any = __ballot(x > 0.0);
+        if (any != 0) {
+            const int pick = hit ? __builtin_ctzl(hit) : 63 - __builtin_clzl(any);
+            slice = base + pick;
+            before = __shfl(at, pick);
         }
-        if (run + x > want) {
-            slice = i;
-            before = run;
-            break;
-        }
-        run += x;
-    }
-    if (slice < 0) {
-        slice = heavy;
-        before = heavy_before;
+        if (hit != 0) break;
+        run += __shfl(c, 63);
     }
     int token = -1;  // no weight anywhere
     if (slice >= 0) {
-        const int lo = slice * a.per, hi = min(lo + a.per, a.V);
-        double at = before;
-        int best = -1;
-        for (int v0 = lo; v0 < hi; v0 += kThreads) {
-            const int v = v0 + threadIdx.x;
-            double x = 0.0, y;
-            if (v < hi) W.at(v, x, y);
-            double c = x;
+        const int lo = slice * a.per, hi = min(lo + a.per, a.V), v0 = lo + kPer * threadIdx.x;
+        double x[kPer], sum = 0.0, y;
 #pragma unroll
-            for (int m = 1; m < 64; m <<= 1) {
-                const double o = __shfl_up(c, m);
-                if (lane >= m) c += o;
+        for (int j = 0; j < kPer; j += 4) {
+            f32x4 p, q;
+            W.load4(v0 + j, hi, p, q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                W.of(v0 + j + i, p[i], q[i], x[j + i], y);
+                sum += x[j + i];
             }
-            if (lane == 63) part[wave] = c;
-            __syncthreads();
-            double base = at;
-            for (int i = 0; i < wave; ++i) base += part[i];
-            const unsigned long hit = __ballot(x > 0.0 && base + c > want), any = __ballot(x > 0.0);
-            if (lane == 0) {
-                found[wave] = hit ? v0 + wave * 64 + __builtin_ctzl(hit) : -1;
-                last[wave] = any ? v0 + wave * 64 + 63 - __builtin_clzl(any) : -1;
-            }
-            __syncthreads();
-            for (int i = 0; i < kWaves; ++i) {
-                at += part[i];
-                if (last[i] >= 0) best = last[i];
-            }
-            for (int i = kWaves - 1; i >= 0; --i)
-                if (found[i] >= 0) token = found[i];
-            __syncthreads();
-            if (token >= 0) break;
         }
-        if (token < 0) token = best;
+        const double c = scan_up(sum, lane);
+        double prev = __shfl_up(c, 1);
+        if (lane == 0) prev = 0.0;
+        if (lane == 63) part[wave] = c;
+        __syncthreads();
+        double base = before;
+        for (int i = 0; i < wave; ++i) base += part[i];
+        const unsigned long hit = __ballot(sum > 0.0 && base + c > want), any = __ballot(sum > 0.0);
+        // the thread's token: the first whose running sum exceeds the wanted one, else its last with weight
+        int mine = -1;
+        double at = base + prev;
+        bool done = false;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            at += x[j];
+            if (x[j] > 0.0 && !done) {
+                mine = v0 + j;
+                done = at > want;
+            }
+        }
+        const int hit_token = __shfl(mine, hit ? __builtin_ctzl(hit) : 0);
+        const int any_token = __shfl(mine, any ? 63 - __builtin_clzl(any) : 0);
+        if (lane == 0) {
+            found[wave] = hit ? hit_token : -1;
+            last[wave] = any ? any_token : -1;
+        }
+        __syncthreads();
+        for (int i = 0; i < kPickWaves; ++i)
+            if (last[i] >= 0) token = last[i];
+        for (int i = kPickWaves - 1; i >= 0; --i)
+            if (found[i] >= 0) token = found[i];
     }
-    for (int j = threadIdx.x; j < n; j += kThreads)
+    for (int j = threadIdx.x; j < n; j += kPickThreads)
         a.out[first + j] = j < acc ? a.ids[first + j] : j == acc ? token : -1;
     if (threadIdx.x == 0) a.accepted[s] = acc;
 }
 
-// slices of a row: about 1024 workgroups over all sequences, of at least 1024 tokens
-int slices_of(int n_seqs, int V) {
-    const int most = (V + 1023) / 1024;
-    return std::max(1, std::min(most, (1024 + n_seqs - 1) / n_seqs));
+// tokens of a slice: about 1024 workgroups over all sequences, 1024 to kMaxSlice tokens each
+int slice_of(int n_seqs, int V) {
+    const int slices = std::max((1024 + n_seqs - 1) / n_seqs, 1);
+    return std::min(std::max((V / slices + 1023) / 1024 * 1024, 1024), kMaxSlice);
 }
 
 }  // namespace
@@ -231,17 +278,19 @@ int slices_of(int n_seqs, int V) {
 namespace detail {
 
 long verify_workspace_bytes(int n_seqs, int vocab) {
-    return static_cast<long>(n_seqs) * dev::slices_of(n_seqs, vocab) * 16;
+    const int per = dev::slice_of(n_seqs, vocab), slices = (vocab - 1) / per + 1;
+    return static_cast<long>(n_seqs) * (slices * 16L + 4);
 }
 
 int launch_verify_drafts(const float* target, long ldt, const float* draft, long ldd, const int* ids, const float* u,
-                         const float* draws, const int* offsets, int n_seqs, int n_rows, int vocab, int* out, int* accepted, double* ws,
-                         hipStream_t stream) {
-    dev::VerifyArgs a{target, draft, ldt, ldd, ids, u, draws, offsets, out, accepted, ws, n_seqs, n_rows, vocab, 0, 0};
-    a.slices = dev::slices_of(n_seqs, vocab);
-    a.per = (vocab + a.slices - 1) / a.slices;
-    hipLaunchKernelGGL(dev::verify_sums_kernel, dim3(static_cast<unsigned>(n_seqs) * a.slices), dim3(dev::kThreads), 0, stream, a);
-    hipLaunchKernelGGL(dev::verify_pick_kernel, dim3(n_seqs), dim3(dev::kThreads), 0, stream, a);
+                         const float* draws, const int* offsets, int n_seqs, int n_rows, int vocab, int* out, int* accepted,
+                         double* ws, hipStream_t stream) {
+    const int per = dev::slice_of(n_seqs, vocab), slices = (vocab - 1) / per + 1;
+    if (static_cast<long>(n_seqs) * slices > 0x7FFFFFFFL) return kDeclined;
+    const dev::VerifyArgs a{target, draft, ldt, ldd, ids, u, draws, offsets, out, accepted, ws,
+                            reinterpret_cast<int*>(ws + 2L * n_seqs * slices), n_seqs, n_rows, vocab, slices, per};
+    hipLaunchKernelGGL(dev::verify_sums_kernel, dim3(static_cast<unsigned>(n_seqs) * slices), dim3(dev::kThreads), 0, stream, a);
+    hipLaunchKernelGGL(dev::verify_pick_kernel, dim3(n_seqs), dim3(dev::kPickThreads), 0, stream, a);
     return 0;
 }
 

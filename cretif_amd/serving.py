@@ -45,72 +45,76 @@ def declare(L):
         f.argtypes, f.restype = args, res
 
 
-def _on_device(t, name):
+def _device():
+    try:
+        return torch._C._cuda_getDevice()
+    except RuntimeError:  # no GPU: the buffers' own checks say so
+        return None
+
+
+def _on_device(t, name, dev=None):
     """The tensor's address; it must be on the current GPU."""
-    if not t.is_cuda:
+    d = t.get_device()
+    if d < 0:
         raise ValueError("%s is on %s; the HIP kernels need device (cuda) tensors" % (name, t.device))
-    if t.get_device() != torch._C._cuda_getDevice():
+    if d != (_device() if dev is None else dev):
         raise ValueError("%s is on %s, not on the current device" % (name, t.device))
     return t.data_ptr()
 
 
-def _rows(t, name):
-    """(address, floats from row to row, rows or None) of a row buffer."""
+def _rows(t, width, name, dev):
+    """(address, floats from row to row, rows or None) of a row buffer of `width` floats a row."""
     if type(t) is tuple:
         return t[0], t[1], None
+    sh, st = t.shape, t.stride()
+    if len(sh) == 2 and sh[0] > 1 and st[1] == 1 and sh[1] == width and t.dtype is torch.float32:  # the usual case first
+        return _on_device(t, name, dev), st[0], sh[0]
     if t.dtype is not torch.float32:
         raise ValueError("%s must be float32, not %s" % (name, t.dtype))
-    d = t.dim()
-    if d == 2:
-        ld, inner = t.stride()
-        tight = inner == 1 or t.shape[1] <= 1
-    elif d == 3:
-        ld, mid, inner = t.stride()
-        tight = (inner == 1 or t.shape[2] <= 1) and (mid == t.shape[2] or t.shape[1] <= 1)
-    else:
+    if len(sh) not in (2, 3):
         raise ValueError("%s must have the shape [rows, width] or [rows, heads, head_dim]" % name)
-    if not tight:
+    inner, wide = sh[-1], sh[1] * (sh[2] if len(sh) == 3 else 1)
+    if wide != width:
+        raise ValueError("%s has rows of %d floats, not %d" % (name, wide, width))
+    if (inner > 1 and st[-1] != 1) or (len(sh) == 3 and sh[1] > 1 and st[1] != inner):
         raise ValueError("%s: the elements of a row must be consecutive" % name)
-    n = t.shape[0]
-    width = t.shape[1] if d == 2 else t.shape[1] * t.shape[2]
-    if n <= 1:
-        ld = max(ld, width)  # the stride of a single row says nothing
-    return _on_device(t, name), ld, n
-
-
-def _wide(t, name, width):
-    if type(t) is not tuple and t.shape[0] and t.numel() // t.shape[0] != width:
-        raise ValueError("%s has rows of %d floats, not %d" % (name, t.numel() // t.shape[0], width))
+    # the stride of a single row says nothing
+    return _on_device(t, name, dev), st[0] if sh[0] > 1 else max(st[0], width), sh[0]
 
 
 def _same_rows(n_rows, *named):
     for name, n in named:
-        if n is None:
-            continue
-        if n_rows is None:
+        if n is not None and n != n_rows:
+            if n_rows is not None:
+                raise ValueError("%s has %d rows, not %d" % (name, n, n_rows))
             n_rows = n
-        elif n != n_rows:
-            raise ValueError("%s has %d rows, not %d" % (name, n, n_rows))
     if n_rows is None:
         raise ValueError("n_rows must be given with (address, ld) buffers")
     return n_rows
 
 
-def _ints(t, name, dims):
+def _ints(t, name, dims, dev=None):
     if t.dtype is not torch.int32 or t.dim() != dims or not t.is_contiguous():
         raise ValueError("%s must be a contiguous int32 tensor of %d dimension(s)" % (name, dims))
-    return _on_device(t, name)
+    return _on_device(t, name, dev)
 
 
-def _room(workspace, need, stream):
-    """(address, bytes, tensor) of the workspace, allocated on the current stream when there is none."""
-    if workspace is None:
-        if stream is not None and need:
-            raise ValueError("give a workspace with an explicit stream (an allocated one belongs to the current stream)")
-        workspace = torch.empty(need, dtype=torch.uint8, device="cuda")
+def _room(workspace, dev):
+    """(address, bytes) of a workspace."""
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    return _on_device(workspace, "workspace"), workspace.numel() * workspace.element_size(), workspace
+    return _on_device(workspace, "workspace", dev), workspace.nbytes
+
+
+def _new_room(need, stream):
+    if stream is not None:
+        raise ValueError("give a workspace with an explicit stream (an allocated one belongs to the current stream)")
+    return torch.empty(need, dtype=torch.uint8, device="cuda")
+
+
+def _on(stream, dev):
+    """The stream's address; the device's current stream when None (the buffers have initialised the GPU)."""
+    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)
 
 
 class Rotation:
@@ -128,10 +132,11 @@ class Rotation:
                             None if k_norm is None else _on_device(k_norm, "k_norm"), eps, theta, rot_dim, PAIRS[pairs])
         self._ref = ctypes.addressof(self._c)
 
+        self._widths = {w.shape[0] for w in (q_norm, k_norm) if w is not None}
+
     def _fits(self, head_dim):
-        for w, name in ((self.q_norm, "q_norm"), (self.k_norm, "k_norm")):
-            if w is not None and w.shape[0] != head_dim:
-                raise ValueError("%s has %d weights, not head_dim=%d" % (name, w.shape[0], head_dim))
+        if self._widths and self._widths != {head_dim}:
+            raise ValueError("the norms have %s weights, not head_dim=%d" % (sorted(self._widths), head_dim))
 
 
 class PagedKV:
@@ -149,7 +154,7 @@ class PagedKV:
         if n > 0 and not k[0].is_contiguous():
             raise ValueError("a page must be contiguous")
         self.k, self.v = k, v
-        self.n_kv_heads, self.head_dim = h, d
+        self.page_size, self.n_kv_heads, self.head_dim = ps, h, d
         stride = k.stride(0) if n > 1 else (ps * h * d + 7) // 8 * 8
         self._c = _PagedKV(_on_device(k, "k"), _on_device(v, "v"), stride, kinds[k.dtype], n, ps, h, d)
         self._ref = ctypes.addressof(self._c)
@@ -169,58 +174,57 @@ class PagedBatch:
         self._by_rows = {}
 
     def _for(self, n_rows):
-        c = self._by_rows.get(n_rows)
+        c = self._by_rows.get(n_rows)  # descriptors differ in their row count alone: one per count, never changed
         if c is None:
-            c = self._by_rows[n_rows] = self._make(n_rows)
-        return ctypes.addressof(c)
+            c = self._make(n_rows)
+            c = self._by_rows[n_rows] = (ctypes.addressof(c), c)
+        return c[0]
 
 
 def qk_norm_rope(rot, q, k, q_out, k_out, positions, n_heads, n_kv_heads, head_dim, n_rows=None, stream=None):
     """q_out and k_out = the heads of q and k, normed and rotated at positions [rows] (int32); q_out may
     be q and k_out k.  q (with n_heads 0) or k (with n_kv_heads 0) may be None."""
-    _torch()
-    pq, lq, nq = _rows(q, "q") if q is not None else (None, 0, None)
-    pk, lk, nk = _rows(k, "k") if k is not None else (None, 0, None)
-    po, lo, no = _rows(q_out, "q_out") if q is not None else (None, 0, None)
-    px, lx, nx = _rows(k_out, "k_out") if k is not None else (None, 0, None)
+    L, dev = _torch(), _device()
     rot._fits(head_dim)
+    pq = lq = po = lo = pk = lk = px = lx = 0
+    nq = no = nk = nx = None
     if q is not None:
-        _wide(q, "q", n_heads * head_dim)
-        _wide(q_out, "q_out", n_heads * head_dim)
+        pq, lq, nq = _rows(q, n_heads * head_dim, "q", dev)
+        po, lo, no = _rows(q_out, n_heads * head_dim, "q_out", dev)
     if k is not None:
-        _wide(k, "k", n_kv_heads * head_dim)
-        _wide(k_out, "k_out", n_kv_heads * head_dim)
-    pp = _ints(positions, "positions", 1)
-    n = _same_rows(n_rows, ("q", nq), ("k", nk), ("q_out", no), ("k_out", nx), ("positions", positions.shape[0]))
-    _check(_lib().cri_qk_norm_rope(rot._ref, pq, lq, pk, lk, po, lo, px, lx, pp, n, n_heads, n_kv_heads, head_dim,
-                                   _stream(stream)))
+        pk, lk, nk = _rows(k, n_kv_heads * head_dim, "k", dev)
+        px, lx, nx = _rows(k_out, n_kv_heads * head_dim, "k_out", dev)
+    pp = _ints(positions, "positions", 1, dev)
+    n = _same_rows(n_rows, ("positions", positions.shape[0]), ("q", nq), ("k", nk), ("q_out", no), ("k_out", nx))
+    st = L.cri_qk_norm_rope(rot._ref, pq, lq, pk, lk, po, lo, px, lx, pp, n, n_heads, n_kv_heads, head_dim,
+                            _on(stream, dev))
+    if st:
+        _check(st)
 
 
 def paged_append(cache, batch, rot, k, v, q=None, q_out=None, n_heads=0, n_rows=None, stream=None):
     """The batch's k rows, normed and rotated, and v rows go to their pages; with q, its heads go to
     q_out, normed and rotated."""
-    _torch()
-    pk, lk, nk = _rows(k, "k")
-    pv, lv, nv = _rows(v, "v")
+    L, dev = _torch(), _device()
     D = cache.head_dim
-    _wide(k, "k", cache.n_kv_heads * D)
-    _wide(v, "v", cache.n_kv_heads * D)
     rot._fits(D)
-    if q is None:
-        pq, lq, nq, po, lo, no = None, 0, None, None, 0, None
-    else:
-        pq, lq, nq = _rows(q, "q")
-        po, lo, no = _rows(q_out, "q_out")
-        _wide(q, "q", n_heads * D)
-        _wide(q_out, "q_out", n_heads * D)
+    pk, lk, nk = _rows(k, cache.n_kv_heads * D, "k", dev)
+    pv, lv, nv = _rows(v, cache.n_kv_heads * D, "v", dev)
+    pq = lq = po = lo = 0
+    nq = no = None
+    if q is not None:
+        pq, lq, nq = _rows(q, n_heads * D, "q", dev)
+        po, lo, no = _rows(q_out, n_heads * D, "q_out", dev)
     n = _same_rows(n_rows, ("k", nk), ("v", nv), ("q", nq), ("q_out", no))
-    _check(_lib().cri_paged_append(cache._ref, batch._for(n), rot._ref, pq, lq, po, lo, n_heads, pk, lk, pv, lv,
-                                   _stream(stream)))
+    st = L.cri_paged_append(cache._ref, batch._for(n), rot._ref, pq, lq, po, lo, n_heads, pk, lk, pv, lv,
+                            _on(stream, dev))
+    if st:
+        _check(st)
 
 
 def paged_attention_workspace_bytes(cache, batch, n_rows, n_heads, prefix_len=0):
     """Workspace bytes of paged_attention for batches of these host numbers."""
-    n = _lib().cri_paged_attention_workspace_bytes(cache._ref, batch._for(n_rows), prefix_len, n_heads)
+    n = _torch().cri_paged_attention_workspace_bytes(cache._ref, batch._for(n_rows), prefix_len, n_heads)
     if n < 0:
         _check(int(n))
     return int(n)
@@ -231,32 +235,30 @@ def paged_attention(cache, batch, q, out, n_heads, scale, prefix_pages=None, pre
     """out = softmax(scale q K^T) V of every row over the positions it sees, those below prefix_len
     through prefix_pages, which all sequences share.  workspace: a device tensor of
     paged_attention_workspace_bytes (one is allocated when None)."""
-    _torch()
-    pq, lq, nq = _rows(q, "q")
-    po, lo, no = _rows(out, "out")
+    L, dev = _torch(), _device()
     width = n_heads * cache.head_dim
-    _wide(q, "q", width)
-    _wide(out, "out", width)
+    pq, lq, nq = _rows(q, width, "q", dev)
+    po, lo, no = _rows(out, width, "out", dev)
     n = _same_rows(n_rows, ("q", nq), ("out", no))
-    pp = None
+    pp = 0
     if prefix_len > 0:
         if prefix_pages is None:
             raise ValueError("prefix_len without prefix_pages")
-        pp = _ints(prefix_pages, "prefix_pages", 1)
-        if prefix_pages.shape[0] * cache._c.page_size < prefix_len:
+        pp = _ints(prefix_pages, "prefix_pages", 1, dev)
+        if prefix_pages.shape[0] * cache.page_size < prefix_len:
             raise ValueError("prefix_pages holds %d pages, too few for prefix_len=%d" % (prefix_pages.shape[0], prefix_len))
-    b = batch._for(n)
     if workspace is None:
-        need = paged_attention_workspace_bytes(cache, batch, n, n_heads, prefix_len)
-        workspace = None if need == 0 else _room(None, need, stream)[2]
-    pw, wb = (0, 0) if workspace is None else _room(workspace, 0, stream)[:2]
-    _check(_lib().cri_paged_attention(cache._ref, b, pp, prefix_len, pq, lq, po, lo, n_heads, scale, pw, wb,
-                                      _stream(stream)))
+        workspace = _new_room(paged_attention_workspace_bytes(cache, batch, n, n_heads, prefix_len), stream)
+    pw, wb = _room(workspace, dev)
+    st = L.cri_paged_attention(cache._ref, batch._for(n), pp, prefix_len, pq, lq, po, lo, n_heads, scale, pw, wb,
+                               _on(stream, dev))
+    if st:
+        _check(st)
 
 
 def verify_drafts_workspace_bytes(n_seqs, vocab):
     """Workspace bytes of verify_drafts."""
-    n = _lib().cri_verify_drafts_workspace_bytes(n_seqs, vocab)
+    n = _torch().cri_verify_drafts_workspace_bytes(n_seqs, vocab)
     if n < 0:
         _check(int(n))
     return int(n)
@@ -267,16 +269,19 @@ def verify_drafts(target, draft, draft_ids, uniforms, draws, offsets, out_ids, n
     [rows, vocab], draft_ids, uniforms (that decide about the drafts) and draws (independent ones,
     that draw the last token) [rows], offsets [n_seqs + 1]; out_ids [rows] gets the accepted drafts,
     the drawn token and -1 behind it, n_accepted [n_seqs] the drafts accepted."""
-    _torch()
-    pt, lt, n = _rows(target, "target")
+    L, dev = _torch(), _device()
+    if target.dim() != 2:
+        raise ValueError("target must have the shape [rows, vocab]")
     V = target.shape[1]
-    pd, ld = None, 0
+    pt, lt, n = _rows(target, V, "target", dev)
+    pd = ld = 0
     if draft is not None:
-        pd, ld, nd = _rows(draft, "draft")
-        if nd != n or draft.shape[1] != V:
+        pd, ld, nd = _rows(draft, V, "draft", dev)
+        if nd != n:
             raise ValueError("draft must have the shape of target")
-    pi, po, pa = _ints(draft_ids, "draft_ids", 1), _ints(out_ids, "out_ids", 1), _ints(n_accepted, "n_accepted", 1)
-    pf = _ints(offsets, "offsets", 1)
+    pi, po, pa = (_ints(draft_ids, "draft_ids", 1, dev), _ints(out_ids, "out_ids", 1, dev),
+                  _ints(n_accepted, "n_accepted", 1, dev))
+    pf = _ints(offsets, "offsets", 1, dev)
     B = n_accepted.shape[0]
     for x, name in ((uniforms, "uniforms"), (draws, "draws")):
         if x.dtype is not torch.float32 or x.shape != (n,) or not x.is_contiguous():
@@ -284,22 +289,25 @@ def verify_drafts(target, draft, draft_ids, uniforms, draws, offsets, out_ids, n
     if draft_ids.shape[0] != n or out_ids.shape[0] != n or offsets.shape[0] != B + 1:
         raise ValueError("draft_ids and out_ids must have target's rows, offsets n_seqs + 1 entries")
     if workspace is None:
-        workspace = _room(None, verify_drafts_workspace_bytes(B, V), stream)[2]
-    pw, wb = _room(workspace, 0, stream)[:2]
-    _check(_lib().cri_verify_drafts(pt, lt, pd, ld, pi, _on_device(uniforms, "uniforms"),
-                                    _on_device(draws, "draws"), pf, B, n, V, po, pa, pw, wb,
-                                    _stream(stream)))
+        workspace = _new_room(verify_drafts_workspace_bytes(B, V), stream)
+    pw, wb = _room(workspace, dev)
+    st = L.cri_verify_drafts(pt, lt, pd, ld, pi, _on_device(uniforms, "uniforms", dev), _on_device(draws, "draws", dev),
+                             pf, B, n, V, po, pa, pw, wb, _on(stream, dev))
+    if st:
+        _check(st)
 
 
-torch = None
+torch = _loaded = None
 
 
 def _torch():
-    global torch
-    if torch is None:
+    """torch and the library are loaded by the first call, not by importing the package."""
+    global torch, _loaded
+    if _loaded is None:
         import torch as t
 
-        torch = t
+        torch, _loaded = t, _lib()
+    return _loaded
 
 
 from . import _check, _stream, lib as _lib  # noqa: E402

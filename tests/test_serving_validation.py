@@ -132,7 +132,7 @@ def verify(t=Q, ldt=100, d=K, ldd=100, ids=FAKE, u=V, dr=V, off=FAKE, B=2, n=5, 
     (dict(B=-1), -1), (dict(n=-1), -1), (dict(vocab=-1), -1), (dict(vocab=0), -2), (dict(t=0), -1), (dict(ids=0), -1),
     (dict(u=0), -1), (dict(dr=0), -1), (dict(dr=V + 2), -3), (dict(off=0), -1), (dict(out=0), -1), (dict(acc=0), -1), (dict(t=Q + 2), -3), (dict(d=K + 1), -3),
     (dict(ldt=99), -2), (dict(ldd=99), -2), (dict(ldt=1 << 50), -2), (dict(out=FAKE + 4), -1), (dict(ws=0), -1),
-    (dict(ws=WS + 4), -3), (dict(wsb=16), -2), (dict(B=(1 << 20) + 1), -2),
+    (dict(ws=WS + 4), -3), (dict(wsb=16), -2), (dict(B=(1 << 20) + 1), -2), (dict(vocab=1 << 29, ldt=1 << 29, ldd=1 << 29), -2),
 ])
 def test_verify_refuses(kw, want):
     assert verify(**kw) == want
