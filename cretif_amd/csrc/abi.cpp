@@ -681,6 +681,8 @@ int check_paged(const cri_paged_kv* kv, const cri_paged_batch* batch, cri::PageP
         return fail(CRI_ERR_SHAPE, fn, "problem too large");
     if (kv->page_stride < page * kv->head_dim || kv->page_stride % 8 != 0)
         return fail(CRI_ERR_SHAPE, fn, "page_stride must be a multiple of 8 and hold page_size * n_kv_heads * head_dim elements");
+    if (static_cast<long>(kv->n_kv_heads) * kv->head_dim > (1L << 20))
+        return fail(CRI_ERR_SHAPE, fn, "n_kv_heads * head_dim exceeds 2^20");
     if (static_cast<long>(batch->max_pages) * kv->page_size > kMaxPositions)
         return fail(CRI_ERR_SHAPE, fn, "max_pages * page_size exceeds 2^30 positions");
     int l = 0;

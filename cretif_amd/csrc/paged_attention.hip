@@ -1,5 +1,7 @@
 // paged_attention.hip -- how a call of the paged attention is cut into workgroups, and the kernel that joins their
 // records.
+#include <numeric>
+
 #include "paged_attention.hpp"
 
 namespace cri {
@@ -28,11 +30,21 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const float* __restrict
     // 2^lg lanes hold a record's accumulators, the wave's 64 >> lg groups of them take the records in turn
     const int c = lane & ((1 << lg) - 1), grp = lane >> lg, groups = 64 >> lg;
     f32x4 x = {0, 0, 0, 0};
-    for (int k0 = 0; k0 < nrec; k0 += groups) {
-        const int k = k0 + grp;
-        const float w = __shfl(f, min(k, nrec - 1));  // every lane takes part
-        if (k < nrec && w != 0.0f && 4 * c < D)        // a record of weight 0 may hold nothing
-            x += *reinterpret_cast<const f32x4*>(r + static_cast<long>(k) * (D + 4) + 4 + 4 * c) * w;
+    constexpr int kAhead = 4;  // records in flight
+    for (int k0 = 0; k0 < nrec; k0 += kAhead * groups) {
+        float wt[kAhead];
+        f32x4 y[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int k = k0 + j * groups + grp;
+            wt[j] = __shfl(f, min(k, nrec - 1));  // every lane takes part
+            if (k >= nrec || 4 * c >= D) wt[j] = 0.0f;
+            y[j] = f32x4{0, 0, 0, 0};
+            if (wt[j] != 0.0f)  // a record of weight 0 may hold nothing
+                y[j] = *reinterpret_cast<const f32x4*>(r + static_cast<long>(k) * (D + 4) + 4 + 4 * c);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) x += y[j] * wt[j];
     }
     for (int m = 1 << lg; m < 64; m <<= 1)
 #pragma unroll
@@ -44,46 +56,58 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const float* __restrict
 
 // the cut of a call, from what the host knows of it
 struct Cut {
-    bool even;
-    int nc, pre_wq, pre_tiles, pre_chunks, pre_blocks, own_wq, own_tiles, own_chunks, nrec;
+    bool even, staged;  // staged: the prefix goes to the kernel that shares it through LDS
+    int pre_wq, pre_tiles, pre_chunks, pre_per, pre_blocks, own_wq, own_tiles, own_chunks, own_per, nrec;
     long own_blocks;
 };
 
 constexpr int kMaxRecords = 64;  // the joining wave keeps one record's maximum per lane
+constexpr int kSlots = 512;      // workgroups on the GPU at a time: two per CU
+
+int round_up(int x, int to) { return (x + to - 1) / to * to; }
 
 Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int prefix_len) {
     Cut c{};
     const int D = P.head_dim, G = n_heads / P.n_kv_heads;
     c.even = (D == 64 || D == 128 || D == 256) && P.page_size % 16 == 0;
-    const long rows = static_cast<long>(B.n_rows) * G;         // of a KV head
-    const long mean = (rows + B.n_seqs - 1) / B.n_seqs;        // of a KV head and sequence
+    const long rows = static_cast<long>(B.n_rows) * G;   // of a KV head
+    const long mean = (rows + B.n_seqs - 1) / B.n_seqs;  // of a KV head and sequence
+    c.staged = c.even && type != kKvF32 && D <= 128 && rows > 64 && prefix_len >= 256;
     const int tile = type == kKvF32 ? 16 : 32;
-    c.nc = c.even && D <= 128 && (mean > 16 || (prefix_len > 0 && rows > 16)) ? 2 : 1;
-    const int block = 16 * c.nc;
+    constexpr int block = 16;  // rows of a wave
     auto waves_of = [&](long r) { return r <= block ? 1 : r <= 2 * block ? 2 : 4; };
     c.pre_wq = waves_of(rows);
     c.own_wq = waves_of(mean);
-    const int target = 512;  // workgroups of each kind: two per CU
     if (prefix_len > 0) {
-        c.pre_tiles = static_cast<int>((rows + block * c.pre_wq - 1) / (block * c.pre_wq));
+        const int tile_rows = c.staged ? kPrefixRows : block * c.pre_wq;
+        const int unit = c.staged ? kPrefixStage : tile * (kPagedWaves / c.pre_wq);
+        c.pre_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
         const long streams = static_cast<long>(P.n_kv_heads) * c.pre_tiles;
-        const int wk = kPagedWaves / c.pre_wq, tiles = (prefix_len + tile - 1) / tile;
-        long n = (target + streams - 1) / streams;
-        n = std::min<long>(n, (tiles + 2 * wk - 1) / (2 * wk));  // at least two tiles to a wave
-        c.pre_chunks = static_cast<int>(std::min<long>(std::max<long>(n, 1), kMaxRecords / 2));
-        const int groups = (P.n_kv_heads * c.pre_chunks + kPagedXcds - 1) / kPagedXcds;
-        c.pre_blocks = groups * kPagedXcds * c.pre_tiles;
+        const int units = (prefix_len + unit - 1) / unit;
+        // chunks: fewest rounds of workgroups times units of each, a workgroup's start and its records counted as two
+        long best = 0;
+        for (int n = 1; n <= kMaxRecords / 2 && n <= units; ++n) {
+            const long rounds = (streams * n + kSlots - 1) / kSlots, cost = rounds * ((units + n - 1) / n + 2);
+            if (best == 0 || cost < best) {
+                best = cost;
+                c.pre_per = (units + n - 1) / n * unit;
+            }
+        }
+        c.pre_chunks = (prefix_len + c.pre_per - 1) / c.pre_per;
+        c.pre_blocks = static_cast<int>((streams * c.pre_chunks + kPagedXcds - 1) / kPagedXcds * kPagedXcds);
     }
-    const long cap = static_cast<long>(B.max_pages) * P.page_size, own = std::max(cap - prefix_len, 0L);
-    const int rt = block * c.own_wq;
-    c.own_tiles = static_cast<int>(rows / rt + std::min<long>(B.n_seqs, B.n_rows));
-    {
-        const long streams = static_cast<long>(P.n_kv_heads) * c.own_tiles;
-        const int wk = kPagedWaves / c.own_wq;
-        long n = (target + streams - 1) / streams;
-        n = std::min<long>(n, (own + 2 * wk * tile - 1) / (2 * wk * tile));
-        c.own_chunks = static_cast<int>(std::min<long>(std::max<long>(n, 1), kMaxRecords / 2));
-    }
+    // a sequence's own positions: chunks of one size, so that a long sequence has more of them and none is waited for;
+    // 512 positions, or less where the batch would leave CUs idle
+    const long cap = static_cast<long>(B.max_pages) * P.page_size;
+    const long own = std::max(cap - prefix_len / tile * tile, 1L);
+    const int rt = block * c.own_wq, unit = tile * (kPagedWaves / c.own_wq);
+    // sum of ceil(n G / rt) over the sequences that have rows: n G is a multiple of gcd(G, rt)
+    c.own_tiles = static_cast<int>((rows + std::min<long>(B.n_seqs, B.n_rows) * (rt - std::gcd(G, rt))) / rt);
+    const long streams = static_cast<long>(P.n_kv_heads) * c.own_tiles;
+    const long fill = own * streams / kSlots;  // positions per workgroup that fill the GPU once
+    const long least = (own + kMaxRecords / 2 - 1) / (kMaxRecords / 2);
+    c.own_per = round_up(static_cast<int>(std::max({std::min(fill, 512L), least, 1L})), 2 * unit);
+    c.own_chunks = static_cast<int>((own + c.own_per - 1) / c.own_per);
     c.own_blocks = static_cast<long>(c.own_tiles) * c.own_chunks * P.n_kv_heads;
     c.nrec = c.pre_chunks + c.own_chunks;
     return c;
@@ -108,13 +132,21 @@ int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, cons
     a.P = P, a.B = B;
     a.prefix_pages = prefix_pages, a.prefix_len = prefix_len;
     a.H = n_heads, a.G = n_heads / P.n_kv_heads, a.nrec = c.nrec;
-    a.pre_wq = c.pre_wq, a.pre_tiles = c.pre_tiles, a.pre_chunks = c.pre_chunks, a.pre_blocks = c.pre_blocks;
-    a.own_wq = c.own_wq, a.own_tiles = c.own_tiles, a.own_chunks = c.own_chunks;
+    a.pre_wq = c.pre_wq, a.pre_tiles = c.pre_tiles, a.pre_chunks = c.pre_chunks, a.pre_per = c.pre_per;
+    a.pre_blocks = c.pre_blocks;
+    a.own_wq = c.own_wq, a.own_tiles = c.own_tiles, a.own_chunks = c.own_chunks, a.own_per = c.own_per;
     a.qscale = scale * 1.44269504088896340736f;
-    const long blocks = c.pre_blocks + c.own_blocks;
+    a.staged = c.staged;
+    if (c.staged) {
+        (type == kKvF16 ? dev::run_paged_prefix_f16 : dev::run_paged_prefix_bf16)(a, stream);
+        a.pre_blocks = 0;
+    }
+    const long blocks = a.pre_blocks + c.own_blocks;
     if (blocks > 0x7FFFFFFFL) return kDeclined;
-    const auto run = type == kKvF32 ? dev::run_paged_attn_f32 : type == kKvF16 ? dev::run_paged_attn_f16 : dev::run_paged_attn_bf16;
-    run(a, c.even, c.nc, static_cast<int>(blocks), stream);
+    const auto run = type == kKvF32   ? dev::run_paged_attn_f32
+                     : type == kKvF16 ? dev::run_paged_attn_f16
+                                      : dev::run_paged_attn_bf16;
+    run(a, c.even, static_cast<int>(blocks), stream);
     if (c.nrec > 1) {
         const long waves = static_cast<long>(B.n_rows) * n_heads;
         int lg = 0;

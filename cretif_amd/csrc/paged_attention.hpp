@@ -4,7 +4,7 @@
 // with the rows of all sequences at once, so its K and V are read once for the batch; each sequence's own
 // positions are multiplied with its own rows.  Both leave (max, sum, acc) records that a second kernel joins.
 //
-// One wave takes 16 NC query rows ("columns": query q = token x G + g of the heads g that share a KV head) and a
+// One wave takes 16 query rows ("columns": query q = token x G + g of the heads g that share a KV head) and a
 // tile of positions at a time, straight from the pool into registers:
 //   * S^T = K Q^T: K is the A operand, whose 16 bytes per lane are consecutive dims of a position's row.
 //   * O^T += V^T P^T: a lane owns one column, and the positions of its scores are the positions whose
@@ -35,9 +35,10 @@ struct PagedAttnArgs {
     PageBatch B;
     const int* prefix_pages;
     int prefix_len, H, G, nrec;
-    int pre_wq, pre_tiles, pre_chunks, pre_blocks;  // the prefix's workgroups: [stream / 8][tile][stream % 8]
-    int own_wq, own_tiles, own_chunks;              // the sequences': [tile][chunk][KV head]
-    float qscale;                                   // scale * log2 e: scores are in base 2
+    int pre_wq, pre_tiles, pre_chunks, pre_per, pre_blocks;  // the prefix's workgroups: [chunk][KV head][tile] by XCD
+    int own_wq, own_tiles, own_chunks, own_per;              // the sequences': [tile][chunk][KV head]
+    float qscale;  // scale * log2 e: scores are in base 2
+    bool staged;   // the prefix went to paged_prefix_kernel
 };
 
 constexpr int kPagedWaves = 4;
@@ -93,74 +94,117 @@ __device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&p)[PARTS]) {
     }
 }
 
+// fp16 parts of a query row of largest magnitude m: it is scaled by f, a power of two that takes m to [2^13, 2^14), and
+// the scores' factor kf by 1 / f; the parts are then off by 2^-23 of an element or 2^-39 of the largest
+__device__ __forceinline__ void q_scale(float m, float& f, float& kf) {
+    const int sh = min(13 + 127 - static_cast<int>(__builtin_bit_cast(uint32_t, m) >> 23), 126);
+    f = __builtin_bit_cast(float, (127 + sh) << 23);
+    kf *= __builtin_bit_cast(float, (127 - sh) << 23);
+}
 __device__ __forceinline__ float col_max(float v) { return swap_max32(swap_max16(v, v), swap_max16(v, v)); }
 __device__ __forceinline__ float col_sum(float v) {
     const float s = swap_add16(v, v);
     return swap_add32(s, s);
 }
-__device__ __forceinline__ int wave_max_i(int v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v = max(v, __shfl_xor(v, m));
-    return v;
+template <int CTRL>
+__device__ __forceinline__ int dpp_i(int old, int v) {
+    return __builtin_amdgcn_update_dpp(old, v, CTRL, 0xF, 0xF, false);
 }
-__device__ __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v = min(v, __shfl_xor(v, m));
-    return v;
+// the largest of the first 16 lanes (all rows of 16 hold the same values), in a scalar register
+__device__ __forceinline__ int row_max_i(int v) {
+    v = max(v, dpp_i<kQuadPerm1032>(v, v));
+    v = max(v, dpp_i<kQuadPerm2301>(v, v));
+    v = max(v, dpp_i<kRowHalfMirror>(v, v));
+    v = max(v, dpp_i<kRowMirror>(v, v));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+// sums over the lanes up to and with each
+__device__ __forceinline__ int wave_scan_i(int v) {
+    v += dpp_i<0x111>(0, v);  // row_shr 1, 2, 4, 8: within 16 lanes, zeros from outside
+    v += dpp_i<0x112>(0, v);
+    v += dpp_i<0x114>(0, v);
+    v += dpp_i<0x118>(0, v);
+    const int lane = threadIdx.x & 63;
+    const int a = __builtin_amdgcn_readlane(v, 15), b = __builtin_amdgcn_readlane(v, 31), c = __builtin_amdgcn_readlane(v, 47);
+    return v + (lane >= 16 ? a : 0) + (lane >= 32 ? b : 0) + (lane >= 48 ? c : 0);
+}
+// int arrays that no kernel here writes, read at uniform places with scalar loads
+typedef const __attribute__((address_space(4))) int* UniformInts;
+__device__ __forceinline__ UniformInts uniform(const int* p) { return (UniformInts)p; }
+
+// The sequences of up to 64 consecutive tokens t0 .. t0 + n - 1, lane l's being t0 + l's k: 64 offsets are read at a time
+// and compared with every token, so that the searches of a wave cost one trip to memory.  Returns the position of token
+// t0 + k in its sequence, or a negative number for a token of none (any below 0 is "before all positions").
+__device__ __forceinline__ int position_of(const PageBatch& B, int t0, int n, int k, bool& found) {
+    const int lane = threadIdx.x & 63;
+    int s = 0;
+    for (int base = 0; base < B.n_seqs; base += 64) {
+        const int i = base + lane;
+        const int end = i < B.n_seqs ? B.offsets[i + 1] : 0x7FFFFFFF;
+        bool all = true;
+        for (int j = 0; j < n; ++j) {
+            const int before = __popcll(__ballot(end <= t0 + j));
+            if (j == k) s += before;
+            all = all && before < 64;
+        }
+        if (all) break;
+    }
+    found = false;
+    if (k < n && s < B.n_seqs) {
+        const int t = t0 + k, lo = B.offsets[s], hi = B.offsets[s + 1], len = B.lens[s];
+        found = t >= lo && t < hi;
+        return len - (hi - t);
+    }
+    return -1;
 }
 
-// the sequence of row t by bisection, one search per lane; -1 for a row of none
-__device__ __forceinline__ int sequence_of(const PageBatch& B, int t) {
-    int lo = 0, hi = B.n_seqs;  // the first s with offsets[s + 1] > t
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (B.offsets[mid + 1] > t)
-            hi = mid;
-        else
-            lo = mid + 1;
-    }
-    return lo < B.n_seqs && B.offsets[lo] <= t ? lo : -1;
+// the prefix's work of this workgroup: consecutive items (the row tiles of one chunk and KV head, which read the same
+// K and V) go to one XCD and its L2
+__device__ __forceinline__ bool prefix_item(const PagedAttnArgs& a, int b, int Hkv, int& chunk, int& kvh, int& tile) {
+    const int wi = b % kPagedXcds * (a.pre_blocks / kPagedXcds) + b / kPagedXcds;
+    const int stream = wi / a.pre_tiles;
+    tile = wi % a.pre_tiles;
+    chunk = stream / Hkv;
+    kvh = stream % Hkv;
+    return chunk < a.pre_chunks;
 }
 
 // EVEN: head_dim is DP and the page size a multiple of 16, so the 16 positions of a tile's row block lie in one page
-template <int TYPE, int DP, int NC, bool EVEN>
-__global__ __launch_bounds__(64 * kPagedWaves) void paged_attn_kernel(const PagedAttnArgs a) {
+template <int TYPE, int DP, bool EVEN>
+__global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_attn_kernel(const PagedAttnArgs a) {
     typedef PagedShape<TYPE, DP> S;
     typedef typename KvType<TYPE>::elem elem;
     typedef std::integral_constant<int, TYPE> Type;
     constexpr int kTile = S::kTile, kT = S::kT, kKs = S::kKs, kVe = S::kVe, kNh = S::kNh, kAcc = S::kAcc;
-    constexpr int kRowF = DP + 4;                // floats of a column's record in LDS
-    constexpr int kNs = 4 * kT;                  // scores of a lane and column
-    extern __shared__ __attribute__((aligned(16))) float lds[];  // 3 waves' records
+    constexpr int kEs = sizeof(elem), kNs = 4 * kT;  // scores of a lane
+    extern __shared__ __attribute__((aligned(16))) float lds[];  // the waves' records
 
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int D = EVEN ? DP : a.P.head_dim;
     const int Hkv = a.P.n_kv_heads, G = a.G;
-    const long row_elems = static_cast<long>(Hkv) * D;
-    const int cap = static_cast<int>(min(static_cast<long>(a.B.max_pages) * a.P.page_size, 0x7FFFFFFFL));
+    const uint32_t row_bytes = static_cast<uint32_t>(Hkv * D * kEs);
+    const int cap = a.B.max_pages * a.P.page_size;
+    const UniformInts offsets = uniform(a.B.offsets), lens = uniform(a.B.lens);
 
     // ---- what this workgroup does: a KV head, a tile of rows, a range of positions
     const bool prefix = static_cast<int>(blockIdx.x) < a.pre_blocks;
-    int kvh, wq, row0, nrows, tok0, pos0 = 0, rec_at, p_lo, p_hi;
-    const int* table;
-    int table_len;
+    int kvh, wq, row0, nrows, tok0, pos0 = 0, rec_at, own_lo, own_hi;
+    UniformInts own_table;
+    int own_len, before_lo = 0, before_hi = 0;  // (before: the prefix's positions for rows that do not see all of it)
+    const int prefix_pages = (a.prefix_len + a.P.page_size - 1) / a.P.page_size;
     if (prefix) {
-        const int b = blockIdx.x, grp = kPagedXcds * a.pre_tiles;
-        const int stream = b / grp * kPagedXcds + b % kPagedXcds, tile = b % grp / kPagedXcds;
-        if (stream >= Hkv * a.pre_chunks) return;
-        kvh = stream % Hkv;
-        const int chunk = stream / Hkv;
+        int chunk, tile;
+        if (!prefix_item(a, blockIdx.x, Hkv, chunk, kvh, tile)) return;
         wq = a.pre_wq;
-        row0 = tile * 16 * NC * wq;
+        row0 = tile * 16 * wq;
         nrows = a.B.n_rows * G;
         tok0 = 0;
         rec_at = chunk;
-        const int ntiles = (a.prefix_len + kTile - 1) / kTile, per = (ntiles + a.pre_chunks - 1) / a.pre_chunks;
-        p_lo = min(chunk * per * kTile, a.prefix_len);
-        p_hi = min(p_lo + per * kTile, a.prefix_len);
-        table = a.prefix_pages;
-        table_len = (a.prefix_len + a.P.page_size - 1) / a.P.page_size;
+        own_lo = chunk * a.pre_per;
+        own_hi = min(own_lo + a.pre_per, a.prefix_len);
+        own_table = uniform(a.prefix_pages);
+        own_len = prefix_pages;
     } else {
         int b = static_cast<int>(blockIdx.x) - a.pre_blocks;
         kvh = b % Hkv;
@@ -169,205 +213,204 @@ __global__ __launch_bounds__(64 * kPagedWaves) void paged_attn_kernel(const Page
         int tile = b / a.own_chunks;
         wq = a.own_wq;
         // the tile-th tile of rows of the batch: 64 sequences' tile counts summed at a time
-        const int rt = 16 * NC * wq;
+        const int rt = 16 * wq;
         int seq = -1;
         for (int base = 0; base < a.B.n_seqs; base += 64) {
             const int i = base + lane;
             int n = 0;
             if (i < a.B.n_seqs) n = min(max(a.B.offsets[i + 1] - a.B.offsets[i], 0), a.B.n_rows);
-            n = (n * G + rt - 1) / rt;
-            int sum = n;
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) {
-                const int o = __shfl_up(sum, m);
-                if (lane >= m) sum += o;
-            }
+            const int sum = wave_scan_i((n * G + rt - 1) / rt);
             const int before = __popcll(__ballot(sum <= tile));
             if (before < 64) {
                 seq = base + before;
-                if (before > 0) tile -= __shfl(sum, before - 1);
+                if (before > 0) tile -= __builtin_amdgcn_readlane(sum, before - 1);
                 break;
             }
-            tile -= __shfl(sum, 63);
+            tile -= __builtin_amdgcn_readlane(sum, 63);
         }
         if (seq < 0 || seq >= a.B.n_seqs) return;
-        seq = __builtin_amdgcn_readfirstlane(seq);
-        tile = __builtin_amdgcn_readfirstlane(tile);
-        tok0 = a.B.offsets[seq];
-        const int n = min(max(a.B.offsets[seq + 1] - tok0, 0), a.B.n_rows);
+        tok0 = offsets[seq];
+        const int n = min(max(offsets[seq + 1] - tok0, 0), a.B.n_rows);
+        const int len = lens[seq];
         row0 = tile * rt;
         nrows = n * G;
-        const int len = a.B.lens[seq];
         pos0 = len - n;  // position of the sequence's first row
         rec_at = a.pre_chunks + chunk;
         const int end = min(len, cap), start = a.prefix_len / kTile * kTile;
-        const int ntiles = (max(end - start, 0) + kTile - 1) / kTile, per = (ntiles + a.own_chunks - 1) / a.own_chunks;
-        p_lo = min(start + chunk * per * kTile, end);
-        p_hi = min(p_lo + per * kTile, end);
-        p_lo = max(p_lo, min(a.prefix_len, end));
-        table = a.B.pages + static_cast<long>(seq) * a.B.max_pages;
-        table_len = a.B.max_pages;
-    }
-    const int wk = kPagedWaves / wq;  // waves that share rows and split positions
-    const int wrow = row0 + w / wk * 16 * NC, wpos = w % wk;
-
-    // ---- the wave's columns: row, limit (positions it sees), query operand
-    int lim[NC], tok[NC], head[NC];
-    int most = 0, least = 0x7FFFFFFF;
-    int ncols = 0;  // column blocks with a row
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        const int r = wrow + 16 * n + c;
-        if (wrow + 16 * n < nrows) ncols = n + 1;
-        tok[n] = -1;
-        lim[n] = 0x7FFFFFFF;  // no row: sees everything, is stored nowhere
-        head[n] = 0;
-        if (r < nrows) {
-            const int i = r / G, t = tok0 + i;
-            int p = pos0 + i;
-            bool ok = t >= 0 && t < a.B.n_rows;
-            if (prefix && ok) {
-                const int s = sequence_of(a.B, t);
-                ok = s >= 0;
-                if (ok) p = a.B.lens[s] - (a.B.offsets[s + 1] - t);
-            }
-            if (ok) {
-                tok[n] = t;
-                head[n] = kvh * G + r % G;
-                lim[n] = min(max(p + 1, 0), prefix ? a.prefix_len : cap);
-                most = max(most, lim[n]);
-                least = min(least, lim[n]);
-            }
+        own_lo = min(start + chunk * a.own_per, end);
+        own_hi = min(own_lo + a.own_per, end);
+        own_lo = max(own_lo, min(a.prefix_len, end));
+        own_table = uniform(a.B.pages + static_cast<long>(seq) * a.B.max_pages);
+        own_len = a.B.max_pages;
+        if (a.staged && pos0 + row0 / G + 1 < a.prefix_len) {
+            const int hi = min(a.prefix_len, len);
+            const int per = ((hi + a.own_chunks - 1) / a.own_chunks + kTile - 1) / kTile * kTile;
+            before_lo = min(chunk * per, hi);
+            before_hi = min(before_lo + per, hi);
         }
     }
-    most = __builtin_amdgcn_readfirstlane(wave_max_i(most));
-    least = __builtin_amdgcn_readfirstlane(wave_min_i(least));
+    const int wk = kPagedWaves / wq;  // waves that share rows and split positions
+    const int wrow = row0 + w / wk * 16, wpos = w % wk;
 
-    float kf[NC], qmax[NC];
-    u32x4 q[NC][S::kWide ? 1 : kKs][S::kParts];
-    f32x4 q32[NC][S::kWide ? kKs : 1];
+    // ---- the lane's column: its row, the positions up to and with the row's own, its query operand
+    int tok = -1, head = 0, sees = 0;
+    {
+        const int r = wrow + c, i0 = wrow / G, i = r / G, t = tok0 + i;
+        bool ok = r < nrows && t >= 0 && t < a.B.n_rows;
+        int p = pos0 + i;
+        if (prefix) {
+            bool found;
+            p = position_of(a.B, i0, min((wrow + 15) / G, a.B.n_rows - 1) - i0 + 1, i - i0, found);
+            ok = ok && found;
+        }
+        if (ok) {
+            tok = t;
+            head = kvh * G + r - i * G;
+            sees = max(p + 1, 0);
+        }
+    }
+    // ---- the tiles
+    const char* const kbase = static_cast<const char*>(a.P.k) + static_cast<long>(kvh) * D * kEs;
+    const char* const vbase = static_cast<const char*>(a.P.v) + static_cast<long>(kvh) * D * kEs;
+    // EVEN: a lane's bytes from the first row of a 16-position block; its address is that row's and these
+    const uint32_t k_off = c * row_bytes + 16 * g, v_off = 4 * g * row_bytes + kVe * kEs * c;
+    typedef uint32_t vreg __attribute__((ext_vector_type(S::kWide ? 4 : kVe / 2)));
+
+    // A sequence's workgroup may have two ranges: where the prefix is left to paged_prefix_kernel, first that part of it
+    // that rows see which do not see it whole.
+    int part = before_lo < before_hi ? 0 : 1, p_lo, p_hi, table_len, lim, least, first, last;
+    UniformInts table;
+    auto set_part = [&]() {
+        p_lo = part ? own_lo : before_lo;
+        p_hi = part ? own_hi : before_hi;
+        table = part ? own_table : uniform(a.prefix_pages);
+        table_len = part ? own_len : prefix_pages;
+        // the positions the column sees; no row: everything, it is stored nowhere
+        lim = tok < 0   ? 0x7FFFFFFF
+              : prefix  ? min(sees, a.prefix_len)
+              : part    ? min(sees, cap)
+                        : sees < a.prefix_len ? sees : 0;
+        least = -row_max_i(-lim);
+        first = p_lo / kTile + wpos;
+        last = (min(p_hi, row_max_i(tok < 0 ? 0 : lim)) + kTile - 1) / kTile;  // tiles [first, last) in steps of wk
+    };
+    auto page_at = [&](int pi) {
+        const int pg = table[min(pi, table_len - 1)];
+        return (static_cast<unsigned>(pg) < static_cast<unsigned>(a.P.n_pages) ? pg : 0) * a.P.stride * kEs;
+    };
+    auto row_at = [&](int pos) {  // byte offset of a position's row; uniform positions only where EVEN
+        const int pi = page_index(a.P, pos);
+        return page_at(pi) + static_cast<long>(pos - pi * a.P.page_size) * row_bytes;
+    };
+    auto lane_row = [&](int pos) {  // the same for a position of the lane's own
+        const int pi = page_index(a.P, pos);
+        const int pg = ((const int*)table)[min(pi, table_len - 1)];
+        return (static_cast<unsigned>(pg) < static_cast<unsigned>(a.P.n_pages) ? pg : 0) * a.P.stride * kEs +
+               static_cast<long>(pos - pi * a.P.page_size) * row_bytes;
+    };
+    auto load_k = [&](int p0, const long (&at)[kT], u32x4 (&k)[kT][kKs]) {
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        kf[n] = a.qscale;
-        const float* src = a.q + static_cast<long>(max(tok[n], 0)) * a.ldq + static_cast<long>(head[n]) * D;
-        const bool ok = tok[n] >= 0;
+        for (int t = 0; t < kT; ++t) {
+            if constexpr (EVEN) {
+                const char* row = kbase + at[t];
+#pragma unroll
+                for (int j = 0; j < kKs; ++j) k[t][j] = *reinterpret_cast<const u32x4*>(row + k_off + 64 * j);
+            } else {
+                const char* row = kbase + lane_row(p0 + 16 * t + c);
+#pragma unroll
+                for (int j = 0; j < kKs; ++j) {
+                    const int d = 64 * j + 16 * g;  // bytes
+                    const bool in = d < D * kEs;
+                    k[t][j] = *reinterpret_cast<const u32x4*>(row + (in ? d : 0));
+                    if (!in) k[t][j] = u32x4{0, 0, 0, 0};
+                }
+            }
+        }
+    };
+    auto load_v = [&](int p0, const long (&at)[kT], vreg (&v)[kT][4][kNh]) {
+#pragma unroll
+        for (int t = 0; t < kT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (EVEN) {
+                    const char* row = vbase + at[t] + static_cast<long>(i) * row_bytes;
+#pragma unroll
+                    for (int h = 0; h < kNh; ++h)
+                        v[t][i][h] = *reinterpret_cast<const vreg*>(row + v_off + 16 * kVe * kEs * h);
+                } else {
+                    const char* row = vbase + lane_row(p0 + 16 * t + 4 * g + i);
+#pragma unroll
+                    for (int h = 0; h < kNh; ++h) {
+                        const int d = (16 * h + c) * kVe;
+                        v[t][i][h] = *reinterpret_cast<const vreg*>(row + (d < D ? d * kEs : 0));
+                    }
+                }
+            }
+    };
+    u32x4 k[kT][kKs];
+    vreg v[kT][4][kNh];
+    long at[kT] = {};
+    auto load_tile = [&](int tile) {
+        if constexpr (EVEN) {
+#pragma unroll
+            for (int t = 0; t < kT; ++t) at[t] = row_at(tile * kTile + 16 * t);
+        }
+        load_k(tile * kTile, at, k);
+        load_v(tile * kTile, at, v);
+    };
+    set_part();
+    if (first < last) load_tile(first);
+
+    float kf = a.qscale;
+    u32x4 q[S::kWide ? 1 : kKs][S::kParts];
+    f32x4 q32[S::kWide ? kKs : 1];
+    {
+        const float* src = a.q + static_cast<long>(max(tok, 0)) * a.ldq + static_cast<long>(head) * D;
         if constexpr (S::kWide) {
 #pragma unroll
             for (int j = 0; j < kKs; ++j) {
                 const int d = 16 * j + 4 * g;
-                q32[n][j] = ok && d < D ? ld_f32x4(src + d) : f32x4{0, 0, 0, 0};
+                q32[j] = tok >= 0 && (EVEN || d < D) ? ld_f32x4(src + d) : f32x4{0, 0, 0, 0};
             }
         } else {
-            float x[kKs][8];
-            float m = 0.0f;
+            float x[kKs][8], m = 0.0f;
 #pragma unroll
             for (int j = 0; j < kKs; ++j) {
                 const int d = 32 * j + 8 * g;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const f32x4 v = ok && d < D ? ld_f32x4(src + d + 4 * h) : f32x4{0, 0, 0, 0};
+                for (int e = 0; e < 8; e += 4) {
+                    const f32x4 v = tok >= 0 && (EVEN || d < D) ? ld_f32x4(src + d + e) : f32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[j][4 * h + e] = v[e];
-                        m = fmaxf(m, fabsf(v[e]));
+                    for (int i = 0; i < 4; ++i) {
+                        x[j][e + i] = v[i];
+                        m = fmaxf(m, fabsf(v[i]));
                     }
                 }
             }
             float f = 1.0f;
-            if constexpr (TYPE == kKvF16) {
-                // the row's largest magnitude goes to [2^13, 2^14): the parts are off by 2^-23 of an element or
-                // 2^-39 of the largest
-                qmax[n] = col_max(m);
-                const int ex = static_cast<int>(__builtin_bit_cast(uint32_t, qmax[n]) >> 23) - 127;
-                const int sh = min(13 - ex, 126);
-                f = __builtin_bit_cast(float, (sh + 127) << 23);
-                kf[n] = a.qscale * __builtin_bit_cast(float, (127 - max(sh, -126)) << 23);
-            }
+            if constexpr (TYPE == kKvF16) q_scale(col_max(m), f, kf);
 #pragma unroll
             for (int j = 0; j < kKs; ++j) {
                 if constexpr (TYPE == kKvF16) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[j][e] *= f;
                 }
-                split8<TYPE, S::kParts>(x[j], q[n][j]);
+                split8<TYPE, S::kParts>(x[j], q[j]);
             }
         }
     }
 
-    f32x4 acc[NC][kAcc];
-    float mx[NC], sum[NC];
+    f32x4 acc[kAcc];
+    float mx = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        mx[n] = -INFINITY;
-        sum[n] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kAcc; ++i) acc[n][i] = f32x4{0, 0, 0, 0};
-    }
+    for (int i = 0; i < kAcc; ++i) acc[i] = f32x4{0, 0, 0, 0};
 
-    // ---- the tiles
-    const elem* const kbase = static_cast<const elem*>(a.P.k) + static_cast<long>(kvh) * D;
-    const elem* const vbase = static_cast<const elem*>(a.P.v) + static_cast<long>(kvh) * D;
-    auto page_of = [&](int pi) {
-        const int pg = table[min(pi, table_len - 1)];
-        return static_cast<unsigned>(pg) < static_cast<unsigned>(a.P.n_pages) ? pg : 0;
-    };
-    auto row_at = [&](int pos) {  // element offset of a position's row
-        const int pi = page_index(a.P, pos);
-        return page_of(pi) * a.P.stride + (pos - pi * a.P.page_size) * row_elems;
-    };
-    // first row of each 16-position block of a tile (EVEN)
-    auto block_rows = [&](int p0, long (&at)[kT]) {
-#pragma unroll
-        for (int t = 0; t < kT; ++t) at[t] = row_at(p0 + 16 * t);
-    };
-    auto load_k = [&](int p0, const long (&at)[kT], u32x4 (&k)[kT][kKs]) {
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-            const elem* row = kbase + (EVEN ? at[t] + c * row_elems : row_at(p0 + 16 * t + c));
-#pragma unroll
-            for (int j = 0; j < kKs; ++j) {
-                const int d = S::kWide ? 16 * j + 4 * g : 32 * j + 8 * g;
-                if constexpr (EVEN) {
-                    k[t][j] = *reinterpret_cast<const u32x4*>(row + d);
-                } else {
-                    k[t][j] = *reinterpret_cast<const u32x4*>(row + (d < D ? d : 0));
-                    if (d >= D) k[t][j] = u32x4{0, 0, 0, 0};
-                }
-            }
-        }
-    };
-    typedef uint32_t vreg __attribute__((ext_vector_type(S::kWide ? 4 : kVe / 2)));
-    auto load_v = [&](int p0, const long (&at)[kT], vreg (&v)[kT][4][kNh]) {
-#pragma unroll
-        for (int t = 0; t < kT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const elem* row = vbase + (EVEN ? at[t] + (4 * g + i) * row_elems : row_at(p0 + 16 * t + 4 * g + i));
-#pragma unroll
-                for (int h = 0; h < kNh; ++h) {
-                    const int d = 16 * kVe * h + kVe * c;
-                    v[t][i][h] = *reinterpret_cast<const vreg*>(row + (EVEN || d < D ? d : 0));
-                }
-            }
-    };
-    const int first = p_lo / kTile + wpos;
-    const int last = (min(p_hi, most) + kTile - 1) / kTile;  // tiles [first, last) in steps of wk
-
-    u32x4 k[kT][kKs];
-    long at[kT] = {};
-    if (first < last) {
-        if constexpr (EVEN) block_rows(first * kTile, at);
-        load_k(first * kTile, at, k);
-    }
-    for (int tile = first; tile < last; tile += wk) {
-        const int p0 = tile * kTile;
-        vreg v[kT][4][kNh];
-        load_v(p0, at, v);
-        const bool whole = p0 >= p_lo && p0 + kTile <= min(p_hi, least);
-        float s[NC][kNs];
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            if (n > 0 && n >= ncols) continue;
+#pragma unroll 1
+    for (;;) {
+#pragma unroll 1
+        for (int tile = first; tile < last; tile += wk) {
+            const int p0 = tile * kTile;
+            float s[kNs];
 #pragma unroll
             for (int t = 0; t < kT; ++t) {
                 f32x4 x = {0, 0, 0, 0};
@@ -376,195 +419,137 @@ __global__ __launch_bounds__(64 * kPagedWaves) void paged_attn_kernel(const Page
                     for (int j = 0; j < kKs; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            x = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, static_cast<uint32_t>(k[t][j][e])), q32[n][j][e], x,
-                                                                     0, 0, 0);
+                            x = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                __builtin_bit_cast(float, static_cast<uint32_t>(k[t][j][e])), q32[j][e], x, 0, 0, 0);
                 } else {
 #pragma unroll
                     for (int p = S::kParts - 1; p >= 0; --p)
 #pragma unroll
-                        for (int j = 0; j < kKs; ++j) x = mma16(k[t][j], q[n][j][p], x, Type{});
+                        for (int j = 0; j < kKs; ++j) x = mma16(k[t][j], q[j][p], x, Type{});
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[n][4 * t + i] = x[i] * kf[n];
+                for (int i = 0; i < 4; ++i) s[4 * t + i] = x[i] * kf;
             }
-        }
-        if (tile + wk < last) {  // the next tile's keys, in flight during the softmax and the second product
-            long nat[kT] = {};
-            if constexpr (EVEN) block_rows(p0 + wk * kTile, nat);
-            load_k(p0 + wk * kTile, nat, k);
+            const int next = p0 + wk * kTile;
+            const bool more = tile + wk < last;
+            if (more) {  // the next tile's keys, in flight during the softmax and the second product
+                if constexpr (EVEN) {
 #pragma unroll
-            for (int t = 0; t < kT; ++t) at[t] = nat[t];
-        }
-        u32x4 pb[NC][S::kParts];
-        float p32[NC][4];
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            if (n > 0 && n >= ncols) continue;
+                    for (int t = 0; t < kT; ++t) at[t] = row_at(next + 16 * t);
+                }
+                load_k(next, at, k);
+            }
+            const bool whole = p0 >= p_lo && p0 + kTile <= min(p_hi, least);
             if (!whole) {
-                const int hi = min(p_hi, lim[n]);
+                const int hi = min(p_hi, lim);
 #pragma unroll
                 for (int t = 0; t < kT; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int p = p0 + 16 * t + 4 * g + i;
-                        if (p < p_lo || p >= hi) s[n][4 * t + i] = -INFINITY;
+                        if (p < p_lo || p >= hi) s[4 * t + i] = -INFINITY;
                     }
             }
-            float m = s[n][0];
+            float m = s[0];
 #pragma unroll
-            for (int i = 1; i < kNs; ++i) m = fmaxf(m, s[n][i]);
+            for (int i = 1; i < kNs; ++i) m = fmaxf(m, s[i]);
             m = col_max(m);
-            const bool raise = m > mx[n] + S::kSlack;
+            const bool raise = m > mx + S::kSlack;
             if (__ballot(raise) != 0) {
-                const float f = raise ? __builtin_amdgcn_exp2f(mx[n] - m) : 1.0f;
-                if (raise) mx[n] = m;
-                sum[n] *= f;
+                const float f = raise ? __builtin_amdgcn_exp2f(mx - m) : 1.0f;
+                if (raise) mx = m;
+                sum *= f;
 #pragma unroll
-                for (int i = 0; i < kAcc; ++i) acc[n][i] *= f;
+                for (int i = 0; i < kAcc; ++i) acc[i] *= f;
             }
-            const float base = (mx[n] == -INFINITY ? 0.0f : mx[n]) - S::kShift;
+            const float base = (mx == -INFINITY ? 0.0f : mx) - S::kShift;
             float p[8] = {};
-            float l = 0.0f;
 #pragma unroll
             for (int i = 0; i < kNs; ++i) {
-                p[i] = __builtin_amdgcn_exp2f(s[n][i] - base);
-                l += p[i];
+                p[i] = __builtin_amdgcn_exp2f(s[i] - base);
+                sum += p[i];
             }
-            sum[n] += l;
-            if constexpr (S::kWide) {
+            u32x4 pb[S::kParts];
+            if constexpr (!S::kWide) split8<TYPE, S::kParts>(p, pb);
+            // O^T += V^T P^T; `from` zeroes the positions from there on (an index into the tile) and those before p_lo
+            auto multiply = [&](auto masked, int from, bool mine) {
+                constexpr bool kMask = decltype(masked)::value;
+                const int lo = kMask ? p_lo - p0 : 0;
+                uint32_t low = 0x05040100u, high = 0x07060302u;  // byte permutations: the rows' low or high halves
+                // (opaque, or the permuted rows of every limit's round would be kept in registers across the rounds)
+                if (kMask) asm volatile("" : "+s"(low), "+s"(high));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p32[n][i] = p[i];
-            } else {
-                split8<TYPE, S::kParts>(p, pb[n]);
-            }
-        }
-        // O^T += V^T P^T; `from` zeroes the positions from there on (an index into the tile) and those before p_lo
-        auto multiply = [&](auto masked, int from, const int (&rel)[NC]) {
-            constexpr bool kMask = decltype(masked)::value;
-            const int lo = kMask ? p_lo - p0 : 0;
+                for (int h = 0; h < kNh; ++h)
 #pragma unroll
-            for (int h = 0; h < kNh; ++h)
-#pragma unroll
-                for (int e = 0; e < kVe; ++e) {
-                    if constexpr (S::kWide) {
-#pragma unroll
-                        for (int n = 0; n < NC; ++n) {
-                            if (n > 0 && n >= ncols) continue;
-                            f32x4 x = acc[n][h * kVe + e];
+                    for (int e = 0; e < kVe; ++e) {
+                        f32x4 x = acc[h * kVe + e];
+                        if constexpr (S::kWide) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 float u = __builtin_bit_cast(float, static_cast<uint32_t>(v[0][i][h][e]));
                                 if (kMask && (4 * g + i < lo || 4 * g + i >= from)) u = 0.0f;
-                                x = __builtin_amdgcn_mfma_f32_16x16x4f32(u, p32[n][i], x, 0, 0, 0);
+                                x = __builtin_amdgcn_mfma_f32_16x16x4f32(u, p[i], x, 0, 0, 0);
                             }
-                            if (!kMask || rel[n] == from) acc[n][h * kVe + e] = x;
-                        }
-                    } else {
-                        // dim e of the lane's eight positions: halves of two rows' dwords
-                        u32x4 f;
+                        } else {
+                            // dim e of the lane's eight positions: halves of two rows' dwords
+                            u32x4 f;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int t = j >> 1, i = 2 * (j & 1);
-                            const uint32_t x = v[t][i][h][e >> 1], y = v[t][i + 1][h][e >> 1];
-                            f[j] = __builtin_amdgcn_perm(y, x, e & 1 ? 0x07060302u : 0x05040100u);
-                            if (kMask) {
-                                const int at0 = 16 * t + 4 * g + i;
-                                if (at0 < lo || at0 >= from) f[j] &= 0xFFFF0000u;
-                                if (at0 + 1 < lo || at0 + 1 >= from) f[j] &= 0x0000FFFFu;
+                            for (int j = 0; j < 4; ++j) {
+                                const int t = j >> 1, i = 2 * (j & 1);
+                                const uint32_t lo16 = v[t][i][h][e >> 1], hi16 = v[t][i + 1][h][e >> 1];
+                                f[j] = __builtin_amdgcn_perm(hi16, lo16, e & 1 ? high : low);
+                                if (kMask) {
+                                    const int at0 = 16 * t + 4 * g + i;
+                                    if (at0 < lo || at0 >= from) f[j] &= 0xFFFF0000u;
+                                    if (at0 + 1 < lo || at0 + 1 >= from) f[j] &= 0x0000FFFFu;
+                                }
                             }
+#pragma unroll
+                            for (int k = S::kParts - 1; k >= 0; --k) x = mma16(f, pb[k], x, Type{});
                         }
+                        if constexpr (kMask) {
 #pragma unroll
-                        for (int n = 0; n < NC; ++n) {
-                            if (n > 0 && n >= ncols) continue;
-                            f32x4 x = acc[n][h * kVe + e];
-#pragma unroll
-                            for (int p = S::kParts - 1; p >= 0; --p) x = mma16(f, pb[n][p], x, Type{});
-                            if (!kMask || rel[n] == from) acc[n][h * kVe + e] = x;
+                            for (int i = 0; i < 4; ++i) acc[h * kVe + e][i] = mine ? x[i] : acc[h * kVe + e][i];
+                        } else {
+                            acc[h * kVe + e] = x;
                         }
                     }
+            };
+            if (whole) {
+                multiply(std::false_type{}, 0, true);
+            } else {  // once per limit that the tile's columns have
+                const int rel = min(max(min(p_hi, lim) - p0, 0), kTile);
+                for (unsigned long left = __ballot(rel > 0); left != 0;) {
+                    const int from = __builtin_amdgcn_readlane(rel, __builtin_ctzl(left));
+                    multiply(std::true_type{}, from, rel == from);
+                    left &= ~__ballot(rel == from);
                 }
-        };
-        int rel[NC];
-        if (whole) {
-            multiply(std::false_type{}, 0, rel);
-        } else {
-#pragma unroll
-            for (int n = 0; n < NC; ++n) rel[n] = min(max(min(p_hi, lim[n]) - p0, 0), kTile);
-            for (int from = kTile; from > 0; --from) {
-                bool any = false;
-#pragma unroll
-                for (int n = 0; n < NC; ++n) any = any || rel[n] == from;
-                if (__ballot(any) != 0) multiply(std::true_type{}, from, rel);
             }
+            if (more) load_v(next, at, v);
         }
+        if (part == 1) break;
+        part = 1;
+        set_part();
+        if (first < last) load_tile(first);
     }
 
-    // ---- a column's waves meet in LDS, the first of them has the result
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        sum[n] = col_sum(sum[n]);
-        if (sum[n] != sum[n]) mx[n] = INFINITY;  // NaN scores leave no maximum: keep the record from being skipped
-    }
-    auto dim_of = [&](int h, int i) { return 16 * kVe * h + kVe * (4 * g + i); };  // of accumulators h kVe .., element i
-    if (wk > 1) {
-        const int slot = wpos - 1 + w / wk * (wk - 1);  // of kPagedWaves - wq
-        if (wpos > 0) {
-#pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                float* r = lds + (slot * NC * 16 + n * 16 + c) * kRowF;
-                if (g == 0) {
-                    r[DP] = mx[n];
-                    r[DP + 1] = sum[n];
-                }
-#pragma unroll
-                for (int h = 0; h < kNh; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < kVe; e += 4)
-                            *reinterpret_cast<f32x4*>(r + dim_of(h, i) + e) =
-                                f32x4{acc[n][h * kVe + e][i], acc[n][h * kVe + e + 1][i], acc[n][h * kVe + e + 2][i],
-                                      acc[n][h * kVe + e + 3][i]};
-            }
-        }
-        __syncthreads();
-        if (wpos > 0) return;
-        for (int o = 0; o < wk - 1; ++o) {
-#pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                const float* r = lds + ((o + w / wk * (wk - 1)) * NC * 16 + n * 16 + c) * kRowF;
-                const float m2 = r[DP], l2 = r[DP + 1], m = fmaxf(mx[n], m2);
-                const float f1 = mx[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx[n] - m);
-                const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - m);
-                mx[n] = m;
-                sum[n] = sum[n] * f1 + l2 * f2;
-#pragma unroll
-                for (int h = 0; h < kNh; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < kVe; e += 4) {
-                            const f32x4 x = *reinterpret_cast<const f32x4*>(r + dim_of(h, i) + e);
-#pragma unroll
-                            for (int d = 0; d < 4; ++d)
-                                acc[n][h * kVe + e + d][i] = acc[n][h * kVe + e + d][i] * f1 + x[d] * f2;
-                        }
-            }
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        if (tok[n] < 0) continue;
-        float* dst;
+    // ---- the waves of a column meet in LDS, each takes a share of its dims
+    sum = col_sum(sum);
+    if (sum != sum) mx = INFINITY;  // NaN scores leave no maximum: keep the record from being skipped
+    auto dim_of = [&](int h, int i) { return 16 * kVe * h + kVe * (4 * g + i); };  // of acc[h kVe ..][i]
+    float* dst = nullptr;
+    if (tok >= 0)
+        dst = a.nrec == 1 ? a.out + tok * a.ldo + static_cast<long>(head) * D
+                          : a.rec + ((static_cast<long>(tok) * a.H + head) * a.nrec + rec_at) * (D + 4);
+    if (wk == 1) {
+        if (tok < 0) return;
         float f = 1.0f;
         if (a.nrec == 1) {
-            dst = a.out + tok[n] * a.ldo + static_cast<long>(head[n]) * D;
-            f = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];  // a row that sees nothing: zeros
+            f = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing: zeros
         } else {
-            dst = a.rec + ((static_cast<long>(tok[n]) * a.H + head[n]) * a.nrec + rec_at) * (D + 4);
-            if (g == 0) *reinterpret_cast<f32x2*>(dst) = f32x2{mx[n], sum[n]};
+            if (g == 0) *reinterpret_cast<f32x2*>(dst) = f32x2{mx, sum};
             dst += 4;
-            if (mx[n] == -INFINITY) continue;
+            if (mx == -INFINITY) return;
         }
 #pragma unroll
         for (int h = 0; h < kNh; ++h)
@@ -574,42 +559,315 @@ __global__ __launch_bounds__(64 * kPagedWaves) void paged_attn_kernel(const Page
                 for (int e = 0; e < kVe; e += 4) {
                     const int d = dim_of(h, i) + e;
                     if (EVEN || d < D)
-                        *reinterpret_cast<f32x4_a4*>(dst + d) =
-                            f32x4_a4{acc[n][h * kVe + e][i] * f, acc[n][h * kVe + e + 1][i] * f,
-                                     acc[n][h * kVe + e + 2][i] * f, acc[n][h * kVe + e + 3][i] * f};
+                        *reinterpret_cast<f32x4_a4*>(dst + d) = f32x4_a4{acc[h * kVe + e][i] * f, acc[h * kVe + e + 1][i] * f,
+                                                                         acc[h * kVe + e + 2][i] * f,
+                                                                         acc[h * kVe + e + 3][i] * f};
                 }
+        return;
+    }
+    constexpr int kRowF = DP + 4;  // floats of a column's record; the row stride spreads the banks
+    float* const mine = lds + w * 16 * kRowF;
+    if (g == 0) {
+        mine[c * kRowF + DP] = mx;
+        mine[c * kRowF + DP + 1] = sum;
+    }
+    if (mx != -INFINITY) {
+#pragma unroll
+        for (int h = 0; h < kNh; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < kVe; e += 4)
+                    *reinterpret_cast<f32x4*>(mine + c * kRowF + dim_of(h, i) + e) =
+                        f32x4{acc[h * kVe + e][i], acc[h * kVe + e + 1][i], acc[h * kVe + e + 2][i],
+                              acc[h * kVe + e + 3][i]};
+    }
+    __syncthreads();
+    if (tok < 0) return;
+    const float* const rec = lds + w / wk * wk * 16 * kRowF + c * kRowF;  // of the column's first wave
+    float top = -INFINITY;
+    for (int o = 0; o < wk; ++o) top = fmaxf(top, rec[o * 16 * kRowF + DP]);
+    float total = 0.0f, f[kPagedWaves];
+#pragma unroll
+    for (int o = 0; o < kPagedWaves; ++o) {
+        if (o >= wk) break;
+        const float m = rec[o * 16 * kRowF + DP];
+        f[o] = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        total += rec[o * 16 * kRowF + DP + 1] * f[o];
+    }
+    float back = 1.0f;
+    if (a.nrec == 1) {
+        back = total == 0.0f ? 0.0f : 1.0f / total;  // a row that sees nothing: zeros
+    } else {
+        if (g == 0 && wpos == 0) *reinterpret_cast<f32x2*>(dst) = f32x2{top, total};
+        dst += 4;
+        if (top == -INFINITY) return;
+    }
+    for (int d = 4 * (4 * wpos + g); d < D; d += 16 * wk) {
+        f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+        for (int o = 0; o < kPagedWaves; ++o) {
+            if (o >= wk) break;
+            if (f[o] != 0.0f) x += *reinterpret_cast<const f32x4*>(rec + o * 16 * kRowF + d) * f[o];
+        }
+        *reinterpret_cast<f32x4_a4*>(dst + d) = f32x4_a4{x[0] * back, x[1] * back, x[2] * back, x[3] * back};
     }
 }
 
-template <int TYPE, int DP, int NC, bool EVEN>
+// The shared prefix against many rows (16-bit caches, head_dim 64 and 128, pages of 16 n positions).  A workgroup of four
+// waves takes 128 rows, 32 to a wave, and a chunk of the prefix in stages of 64 positions that all its waves read from
+// LDS: straight from the pool every wave would load 16 KB for the 2 x 0.5 MFLOP it does with a tile, more than the L1
+// delivers beside the matrix instructions.  v_mfma_f32_32x32x16: half the instructions of 16x16x32 for the same product.
+//   * K goes to LDS with global_load_lds, whole rows at a time; the 16-byte pieces of a row are exchanged within it so
+//     that the 32 rows of an operand fetch lie in different banks.
+//   * V goes through registers, where 16 positions x dims are transposed with byte permutations, to LDS in operand order.
+//     An operand's "row" i holds the dims (D / 32) i + block, so that a lane's dims are consecutive in memory.
+//   * Two buffers, one barrier per stage; the next stage is under way while the current one is multiplied.
+constexpr int kPrefixStage = 64, kPrefixRows = 128;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c, std::integral_constant<int, kKvF16>) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c, std::integral_constant<int, kKvBF16>) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+}
+
+// 16 bytes per lane from global memory into LDS (lane l at byte 16 l of the wave-uniform lds)
+__device__ __forceinline__ void dma16(const void* g, char* lds) { __builtin_amdgcn_global_load_lds(g, lds, 16, 0, 0); }
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArgs a) {
+    typedef PagedShape<TYPE, D> S;
+    typedef typename KvType<TYPE>::elem elem;
+    typedef std::integral_constant<int, TYPE> Type;
+    constexpr int kParts = S::kParts, kKs = D / 16, kDb = D / 32, kRowB = 2 * D, kPieces = kRowB / 16;
+    constexpr int kBuf = kPrefixStage * kRowB;  // bytes of a stage's K or V
+    extern __shared__ __attribute__((aligned(16))) char stage_lds[];  // K twice, V twice
+    typedef uint32_t vreg __attribute__((ext_vector_type(D / 64)));   // a lane's dims of a row of V
+
+    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int Hkv = a.P.n_kv_heads, G = a.G, nrows = a.B.n_rows * G;
+    const long row_elems = static_cast<long>(Hkv) * D;
+    int chunk, kvh, tile;
+    if (!prefix_item(a, blockIdx.x, Hkv, chunk, kvh, tile)) return;
+    const int p_lo = chunk * a.pre_per, p_hi = min(p_lo + a.pre_per, a.prefix_len);
+    const int table_len = (a.prefix_len + a.P.page_size - 1) / a.P.page_size;
+
+    const elem* const kbase = static_cast<const elem*>(a.P.k) + static_cast<long>(kvh) * D;
+    const elem* const vbase = static_cast<const elem*>(a.P.v) + static_cast<long>(kvh) * D;
+    // the 16 positions of a stage that this wave copies lie in one page
+    auto rows_at = [&](int p0) {
+        const int pos = p0 + 16 * w, pi = page_index(a.P, pos);
+        const int pg = uniform(a.prefix_pages)[min(pi, table_len - 1)];
+        return (static_cast<unsigned>(pg) < static_cast<unsigned>(a.P.n_pages) ? pg : 0) * a.P.stride +
+               (pos - pi * a.P.page_size) * row_elems;
+    };
+    // a piece's place in its row of LDS
+    auto mix = [&](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
+    auto copy_k = [&](long at, int buf) {
+        constexpr int kRows = 64 / kPieces;  // of a copy
+#pragma unroll
+        for (int n = 0; n < 16 / kRows; ++n) {
+            const int r = n * kRows + lane / kPieces, piece = lane % kPieces ^ mix(r);
+            dma16(kbase + at + r * row_elems + 8 * piece, stage_lds + buf * kBuf + (16 * w + n * kRows) * kRowB);
+        }
+    };
+    auto load_v = [&](long at, vreg (&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = *reinterpret_cast<const vreg*>(vbase + at + (8 * (e >> 2) + 4 * h + (e & 3)) * row_elems + kDb * i);
+    };
+    auto store_v = [&](vreg (&v)[8], int p0, int buf) {
+        if (p0 + 16 * w + 16 > p_hi) {  // positions past the prefix: zeros, whatever their page holds
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (p0 + 16 * w + 8 * (e >> 2) + 4 * h + (e & 3) >= p_hi) v[e] = vreg(0u);
+        }
+        char* const dst = stage_lds + 2 * kBuf + buf * kBuf + w * kDb * 1024 + 16 * lane;
+#pragma unroll
+        for (int d = 0; d < kDb; ++d) {
+            u32x4 f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                f[j] = __builtin_amdgcn_perm(v[2 * j + 1][d >> 1], v[2 * j][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+            *reinterpret_cast<u32x4*>(dst + d * 1024) = f;
+        }
+    };
+
+    vreg v[8];
+    {
+        const long at = rows_at(p_lo);
+        copy_k(at, 0);
+        load_v(at, v);
+    }
+    // ---- the lane's row and query operand.  Rows that do not see the whole prefix are left to the workgroups of their
+    // sequences: here they get empty records.
+    const int row0 = tile * kPrefixRows + 32 * w, r = row0 + i, t0 = row0 / G, t = r / G;
+    bool found;
+    const int pos = position_of(a.B, t0, min((row0 + 31) / G, a.B.n_rows - 1) - t0 + 1, t - t0, found);
+    const int tok = found && r < nrows ? t : -1, head = kvh * G + r - t * G;
+    const bool sees = tok >= 0 && pos + 1 >= a.prefix_len;
+    const bool active = __ballot(sees) != 0;
+    u32x4 q[kKs][kParts];
+    float kf = a.qscale;
+    {
+        const float* src = a.q + static_cast<long>(max(tok, 0)) * a.ldq + static_cast<long>(head) * D + 8 * h;
+        float x[kKs][8], m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kKs; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const f32x4 v = sees ? ld_f32x4(src + 16 * j + e) : f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    x[j][e + d] = v[d];
+                    m = fmaxf(m, fabsf(v[d]));
+                }
+            }
+        float f = 1.0f;
+        if constexpr (TYPE == kKvF16) q_scale(swap_max32(m, m), f, kf);
+#pragma unroll
+        for (int j = 0; j < kKs; ++j) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[j][e] *= f;
+            split8<TYPE, kParts>(x[j], q[j]);
+        }
+    }
+
+    f32x16 o[kDb];
+#pragma unroll
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
+    float mx = -INFINITY, sum = 0.0f;
+
+    auto multiply_tile = [&](const char* kt, const char* vt, int p0) {
+        f32x16 s;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < kKs; ++ks) {
+            const u32x4 k = *reinterpret_cast<const u32x4*>(kt + i * kRowB + 16 * ((2 * ks + h) ^ mix(i)));
+#pragma unroll
+            for (int p = kParts - 1; p >= 0; --p) s = mma32(k, q[ks][p], s, Type{});
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] *= kf;
+        if (p0 + 32 > p_hi) {  // the prefix ends in this tile
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                if (p0 + 8 * (v >> 2) + 4 * h + (v & 3) >= p_hi) s[v] = -INFINITY;
+        }
+        float m = s[0];
+#pragma unroll
+        for (int v = 1; v < 16; ++v) m = fmaxf(m, s[v]);
+        m = swap_max32(m, m);
+        const bool raise = m > mx + S::kSlack;
+        if (__ballot(raise) != 0) {
+            const float f = raise ? __builtin_amdgcn_exp2f(mx - m) : 1.0f;
+            if (raise) mx = m;
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < kDb; ++d) o[d] *= f;
+        }
+        const float base = (mx == -INFINITY ? 0.0f : mx) - S::kShift;
+        u32x4 pb[2][kParts];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(s[8 * b + e] - base);
+                sum += p[e];
+            }
+            split8<TYPE, kParts>(p, pb[b]);
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int d = 0; d < kDb; ++d) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(vt + (b * kDb + d) * 1024 + 16 * lane);
+#pragma unroll
+                for (int p = kParts - 1; p >= 0; --p) o[d] = mma32(v, pb[b][p], o[d], Type{});
+            }
+    };
+
+    const int stages = (p_hi - p_lo + kPrefixStage - 1) / kPrefixStage;
+    {
+        store_v(v, p_lo, 0);
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the copies to LDS
+        __syncthreads();
+    }
+    for (int st = 0; st < stages; ++st) {
+        const int p0 = p_lo + st * kPrefixStage, buf = st & 1;
+        const bool more = st + 1 < stages;
+        if (more) {
+            const long at = rows_at(p0 + kPrefixStage);
+            copy_k(at, buf ^ 1);
+            load_v(at, v);
+        }
+        const char* const kt = stage_lds + buf * kBuf;
+        const char* const vt = stage_lds + 2 * kBuf + buf * kBuf;
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t)
+            if (active && p0 + 32 * t < p_hi) multiply_tile(kt + t * 32 * kRowB, vt + t * 2 * kDb * 1024, p0 + 32 * t);
+        if (more) {
+            store_v(v, p0 + kPrefixStage, buf ^ 1);
+            __builtin_amdgcn_s_waitcnt(0x0F70);
+            __syncthreads();
+        }
+    }
+
+    sum = swap_add32(sum, sum);
+    if (sum != sum) mx = INFINITY;  // NaN scores leave no maximum: keep the record from being skipped
+    if (!sees) mx = -INFINITY;
+    if (tok < 0) return;
+    float* dst = a.rec + ((static_cast<long>(tok) * a.H + head) * a.nrec + chunk) * (D + 4);
+    if (h == 0) *reinterpret_cast<f32x2*>(dst) = f32x2{mx, sees ? sum : 0.0f};
+    if (mx == -INFINITY) return;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        float* x = dst + 4 + kDb * (8 * (e >> 2) + 4 * h + (e & 3));
+        if constexpr (kDb == 4)
+            *reinterpret_cast<f32x4*>(x) = f32x4{o[0][e], o[1][e], o[2][e], o[3][e]};
+        else
+            *reinterpret_cast<f32x2*>(x) = f32x2{o[0][e], o[1][e]};
+    }
+}
+
+template <int TYPE, int DP, bool EVEN>
 void run_paged_attn(const PagedAttnArgs& a, int blocks, hipStream_t stream) {
-    const int lds = (kPagedWaves - 1) * NC * 16 * (DP + 4) * 4;
-    hipLaunchKernelGGL((paged_attn_kernel<TYPE, DP, NC, EVEN>), dim3(blocks), dim3(64 * kPagedWaves), lds, stream, a);
+    hipLaunchKernelGGL((paged_attn_kernel<TYPE, DP, EVEN>), dim3(blocks), dim3(64 * kPagedWaves),
+                       kPagedWaves * 16 * (DP + 4) * 4, stream, a);
 }
 
 template <int TYPE>
-void run_paged_attn_type(const PagedAttnArgs& a, bool even, int nc, int blocks, hipStream_t stream) {
+void run_paged_attn_type(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream) {
     const int D = a.P.head_dim;
-    if (even) {
-        if (D == 64)
-            nc == 2 ? run_paged_attn<TYPE, 64, 2, true>(a, blocks, stream) : run_paged_attn<TYPE, 64, 1, true>(a, blocks, stream);
-        else if (D == 128)
-            nc == 2 ? run_paged_attn<TYPE, 128, 2, true>(a, blocks, stream) : run_paged_attn<TYPE, 128, 1, true>(a, blocks, stream);
-        else
-            run_paged_attn<TYPE, 256, 1, true>(a, blocks, stream);
-    } else {
-        if (D <= 64)
-            run_paged_attn<TYPE, 64, 1, false>(a, blocks, stream);
-        else if (D <= 128)
-            run_paged_attn<TYPE, 128, 1, false>(a, blocks, stream);
-        else
-            run_paged_attn<TYPE, 256, 1, false>(a, blocks, stream);
-    }
+    if (D <= 64)
+        even ? run_paged_attn<TYPE, 64, true>(a, blocks, stream) : run_paged_attn<TYPE, 64, false>(a, blocks, stream);
+    else if (D <= 128)
+        even ? run_paged_attn<TYPE, 128, true>(a, blocks, stream) : run_paged_attn<TYPE, 128, false>(a, blocks, stream);
+    else
+        even ? run_paged_attn<TYPE, 256, true>(a, blocks, stream) : run_paged_attn<TYPE, 256, false>(a, blocks, stream);
 }
 
-void run_paged_attn_f32(const PagedAttnArgs& a, bool even, int nc, int blocks, hipStream_t stream);
-void run_paged_attn_f16(const PagedAttnArgs& a, bool even, int nc, int blocks, hipStream_t stream);
-void run_paged_attn_bf16(const PagedAttnArgs& a, bool even, int nc, int blocks, hipStream_t stream);
+template <int TYPE>
+void run_paged_prefix_type(const PagedAttnArgs& a, hipStream_t stream) {
+    const int lds = 4 * kPrefixStage * a.P.head_dim * 2;
+    if (a.P.head_dim == 64)
+        hipLaunchKernelGGL((paged_prefix_kernel<TYPE, 64>), dim3(a.pre_blocks), dim3(256), lds, stream, a);
+    else
+        hipLaunchKernelGGL((paged_prefix_kernel<TYPE, 128>), dim3(a.pre_blocks), dim3(256), lds, stream, a);
+}
+
+void run_paged_prefix_f16(const PagedAttnArgs& a, hipStream_t stream);
+void run_paged_prefix_bf16(const PagedAttnArgs& a, hipStream_t stream);
+void run_paged_attn_f32(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream);
+void run_paged_attn_f16(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream);
+void run_paged_attn_bf16(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream);
 
 }  // namespace dev
 }  // namespace cri

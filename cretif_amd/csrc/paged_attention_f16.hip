@@ -4,9 +4,11 @@
 namespace cri {
 namespace dev {
 
-void run_paged_attn_f16(const PagedAttnArgs& a, bool even, int nc, int blocks, hipStream_t stream) {
-    run_paged_attn_type<kKvF16>(a, even, nc, blocks, stream);
+void run_paged_attn_f16(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream) {
+    run_paged_attn_type<kKvF16>(a, even, blocks, stream);
 }
+
+void run_paged_prefix_f16(const PagedAttnArgs& a, hipStream_t stream) { run_paged_prefix_type<kKvF16>(a, stream); }
 
 }  // namespace dev
 }  // namespace cri

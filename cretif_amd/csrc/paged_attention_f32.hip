@@ -4,8 +4,8 @@
 namespace cri {
 namespace dev {
 
-void run_paged_attn_f32(const PagedAttnArgs& a, bool even, int nc, int blocks, hipStream_t stream) {
-    run_paged_attn_type<kKvF32>(a, even, nc, blocks, stream);
+void run_paged_attn_f32(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream) {
+    run_paged_attn_type<kKvF32>(a, even, blocks, stream);
 }
 
 }  // namespace dev
