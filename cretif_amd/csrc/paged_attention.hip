@@ -80,7 +80,7 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
     c.own_wq = waves_of(mean);
     if (prefix_len > 0) {
         const int tile_rows = c.staged ? kPrefixRows : block * c.pre_wq;
-        const int unit = c.staged ? kPrefixStage : tile * (kPagedWaves / c.pre_wq);
+        const int unit = c.staged ? kPrefixTile : tile * (kPagedWaves / c.pre_wq);
         c.pre_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
         const long streams = static_cast<long>(P.n_kv_heads) * c.pre_tiles;
         const int units = (prefix_len + unit - 1) / unit;

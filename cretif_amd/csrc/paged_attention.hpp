@@ -68,7 +68,10 @@ __device__ __forceinline__ f32x4 mma16(const u32x4& a, const u32x4& b, const f32
 // the parts of eight floats (times f for fp16): x = p[0] + p[1] (+ p[2]), each the rest's rounding
 template <int TYPE, int PARTS>
 __device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&p)[PARTS]) {
-    float r[8];
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    float r[8], one = 1.0f;
+    h2 hi[4];
+    if (TYPE == kKvF16) asm("" : "+s"(one));  // (opaque: a product by 1 would be folded away, and with it the v_fma_mix)
 #pragma unroll
     for (int e = 0; e < 8; ++e) r[e] = x[e];
 #pragma unroll
@@ -77,11 +80,15 @@ __device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&p)[PARTS]) {
         for (int e = 0; e < 4; ++e) {
             const f32x2 v = {r[2 * e], r[2 * e + 1]};
             if constexpr (TYPE == kKvF16) {
-                typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-                const h2 w = __builtin_convertvector(v, h2);
+                h2 w;
+                if (k == 0) {
+                    w = __builtin_convertvector(v, h2);
+                    hi[e] = w;
+                } else {  // the rest and its rounding in one v_fma_mix each
+                    w = h2{static_cast<_Float16>(fmaf(v.x, one, -static_cast<float>(hi[e].x))),
+                           static_cast<_Float16>(fmaf(v.y, one, -static_cast<float>(hi[e].y)))};
+                }
                 p[k][e] = __builtin_bit_cast(uint32_t, w);
-                r[2 * e] -= static_cast<float>(w.x);
-                r[2 * e + 1] -= static_cast<float>(w.y);
             } else {
                 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
                 const b2 w = __builtin_convertvector(v, b2);
@@ -615,15 +622,20 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
 }
 
 // The shared prefix against many rows (16-bit caches, head_dim 64 and 128, pages of 16 n positions).  A workgroup of four
-// waves takes 128 rows, 32 to a wave, and a chunk of the prefix in stages of 64 positions that all its waves read from
-// LDS: straight from the pool every wave would load 16 KB for the 2 x 0.5 MFLOP it does with a tile, more than the L1
-// delivers beside the matrix instructions.  v_mfma_f32_32x32x16: half the instructions of 16x16x32 for the same product.
-//   * K goes to LDS with global_load_lds, whole rows at a time; the 16-byte pieces of a row are exchanged within it so
-//     that the 32 rows of an operand fetch lie in different banks.
-//   * V goes through registers, where 16 positions x dims are transposed with byte permutations, to LDS in operand order.
-//     An operand's "row" i holds the dims (D / 32) i + block, so that a lane's dims are consecutive in memory.
-//   * Two buffers, one barrier per stage; the next stage is under way while the current one is multiplied.
-constexpr int kPrefixStage = 64, kPrefixRows = 128;
+// waves takes 128 rows, 32 to a wave, and a chunk of the prefix in tiles of 32 positions that all its waves read from LDS:
+// straight from the pool every wave would load 16 KB for the 2 x 0.5 MFLOP it does with a tile, more than the L1 delivers
+// beside the matrix instructions.  v_mfma_f32_32x32x16: half the instructions of 16x16x32 for the same product.
+//   * Tiles go to LDS with global_load_lds, whole rows at a time, into rings of four, two to three tiles ahead; one barrier
+//     per tile.  The 16-byte pieces of a row are exchanged within it: K's so that the 32 rows of an operand fetch lie in
+//     different banks, V's so that the four rows that ds_read_b64_tr_b16 takes apart do (16 lanes read 4 positions x 16
+//     dims and get a dim's 4 positions each: V^T's operand without a byte permutation).
+//   * The scores of the next tile are issued between the exponentials of the current one, the next tile's maximum between
+//     the products with V: a wave's matrix instructions and its vector ones run side by side.
+//   * kf, the scores' factor, is applied within the exponential's fma.  It is not negative (a negative scale turns the
+//     query's sign), so the raw scores' maximum is the scaled ones'.
+// Bound by the vector instructions beside the matrix ones: about 100 and 16 exponentials per tile and wave to 32
+// products of 32 cycles.
+constexpr int kPrefixRows = 128, kPrefixTile = 32, kRing = 4;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c, std::integral_constant<int, kKvF16>) {
@@ -632,9 +644,18 @@ __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f3
 __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c, std::integral_constant<int, kKvBF16>) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
 }
-
 // 16 bytes per lane from global memory into LDS (lane l at byte 16 l of the wave-uniform lds)
 __device__ __forceinline__ void dma16(const void* g, char* lds) { __builtin_amdgcn_global_load_lds(g, lds, 16, 0, 0); }
+// lanes 4 k + a of each 16 give the address of row k's 4 a-th element, lane i gets element i of rows 0 .. 3
+__device__ __forceinline__ u32x2 read_transposed(const char* p) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* Ptr;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(p)));
+}
+template <int N>
+__device__ __forceinline__ void wait_copies() {  // all but the last N copies of this wave have arrived
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
 
 template <int TYPE, int D>
 __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArgs a) {
@@ -642,66 +663,48 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
     typedef typename KvType<TYPE>::elem elem;
     typedef std::integral_constant<int, TYPE> Type;
     constexpr int kParts = S::kParts, kKs = D / 16, kDb = D / 32, kRowB = 2 * D, kPieces = kRowB / 16;
-    constexpr int kBuf = kPrefixStage * kRowB;  // bytes of a stage's K or V
-    extern __shared__ __attribute__((aligned(16))) char stage_lds[];  // K twice, V twice
-    typedef uint32_t vreg __attribute__((ext_vector_type(D / 64)));   // a lane's dims of a row of V
+    constexpr int kTileB = kPrefixTile * kRowB;  // bytes of a tile's K or V
+    constexpr int kCopies = kTileB / 1024 / 4;   // of a wave, of a tile's K or V
+    extern __shared__ __attribute__((aligned(16))) char ring[];  // K's tiles, V's tiles
 
     const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.P.n_kv_heads, G = a.G, nrows = a.B.n_rows * G;
-    const long row_elems = static_cast<long>(Hkv) * D;
+    const uint32_t row_bytes = static_cast<uint32_t>(Hkv) * kRowB;
     int chunk, kvh, tile;
     if (!prefix_item(a, blockIdx.x, Hkv, chunk, kvh, tile)) return;
     const int p_lo = chunk * a.pre_per, p_hi = min(p_lo + a.pre_per, a.prefix_len);
+    const int ntiles = (p_hi - p_lo + kPrefixTile - 1) / kPrefixTile;
     const int table_len = (a.prefix_len + a.P.page_size - 1) / a.P.page_size;
 
-    const elem* const kbase = static_cast<const elem*>(a.P.k) + static_cast<long>(kvh) * D;
-    const elem* const vbase = static_cast<const elem*>(a.P.v) + static_cast<long>(kvh) * D;
-    // the 16 positions of a stage that this wave copies lie in one page
-    auto rows_at = [&](int p0) {
-        const int pos = p0 + 16 * w, pi = page_index(a.P, pos);
-        const int pg = uniform(a.prefix_pages)[min(pi, table_len - 1)];
-        return (static_cast<unsigned>(pg) < static_cast<unsigned>(a.P.n_pages) ? pg : 0) * a.P.stride +
-               (pos - pi * a.P.page_size) * row_elems;
-    };
-    // a piece's place in its row of LDS
-    auto mix = [&](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
-    auto copy_k = [&](long at, int buf) {
-        constexpr int kRows = 64 / kPieces;  // of a copy
+    // ---- the copies: a wave's rows of a tile lie in one page (8 rows each; 16 share a page)
+    const char* const kbase = static_cast<const char*>(a.P.k) + static_cast<long>(kvh) * kRowB;
+    const char* const vbase = static_cast<const char*>(a.P.v) + static_cast<long>(kvh) * kRowB;
+    auto k_mix = [&](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
+    auto v_mix = [&](int row) { return D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; };
+    constexpr int kCopyRows = 64 / kPieces;
+    uint32_t k_off[kCopies], v_off[kCopies];  // bytes of the lane's pieces from the wave's first row
 #pragma unroll
-        for (int n = 0; n < 16 / kRows; ++n) {
-            const int r = n * kRows + lane / kPieces, piece = lane % kPieces ^ mix(r);
-            dma16(kbase + at + r * row_elems + 8 * piece, stage_lds + buf * kBuf + (16 * w + n * kRows) * kRowB);
-        }
-    };
-    auto load_v = [&](long at, vreg (&v)[8]) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            v[e] = *reinterpret_cast<const vreg*>(vbase + at + (8 * (e >> 2) + 4 * h + (e & 3)) * row_elems + kDb * i);
-    };
-    auto store_v = [&](vreg (&v)[8], int p0, int buf) {
-        if (p0 + 16 * w + 16 > p_hi) {  // positions past the prefix: zeros, whatever their page holds
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (p0 + 16 * w + 8 * (e >> 2) + 4 * h + (e & 3) >= p_hi) v[e] = vreg(0u);
-        }
-        char* const dst = stage_lds + 2 * kBuf + buf * kBuf + w * kDb * 1024 + 16 * lane;
-#pragma unroll
-        for (int d = 0; d < kDb; ++d) {
-            u32x4 f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                f[j] = __builtin_amdgcn_perm(v[2 * j + 1][d >> 1], v[2 * j][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
-            *reinterpret_cast<u32x4*>(dst + d * 1024) = f;
-        }
-    };
-
-    vreg v[8];
-    {
-        const long at = rows_at(p_lo);
-        copy_k(at, 0);
-        load_v(at, v);
+    for (int n = 0; n < kCopies; ++n) {
+        const int r = n * kCopyRows + lane / kPieces, row = 8 * w + r;
+        k_off[n] = r * row_bytes + 16 * (lane % kPieces ^ k_mix(row));
+        v_off[n] = r * row_bytes + 16 * (lane % kPieces ^ v_mix(row));
     }
+    auto copy = [&](int t) {  // tile t (past the last one: that one again, so that every turn issues as many)
+        const int pos = p_lo + min(t, ntiles - 1) * kPrefixTile + 8 * w, pi = page_index(a.P, pos);
+        const int pg = uniform(a.prefix_pages)[min(pi, table_len - 1)];
+        const long at = (static_cast<unsigned>(pg) < static_cast<unsigned>(a.P.n_pages) ? pg : 0) * a.P.stride * 2 +
+                        static_cast<long>(pos - pi * a.P.page_size) * row_bytes;
+        char* const dst = ring + t % kRing * kTileB + 8 * w * kRowB;
+#pragma unroll
+        for (int n = 0; n < kCopies; ++n) dma16(kbase + at + k_off[n], dst + n * 1024);
+#pragma unroll
+        for (int n = 0; n < kCopies; ++n) dma16(vbase + at + v_off[n], dst + kRing * kTileB + n * 1024);
+    };
+    copy(0);
+    copy(1);
+    copy(2);
+
     // ---- the lane's row and query operand.  Rows that do not see the whole prefix are left to the workgroups of their
     // sequences: here they get empty records.
     const int row0 = tile * kPrefixRows + 32 * w, r = row0 + i, t0 = row0 / G, t = r / G;
@@ -709,9 +712,8 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
     const int pos = position_of(a.B, t0, min((row0 + 31) / G, a.B.n_rows - 1) - t0 + 1, t - t0, found);
     const int tok = found && r < nrows ? t : -1, head = kvh * G + r - t * G;
     const bool sees = tok >= 0 && pos + 1 >= a.prefix_len;
-    const bool active = __ballot(sees) != 0;
     u32x4 q[kKs][kParts];
-    float kf = a.qscale;
+    float kf = fmaxf(fabsf(a.qscale), 1.17549435e-38f);  // (not 0: it meets masked scores of -infinity)
     {
         const float* src = a.q + static_cast<long>(max(tok, 0)) * a.ldq + static_cast<long>(head) * D + 8 * h;
         float x[kKs][8], m = 0.0f;
@@ -728,6 +730,9 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
             }
         float f = 1.0f;
         if constexpr (TYPE == kKvF16) q_scale(swap_max32(m, m), f, kf);
+        kf = fmaxf(kf, 1.17549435e-38f);
+        f = __builtin_copysignf(f, a.qscale);
+        if (a.qscale == 0.0f) f = 0.0f;
 #pragma unroll
         for (int j = 0; j < kKs; ++j) {
 #pragma unroll
@@ -743,27 +748,45 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
         for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
     float mx = -INFINITY, sum = 0.0f;
 
-    auto multiply_tile = [&](const char* kt, const char* vt, int p0) {
-        f32x16 s;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+    // the raw scores of tile t, a lane's 16: positions 8 (v >> 2) + 4 h + (v & 3)
+    const char* const k_at = ring + i * kRowB;
+    auto scores = [&](int t, f32x16& s) {
+        const char* const kt = k_at + t % kRing * kTileB;
+        const f32x16 zero = {};
 #pragma unroll
         for (int ks = 0; ks < kKs; ++ks) {
-            const u32x4 k = *reinterpret_cast<const u32x4*>(kt + i * kRowB + 16 * ((2 * ks + h) ^ mix(i)));
+            const u32x4 k = *reinterpret_cast<const u32x4*>(kt + 16 * ((2 * ks + h) ^ k_mix(i)));
 #pragma unroll
-            for (int p = kParts - 1; p >= 0; --p) s = mma32(k, q[ks][p], s, Type{});
+            for (int p = kParts - 1; p >= 0; --p) s = mma32(k, q[ks][p], ks == 0 && p == kParts - 1 ? zero : s, Type{});
         }
-#pragma unroll
-        for (int v = 0; v < 16; ++v) s[v] *= kf;
-        if (p0 + 32 > p_hi) {  // the prefix ends in this tile
+    };
+    auto largest = [&](int t, f32x16& s) {
+        const int left = p_hi - p_lo - t * kPrefixTile;
+        if (left < kPrefixTile) {  // the prefix ends in this tile
 #pragma unroll
             for (int v = 0; v < 16; ++v)
-                if (p0 + 8 * (v >> 2) + 4 * h + (v & 3) >= p_hi) s[v] = -INFINITY;
+                if (8 * (v >> 2) + 4 * h + (v & 3) >= left) s[v] = -INFINITY;
         }
         float m = s[0];
 #pragma unroll
         for (int v = 1; v < 16; ++v) m = fmaxf(m, s[v]);
-        m = swap_max32(m, m);
+        return swap_max32(m, m) * kf;
+    };
+    // V^T's operand of dim block d and positions 16 b .. : two reads of 4 x 16
+    const int v_row = 4 * h + ((lane >> 2) & 3), v_col = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);  // row, byte in 64
+    for (int tl = 0; tl < ntiles; ++tl) {
+        wait_copies<4 * kCopies>();  // tile tl
+        __syncthreads();
+        copy(tl + 3);
+        if (p_hi - p_lo - tl * kPrefixTile < kPrefixTile) {  // positions past the prefix: zeros, whatever their page holds
+            const int left = p_hi - p_lo - tl * kPrefixTile;
+            for (int x = threadIdx.x; x < (kPrefixTile - left) * kPieces; x += 256)
+                *reinterpret_cast<u32x4*>(ring + (kRing + tl % kRing) * kTileB + left * kRowB + 16 * x) = u32x4{0, 0, 0, 0};
+            __syncthreads();
+        }
+        f32x16 s;
+        scores(tl, s);
+        const float m = largest(tl, s);
         const bool raise = m > mx + S::kSlack;
         if (__ballot(raise) != 0) {
             const float f = raise ? __builtin_amdgcn_exp2f(mx - m) : 1.0f;
@@ -779,46 +802,29 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
             float p[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(s[8 * b + e] - base);
+                p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * b + e], kf, -base));
                 sum += p[e];
             }
             split8<TYPE, kParts>(p, pb[b]);
         }
+        const char* const vt = ring + (kRing + tl % kRing) * kTileB;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int d = 0; d < kDb; ++d) {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(vt + (b * kDb + d) * 1024 + 16 * lane);
+                u32x4 v;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int row = 16 * b + 8 * x + v_row;  // row & 3 and (row >> 1) & 1 are the lane's own
+                    const u32x2 y = read_transposed(vt + row * kRowB + ((64 * d) ^ (16 * v_mix(v_row))) + v_col);
+                    v[2 * x] = y.x;
+                    v[2 * x + 1] = y.y;
+                }
 #pragma unroll
                 for (int p = kParts - 1; p >= 0; --p) o[d] = mma32(v, pb[b][p], o[d], Type{});
             }
-    };
-
-    const int stages = (p_hi - p_lo + kPrefixStage - 1) / kPrefixStage;
-    {
-        store_v(v, p_lo, 0);
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the copies to LDS
-        __syncthreads();
     }
-    for (int st = 0; st < stages; ++st) {
-        const int p0 = p_lo + st * kPrefixStage, buf = st & 1;
-        const bool more = st + 1 < stages;
-        if (more) {
-            const long at = rows_at(p0 + kPrefixStage);
-            copy_k(at, buf ^ 1);
-            load_v(at, v);
-        }
-        const char* const kt = stage_lds + buf * kBuf;
-        const char* const vt = stage_lds + 2 * kBuf + buf * kBuf;
-#pragma unroll 1
-        for (int t = 0; t < 2; ++t)
-            if (active && p0 + 32 * t < p_hi) multiply_tile(kt + t * 32 * kRowB, vt + t * 2 * kDb * 1024, p0 + 32 * t);
-        if (more) {
-            store_v(v, p0 + kPrefixStage, buf ^ 1);
-            __builtin_amdgcn_s_waitcnt(0x0F70);
-            __syncthreads();
-        }
-    }
+    wait_copies<0>();
 
     sum = swap_add32(sum, sum);
     if (sum != sum) mx = INFINITY;  // NaN scores leave no maximum: keep the record from being skipped
@@ -828,13 +834,10 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
     if (h == 0) *reinterpret_cast<f32x2*>(dst) = f32x2{mx, sees ? sum : 0.0f};
     if (mx == -INFINITY) return;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        float* x = dst + 4 + kDb * (8 * (e >> 2) + 4 * h + (e & 3));
-        if constexpr (kDb == 4)
-            *reinterpret_cast<f32x4*>(x) = f32x4{o[0][e], o[1][e], o[2][e], o[3][e]};
-        else
-            *reinterpret_cast<f32x2*>(x) = f32x2{o[0][e], o[1][e]};
-    }
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4)
+            *reinterpret_cast<f32x4*>(dst + 4 + 32 * d + 2 * v + 4 * h) = f32x4{o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
 }
 
 template <int TYPE, int DP, bool EVEN>
@@ -856,7 +859,7 @@ void run_paged_attn_type(const PagedAttnArgs& a, bool even, int blocks, hipStrea
 
 template <int TYPE>
 void run_paged_prefix_type(const PagedAttnArgs& a, hipStream_t stream) {
-    const int lds = 4 * kPrefixStage * a.P.head_dim * 2;
+    const int lds = 2 * kRing * kPrefixTile * a.P.head_dim * 2;
     if (a.P.head_dim == 64)
         hipLaunchKernelGGL((paged_prefix_kernel<TYPE, 64>), dim3(a.pre_blocks), dim3(256), lds, stream, a);
     else
