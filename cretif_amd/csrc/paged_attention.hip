@@ -84,13 +84,16 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
         c.pre_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
         const long streams = static_cast<long>(P.n_kv_heads) * c.pre_tiles;
         const int units = (prefix_len + unit - 1) / unit;
-        // chunks: fewest rounds of workgroups times units of each, a workgroup's start and its records counted as two
-        long best = 0;
+        // chunks: rounds of workgroups times units of each (a workgroup that has its CU to itself takes two thirds of the
+        // time), five units for a workgroup's start and end, a sixtieth for each one's records
+        double best = 0.0;
         for (int n = 1; n <= kMaxRecords / 2 && n <= units; ++n) {
-            const long rounds = (streams * n + kSlots - 1) / kSlots, cost = rounds * ((units + n - 1) / n + 2);
-            if (best == 0 || cost < best) {
+            const long groups = streams * n, per = (units + n - 1) / n;
+            const double rounds = groups <= kSlots / 2 ? 0.65 : static_cast<double>((groups + kSlots - 1) / kSlots);
+            const double cost = rounds * per + 5.0 * ((groups + kSlots - 1) / kSlots) + groups / 60.0;
+            if (best == 0.0 || cost < best) {
                 best = cost;
-                c.pre_per = (units + n - 1) / n * unit;
+                c.pre_per = static_cast<int>(per * unit);
             }
         }
         c.pre_chunks = (prefix_len + c.pre_per - 1) / c.pre_per;
@@ -135,6 +138,8 @@ int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, cons
     a.pre_wq = c.pre_wq, a.pre_tiles = c.pre_tiles, a.pre_chunks = c.pre_chunks, a.pre_per = c.pre_per;
     a.pre_blocks = c.pre_blocks;
     a.own_wq = c.own_wq, a.own_tiles = c.own_tiles, a.own_chunks = c.own_chunks, a.own_per = c.own_per;
+    a.by_G = dev::fast_div(a.G), a.by_Hkv = dev::fast_div(P.n_kv_heads);
+    a.by_pre_tiles = dev::fast_div(std::max(c.pre_tiles, 1)), a.by_own_tiles = dev::fast_div(std::max(c.own_tiles, 1));
     a.qscale = scale * 1.44269504088896340736f;
     a.staged = c.staged;
     if (c.staged) {

@@ -26,6 +26,20 @@
 namespace cri {
 namespace dev {
 
+// n / d for 0 <= n < 2^31 by a host-made multiplier (page_index says why it is exact)
+struct FastDiv {
+    uint32_t magic;
+    int shift;
+};
+inline FastDiv fast_div(int d) {
+    int l = 0;
+    while ((1L << l) < d) ++l;
+    return FastDiv{static_cast<uint32_t>((1UL << (31 + l)) / d + 1), 31 + l};
+}
+__device__ __forceinline__ int div_by(int n, FastDiv d) {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * d.magic) >> d.shift);
+}
+
 struct PagedAttnArgs {
     const float* q;
     float* out;
@@ -36,7 +50,8 @@ struct PagedAttnArgs {
     const int* prefix_pages;
     int prefix_len, H, G, nrec;
     int pre_wq, pre_tiles, pre_chunks, pre_per, pre_blocks;  // the prefix's workgroups: [chunk][KV head][tile] by XCD
-    int own_wq, own_tiles, own_chunks, own_per;              // the sequences': [tile][chunk][KV head]
+    int own_wq, own_tiles, own_chunks, own_per;              // the sequences': [chunk][tile][KV head]: long ones first
+    FastDiv by_G, by_Hkv, by_pre_tiles, by_own_tiles;
     float qscale;  // scale * log2 e: scores are in base 2
     bool staged;   // the prefix went to paged_prefix_kernel
 };
@@ -169,10 +184,10 @@ __device__ __forceinline__ int position_of(const PageBatch& B, int t0, int n, in
 // K and V) go to one XCD and its L2
 __device__ __forceinline__ bool prefix_item(const PagedAttnArgs& a, int b, int Hkv, int& chunk, int& kvh, int& tile) {
     const int wi = b % kPagedXcds * (a.pre_blocks / kPagedXcds) + b / kPagedXcds;
-    const int stream = wi / a.pre_tiles;
-    tile = wi % a.pre_tiles;
-    chunk = stream / Hkv;
-    kvh = stream % Hkv;
+    const int stream = div_by(wi, a.by_pre_tiles);
+    tile = wi - stream * a.pre_tiles;
+    chunk = div_by(stream, a.by_Hkv);
+    kvh = stream - chunk * Hkv;
     return chunk < a.pre_chunks;
 }
 
@@ -213,11 +228,10 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
         own_table = uniform(a.prefix_pages);
         own_len = prefix_pages;
     } else {
-        int b = static_cast<int>(blockIdx.x) - a.pre_blocks;
-        kvh = b % Hkv;
-        b /= Hkv;
-        const int chunk = b % a.own_chunks;
-        int tile = b / a.own_chunks;
+        const int b = static_cast<int>(blockIdx.x) - a.pre_blocks, rest = div_by(b, a.by_Hkv);
+        kvh = b - rest * Hkv;
+        const int chunk = div_by(rest, a.by_own_tiles);
+        int tile = rest - chunk * a.own_tiles;
         wq = a.own_wq;
         // the tile-th tile of rows of the batch: 64 sequences' tile counts summed at a time
         const int rt = 16 * wq;
@@ -249,7 +263,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
         own_lo = max(own_lo, min(a.prefix_len, end));
         own_table = uniform(a.B.pages + static_cast<long>(seq) * a.B.max_pages);
         own_len = a.B.max_pages;
-        if (a.staged && pos0 + row0 / G + 1 < a.prefix_len) {
+        if (a.staged && pos0 + div_by(row0, a.by_G) + 1 < a.prefix_len) {
             const int hi = min(a.prefix_len, len);
             const int per = ((hi + a.own_chunks - 1) / a.own_chunks + kTile - 1) / kTile * kTile;
             before_lo = min(chunk * per, hi);
@@ -262,12 +276,12 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
     // ---- the lane's column: its row, the positions up to and with the row's own, its query operand
     int tok = -1, head = 0, sees = 0;
     {
-        const int r = wrow + c, i0 = wrow / G, i = r / G, t = tok0 + i;
+        const int r = wrow + c, i0 = div_by(wrow, a.by_G), i = div_by(r, a.by_G), t = tok0 + i;
         bool ok = r < nrows && t >= 0 && t < a.B.n_rows;
         int p = pos0 + i;
         if (prefix) {
             bool found;
-            p = position_of(a.B, i0, min((wrow + 15) / G, a.B.n_rows - 1) - i0 + 1, i - i0, found);
+            p = position_of(a.B, i0, min(div_by(wrow + 15, a.by_G), a.B.n_rows - 1) - i0 + 1, i - i0, found);
             ok = ok && found;
         }
         if (ok) {
@@ -276,6 +290,23 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
             sees = max(p + 1, 0);
         }
     }
+    if (own_lo >= own_hi && before_lo >= before_hi && a.nrec > 1) {  // no positions: an empty record
+        if (wpos == 0 && g == 0 && tok >= 0)
+            *reinterpret_cast<f32x2*>(a.rec + ((static_cast<long>(tok) * a.H + head) * a.nrec + rec_at) * (D + 4)) =
+                f32x2{-INFINITY, 0.0f};
+        return;
+    }
+    // the query's row, under way while the first tile is looked up
+    f32x4 raw[S::kWide ? kKs : 2 * kKs];
+    {
+        const float* src = a.q + static_cast<long>(max(tok, 0)) * a.ldq + static_cast<long>(head) * D;
+#pragma unroll
+        for (int j = 0; j < (S::kWide ? kKs : 2 * kKs); ++j) {
+            const int d = S::kWide ? 16 * j + 4 * g : 32 * (j >> 1) + 8 * g + 4 * (j & 1);
+            raw[j] = tok >= 0 && (EVEN || d < D) ? ld_f32x4(src + d) : f32x4{0, 0, 0, 0};
+        }
+    }
+
     // ---- the tiles
     const char* const kbase = static_cast<const char*>(a.P.k) + static_cast<long>(kvh) * D * kEs;
     const char* const vbase = static_cast<const char*>(a.P.v) + static_cast<long>(kvh) * D * kEs;
@@ -372,28 +403,18 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
     u32x4 q[S::kWide ? 1 : kKs][S::kParts];
     f32x4 q32[S::kWide ? kKs : 1];
     {
-        const float* src = a.q + static_cast<long>(max(tok, 0)) * a.ldq + static_cast<long>(head) * D;
         if constexpr (S::kWide) {
 #pragma unroll
-            for (int j = 0; j < kKs; ++j) {
-                const int d = 16 * j + 4 * g;
-                q32[j] = tok >= 0 && (EVEN || d < D) ? ld_f32x4(src + d) : f32x4{0, 0, 0, 0};
-            }
+            for (int j = 0; j < kKs; ++j) q32[j] = raw[j];
         } else {
             float x[kKs][8], m = 0.0f;
 #pragma unroll
-            for (int j = 0; j < kKs; ++j) {
-                const int d = 32 * j + 8 * g;
+            for (int j = 0; j < kKs; ++j)
 #pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    const f32x4 v = tok >= 0 && (EVEN || d < D) ? ld_f32x4(src + d + e) : f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[j][e + i] = v[i];
-                        m = fmaxf(m, fabsf(v[i]));
-                    }
+                for (int e = 0; e < 8; ++e) {
+                    x[j][e] = raw[2 * j + (e >> 2)][e & 3];
+                    m = fmaxf(m, fabsf(x[j][e]));
                 }
-            }
             float f = 1.0f;
             if constexpr (TYPE == kKvF16) q_scale(col_max(m), f, kf);
 #pragma unroll
@@ -707,9 +728,9 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
 
     // ---- the lane's row and query operand.  Rows that do not see the whole prefix are left to the workgroups of their
     // sequences: here they get empty records.
-    const int row0 = tile * kPrefixRows + 32 * w, r = row0 + i, t0 = row0 / G, t = r / G;
+    const int row0 = tile * kPrefixRows + 32 * w, r = row0 + i, t0 = div_by(row0, a.by_G), t = div_by(r, a.by_G);
     bool found;
-    const int pos = position_of(a.B, t0, min((row0 + 31) / G, a.B.n_rows - 1) - t0 + 1, t - t0, found);
+    const int pos = position_of(a.B, t0, min(div_by(row0 + 31, a.by_G), a.B.n_rows - 1) - t0 + 1, t - t0, found);
     const int tok = found && r < nrows ? t : -1, head = kvh * G + r - t * G;
     const bool sees = tok >= 0 && pos + 1 >= a.prefix_len;
     u32x4 q[kKs][kParts];
