@@ -8,47 +8,84 @@ namespace cri {
 namespace dev {
 namespace {
 
-// One wave per (row, head): the records' maxima and sums weigh the accumulators.  Bound by the records' bytes.
+// The records of a (row, head) joined: their maxima and sums weigh the accumulators.  W waves share one (row, head), each
+// with a W-th of its records, and meet in LDS; 2^lg lanes hold a record's accumulators, the 64 >> lg groups of a wave's
+// lanes take records in turn.  Bound by the records' bytes.
+template <int W>
 __global__ __launch_bounds__(256) void paged_join_kernel(const float* __restrict__ rec, float* __restrict__ out, long ldo,
                                                          const int* __restrict__ offsets, int n_seqs, int n_rows, int H,
-                                                         int D, int lg, int nrec) {
-    const int lane = threadIdx.x & 63;
-    const int id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    const int t = id / H, h = id % H;
-    if (t >= n_rows || t < offsets[0] || t >= offsets[n_seqs]) return;  // rows of no sequence stay as they were
+                                                         FastDiv by_H, int D, int lg, int nrec) {
+    __shared__ float part[W > 1 ? W : 1][256 + 2];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = blockIdx.x * (4 / W) + w / W, mine = w % W;
+    const int t = div_by(id, by_H), h = id - t * H;
+    // rows of no sequence stay as they were
+    const bool on = t < n_rows && t >= offsets[0] && t < offsets[n_seqs];
+    if (W == 1 && !on) return;
     const float* r = rec + static_cast<long>(id) * nrec * (D + 4);
-    float m = -INFINITY, l = 0.0f;
-    if (lane < nrec) {
-        const f32x2 x = *reinterpret_cast<const f32x2*>(r + static_cast<long>(lane) * (D + 4));
-        m = x.x;
-        l = x.y;
-    }
-    const float mx = wave_max(m);
-    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
-    const float total = group_sum(l * f, 6);
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    // 2^lg lanes hold a record's accumulators, the wave's 64 >> lg groups of them take the records in turn
+    const int per = (nrec + W - 1) / W, lo = mine * per, hi = on ? min(lo + per, nrec) : lo;
     const int c = lane & ((1 << lg) - 1), grp = lane >> lg, groups = 64 >> lg;
+    float mx = -INFINITY, total = 0.0f;
     f32x4 x = {0, 0, 0, 0};
-    constexpr int kAhead = 4;  // records in flight
-    for (int k0 = 0; k0 < nrec; k0 += kAhead * groups) {
-        float wt[kAhead];
-        f32x4 y[kAhead];
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            const int k = k0 + j * groups + grp;
-            wt[j] = __shfl(f, min(k, nrec - 1));  // every lane takes part
-            if (k >= nrec || 4 * c >= D) wt[j] = 0.0f;
-            y[j] = f32x4{0, 0, 0, 0};
-            if (wt[j] != 0.0f)  // a record of weight 0 may hold nothing
-                y[j] = *reinterpret_cast<const f32x4*>(r + static_cast<long>(k) * (D + 4) + 4 + 4 * c);
+    for (int base = lo; base < hi; base += 64) {  // 64 records' maxima and sums at a time, one per lane
+        float m = -INFINITY, l = 0.0f;
+        if (base + lane < hi) {
+            const f32x2 v = *reinterpret_cast<const f32x2*>(r + static_cast<long>(base + lane) * (D + 4));
+            m = v.x;
+            l = v.y;
         }
+        const float top = fmaxf(mx, wave_max(m));
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        const float old = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - top);
+        mx = top;
+        total = total * old + group_sum(l * f, 6);
+        x *= old;
+        const int n = min(64, hi - base);
+        constexpr int kAhead = 4;  // records in flight
+        for (int k0 = 0; k0 < n; k0 += kAhead * groups) {
+            float wt[kAhead];
+            f32x4 y[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) x += y[j] * wt[j];
+            for (int j = 0; j < kAhead; ++j) {
+                const int k = k0 + j * groups + grp;
+                wt[j] = __shfl(f, min(k, 63));  // every lane takes part
+                if (k >= n || 4 * c >= D) wt[j] = 0.0f;
+                y[j] = f32x4{0, 0, 0, 0};
+                if (wt[j] != 0.0f)  // a record of weight 0 may hold nothing
+                    y[j] = *reinterpret_cast<const f32x4*>(r + static_cast<long>(base + k) * (D + 4) + 4 + 4 * c);
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) x += y[j] * wt[j];
+        }
     }
     for (int m = 1 << lg; m < 64; m <<= 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], m);
+    if (W > 1) {
+        float* p = part[w];
+        if (grp == 0 && 4 * c < D) *reinterpret_cast<f32x4_a4*>(p + 4 * c) = f32x4_a4{x[0], x[1], x[2], x[3]};
+        if (lane == 0) {
+            p[256] = mx;
+            p[257] = total;
+        }
+        __syncthreads();
+        if (mine != 0 || !on) return;
+        float top = mx;
+#pragma unroll
+        for (int o = 1; o < W; ++o) top = fmaxf(top, part[w + o][256]);
+        const float own = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - top);
+        total *= own;
+        x *= own;
+#pragma unroll
+        for (int o = 1; o < W; ++o) {
+            const float m = part[w + o][256], f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+            total += part[w + o][257] * f;
+            if (grp == 0 && 4 * c < D)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] += part[w + o][4 * c + i] * f;
+        }
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     if (grp == 0 && 4 * c < D)
         *reinterpret_cast<f32x4_a4*>(out + t * ldo + static_cast<long>(h) * D + 4 * c) =
             f32x4_a4{x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
@@ -57,12 +94,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const float* __restrict
 // the cut of a call, from what the host knows of it
 struct Cut {
     bool even, staged;  // staged: the prefix goes to the kernel that shares it through LDS
-    int pre_wq, pre_tiles, pre_chunks, pre_per, pre_blocks, own_wq, own_tiles, own_chunks, own_per, nrec;
-    long own_blocks;
+    int pre_tiles, pre_chunks, pre_per, pre_blocks, own_more, own_chunks, own_per, nrec;
+    long own_first, own_blocks;
 };
 
-constexpr int kMaxRecords = 64;  // the joining wave keeps one record's maximum per lane
-constexpr int kSlots = 512;      // workgroups on the GPU at a time: two per CU
+constexpr int kPreRecords = 64, kOwnRecords = 192;  // chunks at most
+constexpr int kSlots = 512;                         // workgroups on the GPU at a time: two per CU
 
 int round_up(int x, int to) { return (x + to - 1) / to * to; }
 
@@ -70,48 +107,46 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
     Cut c{};
     const int D = P.head_dim, G = n_heads / P.n_kv_heads;
     c.even = (D == 64 || D == 128 || D == 256) && P.page_size % 16 == 0;
-    const long rows = static_cast<long>(B.n_rows) * G;   // of a KV head
-    const long mean = (rows + B.n_seqs - 1) / B.n_seqs;  // of a KV head and sequence
+    const long rows = static_cast<long>(B.n_rows) * G;  // of a KV head
     c.staged = c.even && type != kKvF32 && D <= 128 && rows > 64 && prefix_len >= 256;
     const int tile = type == kKvF32 ? 16 : 32;
-    constexpr int block = 16;  // rows of a wave
-    auto waves_of = [&](long r) { return r <= block ? 1 : r <= 2 * block ? 2 : 4; };
-    c.pre_wq = waves_of(rows);
-    c.own_wq = waves_of(mean);
     if (prefix_len > 0) {
-        const int tile_rows = c.staged ? kPrefixRows : block * c.pre_wq;
-        const int unit = c.staged ? kPrefixTile : tile * (kPagedWaves / c.pre_wq);
+        const int tile_rows = c.staged ? kPrefixRows : 16;
+        const int units = (prefix_len + tile - 1) / tile;
         c.pre_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
         const long streams = static_cast<long>(P.n_kv_heads) * c.pre_tiles;
-        const int units = (prefix_len + unit - 1) / unit;
-        // chunks: rounds of workgroups times units of each (a workgroup that has its CU to itself takes two thirds of the
-        // time), five units for a workgroup's start and end, a sixtieth for each one's records
+        // Chunks: rounds of items times the position tiles of each (a workgroup that has its CU to itself takes two thirds
+        // of the time per tile), five for an item's start and end, and its records: 128 rows' take a 60th of a tile's time
+        // when the whole GPU writes and reads them.
+        const int slots = c.staged ? kSlots : kPagedWaves * kSlots;
+        const double records = c.staged ? 1.0 / 60 : 1.0 / 480;
         double best = 0.0;
-        for (int n = 1; n <= kMaxRecords / 2 && n <= units; ++n) {
-            const long groups = streams * n, per = (units + n - 1) / n;
-            const double rounds = groups <= kSlots / 2 ? 0.65 : static_cast<double>((groups + kSlots - 1) / kSlots);
-            const double cost = rounds * per + 5.0 * ((groups + kSlots - 1) / kSlots) + groups / 60.0;
+        for (int n = 1; n <= kPreRecords && n <= units; ++n) {
+            const long items = streams * n, per = (units + n - 1) / n;
+            const double rounds = items <= slots / 2 ? 0.65 : static_cast<double>((items + slots - 1) / slots);
+            const double cost = rounds * per + 5.0 * ((items + slots - 1) / slots) + items * records;
             if (best == 0.0 || cost < best) {
                 best = cost;
-                c.pre_per = static_cast<int>(per * unit);
+                c.pre_per = static_cast<int>(per * tile);
             }
         }
         c.pre_chunks = (prefix_len + c.pre_per - 1) / c.pre_per;
-        c.pre_blocks = static_cast<int>((streams * c.pre_chunks + kPagedXcds - 1) / kPagedXcds * kPagedXcds);
+        const long groups = c.staged ? streams * c.pre_chunks : (streams * c.pre_chunks + kPagedWaves - 1) / kPagedWaves;
+        c.pre_blocks = static_cast<int>((groups + kPagedXcds - 1) / kPagedXcds * kPagedXcds);
     }
-    // a sequence's own positions: chunks of one size, so that a long sequence has more of them and none is waited for;
-    // 512 positions, or less where the batch would leave CUs idle
+    // A sequence's own positions: chunks of one size, so that a long sequence has more of them and none is waited for; 256
+    // positions, or less where the batch would leave waves idle.
     const long cap = static_cast<long>(B.max_pages) * P.page_size;
     const long own = std::max(cap - prefix_len / tile * tile, 1L);
-    const int rt = block * c.own_wq, unit = tile * (kPagedWaves / c.own_wq);
-    // sum of ceil(n G / rt) over the sequences that have rows: n G is a multiple of gcd(G, rt)
-    c.own_tiles = static_cast<int>((rows + std::min<long>(B.n_seqs, B.n_rows) * (rt - std::gcd(G, rt))) / rt);
-    const long streams = static_cast<long>(P.n_kv_heads) * c.own_tiles;
-    const long fill = own * streams / kSlots;  // positions per workgroup that fill the GPU once
-    const long least = (own + kMaxRecords / 2 - 1) / (kMaxRecords / 2);
-    c.own_per = round_up(static_cast<int>(std::max({std::min(fill, 512L), least, 1L})), 2 * unit);
+    // sum of ceil(n G / 16) - 1 over the sequences that have rows: n G is a multiple of gcd(G, 16)
+    c.own_more = static_cast<int>((rows - std::gcd(G, 16)) / 16);
+    const long streams = static_cast<long>(P.n_kv_heads) * std::min<long>(B.n_seqs + c.own_more, (rows + 15) / 16 + B.n_seqs);
+    const long fill = own * streams / (kPagedWaves * kSlots);  // positions of a wave that fill the GPU once
+    const long least = (own + kOwnRecords - 1) / kOwnRecords;
+    c.own_per = round_up(static_cast<int>(std::max({std::min(fill, 256L), least, 1L})), tile);
     c.own_chunks = static_cast<int>((own + c.own_per - 1) / c.own_per);
-    c.own_blocks = static_cast<long>(c.own_tiles) * c.own_chunks * P.n_kv_heads;
+    c.own_first = static_cast<long>(c.own_chunks) * B.n_seqs * P.n_kv_heads;
+    c.own_blocks = (c.own_first + static_cast<long>(c.own_chunks) * c.own_more * P.n_kv_heads + kPagedWaves - 1) / kPagedWaves;
     c.nrec = c.pre_chunks + c.own_chunks;
     return c;
 }
@@ -135,11 +170,13 @@ int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, cons
     a.P = P, a.B = B;
     a.prefix_pages = prefix_pages, a.prefix_len = prefix_len;
     a.H = n_heads, a.G = n_heads / P.n_kv_heads, a.nrec = c.nrec;
-    a.pre_wq = c.pre_wq, a.pre_tiles = c.pre_tiles, a.pre_chunks = c.pre_chunks, a.pre_per = c.pre_per;
-    a.pre_blocks = c.pre_blocks;
-    a.own_wq = c.own_wq, a.own_tiles = c.own_tiles, a.own_chunks = c.own_chunks, a.own_per = c.own_per;
+    if (c.pre_blocks + c.own_blocks > 0x7FFFFFFFL / 4) return kDeclined;
+    a.pre_tiles = c.pre_tiles, a.pre_chunks = c.pre_chunks, a.pre_per = c.pre_per, a.pre_blocks = c.pre_blocks;
+    a.own_more = c.own_more, a.own_chunks = c.own_chunks, a.own_per = c.own_per;
+    a.own_first = static_cast<int>(c.own_first);
     a.by_G = dev::fast_div(a.G), a.by_Hkv = dev::fast_div(P.n_kv_heads);
-    a.by_pre_tiles = dev::fast_div(std::max(c.pre_tiles, 1)), a.by_own_tiles = dev::fast_div(std::max(c.own_tiles, 1));
+    a.by_pre_tiles = dev::fast_div(std::max(c.pre_tiles, 1)), a.by_seqs = dev::fast_div(B.n_seqs);
+    a.by_more = dev::fast_div(std::max(c.own_more, 1));
     a.qscale = scale * 1.44269504088896340736f;
     a.staged = c.staged;
     if (c.staged) {
@@ -147,17 +184,20 @@ int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, cons
         a.pre_blocks = 0;
     }
     const long blocks = a.pre_blocks + c.own_blocks;
-    if (blocks > 0x7FFFFFFFL) return kDeclined;
     const auto run = type == kKvF32   ? dev::run_paged_attn_f32
                      : type == kKvF16 ? dev::run_paged_attn_f16
                                       : dev::run_paged_attn_bf16;
     run(a, c.even, static_cast<int>(blocks), stream);
     if (c.nrec > 1) {
-        const long waves = static_cast<long>(B.n_rows) * n_heads;
+        const long pairs = static_cast<long>(B.n_rows) * n_heads;
         int lg = 0;
         while ((4 << lg) < P.head_dim) ++lg;
-        hipLaunchKernelGGL(dev::paged_join_kernel, dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, stream, ws,
-                           out, ldo, B.offsets, B.n_seqs, B.n_rows, n_heads, P.head_dim, lg, c.nrec);
+        // few pairs of many records: four waves to each, or a wave reads them one after the other
+        const bool shared = pairs <= 2048 && c.nrec > 16;
+        const auto join = shared ? dev::paged_join_kernel<4> : dev::paged_join_kernel<1>;
+        const long groups = shared ? pairs : (pairs + 3) / 4;
+        hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, stream, ws, out, ldo, B.offsets, B.n_seqs,
+                           B.n_rows, n_heads, dev::fast_div(n_heads), P.head_dim, lg, c.nrec);
     }
     return 0;
 }

@@ -49,9 +49,11 @@ struct PagedAttnArgs {
     PageBatch B;
     const int* prefix_pages;
     int prefix_len, H, G, nrec;
-    int pre_wq, pre_tiles, pre_chunks, pre_per, pre_blocks;  // the prefix's workgroups: [chunk][KV head][tile] by XCD
-    int own_wq, own_tiles, own_chunks, own_per;              // the sequences': [chunk][tile][KV head]: long ones first
-    FastDiv by_G, by_Hkv, by_pre_tiles, by_own_tiles;
+    // work of the prefix, by XCD: [chunk][KV head][row tile], an item per workgroup (staged) or wave; and of the
+    // sequences, an item per wave: their first row tiles [chunk][sequence][KV head], then the others [chunk][KV head][tile]
+    int pre_tiles, pre_chunks, pre_per, pre_blocks;
+    int own_more, own_chunks, own_per, own_first;  // own_first: items of first tiles, own_more: other tiles at most
+    FastDiv by_G, by_Hkv, by_pre_tiles, by_seqs, by_more;
     float qscale;  // scale * log2 e: scores are in base 2
     bool staged;   // the prefix went to paged_prefix_kernel
 };
@@ -180,16 +182,17 @@ __device__ __forceinline__ int position_of(const PageBatch& B, int t0, int n, in
     return -1;
 }
 
-// the prefix's work of this workgroup: consecutive items (the row tiles of one chunk and KV head, which read the same
-// K and V) go to one XCD and its L2
-__device__ __forceinline__ bool prefix_item(const PagedAttnArgs& a, int b, int Hkv, int& chunk, int& kvh, int& tile) {
-    const int wi = b % kPagedXcds * (a.pre_blocks / kPagedXcds) + b / kPagedXcds;
-    const int stream = div_by(wi, a.by_pre_tiles);
-    tile = wi - stream * a.pre_tiles;
+// Work item i of the prefix.  The caller's items are consecutive on an XCD, so the row tiles of one chunk and KV head,
+// which read the same K and V, meet in its L2.
+__device__ __forceinline__ bool prefix_item(const PagedAttnArgs& a, int i, int Hkv, int& chunk, int& kvh, int& tile) {
+    const int stream = div_by(i, a.by_pre_tiles);
+    tile = i - stream * a.pre_tiles;
     chunk = div_by(stream, a.by_Hkv);
     kvh = stream - chunk * Hkv;
     return chunk < a.pre_chunks;
 }
+// workgroup b of n in the order of the XCDs that get them: b mod 8's first, n a multiple of 8
+__device__ __forceinline__ int by_xcd(int b, int n) { return b % kPagedXcds * (n / kPagedXcds) + b / kPagedXcds; }
 
 // EVEN: head_dim is DP and the page size a multiple of 16, so the 16 positions of a tile's row block lie in one page
 template <int TYPE, int DP, bool EVEN>
@@ -199,7 +202,6 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
     typedef std::integral_constant<int, TYPE> Type;
     constexpr int kTile = S::kTile, kT = S::kT, kKs = S::kKs, kVe = S::kVe, kNh = S::kNh, kAcc = S::kAcc;
     constexpr int kEs = sizeof(elem), kNs = 4 * kT;  // scores of a lane
-    extern __shared__ __attribute__((aligned(16))) float lds[];  // the waves' records
 
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -209,17 +211,16 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
     const int cap = a.B.max_pages * a.P.page_size;
     const UniformInts offsets = uniform(a.B.offsets), lens = uniform(a.B.lens);
 
-    // ---- what this workgroup does: a KV head, a tile of rows, a range of positions
+    // ---- what this wave does: a KV head, 16 rows, a range of positions
     const bool prefix = static_cast<int>(blockIdx.x) < a.pre_blocks;
-    int kvh, wq, row0, nrows, tok0, pos0 = 0, rec_at, own_lo, own_hi;
+    int kvh, row0, nrows, tok0, pos0 = 0, rec_at, own_lo, own_hi;
     UniformInts own_table;
     int own_len, before_lo = 0, before_hi = 0;  // (before: the prefix's positions for rows that do not see all of it)
     const int prefix_pages = (a.prefix_len + a.P.page_size - 1) / a.P.page_size;
     if (prefix) {
         int chunk, tile;
-        if (!prefix_item(a, blockIdx.x, Hkv, chunk, kvh, tile)) return;
-        wq = a.pre_wq;
-        row0 = tile * 16 * wq;
+        if (!prefix_item(a, 4 * by_xcd(blockIdx.x, a.pre_blocks) + w, Hkv, chunk, kvh, tile)) return;
+        row0 = tile * 16;
         nrows = a.B.n_rows * G;
         tok0 = 0;
         rec_at = chunk;
@@ -228,32 +229,41 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
         own_table = uniform(a.prefix_pages);
         own_len = prefix_pages;
     } else {
-        const int b = static_cast<int>(blockIdx.x) - a.pre_blocks, rest = div_by(b, a.by_Hkv);
-        kvh = b - rest * Hkv;
-        const int chunk = div_by(rest, a.by_own_tiles);
-        int tile = rest - chunk * a.own_tiles;
-        wq = a.own_wq;
-        // the tile-th tile of rows of the batch: 64 sequences' tile counts summed at a time
-        const int rt = 16 * wq;
-        int seq = -1;
-        for (int base = 0; base < a.B.n_seqs; base += 64) {
-            const int i = base + lane;
-            int n = 0;
-            if (i < a.B.n_seqs) n = min(max(a.B.offsets[i + 1] - a.B.offsets[i], 0), a.B.n_rows);
-            const int sum = wave_scan_i((n * G + rt - 1) / rt);
-            const int before = __popcll(__ballot(sum <= tile));
-            if (before < 64) {
-                seq = base + before;
-                if (before > 0) tile -= __builtin_amdgcn_readlane(sum, before - 1);
-                break;
+        int item = 4 * (static_cast<int>(blockIdx.x) - a.pre_blocks) + w, chunk, seq, tile = 0;
+        if (item < a.own_first) {
+            const int rest = div_by(item, a.by_Hkv);
+            kvh = item - rest * Hkv;
+            chunk = div_by(rest, a.by_seqs);
+            seq = rest - chunk * a.B.n_seqs;
+        } else {
+            item -= a.own_first;
+            const int rest = div_by(item, a.by_more);
+            int more = item - rest * a.own_more;
+            chunk = div_by(rest, a.by_Hkv);
+            kvh = rest - chunk * Hkv;
+            if (chunk >= a.own_chunks) return;
+            // the more-th of the tiles behind the sequences' first ones: 64 sequences' counts summed at a time
+            seq = -1;
+            for (int base = 0; base < a.B.n_seqs; base += 64) {
+                const int i = base + lane;
+                int n = 0;
+                if (i < a.B.n_seqs) n = min(max(a.B.offsets[i + 1] - a.B.offsets[i], 0), a.B.n_rows);
+                const int tiles = max((n * G + 15) / 16 - 1, 0), sum = wave_scan_i(tiles);
+                const int before = __popcll(__ballot(sum <= more));
+                if (before < 64) {
+                    seq = base + before;
+                    tile = 1 + more - (before > 0 ? __builtin_amdgcn_readlane(sum, before - 1) : 0);
+                    break;
+                }
+                more -= __builtin_amdgcn_readlane(sum, 63);
             }
-            tile -= __builtin_amdgcn_readlane(sum, 63);
+            if (seq < 0 || seq >= a.B.n_seqs) return;
         }
-        if (seq < 0 || seq >= a.B.n_seqs) return;
         tok0 = offsets[seq];
         const int n = min(max(offsets[seq + 1] - tok0, 0), a.B.n_rows);
+        if (n == 0) return;
         const int len = lens[seq];
-        row0 = tile * rt;
+        row0 = tile * 16;
         nrows = n * G;
         pos0 = len - n;  // position of the sequence's first row
         rec_at = a.pre_chunks + chunk;
@@ -270,18 +280,16 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
             before_hi = min(before_lo + per, hi);
         }
     }
-    const int wk = kPagedWaves / wq;  // waves that share rows and split positions
-    const int wrow = row0 + w / wk * 16, wpos = w % wk;
 
     // ---- the lane's column: its row, the positions up to and with the row's own, its query operand
     int tok = -1, head = 0, sees = 0;
     {
-        const int r = wrow + c, i0 = div_by(wrow, a.by_G), i = div_by(r, a.by_G), t = tok0 + i;
+        const int r = row0 + c, i0 = div_by(row0, a.by_G), i = div_by(r, a.by_G), t = tok0 + i;
         bool ok = r < nrows && t >= 0 && t < a.B.n_rows;
         int p = pos0 + i;
         if (prefix) {
             bool found;
-            p = position_of(a.B, i0, min(div_by(wrow + 15, a.by_G), a.B.n_rows - 1) - i0 + 1, i - i0, found);
+            p = position_of(a.B, i0, min(div_by(row0 + 15, a.by_G), a.B.n_rows - 1) - i0 + 1, i - i0, found);
             ok = ok && found;
         }
         if (ok) {
@@ -291,7 +299,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
         }
     }
     if (own_lo >= own_hi && before_lo >= before_hi && a.nrec > 1) {  // no positions: an empty record
-        if (wpos == 0 && g == 0 && tok >= 0)
+        if (g == 0 && tok >= 0)
             *reinterpret_cast<f32x2*>(a.rec + ((static_cast<long>(tok) * a.H + head) * a.nrec + rec_at) * (D + 4)) =
                 f32x2{-INFINITY, 0.0f};
         return;
@@ -329,8 +337,8 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
               : part    ? min(sees, cap)
                         : sees < a.prefix_len ? sees : 0;
         least = -row_max_i(-lim);
-        first = p_lo / kTile + wpos;
-        last = (min(p_hi, row_max_i(tok < 0 ? 0 : lim)) + kTile - 1) / kTile;  // tiles [first, last) in steps of wk
+        first = p_lo / kTile;
+        last = (min(p_hi, row_max_i(tok < 0 ? 0 : lim)) + kTile - 1) / kTile;  // tiles [first, last)
     };
     auto page_at = [&](int pi) {
         const int pg = table[min(pi, table_len - 1)];
@@ -436,7 +444,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
 #pragma unroll 1
     for (;;) {
 #pragma unroll 1
-        for (int tile = first; tile < last; tile += wk) {
+        for (int tile = first; tile < last; ++tile) {
             const int p0 = tile * kTile;
             float s[kNs];
 #pragma unroll
@@ -458,8 +466,8 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[4 * t + i] = x[i] * kf;
             }
-            const int next = p0 + wk * kTile;
-            const bool more = tile + wk < last;
+            const int next = p0 + kTile;
+            const bool more = tile + 1 < last;
             if (more) {  // the next tile's keys, in flight during the softmax and the second product
                 if constexpr (EVEN) {
 #pragma unroll
@@ -561,85 +569,33 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
         if (first < last) load_tile(first);
     }
 
-    // ---- the waves of a column meet in LDS, each takes a share of its dims
+    // ---- the record, or the output
     sum = col_sum(sum);
     if (sum != sum) mx = INFINITY;  // NaN scores leave no maximum: keep the record from being skipped
-    auto dim_of = [&](int h, int i) { return 16 * kVe * h + kVe * (4 * g + i); };  // of acc[h kVe ..][i]
-    float* dst = nullptr;
-    if (tok >= 0)
-        dst = a.nrec == 1 ? a.out + tok * a.ldo + static_cast<long>(head) * D
-                          : a.rec + ((static_cast<long>(tok) * a.H + head) * a.nrec + rec_at) * (D + 4);
-    if (wk == 1) {
-        if (tok < 0) return;
-        float f = 1.0f;
-        if (a.nrec == 1) {
-            f = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing: zeros
-        } else {
-            if (g == 0) *reinterpret_cast<f32x2*>(dst) = f32x2{mx, sum};
-            dst += 4;
-            if (mx == -INFINITY) return;
-        }
-#pragma unroll
-        for (int h = 0; h < kNh; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < kVe; e += 4) {
-                    const int d = dim_of(h, i) + e;
-                    if (EVEN || d < D)
-                        *reinterpret_cast<f32x4_a4*>(dst + d) = f32x4_a4{acc[h * kVe + e][i] * f, acc[h * kVe + e + 1][i] * f,
-                                                                         acc[h * kVe + e + 2][i] * f,
-                                                                         acc[h * kVe + e + 3][i] * f};
-                }
-        return;
-    }
-    constexpr int kRowF = DP + 4;  // floats of a column's record; the row stride spreads the banks
-    float* const mine = lds + w * 16 * kRowF;
-    if (g == 0) {
-        mine[c * kRowF + DP] = mx;
-        mine[c * kRowF + DP + 1] = sum;
-    }
-    if (mx != -INFINITY) {
-#pragma unroll
-        for (int h = 0; h < kNh; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < kVe; e += 4)
-                    *reinterpret_cast<f32x4*>(mine + c * kRowF + dim_of(h, i) + e) =
-                        f32x4{acc[h * kVe + e][i], acc[h * kVe + e + 1][i], acc[h * kVe + e + 2][i],
-                              acc[h * kVe + e + 3][i]};
-    }
-    __syncthreads();
     if (tok < 0) return;
-    const float* const rec = lds + w / wk * wk * 16 * kRowF + c * kRowF;  // of the column's first wave
-    float top = -INFINITY;
-    for (int o = 0; o < wk; ++o) top = fmaxf(top, rec[o * 16 * kRowF + DP]);
-    float total = 0.0f, f[kPagedWaves];
-#pragma unroll
-    for (int o = 0; o < kPagedWaves; ++o) {
-        if (o >= wk) break;
-        const float m = rec[o * 16 * kRowF + DP];
-        f[o] = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-        total += rec[o * 16 * kRowF + DP + 1] * f[o];
-    }
+    float* dst;
     float back = 1.0f;
     if (a.nrec == 1) {
-        back = total == 0.0f ? 0.0f : 1.0f / total;  // a row that sees nothing: zeros
+        dst = a.out + tok * a.ldo + static_cast<long>(head) * D;
+        back = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing: zeros
     } else {
-        if (g == 0 && wpos == 0) *reinterpret_cast<f32x2*>(dst) = f32x2{top, total};
+        dst = a.rec + ((static_cast<long>(tok) * a.H + head) * a.nrec + rec_at) * (D + 4);
+        if (g == 0) *reinterpret_cast<f32x2*>(dst) = f32x2{mx, sum};
         dst += 4;
-        if (top == -INFINITY) return;
+        if (mx == -INFINITY) return;
     }
-    for (int d = 4 * (4 * wpos + g); d < D; d += 16 * wk) {
-        f32x4 x = {0, 0, 0, 0};
 #pragma unroll
-        for (int o = 0; o < kPagedWaves; ++o) {
-            if (o >= wk) break;
-            if (f[o] != 0.0f) x += *reinterpret_cast<const f32x4*>(rec + o * 16 * kRowF + d) * f[o];
-        }
-        *reinterpret_cast<f32x4_a4*>(dst + d) = f32x4_a4{x[0] * back, x[1] * back, x[2] * back, x[3] * back};
-    }
+    for (int h = 0; h < kNh; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < kVe; e += 4) {
+                const int d = 16 * kVe * h + kVe * (4 * g + i) + e;  // of acc[h kVe + e ..][i]
+                if (EVEN || d < D)
+                    *reinterpret_cast<f32x4_a4*>(dst + d) =
+                        f32x4_a4{acc[h * kVe + e][i] * back, acc[h * kVe + e + 1][i] * back, acc[h * kVe + e + 2][i] * back,
+                                 acc[h * kVe + e + 3][i] * back};
+            }
 }
 
 // The shared prefix against many rows (16-bit caches, head_dim 64 and 128, pages of 16 n positions).  A workgroup of four
@@ -693,7 +649,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
     const int Hkv = a.P.n_kv_heads, G = a.G, nrows = a.B.n_rows * G;
     const uint32_t row_bytes = static_cast<uint32_t>(Hkv) * kRowB;
     int chunk, kvh, tile;
-    if (!prefix_item(a, blockIdx.x, Hkv, chunk, kvh, tile)) return;
+    if (!prefix_item(a, by_xcd(blockIdx.x, a.pre_blocks), Hkv, chunk, kvh, tile)) return;
     const int p_lo = chunk * a.pre_per, p_hi = min(p_lo + a.pre_per, a.prefix_len);
     const int ntiles = (p_hi - p_lo + kPrefixTile - 1) / kPrefixTile;
     const int table_len = (a.prefix_len + a.P.page_size - 1) / a.P.page_size;
@@ -863,8 +819,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
 
 template <int TYPE, int DP, bool EVEN>
 void run_paged_attn(const PagedAttnArgs& a, int blocks, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_attn_kernel<TYPE, DP, EVEN>), dim3(blocks), dim3(64 * kPagedWaves),
-                       kPagedWaves * 16 * (DP + 4) * 4, stream, a);
+    hipLaunchKernelGGL((paged_attn_kernel<TYPE, DP, EVEN>), dim3(blocks), dim3(64 * kPagedWaves), 0, stream, a);
 }
 
 template <int TYPE>

@@ -113,10 +113,33 @@ __device__ __forceinline__ Weight weight_of(const VerifyArgs& a, int first, int 
     return w;
 }
 
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {  // zero where the source lane is outside
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {  // of a uniform lane
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(u), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+// sums over the lanes up to and with each; prev: without the lane's own
+__device__ __forceinline__ double scan_up(double v, int lane, double& prev) {
+    v += dpp_f64<0x111>(v);  // row_shr 1, 2, 4, 8: within 16 lanes
+    v += dpp_f64<0x112>(v);
+    v += dpp_f64<0x114>(v);
+    v += dpp_f64<0x118>(v);
+    const double a = lane_f64(v, 15), b = a + lane_f64(v, 31), c = b + lane_f64(v, 47);
+    const double base = lane < 16 ? 0.0 : lane < 32 ? a : lane < 48 ? b : c;
+    prev = base + dpp_f64<0x111>(v);
+    return base + v;
+}
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-    return v;
+    double prev;
+    return lane_f64(scan_up(v, threadIdx.x & 63, prev), 63);
 }
 
 // grid (sequences x slices): the slice's sums
@@ -163,15 +186,6 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyArgs 
     }
 }
 
-__device__ __forceinline__ double scan_up(double c, int lane) {  // inclusive sums over the wave
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const double o = __shfl_up(c, m);
-        if (lane >= m) c += o;
-    }
-    return c;
-}
-
 // grid (sequences): the token, the sequence's output rows
 __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyArgs a) {
     __shared__ double part[kPickWaves];
@@ -204,16 +218,16 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
     for (int base = 0; base < a.slices; base += 64) {
         const int i = base + lane;
         const double x = i < a.slices ? sums[2 * i + which] : 0.0;
-        const double c = scan_up(x, lane), prev = __shfl_up(c, 1);
-        const double at = lane ? run + prev : run;
+        double prev;
+        const double c = scan_up(x, lane, prev), at = run + prev;
         const unsigned long hit = __ballot(x > 0.0 && run + c > want), any = __ballot(x > 0.0);
         if (any != 0) {
             const int pick = hit ? __builtin_ctzl(hit) : 63 - __builtin_clzl(any);
             slice = base + pick;
-            before = __shfl(at, pick);
+            before = lane_f64(at, pick);
         }
         if (hit != 0) break;
-        run += __shfl(c, 63);
+        run += lane_f64(c, 63);
     }
     int token = -1;  // no weight anywhere
     if (slice >= 0) {
@@ -229,9 +243,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
                 sum += x[j + i];
             }
         }
-        const double c = scan_up(sum, lane);
-        double prev = __shfl_up(c, 1);
-        if (lane == 0) prev = 0.0;
+        double prev;
+        const double c = scan_up(sum, lane, prev);
         if (lane == 63) part[wave] = c;
         __syncthreads();
         double base = before;
@@ -249,8 +262,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
                 done = at > want;
             }
         }
-        const int hit_token = __shfl(mine, hit ? __builtin_ctzl(hit) : 0);
-        const int any_token = __shfl(mine, any ? 63 - __builtin_clzl(any) : 0);
+        const int hit_token = __builtin_amdgcn_readlane(mine, hit ? __builtin_ctzl(hit) : 0);
+        const int any_token = __builtin_amdgcn_readlane(mine, any ? 63 - __builtin_clzl(any) : 0);
         if (lane == 0) {
             found[wave] = hit ? hit_token : -1;
             last[wave] = any ? any_token : -1;
