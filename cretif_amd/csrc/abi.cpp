@@ -639,6 +639,7 @@ int kv_type(int type) {
 
 constexpr int kMaxPagedHeadDim = 256;
 constexpr long kMaxPositions = 1L << 30;
+constexpr int kMaxRows = 1 << 23;  // a workgroup of 256 threads each: half of what a launch takes
 
 int check_rotation(const cri_rotation* rot, int head_dim, cri::HeadRotation* out, const char* fn) {
     if (!rot) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null rotation");
@@ -717,6 +718,12 @@ bool rows_overlap(const float* a, long wa, long lda, const float* b, long wb, lo
     return true;
 }
 
+bool in_pool(const cri::PagePool& pool, int type, const void* p, long bytes) {
+    const long size = ((pool.n_pages - 1) * pool.stride + static_cast<long>(pool.page_size) * pool.n_kv_heads * pool.head_dim) *
+                      (type == cri::kKvF32 ? 4 : 2);
+    return overlaps(pool.k, size, p, bytes) || overlaps(pool.v, size, p, bytes);
+}
+
 int check_rows(const float* p, int ld, long width, const char* name, const char* fn) {
     if (!p) return fail(CRI_ERR_INVALID_ARGUMENT, fn, std::string("null ") + name);
     if (!aligned(p, 4)) return fail(CRI_ERR_ALIGNMENT, fn, std::string(name) + " must be 4-byte aligned");
@@ -745,7 +752,7 @@ int cri_qk_norm_rope(const cri_rotation* rot, const float* q, int ldq, const flo
     if (n_heads > 0 && ((st = check_rows(q, ldq, wq, "q", fn)) || (st = check_rows(q_out, ldq_out, wq, "q_out", fn)))) return st;
     if (n_kv_heads > 0 && ((st = check_rows(k, ldk, wk, "k", fn)) || (st = check_rows(k_out, ldk_out, wk, "k_out", fn))))
         return st;
-    if (static_cast<long>(M) * std::max({ldq, ldk, ldq_out, ldk_out}) > kMaxElems)
+    if (M > kMaxRows || static_cast<long>(M) * std::max({ldq, ldk, ldq_out, ldk_out}) > kMaxElems)
         return fail(CRI_ERR_SHAPE, fn, "problem too large");
     const bool same_q = q == q_out && ldq == ldq_out, same_k = k == k_out && ldk == ldk_out;
     if ((n_heads > 0 && !same_q && rows_overlap(q, wq, ldq, q_out, wq, ldq_out, M)) ||
@@ -778,12 +785,16 @@ int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const
     const long wq = q ? static_cast<long>(n_heads) * pool.head_dim : 0;
     if ((st = check_rows(k, ldk, wk, "k", fn)) || (st = check_rows(v, ldv, wk, "v", fn))) return st;
     if (wq > 0 && ((st = check_rows(q, ldq, wq, "q", fn)) || (st = check_rows(q_out, ldq_out, wq, "q_out", fn)))) return st;
-    if (static_cast<long>(b.n_rows) * std::max({wq > 0 ? std::max(ldq, ldq_out) : 0, ldk, ldv}) > kMaxElems)
+    if (b.n_rows > kMaxRows || static_cast<long>(b.n_rows) * std::max({wq > 0 ? std::max(ldq, ldq_out) : 0, ldk, ldv}) > kMaxElems)
         return fail(CRI_ERR_SHAPE, fn, "problem too large");
     if (wq > 0 && ((!(q == q_out && ldq == ldq_out) && rows_overlap(q, wq, ldq, q_out, wq, ldq_out, b.n_rows)) ||
                    rows_overlap(k, wk, ldk, q_out, wq, ldq_out, b.n_rows) ||
                    rows_overlap(v, wk, ldv, q_out, wq, ldq_out, b.n_rows)))
         return fail(CRI_ERR_INVALID_ARGUMENT, fn, "q_out overlaps another buffer");
+    if (in_pool(pool, type, k, span_bytes(b.n_rows, wk, ldk)) || in_pool(pool, type, v, span_bytes(b.n_rows, wk, ldv)) ||
+        (wq > 0 && (in_pool(pool, type, q, span_bytes(b.n_rows, wq, ldq)) ||
+                    in_pool(pool, type, q_out, span_bytes(b.n_rows, wq, ldq_out)))))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "the pool overlaps q, k, v or q_out");
     clear_pending_error();
     if (cri::detail::launch_paged_append(pool, type, b, R, wq > 0 ? q : nullptr, ldq, q_out, ldq_out, n_heads, k, ldk, v,
                                          ldv, s) != 0)
@@ -835,6 +846,9 @@ int cri_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, co
     if (static_cast<long>(b.n_rows) * std::max(ldq, ldo) > kMaxElems) return fail(CRI_ERR_SHAPE, fn, "problem too large");
     if (rows_overlap(q, w, ldq, out, w, ldo, b.n_rows))
         return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out overlaps q (other workgroups still read it)");
+    const long out_bytes = span_bytes(b.n_rows, w, ldo);
+    if (in_pool(pool, type, out, out_bytes)) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out overlaps the pool");
+    if (!std::isfinite(scale * 1.44269504f)) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "scale must be finite (and below 2^127)");
     const long need = cri::detail::paged_attention_workspace_bytes(pool, type, b, n_heads, prefix_len);
     if (need > 0) {
         if (!workspace) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null workspace");
@@ -843,10 +857,13 @@ int cri_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, co
             return fail(CRI_ERR_SHAPE, fn, "workspace of " + std::to_string(workspace_bytes) + " bytes, " +
                                                std::to_string(need) + " needed");
     }
+    if (overlaps(workspace, need, out, out_bytes) || overlaps(workspace, need, q, span_bytes(b.n_rows, w, ldq)) ||
+        in_pool(pool, type, workspace, need))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "the workspace overlaps q, out or the pool");
     clear_pending_error();
     if (cri::detail::launch_paged_attention(pool, type, b, prefix_pages, prefix_len, q, ldq, out, ldo, n_heads, scale,
                                             static_cast<float*>(workspace), s) != 0)
-        return fail(CRI_ERR_UNSUPPORTED, fn, "no kernel for this shape");
+        return fail(CRI_ERR_UNSUPPORTED, fn, "too many sequences x KV heads x chunks for one launch");
     return check_launch(fn);
 }
 

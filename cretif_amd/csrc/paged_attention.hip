@@ -170,7 +170,7 @@ int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, cons
     a.P = P, a.B = B;
     a.prefix_pages = prefix_pages, a.prefix_len = prefix_len;
     a.H = n_heads, a.G = n_heads / P.n_kv_heads, a.nrec = c.nrec;
-    if (c.pre_blocks + c.own_blocks > 0x7FFFFFFFL / 4) return kDeclined;
+    if (c.pre_blocks + c.own_blocks >= 1L << 24) return kDeclined;  // 256 threads each: a launch's limit
     a.pre_tiles = c.pre_tiles, a.pre_chunks = c.pre_chunks, a.pre_per = c.pre_per, a.pre_blocks = c.pre_blocks;
     a.own_more = c.own_more, a.own_chunks = c.own_chunks, a.own_per = c.own_per;
     a.own_first = static_cast<int>(c.own_first);

@@ -175,7 +175,7 @@ __device__ __forceinline__ int position_of(const PageBatch& B, int t0, int n, in
     }
     found = false;
     if (k < n && s < B.n_seqs) {
-        const int t = t0 + k, lo = B.offsets[s], hi = B.offsets[s + 1], len = B.lens[s];
+        const int t = t0 + k, lo = B.offsets[s], hi = B.offsets[s + 1], len = max(B.lens[s], 0);
         found = t >= lo && t < hi;
         return len - (hi - t);
     }
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
         tok0 = offsets[seq];
         const int n = min(max(offsets[seq + 1] - tok0, 0), a.B.n_rows);
         if (n == 0) return;
-        const int len = lens[seq];
+        const int len = max(lens[seq], 0);
         row0 = tile * 16;
         nrows = n * G;
         pos0 = len - n;  // position of the sequence's first row
@@ -718,6 +718,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
         }
     }
 
+    const bool active = __ballot(sees) != 0;  // (a wave without rows copies and waits with the others)
     f32x16 o[kDb];
 #pragma unroll
     for (int d = 0; d < kDb; ++d)
@@ -761,6 +762,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
                 *reinterpret_cast<u32x4*>(ring + (kRing + tl % kRing) * kTileB + left * kRowB + 16 * x) = u32x4{0, 0, 0, 0};
             __syncthreads();
         }
+        if (!active) continue;
         f32x16 s;
         scores(tl, s);
         const float m = largest(tl, s);

@@ -299,7 +299,7 @@ int launch_verify_drafts(const float* target, long ldt, const float* draft, long
                          const float* draws, const int* offsets, int n_seqs, int n_rows, int vocab, int* out, int* accepted,
                          double* ws, hipStream_t stream) {
     const int per = dev::slice_of(n_seqs, vocab), slices = (vocab - 1) / per + 1;
-    if (static_cast<long>(n_seqs) * slices > 0x7FFFFFFFL) return kDeclined;
+    if (static_cast<long>(n_seqs) * slices >= 1L << 24) return kDeclined;  // 256 threads each: a launch's limit
     const dev::VerifyArgs a{target, draft, ldt, ldd, ids, u, draws, offsets, out, accepted, ws,
                             reinterpret_cast<int*>(ws + 2L * n_seqs * slices), n_seqs, n_rows, vocab, slices, per};
     hipLaunchKernelGGL(dev::verify_sums_kernel, dim3(static_cast<unsigned>(n_seqs) * slices), dim3(dev::kThreads), 0, stream, a);

@@ -413,13 +413,13 @@ int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const
  * through prefix_pages (device [ceil(prefix_len / page_size)]) instead of the sequence's own table:
  * a prefix that all sequences share, whose K and V are read once for the batch (its last page may
  * be partly filled; the sequences' own positions start at prefix_len of their own tables).
- * prefix_len 0: every position through its sequence's table.  A row at a position below 0 sees
- * nothing and gets zeros; positions past the table (max_pages * page_size) are not seen.  Nothing
+ * prefix_len 0: every position through its sequence's table.  A row at a position below 0 (a
+ * negative lens counts as 0) sees nothing and gets zeros; positions past the table (max_pages * page_size) are not seen.  Nothing
  * behind a row's last position reaches it, whatever its pages hold there.  Table entries of positions
  * that rows see must be inside the pool (others give unspecified numbers in their sequence's rows).
  *
  * q rows are ldq floats apart, out rows ldo; out must not overlap q or the pool.  n_heads a multiple
- * of n_kv_heads.  q, out 4-byte aligned, workspace 16-byte, cri_paged_attention_workspace_bytes of
+ * of n_kv_heads; scale finite.  q, out 4-byte aligned, workspace 16-byte, cri_paged_attention_workspace_bytes of
  * it (the same kv, batch and prefix_len; only their host numbers count, so the bytes of a batch's
  * n_seqs, n_rows and max_pages serve every step of it).  Sums, maxima and products are in fp32
  * accuracy for every cache type; the order of sums is fixed by the host numbers. */

@@ -169,6 +169,35 @@ def test_append(kind, counts, past, ps, H, Hkv, D, rot, halves, norm, mixed):
     assert torch.equal(pool.k, pk) and torch.equal(pool.v, pv)
 
 
+def test_lens_out_of_range():
+    """Lengths of no meaning touch nothing: far below 0, below the rows."""
+    ps, Hkv, D, H = 16, 2, 64, 4
+    pool = Pool(4, ps, Hkv, D, "fp16")
+    k0, v0 = pool.k.clone(), pool.v.clone()
+    counts, held, rows = [1, 2, 1], [-2 ** 31, -5, -2 ** 31 + 1], [[0, 1], [2, 3], [1, 2]]
+    b = cri.PagedBatch(ints(starts(counts)), ints(held), ints(rows))
+    q, kv, q_out = randn(4, H * D), randn(4, Hkv * D, seed=1), torch.full((4, H * D), 7.0, device="cuda")
+    cri.paged_append(pool.kv, b, cri.Rotation(1e4, 64), kv, kv, q, q_out, H)
+    assert torch.equal(pool.k, k0) and torch.equal(pool.v, v0) and (q_out == 7).all()
+    for P in (0, 20):
+        out = torch.full((4, H * D), 7.0, device="cuda")
+        cri.paged_attention(pool.kv, b, q, out, H, 0.125, ints([3, 0]), P)
+        assert (out == 0).all()
+
+
+def test_in_place_on_the_fused_rows():
+    """q and k normed and rotated where the fused product left them; the values beside them untouched."""
+    M, H, Hkv, D = 5, 4, 2, 64
+    qkv = randn(M, (H + 2 * Hkv) * D, seed=8)
+    src = qkv.clone()
+    q, k = qkv[:, :H * D], qkv[:, H * D:(H + Hkv) * D]
+    pos = [5, 900, 17, 0, 3]
+    cri.qk_norm_rope(cri.Rotation(1e4, D, "halves"), q, k, q, k, ints(pos), H, Hkv, D)
+    check_rotated(q, src[:, :H * D], None, pos, D, True, 1e4, D)
+    check_rotated(k, src[:, H * D:(H + Hkv) * D], None, pos, D, True, 1e4, D)
+    assert torch.equal(qkv[:, (H + Hkv) * D:], src[:, (H + Hkv) * D:])
+
+
 def test_append_leaves_out_what_has_no_page():
     """Positions below 0 and past the table, page numbers outside the pool: those rows leave no trace."""
     ps, Hkv, D, H = 4, 1, 64, 2
@@ -275,6 +304,96 @@ def test_attention(kind, shape):
     assert torch.equal(out, again)  # sums in a fixed order
 
 
+# more than 64 rows of a KV head on a prefix from 256 positions on: with 16-bit caches, heads of 64 and 128 and pages of
+# 16 n positions the prefix is shared through LDS (fp32, other heads and pages: waves of their own)
+MANY = [
+    # counts, own, P, ps, H, Hkv, D
+    ([1] * 33, [1 + 7 * i for i in range(33)], 256, 16, 4, 1, 64),         # a few rows, one tile, a whole number of tiles
+    ([1] * 70, [1 + i % 40 for i in range(70)], 1000, 16, 8, 4, 128),      # ends inside a page and a tile
+    ([3, 0, 5, 1] * 9, [3, 2, 50, 700] * 9, 481, 32, 8, 1, 128),           # 648 rows, ragged, sequences without any
+    ([2] * 100, [2 + i for i in range(100)], 289, 64, 3, 3, 64),           # one position past a tile
+    ([5] * 30, [5 + i for i in range(30)], 3000, 48, 10, 5, 64),           # many chunks
+    ([40, 90], [40, 300], 320, 16, 4, 1, 128),                             # pieces of prompts: rows of two sequences in a tile
+    ([1] * 40, [1 + i for i in range(40)], 300, 20, 8, 2, 128),            # pages of 20
+    ([1] * 40, [1 + i for i in range(40)], 300, 16, 8, 2, 256),
+]
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("shape", MANY, ids=[str(i) for i in range(len(MANY))])
+def test_many_rows_on_a_prefix(kind, shape):
+    counts, own, P, ps, H, Hkv, D = shape
+    pool, off, held, rows, prefix, q = case(kind, counts, own, P, ps, H, Hkv, D, ahead=2, behind=3)
+    bad = torch.ones(pool.k.shape[:2], dtype=torch.bool)  # what no position holds: never met, not even times zero
+    for s, n in enumerate(held):
+        for p in range(P, n):
+            bad[rows[s][p // ps], p % ps] = False
+    for p in range(P):
+        bad[prefix[p // ps], p % ps] = False
+    pool.k[bad.cuda()], pool.v[bad.cuda()] = float("nan"), float("inf")
+    out = attend(pool, off, held, rows, q, H, D ** -0.5, prefix, P)
+    want = ref.attention(q, pool.k, pool.v, off, held, rows, prefix, P, H, D ** -0.5, torch.full(q.shape, 7.0))
+    check_rows(out, want)
+    assert (out[:2] == 7).all() and (out[-3:] == 7).all()
+    assert torch.equal(attend(pool, off, held, rows, q, H, D ** -0.5, prefix, P), out)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_rows_some_inside_the_prefix(kind, D):
+    """Rows that do not see the whole prefix, rows that see nothing and rows past their table, beside ordinary ones."""
+    H, Hkv, P, ps = 4, 1, 400, 16
+    counts = [1] * 20 + [30, 6, 9, 1, 2, 1]
+    held = [P + 5 + i for i in range(20)] + [P + 10, 3, P - 60, 1, 0, 5000]
+    total, rows, _ = tables([P + 64] * len(held), ps)
+    rows = [r[:(P + 64) // ps] for r in rows]
+    pool = Pool(total, ps, Hkv, D, kind)
+    prefix = [int(x) for x in np.random.default_rng(1).permutation(total)[:P // ps]]
+    off = starts(counts)
+    q = randn(sum(counts), H * D, seed=2)
+    out = attend(pool, off, held, rows, q, H, D ** -0.5, prefix, P)
+    pos = {t: p for t, _, p in ref.places(off, held, len(q))}
+    want = ref.attention(q, pool.k, pool.v, off, held[:-1] + [P + 64], rows, prefix, P, H, D ** -0.5, torch.zeros(q.shape))
+    lost = [t for t in range(len(q)) if pos[t] < 0]
+    assert len(lost) == 3 + 2 and (out[lost] == 0).all()
+    keep = [t for t in range(len(q)) if pos[t] >= 0]
+    check_rows(out[keep], want[keep])
+    # a NaN at position 350 of the prefix reaches the rows that see it, no other
+    pool.v[prefix[350 // ps], 350 % ps] = float("nan")
+    got = attend(pool, off, held, rows, q, H, D ** -0.5, prefix, P)
+    blind = [t for t in range(len(q)) if pos[t] < 350]
+    assert len(blind) == 6 + 9 + 1 + 2 and torch.equal(got[blind], out[blind])
+    assert torch.isnan(got[[t for t in range(len(q)) if pos[t] >= 350]]).all()
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("what", ["peak", "rising", "tiny_q", "huge_q", "large_v", "zero_q", "no_scale", "minus"])
+def test_many_rows_ranges(kind, what):
+    H, Hkv, D, P, ps, scale = 8, 1, 128, 700, 16, 128 ** -0.5
+    pool, off, held, rows, prefix, q = case(kind, [2] * 12, [40 + i for i in range(12)], P, ps, H, Hkv, D)
+    if what == "peak":
+        pool.k[prefix[20], 3] *= 8
+    elif what == "rising":
+        for i, pg in enumerate(prefix):
+            pool.k[pg] *= 0.05 * (1 + i)
+    elif what == "tiny_q":
+        q *= 2.0 ** -100
+    elif what == "huge_q":
+        q *= 2.0 ** 60
+        scale *= 2.0 ** -60
+    elif what == "large_v":
+        pool.v[prefix[3]] *= 1000.0
+    elif what == "zero_q":
+        q[:5] = 0
+    elif what == "no_scale":
+        scale = 0.0
+    else:
+        scale = -scale
+    out = attend(pool, off, held, rows, q, H, scale, prefix, P)
+    want = ref.attention(q, pool.k, pool.v, off, held, rows, prefix, P, H, np.float32(scale).astype(np.float64), torch.zeros(q.shape))
+    check_rows(out, want)
+
+
 @pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
 def test_attention_without_a_prefix_is_the_same_mathematics(kind):
     """The prefix through the sequences' own tables gives what prefix_pages give."""
@@ -345,7 +464,7 @@ def test_a_nan_reaches_the_rows_that_see_it(kind):
 
 
 @pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
-@pytest.mark.parametrize("what", ["peak", "rising", "tiny_q", "huge_q", "large_v", "spread_q", "zero_q", "no_scale"])
+@pytest.mark.parametrize("what", ["peak", "rising", "tiny_q", "huge_q", "large_v", "spread_q", "zero_q", "no_scale", "minus"])
 def test_attention_ranges(kind, what):
     H, Hkv, D, P, ps, scale = 8, 2, 128, 300, 16, 128 ** -0.5
     pool, off, held, rows, prefix, q = case(kind, [1, 3], [50, 700], P, ps, H, Hkv, D)
@@ -366,8 +485,10 @@ def test_attention_ranges(kind, what):
         q[:, ::2] *= 2.0 ** -12
     elif what == "zero_q":
         q[0] = 0
-    else:
+    elif what == "no_scale":
         scale = 0.0
+    else:
+        scale = -scale
     out = attend(pool, off, held, rows, q, H, scale, prefix, P)
     want = ref.attention(q, pool.k, pool.v, off, held, rows, prefix, P, H, np.float32(scale).astype(np.float64), torch.zeros(q.shape))
     check_rows(out, want)

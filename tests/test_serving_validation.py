@@ -54,7 +54,7 @@ def norm_rope(r=None, q=Q, ldq=256, k=K, ldk=128, qo=O, ldqo=256, ko=O2, ldko=12
     (dict(r=rot(q_norm=FAKE, eps=-1.0)), -1), (dict(r=rot(q_norm=FAKE + 2)), -3), (dict(pos=0), -1), (dict(pos=FAKE + 1), -3),
     (dict(q=0), -1), (dict(qo=0), -1), (dict(k=0), -1), (dict(ko=0), -1), (dict(q=Q + 2), -3), (dict(ldq=255), -2),
     (dict(ldk=127), -2), (dict(ldqo=8), -2), (dict(qo=Q + 16), -1), (dict(ko=Q), -1), (dict(qo=Q, ldqo=512), -1),
-    (dict(ko=O + 4 * 128, ldko=256), -1), (dict(M=1 << 30, ldq=1 << 20), -2),
+    (dict(ko=O + 4 * 128, ldko=256), -1), (dict(M=1 << 30, ldq=1 << 20), -2), (dict(M=(1 << 23) + 1), -2),
 ])
 def test_norm_rope_refuses(kw, want):
     assert norm_rope(**kw) == want
@@ -88,6 +88,8 @@ POOL = [
 @pytest.mark.parametrize("kw,want", POOL + [
     (dict(r=rot(rot_dim=4)), -2), (dict(H=-1), -1), (dict(k=0), -1), (dict(v=0), -1), (dict(v=V + 1), -3), (dict(ldv=127), -2),
     (dict(qo=0), -1), (dict(ldq=255), -2), (dict(qo=K), -1), (dict(qo=V), -1), (dict(qo=Q, ldqo=257), -1),
+    (dict(k=FAKE + 64), -1), (dict(v=FAKE + 64), -1), (dict(qo=FAKE + 64), -1), (dict(q=FAKE - 64), -1),
+    (dict(b=batch(n_rows=(1 << 23) + 1)), -2),
 ])
 def test_append_refuses(kw, want):
     assert append(**kw) == want
@@ -98,16 +100,18 @@ def test_append_empty():
     assert append(b=batch(n_rows=0), k=0, v=0, q=0, qo=0) == 0
 
 
-def attend(p=None, b=None, pp=FAKE, P=20, q=Q, ldq=256, o=O, ldo=256, H=4, ws=WS, wsb=1 << 40):
+def attend(p=None, b=None, pp=FAKE, P=20, q=Q, ldq=256, o=O, ldo=256, H=4, scale=0.125, ws=WS, wsb=1 << 40):
     p, b = kv() if p is None else p, batch() if b is None else b
-    return status("cri_paged_attention", ref_of(p), ref_of(b), pp, P, q, ldq, o, ldo, H, 0.125, ws, wsb, None)
+    return status("cri_paged_attention", ref_of(p), ref_of(b), pp, P, q, ldq, o, ldo, H, scale, ws, wsb, None)
 
 
 @pytest.mark.parametrize("kw,want", POOL + [
     (dict(H=3), -2), (dict(H=-2), -1), (dict(P=-1), -1), (dict(P=(1 << 30) + 1), -2), (dict(pp=0), -1), (dict(pp=FAKE + 2), -3),
     (dict(q=0), -1), (dict(o=0), -1), (dict(ldq=255), -2), (dict(ldo=100), -2), (dict(o=Q), -1), (dict(o=Q + 1024), -1),
     (dict(ws=0), -1), (dict(ws=WS + 8), -3), (dict(wsb=100), -2), (dict(b=batch(max_pages=0)), -2),
-    (dict(b=batch(n_rows=1 << 23)), -2),
+    (dict(b=batch(n_rows=1 << 23)), -2), (dict(o=FAKE + 64), -1), (dict(ws=FAKE + 64), -1), (dict(ws=Q + 16), -1),
+    (dict(ws=O + 16), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(scale=3e38), -1),
+    (dict(b=batch(n_seqs=1 << 26)), -5),
 ])
 def test_attention_refuses(kw, want):
     assert attend(**kw) == want
