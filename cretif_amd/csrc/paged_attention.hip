@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const float* __restrict
 
 // the cut of a call, from what the host knows of it
 struct Cut {
-    bool even, staged;  // staged: the prefix goes to the kernel that shares it through LDS
+    bool even, staged;  // staged: the prefix goes to workgroups that share it through LDS
     int pre_tiles, pre_chunks, pre_per, pre_blocks, own_more, own_chunks, own_per, nrec;
     long own_first, own_blocks;
 };
@@ -110,21 +110,32 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
     const long rows = static_cast<long>(B.n_rows) * G;  // of a KV head
     c.staged = c.even && type != kKvF32 && D <= 128 && rows > 64 && prefix_len >= 256;
     const int tile = type == kKvF32 ? 16 : 32;
+    const long cap = static_cast<long>(B.max_pages) * P.page_size;
+    const long own = std::max(cap - prefix_len / tile * tile, 1L);
     if (prefix_len > 0) {
         const int tile_rows = c.staged ? kPrefixRows : 16;
         const int units = (prefix_len + tile - 1) / tile;
         c.pre_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
         const long streams = static_cast<long>(P.n_kv_heads) * c.pre_tiles;
-        // Chunks: rounds of items times the position tiles of each (a workgroup that has its CU to itself takes two thirds
-        // of the time per tile), five for an item's start and end, and its records: 128 rows' take a 60th of a tile's time
-        // when the whole GPU writes and reads them.
-        const int slots = c.staged ? kSlots : kPagedWaves * kSlots;
-        const double records = c.staged ? 1.0 / 60 : 1.0 / 480;
+        // Chunks: the fewest microseconds of a model of the GPU.  Staged: a workgroup takes 9 and 1.4 per tile (2.1 where two
+        // share a CU), fills one of 512 slots, the sequences' workgroups the others (at half their tables' length: bytes
+        // at 4.7 TB/s), and 128 rows' record is written and read at that rate.  Else an item is a wave of 16 rows; 5 tiles'
+        // time for its start and end.
+        const double own_us = 0.5 * B.n_seqs * own * P.n_kv_heads * D * (type == kKvF32 ? 8 : 4) / 4.7e6;
+        const double record_us = tile_rows * (D + 4) * 8 / 4.7e6;
         double best = 0.0;
         for (int n = 1; n <= kPreRecords && n <= units; ++n) {
             const long items = streams * n, per = (units + n - 1) / n;
-            const double rounds = items <= slots / 2 ? 0.65 : static_cast<double>((items + slots - 1) / slots);
-            const double cost = rounds * per + 5.0 * ((items + slots - 1) / slots) + items * records;
+            double cost;
+            if (c.staged) {
+                const double alone = 1.4 * per + 9.0, rounds = static_cast<double>((items + kSlots - 1) / kSlots);
+                const double longest = rounds * (items <= kSlots / 2 ? alone : 2.1 * per + 9.0);
+                cost = std::max(longest, items * alone / kSlots + own_us) + items * record_us;
+            } else {
+                const int slots = kPagedWaves * kSlots;
+                const double rounds = items <= slots / 2 ? 0.65 : static_cast<double>((items + slots - 1) / slots);
+                cost = 1.4 * (rounds * per + 5.0 * ((items + slots - 1) / slots)) + items * record_us;
+            }
             if (best == 0.0 || cost < best) {
                 best = cost;
                 c.pre_per = static_cast<int>(per * tile);
@@ -136,8 +147,6 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
     }
     // A sequence's own positions: chunks of one size, so that a long sequence has more of them and none is waited for; 256
     // positions, or less where the batch would leave waves idle.
-    const long cap = static_cast<long>(B.max_pages) * P.page_size;
-    const long own = std::max(cap - prefix_len / tile * tile, 1L);
     // sum of ceil(n G / 16) - 1 over the sequences that have rows: n G is a multiple of gcd(G, 16)
     c.own_more = static_cast<int>((rows - std::gcd(G, 16)) / 16);
     const long streams = static_cast<long>(P.n_kv_heads) * std::min<long>(B.n_seqs + c.own_more, (rows + 15) / 16 + B.n_seqs);
@@ -179,15 +188,13 @@ int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, cons
     a.by_more = dev::fast_div(std::max(c.own_more, 1));
     a.qscale = scale * 1.44269504088896340736f;
     a.staged = c.staged;
-    if (c.staged) {
-        (type == kKvF16 ? dev::run_paged_prefix_f16 : dev::run_paged_prefix_bf16)(a, stream);
-        a.pre_blocks = 0;
-    }
-    const long blocks = a.pre_blocks + c.own_blocks;
-    const auto run = type == kKvF32   ? dev::run_paged_attn_f32
-                     : type == kKvF16 ? dev::run_paged_attn_f16
-                                      : dev::run_paged_attn_bf16;
-    run(a, c.even, static_cast<int>(blocks), stream);
+    const auto run_rows = type == kKvF32   ? dev::run_paged_attn_f32
+                          : type == kKvF16 ? dev::run_paged_attn_f16
+                                           : dev::run_paged_attn_bf16;
+    if (c.staged)
+        (type == kKvF16 ? dev::run_paged_mixed_f16 : dev::run_paged_mixed_bf16)(a, static_cast<int>(c.own_blocks), stream);
+    else
+        run_rows(a, c.even, static_cast<int>(c.pre_blocks + c.own_blocks), stream);
     if (c.nrec > 1) {
         const long pairs = static_cast<long>(B.n_rows) * n_heads;
         int lg = 0;

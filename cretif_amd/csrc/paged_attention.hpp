@@ -55,7 +55,7 @@ struct PagedAttnArgs {
     int own_more, own_chunks, own_per, own_first;  // own_first: items of first tiles, own_more: other tiles at most
     FastDiv by_G, by_Hkv, by_pre_tiles, by_seqs, by_more;
     float qscale;  // scale * log2 e: scores are in base 2
-    bool staged;   // the prefix went to paged_prefix_kernel
+    bool staged;   // the prefix is prefix_body's
 };
 
 constexpr int kPagedWaves = 4;
@@ -195,8 +195,9 @@ __device__ __forceinline__ bool prefix_item(const PagedAttnArgs& a, int i, int H
 __device__ __forceinline__ int by_xcd(int b, int n) { return b % kPagedXcds * (n / kPagedXcds) + b / kPagedXcds; }
 
 // EVEN: head_dim is DP and the page size a multiple of 16, so the 16 positions of a tile's row block lie in one page
+// (block: of pre_blocks workgroups of the prefix, then the sequences')
 template <int TYPE, int DP, bool EVEN>
-__global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_attn_kernel(const PagedAttnArgs a) {
+__device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int block) {
     typedef PagedShape<TYPE, DP> S;
     typedef typename KvType<TYPE>::elem elem;
     typedef std::integral_constant<int, TYPE> Type;
@@ -212,14 +213,14 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
     const UniformInts offsets = uniform(a.B.offsets), lens = uniform(a.B.lens);
 
     // ---- what this wave does: a KV head, 16 rows, a range of positions
-    const bool prefix = static_cast<int>(blockIdx.x) < a.pre_blocks;
+    const bool prefix = block < a.pre_blocks;
     int kvh, row0, nrows, tok0, pos0 = 0, rec_at, own_lo, own_hi;
     UniformInts own_table;
     int own_len, before_lo = 0, before_hi = 0;  // (before: the prefix's positions for rows that do not see all of it)
     const int prefix_pages = (a.prefix_len + a.P.page_size - 1) / a.P.page_size;
     if (prefix) {
         int chunk, tile;
-        if (!prefix_item(a, 4 * by_xcd(blockIdx.x, a.pre_blocks) + w, Hkv, chunk, kvh, tile)) return;
+        if (!prefix_item(a, 4 * by_xcd(block, a.pre_blocks) + w, Hkv, chunk, kvh, tile)) return;
         row0 = tile * 16;
         nrows = a.B.n_rows * G;
         tok0 = 0;
@@ -229,7 +230,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
         own_table = uniform(a.prefix_pages);
         own_len = prefix_pages;
     } else {
-        int item = 4 * (static_cast<int>(blockIdx.x) - a.pre_blocks) + w, chunk, seq, tile = 0;
+        int item = 4 * (block - a.pre_blocks) + w, chunk, seq, tile = 0;
         if (item < a.own_first) {
             const int rest = div_by(item, a.by_Hkv);
             kvh = item - rest * Hkv;
@@ -322,7 +323,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
     const uint32_t k_off = c * row_bytes + 16 * g, v_off = 4 * g * row_bytes + kVe * kEs * c;
     typedef uint32_t vreg __attribute__((ext_vector_type(S::kWide ? 4 : kVe / 2)));
 
-    // A sequence's workgroup may have two ranges: where the prefix is left to paged_prefix_kernel, first that part of it
+    // A sequence's workgroup may have two ranges: where the prefix is left to prefix_body, first that part of it
     // that rows see which do not see it whole.
     int part = before_lo < before_hi ? 0 : 1, p_lo, p_hi, table_len, lim, least, first, last;
     UniformInts table;
@@ -635,21 +636,20 @@ __device__ __forceinline__ void wait_copies() {  // all but the last N copies of
 }
 
 template <int TYPE, int D>
-__global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArgs a) {
+__device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int block, char* const ring) {
     typedef PagedShape<TYPE, D> S;
     typedef typename KvType<TYPE>::elem elem;
     typedef std::integral_constant<int, TYPE> Type;
     constexpr int kParts = S::kParts, kKs = D / 16, kDb = D / 32, kRowB = 2 * D, kPieces = kRowB / 16;
-    constexpr int kTileB = kPrefixTile * kRowB;  // bytes of a tile's K or V
+    constexpr int kTileB = kPrefixTile * kRowB;  // bytes of a tile's K or V (ring: K's tiles, then V's)
     constexpr int kCopies = kTileB / 1024 / 4;   // of a wave, of a tile's K or V
-    extern __shared__ __attribute__((aligned(16))) char ring[];  // K's tiles, V's tiles
 
     const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.P.n_kv_heads, G = a.G, nrows = a.B.n_rows * G;
     const uint32_t row_bytes = static_cast<uint32_t>(Hkv) * kRowB;
     int chunk, kvh, tile;
-    if (!prefix_item(a, by_xcd(blockIdx.x, a.pre_blocks), Hkv, chunk, kvh, tile)) return;
+    if (!prefix_item(a, by_xcd(block, a.pre_blocks), Hkv, chunk, kvh, tile)) return;
     const int p_lo = chunk * a.pre_per, p_hi = min(p_lo + a.pre_per, a.prefix_len);
     const int ntiles = (p_hi - p_lo + kPrefixTile - 1) / kPrefixTile;
     const int table_len = (a.prefix_len + a.P.page_size - 1) / a.P.page_size;
@@ -820,6 +820,22 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
 }
 
 template <int TYPE, int DP, bool EVEN>
+__global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_attn_kernel(const PagedAttnArgs a) {
+    rows_body<TYPE, DP, EVEN>(a, blockIdx.x);
+}
+// The prefix's workgroups and behind them the sequences', in one launch: the former are bound by the matrix instructions,
+// the latter by memory and by the trips to it before their first tile, and a CU holds one of each (64 conversations on
+// 8192 tokens: 70 us, 92 in two launches).
+template <int TYPE, int D>
+__global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_mixed_kernel(const PagedAttnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char ring[];
+    if (static_cast<int>(blockIdx.x) < a.pre_blocks)
+        prefix_body<TYPE, D>(a, blockIdx.x, ring);
+    else
+        rows_body<TYPE, D, true>(a, blockIdx.x);
+}
+
+template <int TYPE, int DP, bool EVEN>
 void run_paged_attn(const PagedAttnArgs& a, int blocks, hipStream_t stream) {
     hipLaunchKernelGGL((paged_attn_kernel<TYPE, DP, EVEN>), dim3(blocks), dim3(64 * kPagedWaves), 0, stream, a);
 }
@@ -836,16 +852,14 @@ void run_paged_attn_type(const PagedAttnArgs& a, bool even, int blocks, hipStrea
 }
 
 template <int TYPE>
-void run_paged_prefix_type(const PagedAttnArgs& a, hipStream_t stream) {
+void run_paged_mixed_type(const PagedAttnArgs& a, int own_blocks, hipStream_t stream) {
     const int lds = 2 * kRing * kPrefixTile * a.P.head_dim * 2;
-    if (a.P.head_dim == 64)
-        hipLaunchKernelGGL((paged_prefix_kernel<TYPE, 64>), dim3(a.pre_blocks), dim3(256), lds, stream, a);
-    else
-        hipLaunchKernelGGL((paged_prefix_kernel<TYPE, 128>), dim3(a.pre_blocks), dim3(256), lds, stream, a);
+    const auto run = a.P.head_dim == 64 ? paged_mixed_kernel<TYPE, 64> : paged_mixed_kernel<TYPE, 128>;
+    hipLaunchKernelGGL(run, dim3(a.pre_blocks + own_blocks), dim3(64 * kPagedWaves), lds, stream, a);
 }
 
-void run_paged_prefix_f16(const PagedAttnArgs& a, hipStream_t stream);
-void run_paged_prefix_bf16(const PagedAttnArgs& a, hipStream_t stream);
+void run_paged_mixed_f16(const PagedAttnArgs& a, int own_blocks, hipStream_t stream);
+void run_paged_mixed_bf16(const PagedAttnArgs& a, int own_blocks, hipStream_t stream);
 void run_paged_attn_f32(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream);
 void run_paged_attn_f16(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream);
 void run_paged_attn_bf16(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream);
