@@ -304,8 +304,8 @@ def test_attention(kind, shape):
     assert torch.equal(out, again)  # sums in a fixed order
 
 
-# more than 64 rows of a KV head on a prefix from 256 positions on: with 16-bit caches, heads of 64 and 128 and pages of
-# 16 n positions the prefix is shared through LDS (fp32, other heads and pages: waves of their own)
+# many rows of a KV head on a long prefix: from 2^18 rows x positions on, with 16-bit caches, heads of 64 and 128 and pages
+# of 16 n positions, the prefix is shared through LDS (else, and with fp32, other heads and pages: waves of their own)
 MANY = [
     # counts, own, P, ps, H, Hkv, D
     ([1] * 33, [1 + 7 * i for i in range(33)], 256, 16, 4, 1, 64),         # a few rows, one tile, a whole number of tiles
@@ -316,6 +316,12 @@ MANY = [
     ([40, 90], [40, 300], 320, 16, 4, 1, 128),                             # pieces of prompts: rows of two sequences in a tile
     ([1] * 40, [1 + i for i in range(40)], 300, 20, 8, 2, 128),            # pages of 20
     ([1] * 40, [1 + i for i in range(40)], 300, 16, 8, 2, 256),
+    ([1] * 260, [1 + i % 90 for i in range(260)], 256, 16, 4, 1, 64),
+    ([1] * 70, [1 + i % 40 for i in range(70)], 1000, 16, 8, 2, 128),
+    ([2] * 155, [2 + i for i in range(155)], 289, 64, 3, 1, 64),
+    ([1] * 9, [1 + 30 * i for i in range(9)], 8200, 32, 8, 2, 64),         # 44 rows
+    ([40, 90], [40, 300], 505, 16, 4, 1, 128),
+    ([1] * 70, [1 + i % 40 for i in range(70)], 1000, 20, 8, 2, 128),
 ]
 
 
@@ -339,21 +345,21 @@ def test_many_rows_on_a_prefix(kind, shape):
 
 
 @pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
-@pytest.mark.parametrize("D", [64, 128])
-def test_many_rows_some_inside_the_prefix(kind, D):
+@pytest.mark.parametrize("D,P", [(64, 400), (128, 400), (64, 1000), (128, 1000)])
+def test_many_rows_some_inside_the_prefix(kind, D, P):
     """Rows that do not see the whole prefix, rows that see nothing and rows past their table, beside ordinary ones."""
-    H, Hkv, P, ps = 4, 1, 400, 16
+    H, Hkv, ps = 4, 1, 16
     counts = [1] * 20 + [30, 6, 9, 1, 2, 1]
     held = [P + 5 + i for i in range(20)] + [P + 10, 3, P - 60, 1, 0, 5000]
     total, rows, _ = tables([P + 64] * len(held), ps)
     rows = [r[:(P + 64) // ps] for r in rows]
     pool = Pool(total, ps, Hkv, D, kind)
-    prefix = [int(x) for x in np.random.default_rng(1).permutation(total)[:P // ps]]
+    prefix = [int(x) for x in np.random.default_rng(1).permutation(total)[:-(-P // ps)]]
     off = starts(counts)
     q = randn(sum(counts), H * D, seed=2)
     out = attend(pool, off, held, rows, q, H, D ** -0.5, prefix, P)
     pos = {t: p for t, _, p in ref.places(off, held, len(q))}
-    want = ref.attention(q, pool.k, pool.v, off, held[:-1] + [P + 64], rows, prefix, P, H, D ** -0.5, torch.zeros(q.shape))
+    want = ref.attention(q, pool.k, pool.v, off, held[:-1] + [len(rows[0]) * ps], rows, prefix, P, H, D ** -0.5, torch.zeros(q.shape))
     lost = [t for t in range(len(q)) if pos[t] < 0]
     assert len(lost) == 3 + 2 and (out[lost] == 0).all()
     keep = [t for t in range(len(q)) if pos[t] >= 0]
@@ -362,14 +368,15 @@ def test_many_rows_some_inside_the_prefix(kind, D):
     pool.v[prefix[350 // ps], 350 % ps] = float("nan")
     got = attend(pool, off, held, rows, q, H, D ** -0.5, prefix, P)
     blind = [t for t in range(len(q)) if pos[t] < 350]
-    assert len(blind) == 6 + 9 + 1 + 2 and torch.equal(got[blind], out[blind])
+    assert len(blind) == 6 + (9 if P == 400 else 0) + 1 + 2 and torch.equal(got[blind], out[blind])
     assert torch.isnan(got[[t for t in range(len(q)) if pos[t] >= 350]]).all()
 
 
 @pytest.mark.parametrize("kind", ["fp16", "bf16"])
 @pytest.mark.parametrize("what", ["peak", "rising", "tiny_q", "huge_q", "large_v", "zero_q", "no_scale", "minus"])
-def test_many_rows_ranges(kind, what):
-    H, Hkv, D, P, ps, scale = 8, 1, 128, 700, 16, 128 ** -0.5
+@pytest.mark.parametrize("P", [700, 1500])
+def test_many_rows_ranges(kind, what, P):
+    H, Hkv, D, ps, scale = 8, 1, 128, 16, 128 ** -0.5
     pool, off, held, rows, prefix, q = case(kind, [2] * 12, [40 + i for i in range(12)], P, ps, H, Hkv, D)
     if what == "peak":
         pool.k[prefix[20], 3] *= 8
@@ -714,6 +721,31 @@ def test_captured_steps_match_eager_ones():
         assert torch.equal(eager.pool.k, graph.pool.k) and torch.equal(eager.pool.v, graph.pool.v), i
         eager.advance()
         graph.advance()
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+def test_captured_attention_of_many_rows(kind):
+    """Captured once, replayed while the sequences grow, with eager work between: the eager bits."""
+    H, Hkv, D, P, ps = 8, 2, 128, 1000, 16
+    own = [1 + i % 40 for i in range(70)]
+    pool, off, held, rows, prefix, q = case(kind, [1] * 70, [x + 60 for x in own], P, ps, H, Hkv, D)
+    lens = ints([P + x for x in own])
+    b = cri.PagedBatch(ints(off), lens, ints(rows))
+    pp, ws = ints(prefix), torch.empty(cri.paged_attention_workspace_bytes(pool.kv, b, 70, H, P), dtype=torch.uint8, device="cuda")
+    out, want = torch.zeros_like(q), torch.zeros_like(q)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        cri.paged_attention(pool.kv, b, q, out, H, D ** -0.5, pp, P, ws)
+    for _ in range(5):
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        cri.paged_attention(pool.kv, b, q, want, H, D ** -0.5, pp, P, ws)
+        assert torch.equal(out, want)
+        lens += 11
+        q.mul_(-0.9)
 
 
 def test_a_side_stream_orders_with_torch():
