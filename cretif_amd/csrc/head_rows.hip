@@ -12,6 +12,9 @@
 //     compute their four angles once: the exponent and the product with the position in 64 bits (at position 10^6 a
 //     32-bit angle is off by 0.06 radians), reduced to a half turn in 64 bits, sine and cosine in 32.
 //   * The sequence of a row is found by the wave: 64 offsets compared at a time.
+//
+// 8192 rows, 32/8 heads of 128 out of a fused product: 65 us, 335 MB at 5.2 TB/s (a large copy moves 4.7); 6921 rows
+// appended in bf16 with their queries 60 us, 312 MB at 5.2; one row 3.0 us, 64 rows 4.1, which are three trips to memory.
 #include "paged.hpp"
 
 namespace cri {
@@ -168,7 +171,8 @@ void set_rows(RowArgs& a, int rows) {
 
 dim3 grid_of(const RowArgs& a, int tokens) {
     const int per = kThreads >> a.lg, parts = (a.nrows + per - 1) / per;
-    // few tokens: a workgroup per part of a token's rows; many: one per token, whose angles serve all its rows
+    // few tokens: a workgroup per part of a token's rows, so that none waits for two; from 1024 on, which fill the GPU, one
+    // per token, whose angles serve all its rows
     return dim3(static_cast<unsigned>(tokens), static_cast<unsigned>(tokens >= 1024 ? 1 : parts));
 }
 

@@ -4,8 +4,12 @@
 // with the rows of all sequences at once, so its K and V are read once for the batch; each sequence's own
 // positions are multiplied with its own rows.  Both leave (max, sum, acc) records that a second kernel joins.
 //
-// One wave takes 16 query rows ("columns": query q = token x G + g of the heads g that share a KV head) and a
-// tile of positions at a time, straight from the pool into registers:
+// rows_body: a wave takes 16 query rows ("columns": query q = token x G + g of the heads g that share a KV head), a
+// range of positions and a tile of them at a time, straight from the pool into registers, without LDS or barriers.  It
+// is bound by memory: 64 sequences of 1500 own positions, 32/8 heads of 128, read their 393 MB of fp16 in 79 us (5.0
+// TB/s; a large copy moves 4.7), fp32 786 MB in 140 us (5.6); a range of 256 positions, half that or a third took the
+// same within a tenth, 512 left waves idle where lengths differ.  Two waves per SIMD (216 registers): three spilled, and
+// were slower (99 -> 130 us before the waves were made independent).
 //   * S^T = K Q^T: K is the A operand, whose 16 bytes per lane are consecutive dims of a position's row.
 //   * O^T += V^T P^T: a lane owns one column, and the positions of its scores are the positions whose
 //     probabilities it supplies, so P never leaves the registers.  V^T's operand is put together in registers from
@@ -17,6 +21,7 @@
 //   * A tile that some column does not see as a whole is multiplied once per limit that its columns have, V zeroed
 //     from the limit on: what lies behind a row's last position (stale pages, infinities) never meets it, not even
 //     times zero.
+// prefix_body, below, takes the prefix where many rows share it.
 #pragma once
 
 #include <algorithm>
@@ -323,7 +328,7 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
     const uint32_t k_off = c * row_bytes + 16 * g, v_off = 4 * g * row_bytes + kVe * kEs * c;
     typedef uint32_t vreg __attribute__((ext_vector_type(S::kWide ? 4 : kVe / 2)));
 
-    // A sequence's workgroup may have two ranges: where the prefix is left to prefix_body, first that part of it
+    // A sequence's wave may have two ranges: where the prefix is left to prefix_body, first that part of it
     // that rows see which do not see it whole.
     int part = before_lo < before_hi ? 0 : 1, p_lo, p_hi, table_len, lim, least, first, last;
     UniformInts table;
@@ -603,16 +608,18 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
 // waves takes 128 rows, 32 to a wave, and a chunk of the prefix in tiles of 32 positions that all its waves read from LDS:
 // straight from the pool every wave would load 16 KB for the 2 x 0.5 MFLOP it does with a tile, more than the L1 delivers
 // beside the matrix instructions.  v_mfma_f32_32x32x16: half the instructions of 16x16x32 for the same product.
-//   * Tiles go to LDS with global_load_lds, whole rows at a time, into rings of four, two to three tiles ahead; one barrier
-//     per tile.  The 16-byte pieces of a row are exchanged within it: K's so that the 32 rows of an operand fetch lie in
+//   * Tiles go to LDS with global_load_lds, whole rows at a time, into rings of four, three tiles ahead; one barrier per
+//     tile.  The 16-byte pieces of a row are exchanged within it: K's so that the 32 rows of an operand fetch lie in
 //     different banks, V's so that the four rows that ds_read_b64_tr_b16 takes apart do (16 lanes read 4 positions x 16
-//     dims and get a dim's 4 positions each: V^T's operand without a byte permutation).
-//   * The scores of the next tile are issued between the exponentials of the current one, the next tile's maximum between
-//     the products with V: a wave's matrix instructions and its vector ones run side by side.
+//     dims and get a dim's 4 positions each: V^T's operand without a byte permutation).  No bank conflicts are counted.
 //   * kf, the scores' factor, is applied within the exponential's fma.  It is not negative (a negative scale turns the
 //     query's sign), so the raw scores' maximum is the scaled ones'.
-// Bound by the vector instructions beside the matrix ones: about 100 and 16 exponentials per tile and wave to 32
-// products of 32 cycles.
+// 480 rows x 32 heads of 128 on 32768 positions of fp16: 482 us, 1075 TFLOP/s of fp16 products, two for each of the
+// formula's, where a large library product runs at 1150 (bf16, three: 618 us, 1257 against 1207).  The matrix units are busy
+// for half the cycles at 1.9 GHz (the clock under this load; nothing but these instructions on random numbers reach 1600
+// TFLOP/s), the rest is the exponentials and parts, about 95 vector instructions and 16 exponentials per wave and tile to
+// 32 products.  Issuing the next tile's scores between them, and operands read ahead, were measured at 562 to 585 us against
+// 541: more registers, the same power.
 constexpr int kPrefixRows = 128, kPrefixTile = 32, kRing = 4;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -638,7 +645,6 @@ __device__ __forceinline__ void wait_copies() {  // all but the last N copies of
 template <int TYPE, int D>
 __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int block, char* const ring) {
     typedef PagedShape<TYPE, D> S;
-    typedef typename KvType<TYPE>::elem elem;
     typedef std::integral_constant<int, TYPE> Type;
     constexpr int kParts = S::kParts, kKs = D / 16, kDb = D / 32, kRowB = 2 * D, kPieces = kRowB / 16;
     constexpr int kTileB = kPrefixTile * kRowB;  // bytes of a tile's K or V (ring: K's tiles, then V's)
@@ -825,7 +831,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
 }
 // The prefix's workgroups and behind them the sequences', in one launch: the former are bound by the matrix instructions,
 // the latter by memory and by the trips to it before their first tile, and a CU holds one of each (64 conversations on
-// 8192 tokens: 70 us, 92 in two launches).
+// 8192 tokens: 67 us, 90 in two launches; 480 rows on 32768: 487 and 510).
 template <int TYPE, int D>
 __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_mixed_kernel(const PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char ring[];

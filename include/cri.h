@@ -414,15 +414,18 @@ int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const
  * a prefix that all sequences share, whose K and V are read once for the batch (its last page may
  * be partly filled; the sequences' own positions start at prefix_len of their own tables).
  * prefix_len 0: every position through its sequence's table.  A row at a position below 0 (a
- * negative lens counts as 0) sees nothing and gets zeros; positions past the table (max_pages * page_size) are not seen.  Nothing
- * behind a row's last position reaches it, whatever its pages hold there.  Table entries of positions
- * that rows see must be inside the pool (others give unspecified numbers in their sequence's rows).
+ * negative lens counts as 0) sees nothing and gets zeros; positions past the table (max_pages *
+ * page_size) are not seen.  Nothing behind a row's last position reaches it, whatever its pages hold
+ * there; a key or value that is not finite makes the rows that see it not finite.  Table entries of
+ * positions that rows see must be inside the pool (others give unspecified numbers in their
+ * sequence's rows).
  *
  * q rows are ldq floats apart, out rows ldo; out must not overlap q or the pool.  n_heads a multiple
- * of n_kv_heads; scale finite.  q, out 4-byte aligned, workspace 16-byte, cri_paged_attention_workspace_bytes of
- * it (the same kv, batch and prefix_len; only their host numbers count, so the bytes of a batch's
- * n_seqs, n_rows and max_pages serve every step of it).  Sums, maxima and products are in fp32
- * accuracy for every cache type; the order of sums is fixed by the host numbers. */
+ * of n_kv_heads; n_rows * n_heads at most 2^24; scale finite.  q, out 4-byte aligned, workspace
+ * 16-byte, cri_paged_attention_workspace_bytes of it (for the same kv, batch and prefix_len; only
+ * their host numbers count, so one workspace serves every step with the same n_seqs, n_rows and
+ * max_pages), not overlapping the others.  Sums, maxima and products are good to fp32 for every cache
+ * type, in an order fixed by the host numbers and lens. */
 int cri_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, const int* prefix_pages, int prefix_len,
                         const float* q, int ldq, float* out, int ldo, int n_heads, float scale, void* workspace,
                         long long workspace_bytes, hipStream_t stream);

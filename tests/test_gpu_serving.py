@@ -373,7 +373,7 @@ def test_many_rows_some_inside_the_prefix(kind, D, P):
 
 
 @pytest.mark.parametrize("kind", ["fp16", "bf16"])
-@pytest.mark.parametrize("what", ["peak", "rising", "tiny_q", "huge_q", "large_v", "zero_q", "no_scale", "minus"])
+@pytest.mark.parametrize("what", ["peak", "rising", "tiny_q", "huge_q", "large_v", "zero_q", "no_scale", "minus", "tiny_kv"])
 @pytest.mark.parametrize("P", [700, 1500])
 def test_many_rows_ranges(kind, what, P):
     H, Hkv, D, ps, scale = 8, 1, 128, 16, 128 ** -0.5
@@ -394,8 +394,12 @@ def test_many_rows_ranges(kind, what, P):
         q[:5] = 0
     elif what == "no_scale":
         scale = 0.0
-    else:
+    elif what == "minus":
         scale = -scale
+    else:  # subnormal fp16 numbers in the cache
+        pool.k *= 2.0 ** -15
+        pool.v *= 2.0 ** -15
+        q *= 2.0 ** 15
     out = attend(pool, off, held, rows, q, H, scale, prefix, P)
     want = ref.attention(q, pool.k, pool.v, off, held, rows, prefix, P, H, np.float32(scale).astype(np.float64), torch.zeros(q.shape))
     check_rows(out, want)
@@ -471,7 +475,7 @@ def test_a_nan_reaches_the_rows_that_see_it(kind):
 
 
 @pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
-@pytest.mark.parametrize("what", ["peak", "rising", "tiny_q", "huge_q", "large_v", "spread_q", "zero_q", "no_scale", "minus"])
+@pytest.mark.parametrize("what", ["peak", "rising", "tiny_q", "huge_q", "large_v", "spread_q", "zero_q", "no_scale", "minus", "tiny_kv"])
 def test_attention_ranges(kind, what):
     H, Hkv, D, P, ps, scale = 8, 2, 128, 300, 16, 128 ** -0.5
     pool, off, held, rows, prefix, q = case(kind, [1, 3], [50, 700], P, ps, H, Hkv, D)
@@ -494,8 +498,12 @@ def test_attention_ranges(kind, what):
         q[0] = 0
     elif what == "no_scale":
         scale = 0.0
-    else:
+    elif what == "minus":
         scale = -scale
+    else:  # subnormal fp16 numbers in the cache
+        pool.k *= 2.0 ** -15
+        pool.v *= 2.0 ** -15
+        q *= 2.0 ** 15
     out = attend(pool, off, held, rows, q, H, scale, prefix, P)
     want = ref.attention(q, pool.k, pool.v, off, held, rows, prefix, P, H, np.float32(scale).astype(np.float64), torch.zeros(q.shape))
     check_rows(out, want)
