@@ -123,12 +123,22 @@ __device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&p)[PARTS]) {
     }
 }
 
-// fp16 parts of a query row of largest magnitude m: it is scaled by f, a power of two that takes m to [2^13, 2^14), and
-// the scores' factor kf by 1 / f; the parts are then off by 2^-23 of an element or 2^-39 of the largest
-__device__ __forceinline__ void q_scale(float m, float& f, float& kf) {
-    const int sh = min(13 + 127 - static_cast<int>(__builtin_bit_cast(uint32_t, m) >> 23), 126);
-    f = __builtin_bit_cast(float, (127 + sh) << 23);
-    kf *= __builtin_bit_cast(float, (127 - sh) << 23);
+// The factors of a query row of largest magnitude m and of its raw scores: f before the products, kf within the
+// exponential's fma, f kf = qscale.  kf is positive (f has the sign, and is 0 for a scale of 0), so the raw scores' maximum
+// is the scaled ones' and a masked score of -infinity stays one.  For fp16 parts f also takes m to [2^13, 2^14): the parts
+// are then off by 2^-23 of an element or 2^-39 of the largest.
+template <int TYPE>
+__device__ __forceinline__ void row_factors(float qscale, float m, float& f, float& kf) {
+    constexpr float kTiny = 1.17549435e-38f;
+    f = 1.0f;
+    kf = fabsf(qscale);
+    if constexpr (TYPE == kKvF16) {
+        const int sh = min(13 + 127 - static_cast<int>(__builtin_bit_cast(uint32_t, m) >> 23), 126);
+        f = __builtin_bit_cast(float, (127 + sh) << 23);
+        kf *= __builtin_bit_cast(float, (127 - sh) << 23);
+    }
+    kf = fmaxf(kf, kTiny);
+    f = qscale == 0.0f ? 0.0f : __builtin_copysignf(f, qscale);
 }
 __device__ __forceinline__ float col_max(float v) { return swap_max32(swap_max16(v, v), swap_max16(v, v)); }
 __device__ __forceinline__ float col_sum(float v) {
@@ -413,32 +423,26 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
     set_part();
     if (first < last) load_tile(first);
 
-    float kf = a.qscale;
+    float kf, f;
     u32x4 q[S::kWide ? 1 : kKs][S::kParts];
     f32x4 q32[S::kWide ? kKs : 1];
-    {
-        if constexpr (S::kWide) {
+    if constexpr (S::kWide) {
+        row_factors<TYPE>(a.qscale, 0.0f, f, kf);
 #pragma unroll
-            for (int j = 0; j < kKs; ++j) q32[j] = raw[j];
-        } else {
-            float x[kKs][8], m = 0.0f;
+        for (int j = 0; j < kKs; ++j) q32[j] = raw[j] * f;
+    } else {
+        float m = 0.0f;
 #pragma unroll
-            for (int j = 0; j < kKs; ++j)
+        for (int j = 0; j < 2 * kKs; ++j)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[j][e] = raw[2 * j + (e >> 2)][e & 3];
-                    m = fmaxf(m, fabsf(x[j][e]));
-                }
-            float f = 1.0f;
-            if constexpr (TYPE == kKvF16) q_scale(col_max(m), f, kf);
+            for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(raw[j][e]));
+        row_factors<TYPE>(a.qscale, col_max(m), f, kf);
 #pragma unroll
-            for (int j = 0; j < kKs; ++j) {
-                if constexpr (TYPE == kKvF16) {
+        for (int j = 0; j < kKs; ++j) {
+            float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[j][e] *= f;
-                }
-                split8<TYPE, S::kParts>(x[j], q[j]);
-            }
+            for (int e = 0; e < 8; ++e) x[e] = raw[2 * j + (e >> 2)][e & 3] * f;
+            split8<TYPE, S::kParts>(x, q[j]);
         }
     }
 
@@ -470,7 +474,7 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
                         for (int j = 0; j < kKs; ++j) x = mma16(k[t][j], q[j][p], x, Type{});
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[4 * t + i] = x[i] * kf;
+                for (int i = 0; i < 4; ++i) s[4 * t + i] = x[i];  // (raw: the factor comes with the exponential)
             }
             const int next = p0 + kTile;
             const bool more = tile + 1 < last;
@@ -495,7 +499,7 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
             float m = s[0];
 #pragma unroll
             for (int i = 1; i < kNs; ++i) m = fmaxf(m, s[i]);
-            m = col_max(m);
+            m = col_max(m) * kf;
             const bool raise = m > mx + S::kSlack;
             if (__ballot(raise) != 0) {
                 const float f = raise ? __builtin_amdgcn_exp2f(mx - m) : 1.0f;
@@ -508,7 +512,7 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
             float p[8] = {};
 #pragma unroll
             for (int i = 0; i < kNs; ++i) {
-                p[i] = __builtin_amdgcn_exp2f(s[i] - base);
+                p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], kf, -base));
                 sum += p[i];
             }
             u32x4 pb[S::kParts];
@@ -612,8 +616,6 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
 //     tile.  The 16-byte pieces of a row are exchanged within it: K's so that the 32 rows of an operand fetch lie in
 //     different banks, V's so that the four rows that ds_read_b64_tr_b16 takes apart do (16 lanes read 4 positions x 16
 //     dims and get a dim's 4 positions each: V^T's operand without a byte permutation).  No bank conflicts are counted.
-//   * kf, the scores' factor, is applied within the exponential's fma.  It is not negative (a negative scale turns the
-//     query's sign), so the raw scores' maximum is the scaled ones'.
 // 480 rows x 32 heads of 128 on 32768 positions of fp16: 482 us, 1075 TFLOP/s of fp16 products, two for each of the
 // formula's, where a large library product runs at 1150 (bf16, three: 618 us, 1257 against 1207).  The matrix units are busy
 // for half the cycles at 1.9 GHz (the clock under this load; nothing but these instructions on random numbers reach 1600
@@ -696,7 +698,7 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
     const int tok = found && r < nrows ? t : -1, head = kvh * G + r - t * G;
     const bool sees = tok >= 0 && pos + 1 >= a.prefix_len;
     u32x4 q[kKs][kParts];
-    float kf = fmaxf(fabsf(a.qscale), 1.17549435e-38f);  // (not 0: it meets masked scores of -infinity)
+    float kf;
     {
         const float* src = a.q + static_cast<long>(max(tok, 0)) * a.ldq + static_cast<long>(head) * D + 8 * h;
         float x[kKs][8], m = 0.0f;
@@ -711,11 +713,8 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
                     m = fmaxf(m, fabsf(v[d]));
                 }
             }
-        float f = 1.0f;
-        if constexpr (TYPE == kKvF16) q_scale(swap_max32(m, m), f, kf);
-        kf = fmaxf(kf, 1.17549435e-38f);
-        f = __builtin_copysignf(f, a.qscale);
-        if (a.qscale == 0.0f) f = 0.0f;
+        float f;
+        row_factors<TYPE>(a.qscale, swap_max32(m, m), f, kf);
 #pragma unroll
         for (int j = 0; j < kKs; ++j) {
 #pragma unroll
