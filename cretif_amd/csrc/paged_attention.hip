@@ -109,29 +109,31 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
     c.even = (D == 64 || D == 128 || D == 256) && P.page_size % 16 == 0;
     const long rows = static_cast<long>(B.n_rows) * G;  // of a KV head
     // Measured, heads of 128, 100 own positions, staged against waves of their own: 64 rows on 4096 positions 19.4 / 19.9 us,
-    // 128 on 1024 18.2 / 17.8, on 4096 24.6 / 25.4, 512 on 512 23.8 / 27.5, on 2048 32.1 / 38.9, 2048 on 1024 80 / 111.
-    c.staged = c.even && type != kKvF32 && D <= 128 && rows > 32 && prefix_len >= 256 && rows * prefix_len >= 1L << 18;
-    const int tile = type == kKvF32 ? 16 : 32;
+    // 128 on 1024 18.2 / 17.8, on 4096 24.6 / 25.4, 512 on 512 23.8 / 27.5, on 2048 32.1 / 38.9, 2048 on 1024 80 / 111
+    // (fp32: 30.7 / 29.0, 25.9 / 23.0, 36 / 41, 38 / 45, 62 / 86, 138 / 210).
+    c.staged = c.even && D <= 128 && rows > 32 && prefix_len >= 256 && rows * prefix_len >= 1L << 18;
+    const int own_tile = type == kKvF32 ? 16 : 32;
     const long cap = static_cast<long>(B.max_pages) * P.page_size;
-    const long own = std::max(cap - prefix_len / tile * tile, 1L);
+    const long own = std::max(cap - prefix_len / own_tile * own_tile, 1L);
     if (prefix_len > 0) {
         const int tile_rows = c.staged ? kPrefixRows : 16;
-        const int units = (prefix_len + tile - 1) / tile;
+        const int tile = c.staged ? kPrefixTile : own_tile, units = (prefix_len + tile - 1) / tile;
         c.pre_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
         const long streams = static_cast<long>(P.n_kv_heads) * c.pre_tiles;
-        // Chunks: the fewest microseconds of a model of the GPU.  Staged: a workgroup takes 9 and 1.4 per tile (2.1 where two
-        // share a CU), fills one of 512 slots, the sequences' workgroups the others (at half their tables' length: bytes
+        // Chunks: the fewest microseconds of a model of the GPU.  Staged: a workgroup takes 9 and 1.4 per tile (fp16, heads of
+        // 128; half as much again where two share a CU), fills one of 512 slots, the sequences' workgroups the others (at half their tables' length: bytes
         // at 4.7 TB/s), and 128 rows' record is written and read at that rate.  Else an item is a wave of 16 rows; 5 tiles'
         // time for its start and end.
         const double own_us = 0.5 * B.n_seqs * own * P.n_kv_heads * D * (type == kKvF32 ? 8 : 4) / 4.7e6;
+        const double tile_us = (type == kKvF16 ? 1.4 : type == kKvBF16 ? 1.9 : 2.8) * D / 128;
         const double record_us = tile_rows * (D + 4) * 8 / 4.7e6;
         double best = 0.0;
         for (int n = 1; n <= kPreRecords && n <= units; ++n) {
             const long items = streams * n, per = (units + n - 1) / n;
             double cost;
             if (c.staged) {
-                const double alone = 1.4 * per + 9.0, rounds = static_cast<double>((items + kSlots - 1) / kSlots);
-                const double longest = rounds * (items <= kSlots / 2 ? alone : 2.1 * per + 9.0);
+                const double alone = tile_us * per + 9.0, rounds = static_cast<double>((items + kSlots - 1) / kSlots);
+                const double longest = rounds * (items <= kSlots / 2 ? alone : 1.5 * tile_us * per + 9.0);
                 cost = std::max(longest, items * alone / kSlots + own_us) + items * record_us;
             } else {
                 const int slots = kPagedWaves * kSlots;
@@ -154,7 +156,7 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
     const long streams = static_cast<long>(P.n_kv_heads) * std::min<long>(B.n_seqs + c.own_more, (rows + 15) / 16 + B.n_seqs);
     const long fill = own * streams / (kPagedWaves * kSlots);  // positions of a wave that fill the GPU once
     const long least = (own + kOwnRecords - 1) / kOwnRecords;
-    c.own_per = round_up(static_cast<int>(std::max({std::min(fill, 256L), least, 1L})), tile);
+    c.own_per = round_up(static_cast<int>(std::max({std::min(fill, 256L), least, 1L})), own_tile);
     c.own_chunks = static_cast<int>((own + c.own_per - 1) / c.own_per);
     c.own_first = static_cast<long>(c.own_chunks) * B.n_seqs * P.n_kv_heads;
     c.own_blocks = (c.own_first + static_cast<long>(c.own_chunks) * c.own_more * P.n_kv_heads + kPagedWaves - 1) / kPagedWaves;
@@ -194,7 +196,9 @@ int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, cons
                           : type == kKvF16 ? dev::run_paged_attn_f16
                                            : dev::run_paged_attn_bf16;
     if (c.staged)
-        (type == kKvF16 ? dev::run_paged_mixed_f16 : dev::run_paged_mixed_bf16)(a, static_cast<int>(c.own_blocks), stream);
+        (type == kKvF32   ? dev::run_paged_mixed_f32
+         : type == kKvF16 ? dev::run_paged_mixed_f16
+                          : dev::run_paged_mixed_bf16)(a, static_cast<int>(c.own_blocks), stream);
     else
         run_rows(a, c.even, static_cast<int>(c.pre_blocks + c.own_blocks), stream);
     if (c.nrec > 1) {

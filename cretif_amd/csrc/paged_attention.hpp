@@ -16,7 +16,7 @@
 //     row loads (16-bit types: byte permutations; fp32: none are needed).
 //   * 16-bit caches, v_mfma_f32_16x16x32: cached numbers are exact operands.  The fp32 queries and probabilities
 //     are taken in parts whose sum is good to fp32: two fp16 parts (queries scaled per row into fp16's upper range,
-//     probabilities by 2^12), three bf16 parts.  fp32 caches: v_mfma_f32_16x16x4.
+//     probabilities by 2^12), three bf16 parts.  fp32 caches: v_mfma_f32_16x16x4, which keeps up with memory.
 //   * The running maximum is raised, and the accumulators rescaled, only when a score exceeds it by kSlack.
 //   * A tile that some column does not see as a whole is multiplied once per limit that its columns have, V zeroed
 //     from the limit on: what lies behind a row's last position (stale pages, infinities) never meets it, not even
@@ -608,14 +608,18 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
             }
 }
 
-// The shared prefix against many rows (16-bit caches, head_dim 64 and 128, pages of 16 n positions).  A workgroup of four
+// The shared prefix against many rows (head_dim 64 and 128, pages of 16 n positions).  A workgroup of four
 // waves takes 128 rows, 32 to a wave, and a chunk of the prefix in tiles of 32 positions that all its waves read from LDS:
 // straight from the pool every wave would load 16 KB for the 2 x 0.5 MFLOP it does with a tile, more than the L1 delivers
 // beside the matrix instructions.  v_mfma_f32_32x32x16: half the instructions of 16x16x32 for the same product.
-//   * Tiles go to LDS with global_load_lds, whole rows at a time, into rings of four, three tiles ahead; one barrier per
+//   * 16-bit tiles go to LDS with global_load_lds, whole rows at a time, into rings of four, three tiles ahead; one barrier per
 //     tile.  The 16-byte pieces of a row are exchanged within it: K's so that the 32 rows of an operand fetch lie in
 //     different banks, V's so that the four rows that ds_read_b64_tr_b16 takes apart do (16 lanes read 4 positions x 16
 //     dims and get a dim's 4 positions each: V^T's operand without a byte permutation).  No bank conflicts are counted.
+//   * fp32 tiles go through registers, where K and V are cut into three bf16 parts, 8 bits of the significand each (exact, and
+//     of fp32's range); a product is the six of parts down to 2^-16, each exact in fp32.  v_mfma_f32_32x32x16_bf16 does 16
+//     times the multiply-adds per cycle of the fp32 instructions, so the six cost 0.38 of their cycles (512 rows of a KV
+//     head on 8192 positions 222 -> 115 us, 256 rows 118 -> 73), at the same distance from float64.
 // 480 rows x 32 heads of 128 on 32768 positions of fp16: 482 us, 1075 TFLOP/s of fp16 products, two for each of the
 // formula's, where a large library product runs at 1150 (bf16, three: 618 us, 1257 against 1207).  The matrix units are busy
 // for half the cycles at 1.9 GHz (the clock under this load; nothing but these instructions on random numbers reach 1600
@@ -639,6 +643,20 @@ __device__ __forceinline__ u32x2 read_transposed(const char* p) {
     typedef __attribute__((address_space(3))) s16x4* Ptr;
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(p)));
 }
+// eight floats as three bf16 parts each, the 8 bits of the significand that remain at a time: exact
+__device__ __forceinline__ void cut8(const f32x4 (&x)[2], u32x4 (&p)[3]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float a = x[e >> 1][2 * (e & 1)], b = x[e >> 1][2 * (e & 1) + 1];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const uint32_t u = __builtin_bit_cast(uint32_t, a), v = __builtin_bit_cast(uint32_t, b);
+            p[k][e] = __builtin_amdgcn_perm(v, u, 0x07060302u);
+            a -= __builtin_bit_cast(float, u & 0xFFFF0000u);
+            b -= __builtin_bit_cast(float, v & 0xFFFF0000u);
+        }
+    }
+}
 template <int N>
 __device__ __forceinline__ void wait_copies() {  // all but the last N copies of this wave have arrived
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
@@ -646,16 +664,20 @@ __device__ __forceinline__ void wait_copies() {  // all but the last N copies of
 
 template <int TYPE, int D>
 __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int block, char* const ring) {
-    typedef PagedShape<TYPE, D> S;
-    typedef std::integral_constant<int, TYPE> Type;
+    constexpr bool kWide = TYPE == kKvF32;                        // K and V, too, are taken in three bf16 parts
+    constexpr int kMath = kWide ? kKvBF16 : TYPE, kKv = kWide ? 3 : 1;
+    typedef PagedShape<kMath, D> S;
+    typedef std::integral_constant<int, kMath> Type;
     constexpr int kParts = S::kParts, kKs = D / 16, kDb = D / 32, kRowB = 2 * D, kPieces = kRowB / 16;
-    constexpr int kTileB = kPrefixTile * kRowB;  // bytes of a tile's K or V (ring: K's tiles, then V's)
-    constexpr int kCopies = kTileB / 1024 / 4;   // of a wave, of a tile's K or V
+    // bytes of (a part of) a tile's K or V; ring: K's tiles or parts, then V's
+    constexpr int kTileB = kPrefixTile * kRowB, kValues = (kWide ? kKv : kRing) * kTileB;
+    constexpr int kCopies = kTileB / 1024 / 4;  // of a wave, of a tile's K or V
 
     const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.P.n_kv_heads, G = a.G, nrows = a.B.n_rows * G;
-    const uint32_t row_bytes = static_cast<uint32_t>(Hkv) * kRowB;
+    constexpr int kEs = kWide ? 4 : 2;
+    const uint32_t row_bytes = static_cast<uint32_t>(Hkv) * D * kEs;
     int chunk, kvh, tile;
     if (!prefix_item(a, by_xcd(block, a.pre_blocks), Hkv, chunk, kvh, tile)) return;
     const int p_lo = chunk * a.pre_per, p_hi = min(p_lo + a.pre_per, a.prefix_len);
@@ -663,8 +685,8 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
     const int table_len = (a.prefix_len + a.P.page_size - 1) / a.P.page_size;
 
     // ---- the copies: a wave's rows of a tile lie in one page (8 rows each; 16 share a page)
-    const char* const kbase = static_cast<const char*>(a.P.k) + static_cast<long>(kvh) * kRowB;
-    const char* const vbase = static_cast<const char*>(a.P.v) + static_cast<long>(kvh) * kRowB;
+    const char* const kbase = static_cast<const char*>(a.P.k) + static_cast<long>(kvh) * D * kEs;
+    const char* const vbase = static_cast<const char*>(a.P.v) + static_cast<long>(kvh) * D * kEs;
     auto k_mix = [&](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
     auto v_mix = [&](int row) { return D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; };
     constexpr int kCopyRows = 64 / kPieces;
@@ -675,20 +697,60 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
         k_off[n] = r * row_bytes + 16 * (lane % kPieces ^ k_mix(row));
         v_off[n] = r * row_bytes + 16 * (lane % kPieces ^ v_mix(row));
     }
-    auto copy = [&](int t) {  // tile t (past the last one: that one again, so that every turn issues as many)
-        const int pos = p_lo + min(t, ntiles - 1) * kPrefixTile + 8 * w, pi = page_index(a.P, pos);
+    auto row_at = [&](int pos) {  // byte offset of a (uniform) position's row
+        const int pi = page_index(a.P, pos);
         const int pg = uniform(a.prefix_pages)[min(pi, table_len - 1)];
-        const long at = (static_cast<unsigned>(pg) < static_cast<unsigned>(a.P.n_pages) ? pg : 0) * a.P.stride * 2 +
-                        static_cast<long>(pos - pi * a.P.page_size) * row_bytes;
+        return (static_cast<unsigned>(pg) < static_cast<unsigned>(a.P.n_pages) ? pg : 0) * a.P.stride * kEs +
+               static_cast<long>(pos - pi * a.P.page_size) * row_bytes;
+    };
+    auto copy = [&](int t) {  // tile t (past the last one: that one again, so that every turn issues as many)
+        const long at = row_at(p_lo + min(t, ntiles - 1) * kPrefixTile + 8 * w);
         char* const dst = ring + t % kRing * kTileB + 8 * w * kRowB;
 #pragma unroll
         for (int n = 0; n < kCopies; ++n) dma16(kbase + at + k_off[n], dst + n * 1024);
 #pragma unroll
-        for (int n = 0; n < kCopies; ++n) dma16(vbase + at + v_off[n], dst + kRing * kTileB + n * 1024);
+        for (int n = 0; n < kCopies; ++n) dma16(vbase + at + v_off[n], dst + kValues + n * 1024);
     };
-    copy(0);
-    copy(1);
-    copy(2);
+    // fp32: a thread's pieces, eight elements of a row each, through registers, cut into parts on their way to LDS
+    constexpr int kMine = kWide ? kPrefixTile * kPieces / 256 : 1;
+    f32x4 kr[kMine][2], vr[kMine][2];
+    auto load = [&](int t) {
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) {
+            const int row = (256 * n + static_cast<int>(threadIdx.x)) / kPieces, row0 = (256 * n + 64 * w) / kPieces;
+            const long at = row_at(p_lo + min(t, ntiles - 1) * kPrefixTile + row0);
+            const uint32_t off = (row - row0) * row_bytes + 32 * (threadIdx.x % kPieces);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                kr[n][x] = *reinterpret_cast<const f32x4*>(kbase + at + off + 16 * x);
+                vr[n][x] = *reinterpret_cast<const f32x4*>(vbase + at + off + 16 * x);
+            }
+        }
+    };
+    auto store = [&](int t) {
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) {
+            const int row = (256 * n + static_cast<int>(threadIdx.x)) / kPieces, piece = threadIdx.x % kPieces;
+            if (t * kPrefixTile + row >= p_hi - p_lo)  // past the prefix: zeros, whatever the page holds
+                kr[n][0] = kr[n][1] = vr[n][0] = vr[n][1] = f32x4{0, 0, 0, 0};
+            u32x4 p[3];
+            cut8(kr[n], p);
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+                *reinterpret_cast<u32x4*>(ring + x * kTileB + row * kRowB + 16 * (piece ^ k_mix(row))) = p[x];
+            cut8(vr[n], p);
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+                *reinterpret_cast<u32x4*>(ring + kValues + x * kTileB + row * kRowB + 16 * (piece ^ v_mix(row))) = p[x];
+        }
+    };
+    if constexpr (kWide) {
+        load(0);
+    } else {
+        copy(0);
+        copy(1);
+        copy(2);
+    }
 
     // ---- the lane's row and query operand.  Rows that do not see the whole prefix are left to the workgroups of their
     // sequences: here they get empty records.
@@ -714,12 +776,12 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
                 }
             }
         float f;
-        row_factors<TYPE>(a.qscale, swap_max32(m, m), f, kf);
+        row_factors<kMath>(a.qscale, swap_max32(m, m), f, kf);
 #pragma unroll
         for (int j = 0; j < kKs; ++j) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[j][e] *= f;
-            split8<TYPE, kParts>(x[j], q[j]);
+            split8<kMath, kParts>(x[j], q[j]);
         }
     }
 
@@ -733,15 +795,22 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
 
     // the raw scores of tile t, a lane's 16: positions 8 (v >> 2) + 4 h + (v & 3)
     const char* const k_at = ring + i * kRowB;
+    // (parts: products of the small ones first, those of a K part and a query part below 2^-24 of the whole left out)
     auto scores = [&](int t, f32x16& s) {
-        const char* const kt = k_at + t % kRing * kTileB;
+        const char* const kt = k_at + (kWide ? 0 : t % kRing * kTileB);
         const f32x16 zero = {};
+        bool first = true;
 #pragma unroll
-        for (int ks = 0; ks < kKs; ++ks) {
-            const u32x4 k = *reinterpret_cast<const u32x4*>(kt + 16 * ((2 * ks + h) ^ k_mix(i)));
+        for (int ks = 0; ks < kKs; ++ks)
 #pragma unroll
-            for (int p = kParts - 1; p >= 0; --p) s = mma32(k, q[ks][p], ks == 0 && p == kParts - 1 ? zero : s, Type{});
-        }
+            for (int x = kKv - 1; x >= 0; --x) {
+                const u32x4 k = *reinterpret_cast<const u32x4*>(kt + x * kTileB + 16 * ((2 * ks + h) ^ k_mix(i)));
+#pragma unroll
+                for (int p = kParts - 1 - x; p >= 0; --p) {
+                    s = mma32(k, q[ks][p], first ? zero : s, Type{});
+                    first = false;
+                }
+            }
     };
     auto largest = [&](int t, f32x16& s) {
         const int left = p_hi - p_lo - t * kPrefixTile;
@@ -758,16 +827,22 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
     // V^T's operand of dim block d and positions 16 b .. : two reads of 4 x 16
     const int v_row = 4 * h + ((lane >> 2) & 3), v_col = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);  // row, byte in 64
     for (int tl = 0; tl < ntiles; ++tl) {
-        wait_copies<4 * kCopies>();  // tile tl
-        __syncthreads();
-        copy(tl + 3);
-        if (p_hi - p_lo - tl * kPrefixTile < kPrefixTile) {  // positions past the prefix: zeros, whatever their page holds
+        if constexpr (kWide) {
+            store(tl);
+            __syncthreads();
+            load(tl + 1);
+        } else {
+            wait_copies<4 * kCopies>();  // tile tl
+            __syncthreads();
+            copy(tl + 3);
+        }
+        if (!kWide && p_hi - p_lo - tl * kPrefixTile < kPrefixTile) {  // positions past the prefix: zeros, whatever their page holds
             const int left = p_hi - p_lo - tl * kPrefixTile;
             for (int x = threadIdx.x; x < (kPrefixTile - left) * kPieces; x += 256)
-                *reinterpret_cast<u32x4*>(ring + (kRing + tl % kRing) * kTileB + left * kRowB + 16 * x) = u32x4{0, 0, 0, 0};
+                *reinterpret_cast<u32x4*>(ring + kValues + tl % kRing * kTileB + left * kRowB + 16 * x) = u32x4{0, 0, 0, 0};
             __syncthreads();
         }
-        if (!active) continue;
+        if (active) {
         f32x16 s;
         scores(tl, s);
         const float m = largest(tl, s);
@@ -789,26 +864,31 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
                 p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * b + e], kf, -base));
                 sum += p[e];
             }
-            split8<TYPE, kParts>(p, pb[b]);
+            split8<kMath, kParts>(p, pb[b]);
         }
-        const char* const vt = ring + (kRing + tl % kRing) * kTileB;
+        const char* const vt = ring + kValues + (kWide ? 0 : tl % kRing * kTileB);
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int d = 0; d < kDb; ++d) {
-                u32x4 v;
+            for (int d = 0; d < kDb; ++d)
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int row = 16 * b + 8 * x + v_row;  // row & 3 and (row >> 1) & 1 are the lane's own
-                    const u32x2 y = read_transposed(vt + row * kRowB + ((64 * d) ^ (16 * v_mix(v_row))) + v_col);
-                    v[2 * x] = y.x;
-                    v[2 * x + 1] = y.y;
+                for (int y = kKv - 1; y >= 0; --y) {
+                    u32x4 v;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int row = 16 * b + 8 * x + v_row;  // row & 3 and (row >> 1) & 1 are the lane's own
+                        const u32x2 z =
+                            read_transposed(vt + y * kTileB + row * kRowB + ((64 * d) ^ (16 * v_mix(v_row))) + v_col);
+                        v[2 * x] = z.x;
+                        v[2 * x + 1] = z.y;
+                    }
+#pragma unroll
+                    for (int p = kParts - 1 - y; p >= 0; --p) o[d] = mma32(v, pb[b][p], o[d], Type{});
                 }
-#pragma unroll
-                for (int p = kParts - 1; p >= 0; --p) o[d] = mma32(v, pb[b][p], o[d], Type{});
-            }
+        }
+        if constexpr (kWide) __syncthreads();  // the parts have been read
     }
-    wait_copies<0>();
+    if constexpr (!kWide) wait_copies<0>();
 
     sum = swap_add32(sum, sum);
     if (sum != sum) mx = INFINITY;  // NaN scores leave no maximum: keep the record from being skipped
@@ -858,11 +938,12 @@ void run_paged_attn_type(const PagedAttnArgs& a, bool even, int blocks, hipStrea
 
 template <int TYPE>
 void run_paged_mixed_type(const PagedAttnArgs& a, int own_blocks, hipStream_t stream) {
-    const int lds = 2 * kRing * kPrefixTile * a.P.head_dim * 2;
+    const int lds = 2 * (TYPE == kKvF32 ? 3 : kRing) * kPrefixTile * a.P.head_dim * 2;
     const auto run = a.P.head_dim == 64 ? paged_mixed_kernel<TYPE, 64> : paged_mixed_kernel<TYPE, 128>;
     hipLaunchKernelGGL(run, dim3(a.pre_blocks + own_blocks), dim3(64 * kPagedWaves), lds, stream, a);
 }
 
+void run_paged_mixed_f32(const PagedAttnArgs& a, int own_blocks, hipStream_t stream);
 void run_paged_mixed_f16(const PagedAttnArgs& a, int own_blocks, hipStream_t stream);
 void run_paged_mixed_bf16(const PagedAttnArgs& a, int own_blocks, hipStream_t stream);
 void run_paged_attn_f32(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream);

@@ -304,8 +304,8 @@ def test_attention(kind, shape):
     assert torch.equal(out, again)  # sums in a fixed order
 
 
-# many rows of a KV head on a long prefix: from 2^18 rows x positions on, with 16-bit caches, heads of 64 and 128 and pages
-# of 16 n positions, the prefix is shared through LDS (else, and with fp32, other heads and pages: waves of their own)
+# many rows of a KV head on a long prefix: from 2^18 rows x positions on, with heads of 64 and 128 and pages of 16 n
+# positions, the prefix is shared through LDS (else, and with other heads and pages: waves of their own)
 MANY = [
     # counts, own, P, ps, H, Hkv, D
     ([1] * 33, [1 + 7 * i for i in range(33)], 256, 16, 4, 1, 64),         # a few rows, one tile, a whole number of tiles
@@ -372,7 +372,7 @@ def test_many_rows_some_inside_the_prefix(kind, D, P):
     assert torch.isnan(got[[t for t in range(len(q)) if pos[t] >= 350]]).all()
 
 
-@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
 @pytest.mark.parametrize("what", ["peak", "rising", "tiny_q", "huge_q", "large_v", "zero_q", "no_scale", "minus", "tiny_kv"])
 @pytest.mark.parametrize("P", [700, 1500])
 def test_many_rows_ranges(kind, what, P):
@@ -507,6 +507,24 @@ def test_attention_ranges(kind, what):
     out = attend(pool, off, held, rows, q, H, scale, prefix, P)
     want = ref.attention(q, pool.k, pool.v, off, held, rows, prefix, P, H, np.float32(scale).astype(np.float64), torch.zeros(q.shape))
     check_rows(out, want)
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_fp32_numbers_far_apart(many):
+    """fp32 keys and values of any size: dims 2^20 apart that the scores all need, values 2^40 apart between heads, 2^100
+    as a whole."""
+    H, Hkv, D, P, ps = 8, 2, 128, 700 if many else 100, 16
+    pool, off, held, rows, prefix, q = case("fp32", [2] * 60 if many else [2] * 3, [40 + i for i in range(60 if many else 3)],
+                                            P, ps, H, Hkv, D)
+    pool.k[..., ::2] *= 2.0 ** 20
+    q[:, ::2] *= 2.0 ** -20
+    pool.v[:, :, 1] *= 2.0 ** -40
+    pool.v *= 2.0 ** 100
+    out = attend(pool, off, held, rows, q, H, D ** -0.5, prefix, P)
+    want = ref.attention(q, pool.k, pool.v, off, held, rows, prefix, P, H, D ** -0.5, torch.zeros(q.shape))
+    for h in range(Hkv):  # each KV head by itself
+        part = slice(h * 4 * D, (h + 1) * 4 * D)
+        check_rows(out[:, part], want[:, part])
 
 
 def test_strided_rows_and_a_given_workspace():
@@ -731,7 +749,7 @@ def test_captured_steps_match_eager_ones():
         graph.advance()
 
 
-@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
 def test_captured_attention_of_many_rows(kind):
     """Captured once, replayed while the sequences grow, with eager work between: the eager bits."""
     H, Hkv, D, P, ps = 8, 2, 128, 1000, 16
