@@ -134,7 +134,7 @@ __global__ __launch_bounds__(kThreads) void head_rows_kernel(const RowArgs a) {
             }
         }
         if (turn && (is_q || is_k)) {
-// pair i: (x[i], x[4 + i]) of two halves, (x[2 i], x[2 i + 1]) of neighbours
+            // pair i: (x[i], x[4 + i]) of two halves, (x[2 i], x[2 i + 1]) of neighbours
             float y[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

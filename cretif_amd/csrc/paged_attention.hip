@@ -120,10 +120,10 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
         const int tile = c.staged ? kPrefixTile : own_tile, units = (prefix_len + tile - 1) / tile;
         c.pre_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
         const long streams = static_cast<long>(P.n_kv_heads) * c.pre_tiles;
-        // Chunks: the fewest microseconds of a model of the GPU.  Staged: a workgroup takes 9 and 1.4 per tile (fp16, heads of
-        // 128; half as much again where two share a CU), fills one of 512 slots, the sequences' workgroups the others (at half their tables' length: bytes
-        // at 4.7 TB/s), and 128 rows' record is written and read at that rate.  Else an item is a wave of 16 rows; 5 tiles'
-        // time for its start and end.
+        // Chunks: the fewest microseconds of a model of the GPU.  Staged: a workgroup takes 9 and 1.4 per tile (fp16, heads
+        // of 128; bf16 and fp32 by their products; half as much again where two share a CU), fills one of 512 slots, the
+        // sequences' workgroups the others (at half their tables' length: bytes at 4.7 TB/s), and 128 rows' record is
+        // written and read at that rate.  Else an item is a wave of 16 rows; 5 tiles' time for its start and end.
         const double own_us = 0.5 * B.n_seqs * own * P.n_kv_heads * D * (type == kKvF32 ? 8 : 4) / 4.7e6;
         const double tile_us = (type == kKvF16 ? 1.4 : type == kKvBF16 ? 1.9 : 2.8) * D / 128;
         const double record_us = tile_rows * (D + 4) * 8 / 4.7e6;

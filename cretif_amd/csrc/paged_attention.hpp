@@ -836,55 +836,55 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
             __syncthreads();
             copy(tl + 3);
         }
-        if (!kWide && p_hi - p_lo - tl * kPrefixTile < kPrefixTile) {  // positions past the prefix: zeros, whatever their page holds
+        if (!kWide && p_hi - p_lo - tl * kPrefixTile < kPrefixTile) {  // past the prefix: zeros, whatever the page holds
             const int left = p_hi - p_lo - tl * kPrefixTile;
             for (int x = threadIdx.x; x < (kPrefixTile - left) * kPieces; x += 256)
                 *reinterpret_cast<u32x4*>(ring + kValues + tl % kRing * kTileB + left * kRowB + 16 * x) = u32x4{0, 0, 0, 0};
             __syncthreads();
         }
         if (active) {
-        f32x16 s;
-        scores(tl, s);
-        const float m = largest(tl, s);
-        const bool raise = m > mx + S::kSlack;
-        if (__ballot(raise) != 0) {
-            const float f = raise ? __builtin_amdgcn_exp2f(mx - m) : 1.0f;
-            if (raise) mx = m;
-            sum *= f;
-#pragma unroll
-            for (int d = 0; d < kDb; ++d) o[d] *= f;
-        }
-        const float base = (mx == -INFINITY ? 0.0f : mx) - S::kShift;
-        u32x4 pb[2][kParts];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            float p[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * b + e], kf, -base));
-                sum += p[e];
+            f32x16 s;
+            scores(tl, s);
+            const float m = largest(tl, s);
+            const bool raise = m > mx + S::kSlack;
+            if (__ballot(raise) != 0) {
+                const float f = raise ? __builtin_amdgcn_exp2f(mx - m) : 1.0f;
+                if (raise) mx = m;
+                sum *= f;
+    #pragma unroll
+                for (int d = 0; d < kDb; ++d) o[d] *= f;
             }
-            split8<kMath, kParts>(p, pb[b]);
-        }
-        const char* const vt = ring + kValues + (kWide ? 0 : tl % kRing * kTileB);
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int d = 0; d < kDb; ++d)
-#pragma unroll
-                for (int y = kKv - 1; y >= 0; --y) {
-                    u32x4 v;
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int row = 16 * b + 8 * x + v_row;  // row & 3 and (row >> 1) & 1 are the lane's own
-                        const u32x2 z =
-                            read_transposed(vt + y * kTileB + row * kRowB + ((64 * d) ^ (16 * v_mix(v_row))) + v_col);
-                        v[2 * x] = z.x;
-                        v[2 * x + 1] = z.y;
-                    }
-#pragma unroll
-                    for (int p = kParts - 1 - y; p >= 0; --p) o[d] = mma32(v, pb[b][p], o[d], Type{});
+            const float base = (mx == -INFINITY ? 0.0f : mx) - S::kShift;
+            u32x4 pb[2][kParts];
+    #pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                float p[8];
+    #pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * b + e], kf, -base));
+                    sum += p[e];
                 }
+                split8<kMath, kParts>(p, pb[b]);
+            }
+            const char* const vt = ring + kValues + (kWide ? 0 : tl % kRing * kTileB);
+    #pragma unroll
+            for (int b = 0; b < 2; ++b)
+    #pragma unroll
+                for (int d = 0; d < kDb; ++d)
+    #pragma unroll
+                    for (int y = kKv - 1; y >= 0; --y) {
+                        u32x4 v;
+    #pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int row = 16 * b + 8 * x + v_row;  // row & 3 and (row >> 1) & 1 are the lane's own
+                            const u32x2 z =
+                                read_transposed(vt + y * kTileB + row * kRowB + ((64 * d) ^ (16 * v_mix(v_row))) + v_col);
+                            v[2 * x] = z.x;
+                            v[2 * x + 1] = z.y;
+                        }
+    #pragma unroll
+                        for (int p = kParts - 1 - y; p >= 0; --p) o[d] = mma32(v, pb[b][p], o[d], Type{});
+                    }
         }
         if constexpr (kWide) __syncthreads();  // the parts have been read
     }

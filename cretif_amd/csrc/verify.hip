@@ -75,19 +75,14 @@ __device__ __forceinline__ void accept(const VerifyArgs& a, int s, int& first, i
     acc = n - 1;
 }
 
-// the weight of a token: what the draft leaves of p, or p itself
+// the weights of tokens: what the draft leaves of p, or p itself
 struct Weight {
     const float* p;
     const float* q;  // null: none
     int sure;        // the token a draft without probabilities is sure of, or -1
-    __device__ __forceinline__ void of(int v, float pv, float qv, double& w, double& t) const {
-        t = pv > 0.0f ? static_cast<double>(pv) : 0.0;  // NaN counts as zero
-        w = t;
-        if (q != nullptr) {
-            w = t - static_cast<double>(qv);
-            w = w > 0.0 ? w : 0.0;
-        }
-        if (v == sure) w = 0.0;
+    // NaN and negative p count as zero, a NaN q leaves nothing (both maxima take the zero)
+    static __device__ __forceinline__ double of(float pv, float qv) {
+        return fmax(static_cast<double>(fmaxf(pv, 0.0f)) - static_cast<double>(qv), 0.0);
     }
     // tokens v .. v + 3, zeros from hi on
     __device__ __forceinline__ void load4(int v, int hi, f32x4& pv, f32x4& qv) const {
@@ -103,6 +98,14 @@ struct Weight {
                     if (q != nullptr) qv[i] = q[v + i];
                 }
             }
+        }
+    }
+    // what load4 read, without the sure token
+    __device__ __forceinline__ void drop4(int v, f32x4& pv) const {
+        if (sure >= 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (v + i == sure) pv[i] = 0.0f;
         }
     }
 };
@@ -162,14 +165,13 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyArgs 
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) W.load4(v0 + 4 * kThreads * j, hi, p[j], q[j]);
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j)
+        for (int j = 0; j < kAhead; ++j) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                double x, y;
-                W.of(v0 + 4 * kThreads * j + i, p[j][i], q[j][i], x, y);
-                w += x;
-                t += y;
-            }
+            for (int i = 0; i < 4; ++i) t += Weight::of(p[j][i], 0.0f);
+            W.drop4(v0 + 4 * kThreads * j, p[j]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w += Weight::of(p[j][i], q[j][i]);
+        }
     }
     w = wave_sum(w);
     t = wave_sum(t);
@@ -189,6 +191,13 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyArgs 
     }
 }
 
+// the sequence's output rows but the drawn one; id: the thread's drafted token
+__device__ __forceinline__ void write_rest(const VerifyArgs& a, int first, int n, int acc, int id) {
+    if (static_cast<int>(threadIdx.x) < acc) a.out[first + threadIdx.x] = id;
+    for (int j = threadIdx.x + kPickThreads; j < acc; j += kPickThreads) a.out[first + j] = a.ids[first + j];
+    for (int j = acc + 1 + threadIdx.x; j < n; j += kPickThreads) a.out[first + j] = -1;
+}
+
 // grid (sequences): the token, the sequence's output rows
 __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyArgs a) {
     __shared__ double part[kPickWaves];
@@ -200,6 +209,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
         return;
     }
     Weight W = weight_of(a, first, n, acc);
+    const float number = a.draws[first + acc];  // (on their way beside the sums)
+    const int id = static_cast<int>(threadIdx.x) < acc ? a.ids[first + threadIdx.x] : -1;
     // every wave: the totals, then the first slice whose running sum exceeds the wanted one, else the last with weight
     const double* sums = a.sums + static_cast<long>(s) * a.slices * 2;
     double total = 0.0, plain = 0.0;
@@ -215,7 +226,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
         W.sure = -1;
         total = plain;
     }
-    const double want = a.draws[first + acc] * total;
+    const double want = number * total;
     double before = 0.0, run = 0.0;
     int slice = -1;
     for (int base = 0; base < a.slices; base += 64) {
@@ -235,14 +246,15 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
     int token = -1;  // no weight anywhere
     if (slice >= 0) {
         const int lo = slice * a.per, hi = min(lo + a.per, a.V), v0 = lo + kPer * threadIdx.x;
-        double x[kPer], sum = 0.0, y;
+        double x[kPer], sum = 0.0;
 #pragma unroll
         for (int j = 0; j < kPer; j += 4) {
             f32x4 p, q;
             W.load4(v0 + j, hi, p, q);
+            W.drop4(v0 + j, p);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                W.of(v0 + j + i, p[i], q[i], x[j + i], y);
+                x[j + i] = Weight::of(p[i], q[i]);
                 sum += x[j + i];
             }
         }
@@ -277,9 +289,118 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
         for (int i = kPickWaves - 1; i >= 0; --i)
             if (found[i] >= 0) token = found[i];
     }
-    for (int j = threadIdx.x; j < n; j += kPickThreads)
-        a.out[first + j] = j < acc ? a.ids[first + j] : j == acc ? token : -1;
-    if (threadIdx.x == 0) a.accepted[s] = acc;
+    if (threadIdx.x == 0) {
+        a.out[first + acc] = token;
+        a.accepted[s] = acc;
+    }
+    write_rest(a, first, n, acc, id);
+}
+
+// grid (sequences), vocabularies up to kRowVocab: the whole of it in one kernel.  Wave w holds the w-th of the row's
+// sixteenths in registers, 256 tokens at a time; the waves' sums name the wave whose tokens are drawn from, which sums its
+// 256s one by one.
+constexpr int kQuads = 8, kRowVocab = 4 * kQuads * kPickThreads;  // kQuads: of a thread
+
+// QUADS: of a thread at most; Q: there are draft probabilities
+template <int QUADS, bool Q>
+__global__ __launch_bounds__(kPickThreads) void verify_row_kernel(const VerifyArgs a) {
+    __shared__ double part[2][kPickWaves];
+    const int s = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int first, n, acc;
+    accept(a, s, first, n, acc);
+    if (n == 0) {
+        if (threadIdx.x == 0) a.accepted[s] = 0;
+        return;
+    }
+    Weight W = weight_of(a, first, n, acc);
+    const int slabs = (a.V + 256 * kPickWaves - 1) / (256 * kPickWaves), v0 = wave * slabs * 256 + 4 * lane;
+    f32x4 p[QUADS], q[Q ? QUADS : 1];
+    const float number = a.draws[first + acc];
+    const int id = static_cast<int>(threadIdx.x) < acc ? a.ids[first + threadIdx.x] : -1;
+    auto load = [&]() {
+#pragma unroll
+        for (int j = 0; j < QUADS; ++j) W.load4(v0 + 256 * j, j < slabs ? a.V : 0, p[j], q[Q ? j : 0]);
+#pragma unroll
+        for (int j = 0; j < QUADS; ++j) W.drop4(v0 + 256 * j, p[j]);
+    };
+    auto weight = [&](int j, int i) { return Weight::of(p[j][i], Q ? q[j][i] : 0.0f); };
+    load();
+
+    double c, want;
+    int pick;
+#pragma unroll 1
+    for (int turn = 0; turn < 2; ++turn) {  // again from p itself where the draft leaves nothing
+        double w = 0.0;
+#pragma unroll
+        for (int j = 0; j < QUADS; ++j)
+            if (j < slabs) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w += weight(j, i);
+            }
+        w = wave_sum(w);
+        if (lane == 0) part[turn][wave] = w;
+        __syncthreads();
+        const double x = lane < kPickWaves ? part[turn][lane] : 0.0;
+        double prev;
+        c = scan_up(x, lane, prev);
+        const double total = lane_f64(c, 63);
+        want = number * total;
+        const unsigned long hit = __ballot(x > 0.0 && c > want), any = __ballot(x > 0.0);
+        pick = hit ? __builtin_ctzl(hit) : any ? 63 - __builtin_clzl(any) : -1;
+        c = prev;
+        if (total > 0.0) break;
+        W.q = nullptr;
+        W.sure = -1;
+        load();
+    }
+    if (wave == max(pick, 0)) {
+        int token = -1;
+        if (pick >= 0) {
+            double run = lane_f64(c, pick), at = run, x[4] = {};
+            int slab = 0;
+            bool done = false;
+#pragma unroll
+            for (int j = 0; j < QUADS; ++j) {
+                if (j >= slabs || done) continue;
+                double y[4], sum = 0.0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    y[i] = weight(j, i);
+                    sum += y[i];
+                }
+                sum = wave_sum(sum);
+                if (sum > 0.0) {  // the first whose running sum exceeds the wanted one, else the last with weight
+                    slab = j, at = run;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = y[i];
+                    done = run + sum > want;
+                }
+                run += sum;
+            }
+            const double sum = ((x[0] + x[1]) + x[2]) + x[3];
+            double prev;
+            const double up = scan_up(sum, lane, prev);
+            const unsigned long hit = __ballot(sum > 0.0 && at + up > want), any = __ballot(sum > 0.0);
+            int mine = 0;
+            double here = at + prev;
+            done = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                here += x[i];
+                if (x[i] > 0.0 && !done) {
+                    mine = i;
+                    done = here > want;
+                }
+            }
+            const int who = hit ? __builtin_ctzl(hit) : 63 - __builtin_clzl(any);
+            token = wave * slabs * 256 + slab * 256 + 4 * who + __builtin_amdgcn_readlane(mine, who);
+        }
+        if (lane == 0) {
+            a.out[first + acc] = token;
+            a.accepted[s] = acc;
+        }
+    }
+    write_rest(a, first, n, acc, id);
 }
 
 // tokens of a slice: about 1024 workgroups over all sequences, 1024 to kMaxSlice tokens each
@@ -301,6 +422,16 @@ long verify_workspace_bytes(int n_seqs, int vocab) {
 int launch_verify_drafts(const float* target, long ldt, const float* draft, long ldd, const int* ids, const float* u,
                          const float* draws, const int* offsets, int n_seqs, int n_rows, int vocab, int* out, int* accepted,
                          double* ws, hipStream_t stream) {
+    if (vocab <= dev::kRowVocab) {
+        const dev::VerifyArgs a{target, draft, ldt, ldd, ids, u, draws, offsets, out, accepted, nullptr, nullptr,
+                                n_seqs, n_rows, vocab, 1, vocab};
+        const auto run = vocab <= dev::kRowVocab / 4 ? (draft ? dev::verify_row_kernel<dev::kQuads / 4, true>
+                                                              : dev::verify_row_kernel<dev::kQuads / 4, false>)
+                                                     : (draft ? dev::verify_row_kernel<dev::kQuads, true>
+                                                              : dev::verify_row_kernel<dev::kQuads, false>);
+        hipLaunchKernelGGL(run, dim3(n_seqs), dim3(dev::kPickThreads), 0, stream, a);
+        return 0;
+    }
     const int per = dev::slice_of(n_seqs, vocab), slices = (vocab - 1) / per + 1;
     if (static_cast<long>(n_seqs) * slices >= 1L << 24) return kDeclined;  // 256 threads each: a launch's limit
     const dev::VerifyArgs a{target, draft, ldt, ldd, ids, u, draws, offsets, out, accepted, ws,

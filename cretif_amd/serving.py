@@ -62,6 +62,13 @@ def _on_device(t, name, dev=None):
     return t.data_ptr()
 
 
+def _all_on(dev, *descriptors):
+    """What the descriptors hold must be on the device that is current at the call, too."""
+    for d in descriptors:
+        if d._dev is not None and d._dev != dev:
+            raise ValueError("the tensors of a %s are on cuda:%d, not on the current device" % (type(d).__name__, d._dev))
+
+
 def _rows(t, width, name, dev):
     """(address, floats from row to row, rows or None) of a row buffer of `width` floats a row."""
     if type(t) is tuple:
@@ -131,7 +138,7 @@ class Rotation:
         self._c = _Rotation(None if q_norm is None else _on_device(q_norm, "q_norm"),
                             None if k_norm is None else _on_device(k_norm, "k_norm"), eps, theta, rot_dim, PAIRS[pairs])
         self._ref = ctypes.addressof(self._c)
-
+        self._dev = None if q_norm is None and k_norm is None else _device()
         self._widths = {w.shape[0] for w in (q_norm, k_norm) if w is not None}
 
     def _fits(self, head_dim):
@@ -158,6 +165,7 @@ class PagedKV:
         stride = k.stride(0) if n > 1 else (ps * h * d + 7) // 8 * 8
         self._c = _PagedKV(_on_device(k, "k"), _on_device(v, "v"), stride, kinds[k.dtype], n, ps, h, d)
         self._ref = ctypes.addressof(self._c)
+        self._dev = _device()
 
 
 class PagedBatch:
@@ -172,6 +180,7 @@ class PagedBatch:
         self.offsets, self.lens, self.pages = offsets, lens, pages
         self._make = lambda rows: _PagedBatch(po, pl, pp, n, rows, pages.shape[1])
         self._by_rows = {}
+        self._dev = _device()
 
     def _for(self, n_rows):
         c = self._by_rows.get(n_rows)  # descriptors differ in their row count alone: one per count, never changed
@@ -186,6 +195,7 @@ def qk_norm_rope(rot, q, k, q_out, k_out, positions, n_heads, n_kv_heads, head_d
     be q and k_out k.  q (with n_heads 0) or k (with n_kv_heads 0) may be None."""
     L, dev = _torch(), _device()
     rot._fits(head_dim)
+    _all_on(dev, rot)
     pq = lq = po = lo = pk = lk = px = lx = 0
     nq = no = nk = nx = None
     if q is not None:
@@ -208,6 +218,7 @@ def paged_append(cache, batch, rot, k, v, q=None, q_out=None, n_heads=0, n_rows=
     L, dev = _torch(), _device()
     D = cache.head_dim
     rot._fits(D)
+    _all_on(dev, cache, batch, rot)
     pk, lk, nk = _rows(k, cache.n_kv_heads * D, "k", dev)
     pv, lv, nv = _rows(v, cache.n_kv_heads * D, "v", dev)
     pq = lq = po = lo = 0
@@ -237,6 +248,7 @@ def paged_attention(cache, batch, q, out, n_heads, scale, prefix_pages=None, pre
     paged_attention_workspace_bytes (one is allocated when None)."""
     L, dev = _torch(), _device()
     width = n_heads * cache.head_dim
+    _all_on(dev, cache, batch)
     pq, lq, nq = _rows(q, width, "q", dev)
     po, lo, no = _rows(out, width, "out", dev)
     n = _same_rows(n_rows, ("q", nq), ("out", no))

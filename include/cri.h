@@ -446,8 +446,9 @@ long long cri_paged_attention_workspace_bytes(const cri_paged_kv* kv, const cri_
  * that has decided about its draft must not draw its replacement too.
  * out_ids [n_rows]: the accepted drafts, the drawn token, -1 in the sequence's remaining rows;
  * n_accepted [n_seqs].  Rows outside [offsets[0], offsets[n_seqs]) are neither read nor written, a
- * sequence of no rows gets n_accepted 0.  NaN and negative probabilities count as zero.  Comparisons
- * and sums are in 64 bits and in a fixed order.
+ * sequence of no rows gets n_accepted 0.  A target probability that is NaN or negative counts as
+ * zero; where a draft's is NaN its token is not accepted and has no weight.  Comparisons and sums
+ * are in 64 bits and in a fixed order.
  * out_ids must not overlap draft_ids.  workspace: 8-byte aligned, cri_verify_drafts_workspace_bytes. */
 int cri_verify_drafts(const float* target, long long ldt, const float* draft, long long ldd, const int* draft_ids,
                       const float* uniforms, const float* draws, const int* offsets, int n_seqs, int n_rows,

@@ -185,6 +185,26 @@ def test_lens_out_of_range():
         assert (out == 0).all()
 
 
+def test_descriptors_of_another_device():
+    """Descriptors made on one device are refused where another is current (their pointers are not that one's)."""
+    pool = Pool(4, 16, 1, 64, "fp16")
+    b = cri.PagedBatch(ints([0, 1]), ints([5]), ints([[0, 1]]))
+    rot = cri.Rotation(1e4, 64, q_norm=randn(64))
+    x, out = randn(1, 64), torch.zeros(1, 64, device="cuda")
+    for thing in (pool.kv, b, rot):
+        thing._dev += 1
+        with pytest.raises(ValueError, match="current device"):
+            cri.paged_append(pool.kv, b, rot, x, x)
+        with pytest.raises(ValueError, match="current device"):
+            if thing is rot:
+                cri.qk_norm_rope(rot, x, None, out, None, ints([3]), 1, 0, 64)
+            else:
+                cri.paged_attention(pool.kv, b, x, out, 1, 0.125)
+        thing._dev -= 1
+    cri.paged_append(pool.kv, b, rot, x, x)
+    cri.paged_attention(pool.kv, b, x, out, 1, 0.125)
+
+
 def test_in_place_on_the_fused_rows():
     """q and k normed and rotated where the fused product left them; the values beside them untouched."""
     M, H, Hkv, D = 5, 4, 2, 64
@@ -576,6 +596,8 @@ def drafts(counts, V, seed, sure, near=1.0, first=0, behind=0):
 @pytest.mark.parametrize("counts,V", [
     ([1], 1), ([2], 2), ([1], 1000), ([5], 128256), ([3, 0, 1, 6, 2], 1023), ([4] * 9, 1024), ([9, 1, 2], 1025),
     ([70, 3], 50), ([2] * 300, 257), ([1 + i % 7 for i in range(40)], 5000),
+    ([1100, 3], 40), ([2, 1, 4], 4096), ([3, 3], 4097), ([4, 2], 32767), ([3, 1, 2, 5], 32768), ([2, 4, 1], 32769),
+    ([5, 3], 20000), ([1030, 2], 32800),
 ])
 def test_verify(sure, counts, V):
     check_verify(*drafts(counts, V, seed=V + len(counts), sure=sure, first=2, behind=1))
@@ -596,7 +618,7 @@ def test_verify_the_same_distribution_accepts_all():
 
 
 @pytest.mark.parametrize("d", [0.0, 0.5, 1 - 2.0 ** -24, 1.0, 5.0, -1.0, float("nan")])
-@pytest.mark.parametrize("V", [8, 2048, 5000])
+@pytest.mark.parametrize("V", [8, 2048, 5000, 40000])
 def test_verify_borders(d, V):
     """Equal weights of a power of two: the running sum meets the number exactly; zeros at both ends."""
     p = torch.zeros(2, V, device="cuda")
@@ -605,9 +627,9 @@ def test_verify_borders(d, V):
     assert out[0].item() == {0.0: 2, 0.5: 4, -1.0: 2}.get(d, 5)
 
 
-def test_verify_odd_probabilities():
+@pytest.mark.parametrize("V", [1500, 33000])
+def test_verify_odd_probabilities(V):
     """Invalid drafted tokens, drafts that leave nothing, rows of zeros, of NaN, of negatives."""
-    V = 1500
     t = torch.softmax(randn(12, V, seed=3), -1)
     q = torch.softmax(randn(12, V, seed=4), -1)
     q[0] = 2.0           # row 0: the draft leaves nothing of the target
@@ -624,9 +646,10 @@ def test_verify_odd_probabilities():
     check_verify(t, q, [V] * 12, u, d, [0, 12])
 
 
-def test_verify_leaves_no_trace_in_the_workspace_of_others():
-    target, draft, ids, u, d, off = drafts([3, 4, 2], 3000, seed=6, sure=False)
-    n = cri.verify_drafts_workspace_bytes(3, 3000)
+@pytest.mark.parametrize("V", [3000, 50000])
+def test_verify_leaves_no_trace_in_the_workspace_of_others(V):
+    target, draft, ids, u, d, off = drafts([3, 4, 2], V, seed=6, sure=False)
+    n = cri.verify_drafts_workspace_bytes(3, V)
     room = torch.full((n + 64,), 255, dtype=torch.uint8, device="cuda")
     out, acc = torch.zeros(9, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
     cri.verify_drafts(target, draft, ints(ids), u, d, ints(off), out, acc, room[:n])
