@@ -8,13 +8,15 @@
 //
 //   * u q(x) < p(x) is decided in 64 bits, where the product of two 32-bit numbers is exact.
 //   * Weights are differences in 64 bits and so are their sums, whose order is fixed: thread, wave, slice.
-//   * Bound by memory: one row of p and of q per sequence (2 V floats), whatever the number of drafts.  A sequence's
-//     rows are cut into slices over workgroups, so that a single sequence, too, is read by many CUs.  The second
-//     kernel finds the slice by the slices' sums and the token within it in one pass of 1024 threads, eight tokens
-//     each, over that slice alone, which the first kernel has left in the caches.
-//
-// Vocabulary 128256: 64 sequences 12.5 us (65.7 MB at 5.3 TB/s) and 6.3 us for the two kernels, one sequence 4.0 and 6.2;
-// 200 sequences at 32000 10.6 and 6.0.  The second is the chain of trips to memory behind the first's sums.
+//   * Bound by memory: one row of p and of q per sequence (2 V floats), whatever the number of drafts.
+//   * Up to 32768 tokens a sequence's row fits the registers of one workgroup of 1024 threads, and one kernel does it all
+//     (verify_row_kernel).  Us in a graph, against the two kernels below at 33000: one sequence 7.0 / 9.0, 64 9.2 / 12.8, 200
+//     12.0 / 19.3, 256 14.0 / 20.3; 200 with sure drafts, 25.6 MB, 9.7.  1000 tokens: 3.9 for one sequence, 4.5 for 256.
+//   * Longer rows are cut into slices over workgroups, so that a single sequence, too, is read by many CUs
+//     (verify_sums_kernel).  The second kernel finds the slice by the slices' sums and the token within it in one pass of
+//     1024 threads, eight tokens each, over that slice alone, which the first kernel has left in the caches.  128256
+//     tokens: 64 sequences 12.6 us (65.7 MB at 5.2 TB/s) and 6.3 us, one sequence 4.0 and 6.3, the second being the chain of
+//     trips to memory behind the first's sums.
 #include <algorithm>
 
 #include "common.hpp"
@@ -102,11 +104,8 @@ struct Weight {
     }
     // what load4 read, without the sure token
     __device__ __forceinline__ void drop4(int v, f32x4& pv) const {
-        if (sure >= 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (v + i == sure) pv[i] = 0.0f;
-        }
+        for (int i = 0; i < 4; ++i) pv[i] = v + i == sure ? 0.0f : pv[i];
     }
 };
 __device__ __forceinline__ Weight weight_of(const VerifyArgs& a, int first, int n, int acc) {
@@ -320,8 +319,10 @@ __global__ __launch_bounds__(kPickThreads) void verify_row_kernel(const VerifyAr
     auto load = [&]() {
 #pragma unroll
         for (int j = 0; j < QUADS; ++j) W.load4(v0 + 256 * j, j < slabs ? a.V : 0, p[j], q[Q ? j : 0]);
+        if constexpr (!Q) {
 #pragma unroll
-        for (int j = 0; j < QUADS; ++j) W.drop4(v0 + 256 * j, p[j]);
+            for (int j = 0; j < QUADS; ++j) W.drop4(v0 + 256 * j, p[j]);
+        }
     };
     auto weight = [&](int j, int i) { return Weight::of(p[j][i], Q ? q[j][i] : 0.0f); };
     load();
