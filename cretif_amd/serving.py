@@ -74,8 +74,11 @@ def _rows(t, width, name, dev):
     if type(t) is tuple:
         return t[0], t[1], None
     sh, st = t.shape, t.stride()
-    if len(sh) == 2 and sh[0] > 1 and st[1] == 1 and sh[1] == width and t.dtype is torch.float32:  # the usual case first
-        return _on_device(t, name, dev), st[0], sh[0]
+    if len(sh) == 2:  # the usual case first
+        n, w = sh
+        ld, one = st
+        if w == width and one == 1 and t.dtype is torch.float32 and t.get_device() == dev:
+            return t.data_ptr(), ld if n > 1 or ld > width else width, n  # (the stride of a single row says nothing)
     if t.dtype is not torch.float32:
         raise ValueError("%s must be float32, not %s" % (name, t.dtype))
     if len(sh) not in (2, 3):
@@ -85,7 +88,6 @@ def _rows(t, width, name, dev):
         raise ValueError("%s has rows of %d floats, not %d" % (name, wide, width))
     if (inner > 1 and st[-1] != 1) or (len(sh) == 3 and sh[1] > 1 and st[1] != inner):
         raise ValueError("%s: the elements of a row must be consecutive" % name)
-    # the stride of a single row says nothing
     return _on_device(t, name, dev), st[0] if sh[0] > 1 else max(st[0], width), sh[0]
 
 
@@ -103,6 +105,8 @@ def _same_rows(n_rows, *named):
 def _ints(t, name, dims, dev=None):
     if t.dtype is not torch.int32 or t.dim() != dims or not t.is_contiguous():
         raise ValueError("%s must be a contiguous int32 tensor of %d dimension(s)" % (name, dims))
+    if t.get_device() == dev:
+        return t.data_ptr()
     return _on_device(t, name, dev)
 
 
