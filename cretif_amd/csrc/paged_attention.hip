@@ -111,7 +111,12 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
     // Measured, heads of 128, 100 own positions, staged against waves of their own: 64 rows on 4096 positions 19.4 / 19.9 us,
     // 128 on 1024 18.2 / 17.8, on 4096 24.6 / 25.4, 512 on 512 23.8 / 27.5, on 2048 32.1 / 38.9, 2048 on 1024 80 / 111
     // (fp32: 30.7 / 29.0, 25.9 / 23.0, 36 / 41, 38 / 45, 62 / 86, 138 / 210).
-    c.staged = c.even && D <= 128 && rows > 32 && prefix_len >= 256 && rows * prefix_len >= 1L << 18;
+    // Other heads and pages of 20: 128 rows on 4096 positions 26.7 / 30.4 (heads of 128), 21.1 / 27.0 (80; fp32 31.2 / 48.2),
+    // 15.9 / 21.9 (40), 512 on 2048 34.3 / 47.7, 30.2 / 43.6 (49.5 / 87.9), 23.0 / 33.0, 1920 on 32768 518 / 1407, 411 / 1328 (1053 /
+    // 3651), 299 / 974.  Heads of 256, a workgroup to a CU: fp16 512 on 1024 47 / 44, 512 on 4096 63 / 72, 1920 on 32768 606 / 1315,
+    // bf16 512 on 4096 80 / 78, 1920 on 32768 1028 / 1347; fp32 was slower or equal everywhere.
+    const int from = D <= 128 ? 18 : type == kKvF16 ? 20 : type == kKvBF16 ? 22 : 62;
+    c.staged = rows > 32 && prefix_len >= 256 && rows * prefix_len >= 1L << from;
     const int own_tile = type == kKvF32 ? 16 : 32;
     const long cap = static_cast<long>(B.max_pages) * P.page_size;
     const long own = std::max(cap - prefix_len / own_tile * own_tile, 1L);
@@ -126,19 +131,20 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
         // written and read at that rate.  Else an item is a wave of 16 rows; 5 tiles' time for its start and end.
         const double own_us = 0.5 * B.n_seqs * own * P.n_kv_heads * D * (type == kKvF32 ? 8 : 4) / 4.7e6;
         const double tile_us = (type == kKvF16 ? 1.4 : type == kKvBF16 ? 1.9 : 2.8) * D / 128;
+        const int slots = D <= 128 ? kSlots : kSlots / 2;
         const double record_us = tile_rows * (D + 4) * 8 / 4.7e6;
         double best = 0.0;
         for (int n = 1; n <= kPreRecords && n <= units; ++n) {
             const long items = streams * n, per = (units + n - 1) / n;
             double cost;
             if (c.staged) {
-                const double alone = tile_us * per + 9.0, rounds = static_cast<double>((items + kSlots - 1) / kSlots);
-                const double longest = rounds * (items <= kSlots / 2 ? alone : 1.5 * tile_us * per + 9.0);
-                cost = std::max(longest, items * alone / kSlots + own_us) + items * record_us;
+                const double alone = tile_us * per + 9.0, rounds = static_cast<double>((items + slots - 1) / slots);
+                const double longest = rounds * (items <= slots / 2 || D > 128 ? alone : 1.5 * tile_us * per + 9.0);
+                cost = std::max(longest, items * alone / slots + (D <= 128 ? own_us : 0.0)) + items * record_us;
             } else {
-                const int slots = kPagedWaves * kSlots;
-                const double rounds = items <= slots / 2 ? 0.65 : static_cast<double>((items + slots - 1) / slots);
-                cost = 1.4 * (rounds * per + 5.0 * ((items + slots - 1) / slots)) + items * record_us;
+                const int waves = kPagedWaves * kSlots;
+                const double rounds = items <= waves / 2 ? 0.65 : static_cast<double>((items + waves - 1) / waves);
+                cost = 1.4 * (rounds * per + 5.0 * ((items + waves - 1) / waves)) + items * record_us;
             }
             if (best == 0.0 || cost < best) {
                 best = cost;
@@ -198,7 +204,7 @@ int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, cons
     if (c.staged)
         (type == kKvF32   ? dev::run_paged_mixed_f32
          : type == kKvF16 ? dev::run_paged_mixed_f16
-                          : dev::run_paged_mixed_bf16)(a, static_cast<int>(c.own_blocks), stream);
+                          : dev::run_paged_mixed_bf16)(a, c.even, static_cast<int>(c.own_blocks), stream);
     else
         run_rows(a, c.even, static_cast<int>(c.pre_blocks + c.own_blocks), stream);
     if (c.nrec > 1) {

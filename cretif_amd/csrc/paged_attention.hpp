@@ -608,9 +608,8 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
             }
 }
 
-// The shared prefix against many rows (head_dim 64 and 128, pages of 16 n positions).  A workgroup of four
-// waves takes 128 rows, 32 to a wave, and a chunk of the prefix in tiles of 32 positions that all its waves read from LDS:
-// straight from the pool every wave would load 16 KB for the 2 x 0.5 MFLOP it does with a tile, more than the L1 delivers
+// The shared prefix against many rows.  A workgroup of four waves takes 128 rows, 32 to a wave, and a chunk of the prefix in
+// tiles of 32 positions that all its waves read from LDS: straight from the pool every wave would load 16 KB for the 2 x 0.5 MFLOP it does with a tile, more than the L1 delivers
 // beside the matrix instructions.  v_mfma_f32_32x32x16: half the instructions of 16x16x32 for the same product.
 //   * 16-bit tiles go to LDS with global_load_lds, whole rows at a time, into rings of four, three tiles ahead; one barrier per
 //     tile.  The 16-byte pieces of a row are exchanged within it: K's so that the 32 rows of an operand fetch lie in
@@ -627,6 +626,7 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
 // 32 products.  Issuing the next tile's scores between them, and operands read ahead, were measured at 562 to 585 us against
 // 541: more registers, the same power.
 constexpr int kPrefixRows = 128, kPrefixTile = 32, kRing = 4;
+constexpr int prefix_lds(int type, int dp) { return 2 * (type == kKvF32 ? 3 : kRing) * kPrefixTile * dp * 2; }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c, std::integral_constant<int, kKvF16>) {
@@ -662,20 +662,24 @@ __device__ __forceinline__ void wait_copies() {  // all but the last N copies of
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
 }
 
-template <int TYPE, int D>
+// EVEN: head_dim is DP and the page size a multiple of 16.  Else every lane looks up the page of its own row (a tile ahead of
+// the copy that needs it), pieces behind head_dim are the row's first one again (the query is zero there) and blocks of dims
+// behind it are not multiplied: 480 rows x 32 heads on 32768 positions, pages of 20 525 us (waves of their own 1407), heads of
+// 80 411 (1328), 40 299 (974).
+template <int TYPE, int DP, bool EVEN>
 __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int block, char* const ring) {
     constexpr bool kWide = TYPE == kKvF32;                        // K and V, too, are taken in three bf16 parts
     constexpr int kMath = kWide ? kKvBF16 : TYPE, kKv = kWide ? 3 : 1;
-    typedef PagedShape<kMath, D> S;
+    typedef PagedShape<kMath, DP> S;
     typedef std::integral_constant<int, kMath> Type;
-    constexpr int kParts = S::kParts, kKs = D / 16, kDb = D / 32, kRowB = 2 * D, kPieces = kRowB / 16;
+    constexpr int kParts = S::kParts, kKs = DP / 16, kDb = DP / 32, kRowB = 2 * DP, kPieces = kRowB / 16;
     // bytes of (a part of) a tile's K or V; ring: K's tiles or parts, then V's
     constexpr int kTileB = kPrefixTile * kRowB, kValues = (kWide ? kKv : kRing) * kTileB;
     constexpr int kCopies = kTileB / 1024 / 4;  // of a wave, of a tile's K or V
 
     const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int Hkv = a.P.n_kv_heads, G = a.G, nrows = a.B.n_rows * G;
+    const int Hkv = a.P.n_kv_heads, G = a.G, nrows = a.B.n_rows * G, D = EVEN ? DP : a.P.head_dim;
     constexpr int kEs = kWide ? 4 : 2;
     const uint32_t row_bytes = static_cast<uint32_t>(Hkv) * D * kEs;
     int chunk, kvh, tile;
@@ -687,15 +691,16 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
     // ---- the copies: a wave's rows of a tile lie in one page (8 rows each; 16 share a page)
     const char* const kbase = static_cast<const char*>(a.P.k) + static_cast<long>(kvh) * D * kEs;
     const char* const vbase = static_cast<const char*>(a.P.v) + static_cast<long>(kvh) * D * kEs;
-    auto k_mix = [&](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
-    auto v_mix = [&](int row) { return D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; };
+    auto k_mix = [&](int row) { return DP >= 128 ? row & 15 : (row >> 1) & 7; };
+    auto v_mix = [&](int row) { return DP >= 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; };
+    auto real = [&](int piece) { return EVEN || 8 * piece < D ? piece : 0; };
     constexpr int kCopyRows = 64 / kPieces;
-    uint32_t k_off[kCopies], v_off[kCopies];  // bytes of the lane's pieces from the wave's first row
+    uint32_t k_off[kCopies], v_off[kCopies];  // bytes of the lane's pieces from the wave's first row (not EVEN: from their own)
 #pragma unroll
     for (int n = 0; n < kCopies; ++n) {
         const int r = n * kCopyRows + lane / kPieces, row = 8 * w + r;
-        k_off[n] = r * row_bytes + 16 * (lane % kPieces ^ k_mix(row));
-        v_off[n] = r * row_bytes + 16 * (lane % kPieces ^ v_mix(row));
+        k_off[n] = (EVEN ? r * row_bytes : 0) + 16 * real(lane % kPieces ^ k_mix(row));
+        v_off[n] = (EVEN ? r * row_bytes : 0) + 16 * real(lane % kPieces ^ v_mix(row));
     }
     auto row_at = [&](int pos) {  // byte offset of a (uniform) position's row
         const int pi = page_index(a.P, pos);
@@ -703,29 +708,58 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
         return (static_cast<unsigned>(pg) < static_cast<unsigned>(a.P.n_pages) ? pg : 0) * a.P.stride * kEs +
                static_cast<long>(pos - pi * a.P.page_size) * row_bytes;
     };
-    auto copy = [&](int t) {  // tile t (past the last one: that one again, so that every turn issues as many)
-        const long at = row_at(p_lo + min(t, ntiles - 1) * kPrefixTile + 8 * w);
-        char* const dst = ring + t % kRing * kTileB + 8 * w * kRowB;
-#pragma unroll
-        for (int n = 0; n < kCopies; ++n) dma16(kbase + at + k_off[n], dst + n * 1024);
-#pragma unroll
-        for (int n = 0; n < kCopies; ++n) dma16(vbase + at + v_off[n], dst + kValues + n * 1024);
-    };
     // fp32: a thread's pieces, eight elements of a row each, through registers, cut into parts on their way to LDS
     constexpr int kMine = kWide ? kPrefixTile * kPieces / 256 : 1;
+    constexpr int kIds = kWide ? kMine : kCopies;  // rows of a tile that a lane has pieces of
+    auto lane_pos = [&](int t, int n) {
+        const int row = kWide ? (256 * n + static_cast<int>(threadIdx.x)) / kPieces : 8 * w + n * kCopyRows + lane / kPieces;
+        return p_lo + min(t, ntiles - 1) * kPrefixTile + row;
+    };
+    int ids[kIds] = {};  // their pages, of the tile that is copied next
+    auto look_up = [&](int t, int (&ids)[kIds]) {
+#pragma unroll
+        for (int n = 0; n < kIds; ++n) ids[n] = a.prefix_pages[min(page_index(a.P, lane_pos(t, n)), table_len - 1)];
+    };
+    auto lane_row = [&](int t, int n, int pg) {  // byte offset of a lane's row
+        const int pos = lane_pos(t, n);
+        return (static_cast<unsigned>(pg) < static_cast<unsigned>(a.P.n_pages) ? pg : 0) * a.P.stride * kEs +
+               static_cast<long>(pos - page_index(a.P, pos) * a.P.page_size) * row_bytes;
+    };
+    // tile t (past the last one: that one again, so that every turn issues as many), its lanes' pages in ids, which get those
+    // of tile t + ahead
+    auto copy = [&](int t, int (&ids)[kIds], int ahead) {
+        char* const dst = ring + t % kRing * kTileB + 8 * w * kRowB;
+        if constexpr (EVEN) {
+            const long at = row_at(p_lo + min(t, ntiles - 1) * kPrefixTile + 8 * w);
+#pragma unroll
+            for (int n = 0; n < kCopies; ++n) dma16(kbase + at + k_off[n], dst + n * 1024);
+#pragma unroll
+            for (int n = 0; n < kCopies; ++n) dma16(vbase + at + v_off[n], dst + kValues + n * 1024);
+        } else {
+            long at[kCopies];
+#pragma unroll
+            for (int n = 0; n < kCopies; ++n) at[n] = lane_row(t, n, ids[n]);
+            if (ahead > 0) look_up(t + ahead, ids);
+#pragma unroll
+            for (int n = 0; n < kCopies; ++n) dma16(kbase + at[n] + k_off[n], dst + n * 1024);
+#pragma unroll
+            for (int n = 0; n < kCopies; ++n) dma16(vbase + at[n] + v_off[n], dst + kValues + n * 1024);
+        }
+    };
     f32x4 kr[kMine][2], vr[kMine][2];
     auto load = [&](int t) {
 #pragma unroll
         for (int n = 0; n < kMine; ++n) {
             const int row = (256 * n + static_cast<int>(threadIdx.x)) / kPieces, row0 = (256 * n + 64 * w) / kPieces;
-            const long at = row_at(p_lo + min(t, ntiles - 1) * kPrefixTile + row0);
-            const uint32_t off = (row - row0) * row_bytes + 32 * (threadIdx.x % kPieces);
+            const long at = EVEN ? row_at(p_lo + min(t, ntiles - 1) * kPrefixTile + row0) : lane_row(t, n, ids[n]);
+            const uint32_t off = (EVEN ? (row - row0) * row_bytes : 0) + 32 * real(threadIdx.x % kPieces);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 kr[n][x] = *reinterpret_cast<const f32x4*>(kbase + at + off + 16 * x);
                 vr[n][x] = *reinterpret_cast<const f32x4*>(vbase + at + off + 16 * x);
             }
         }
+        if constexpr (!EVEN) look_up(t + 1, ids);
     };
     auto store = [&](int t) {
 #pragma unroll
@@ -745,11 +779,18 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
         }
     };
     if constexpr (kWide) {
+        if constexpr (!EVEN) look_up(0, ids);
         load(0);
     } else {
-        copy(0);
-        copy(1);
-        copy(2);
+        int ids1[kIds] = {}, ids2[kIds] = {};
+        if constexpr (!EVEN) {
+            look_up(0, ids);
+            look_up(1, ids1);
+            look_up(2, ids2);
+        }
+        copy(0, ids, 3);
+        copy(1, ids1, 0);
+        copy(2, ids2, 0);
     }
 
     // ---- the lane's row and query operand.  Rows that do not see the whole prefix are left to the workgroups of their
@@ -768,7 +809,7 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
         for (int j = 0; j < kKs; ++j)
 #pragma unroll
             for (int e = 0; e < 8; e += 4) {
-                const f32x4 v = sees ? ld_f32x4(src + 16 * j + e) : f32x4{0, 0, 0, 0};
+                const f32x4 v = sees && (EVEN || 16 * j + 8 * h + e < D) ? ld_f32x4(src + 16 * j + e) : f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
                     x[j][e + d] = v[d];
@@ -801,7 +842,8 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
         const f32x16 zero = {};
         bool first = true;
 #pragma unroll
-        for (int ks = 0; ks < kKs; ++ks)
+        for (int ks = 0; ks < kKs; ++ks) {
+            if (!EVEN && 16 * ks >= D) break;
 #pragma unroll
             for (int x = kKv - 1; x >= 0; --x) {
                 const u32x4 k = *reinterpret_cast<const u32x4*>(kt + x * kTileB + 16 * ((2 * ks + h) ^ k_mix(i)));
@@ -811,6 +853,7 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
                     first = false;
                 }
             }
+        }
     };
     auto largest = [&](int t, f32x16& s) {
         const int left = p_hi - p_lo - t * kPrefixTile;
@@ -834,7 +877,7 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
         } else {
             wait_copies<4 * kCopies>();  // tile tl
             __syncthreads();
-            copy(tl + 3);
+            copy(tl + 3, ids, 1);
         }
         if (!kWide && p_hi - p_lo - tl * kPrefixTile < kPrefixTile) {  // past the prefix: zeros, whatever the page holds
             const int left = p_hi - p_lo - tl * kPrefixTile;
@@ -851,15 +894,15 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
                 const float f = raise ? __builtin_amdgcn_exp2f(mx - m) : 1.0f;
                 if (raise) mx = m;
                 sum *= f;
-    #pragma unroll
+#pragma unroll
                 for (int d = 0; d < kDb; ++d) o[d] *= f;
             }
             const float base = (mx == -INFINITY ? 0.0f : mx) - S::kShift;
             u32x4 pb[2][kParts];
-    #pragma unroll
+#pragma unroll
             for (int b = 0; b < 2; ++b) {
                 float p[8];
-    #pragma unroll
+#pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * b + e], kf, -base));
                     sum += p[e];
@@ -867,14 +910,15 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
                 split8<kMath, kParts>(p, pb[b]);
             }
             const char* const vt = ring + kValues + (kWide ? 0 : tl % kRing * kTileB);
-    #pragma unroll
+#pragma unroll
             for (int b = 0; b < 2; ++b)
-    #pragma unroll
-                for (int d = 0; d < kDb; ++d)
-    #pragma unroll
+#pragma unroll
+                for (int d = 0; d < kDb; ++d) {
+                    if (!EVEN && 32 * d >= D) break;
+#pragma unroll
                     for (int y = kKv - 1; y >= 0; --y) {
                         u32x4 v;
-    #pragma unroll
+#pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             const int row = 16 * b + 8 * x + v_row;  // row & 3 and (row >> 1) & 1 are the lane's own
                             const u32x2 z =
@@ -882,9 +926,10 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
                             v[2 * x] = z.x;
                             v[2 * x + 1] = z.y;
                         }
-    #pragma unroll
+#pragma unroll
                         for (int p = kParts - 1 - y; p >= 0; --p) o[d] = mma32(v, pb[b][p], o[d], Type{});
                     }
+                }
         }
         if constexpr (kWide) __syncthreads();  // the parts have been read
     }
@@ -901,23 +946,32 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
     for (int d = 0; d < kDb; ++d)
 #pragma unroll
         for (int v = 0; v < 16; v += 4)
-            *reinterpret_cast<f32x4*>(dst + 4 + 32 * d + 2 * v + 4 * h) = f32x4{o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
+            if (EVEN || 32 * d + 2 * v + 4 * h < D)
+                *reinterpret_cast<f32x4*>(dst + 4 + 32 * d + 2 * v + 4 * h) = f32x4{o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
 }
 
 template <int TYPE, int DP, bool EVEN>
 __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_attn_kernel(const PagedAttnArgs a) {
-    rows_body<TYPE, DP, EVEN>(a, blockIdx.x);
+    rows_body<TYPE, DP, EVEN>(a, blockIdx.x + (a.staged ? a.pre_blocks : 0));
 }
 // The prefix's workgroups and behind them the sequences', in one launch: the former are bound by the matrix instructions,
 // the latter by memory and by the trips to it before their first tile, and a CU holds one of each (64 conversations on
 // 8192 tokens: 67 us, 90 in two launches; 480 rows on 32768: 487 and 510).
-template <int TYPE, int D>
+template <int TYPE, int DP, bool EVEN>
 __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_mixed_kernel(const PagedAttnArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char ring[];
+    __shared__ __attribute__((aligned(16))) char ring[prefix_lds(TYPE, DP)];
     if (static_cast<int>(blockIdx.x) < a.pre_blocks)
-        prefix_body<TYPE, D>(a, blockIdx.x, ring);
+        prefix_body<TYPE, DP, EVEN>(a, blockIdx.x, ring);
     else
-        rows_body<TYPE, D, true>(a, blockIdx.x);
+        rows_body<TYPE, DP, EVEN>(a, blockIdx.x);
+}
+// Heads over 128: the queries and accumulators alone take more than half of a SIMD's registers and the ring 128 KB, one
+// workgroup to a CU, so the sequences' workgroups have a launch of their own.  16 heads of 256, 480 rows on 32768 positions of
+// fp16: 571 us (waves of their own 1315); bf16's third part spills 37 registers, 1024 (1347).
+template <int TYPE, bool EVEN>
+__global__ __launch_bounds__(64 * kPagedWaves, 1) void paged_prefix_kernel(const PagedAttnArgs a) {
+    __shared__ __attribute__((aligned(16))) char ring[prefix_lds(TYPE, 256)];
+    prefix_body<TYPE, 256, EVEN>(a, blockIdx.x, ring);
 }
 
 template <int TYPE, int DP, bool EVEN>
@@ -937,15 +991,22 @@ void run_paged_attn_type(const PagedAttnArgs& a, bool even, int blocks, hipStrea
 }
 
 template <int TYPE>
-void run_paged_mixed_type(const PagedAttnArgs& a, int own_blocks, hipStream_t stream) {
-    const int lds = 2 * (TYPE == kKvF32 ? 3 : kRing) * kPrefixTile * a.P.head_dim * 2;
-    const auto run = a.P.head_dim == 64 ? paged_mixed_kernel<TYPE, 64> : paged_mixed_kernel<TYPE, 128>;
-    hipLaunchKernelGGL(run, dim3(a.pre_blocks + own_blocks), dim3(64 * kPagedWaves), lds, stream, a);
+void run_paged_mixed_type(const PagedAttnArgs& a, bool even, int own_blocks, hipStream_t stream) {
+    const int D = a.P.head_dim;
+    if (D > 128) {
+        if constexpr (TYPE != kKvF32)  // (three parts of both, and of 256 dims, do not fit the registers)
+            hipLaunchKernelGGL((even ? paged_prefix_kernel<TYPE, true> : paged_prefix_kernel<TYPE, false>), dim3(a.pre_blocks),
+                               dim3(64 * kPagedWaves), 0, stream, a);
+        return run_paged_attn_type<TYPE>(a, even, own_blocks, stream);
+    }
+    const auto run = D <= 64 ? (even ? paged_mixed_kernel<TYPE, 64, true> : paged_mixed_kernel<TYPE, 64, false>)
+                             : (even ? paged_mixed_kernel<TYPE, 128, true> : paged_mixed_kernel<TYPE, 128, false>);
+    hipLaunchKernelGGL(run, dim3(a.pre_blocks + own_blocks), dim3(64 * kPagedWaves), 0, stream, a);
 }
 
-void run_paged_mixed_f32(const PagedAttnArgs& a, int own_blocks, hipStream_t stream);
-void run_paged_mixed_f16(const PagedAttnArgs& a, int own_blocks, hipStream_t stream);
-void run_paged_mixed_bf16(const PagedAttnArgs& a, int own_blocks, hipStream_t stream);
+void run_paged_mixed_f32(const PagedAttnArgs& a, bool even, int own_blocks, hipStream_t stream);
+void run_paged_mixed_f16(const PagedAttnArgs& a, bool even, int own_blocks, hipStream_t stream);
+void run_paged_mixed_bf16(const PagedAttnArgs& a, bool even, int own_blocks, hipStream_t stream);
 void run_paged_attn_f32(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream);
 void run_paged_attn_f16(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream);
 void run_paged_attn_bf16(const PagedAttnArgs& a, bool even, int blocks, hipStream_t stream);

@@ -8,8 +8,8 @@ void run_paged_attn_f16(const PagedAttnArgs& a, bool even, int blocks, hipStream
     run_paged_attn_type<kKvF16>(a, even, blocks, stream);
 }
 
-void run_paged_mixed_f16(const PagedAttnArgs& a, int own_blocks, hipStream_t stream) {
-    run_paged_mixed_type<kKvF16>(a, own_blocks, stream);
+void run_paged_mixed_f16(const PagedAttnArgs& a, bool even, int own_blocks, hipStream_t stream) {
+    run_paged_mixed_type<kKvF16>(a, even, own_blocks, stream);
 }
 
 }  // namespace dev

@@ -342,6 +342,19 @@ MANY = [
     ([1] * 9, [1 + 30 * i for i in range(9)], 8200, 32, 8, 2, 64),         # 44 rows
     ([40, 90], [40, 300], 505, 16, 4, 1, 128),
     ([1] * 70, [1 + i % 40 for i in range(70)], 1000, 20, 8, 2, 128),
+    # other heads and pages, enough rows and positions that the prefix goes through LDS
+    ([1] * 70, [1 + i % 40 for i in range(70)], 1001, 16, 8, 2, 80),
+    ([2] * 60, [2 + i % 40 for i in range(60)], 1200, 16, 4, 2, 256),
+    ([3, 0, 5, 1] * 9, [3, 2, 50, 90] * 9, 1000, 20, 8, 1, 256),
+    ([1] * 70, [1 + i % 40 for i in range(70)], 1003, 1, 8, 2, 40),
+    ([1] * 66, [1 + i % 40 for i in range(66)], 1070, 7, 8, 2, 200),
+    ([1] * 70, [1 + i % 40 for i in range(70)], 1001, 24, 4, 1, 128),
+    ([2] * 70, [2 + i % 40 for i in range(70)], 1024, 20, 4, 2, 64),
+    ([5] * 30, [5 + i for i in range(30)], 3000, 50, 10, 5, 96),
+    ([1] * 40, [1 + i for i in range(40)], 3301, 16, 4, 2, 8),
+    ([1] * 36, [1 + i for i in range(36)], 7300, 33, 2, 2, 136),
+    ([5] * 60, [5 + i for i in range(60)], 7001, 16, 4, 2, 256),
+    ([4] * 40, [4 + i for i in range(40)], 6600, 33, 4, 1, 136),
 ]
 
 
@@ -365,10 +378,12 @@ def test_many_rows_on_a_prefix(kind, shape):
 
 
 @pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
-@pytest.mark.parametrize("D,P", [(64, 400), (128, 400), (64, 1000), (128, 1000)])
-def test_many_rows_some_inside_the_prefix(kind, D, P):
+@pytest.mark.parametrize("D,P,ps", [(64, 400, 16), (128, 400, 16), (64, 1000, 16), (128, 1000, 16), (256, 1000, 16),
+                                    (80, 1000, 16), (128, 1000, 20), (200, 1000, 12), (256, 3900, 16),
+                                    (200, 3900, 12)])
+def test_many_rows_some_inside_the_prefix(kind, D, P, ps):
     """Rows that do not see the whole prefix, rows that see nothing and rows past their table, beside ordinary ones."""
-    H, Hkv, ps = 4, 1, 16
+    H, Hkv = 4, 1
     counts = [1] * 20 + [30, 6, 9, 1, 2, 1]
     held = [P + 5 + i for i in range(20)] + [P + 10, 3, P - 60, 1, 0, 5000]
     total, rows, _ = tables([P + 64] * len(held), ps)
