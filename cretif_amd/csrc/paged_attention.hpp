@@ -608,9 +608,10 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
             }
 }
 
-// The shared prefix against many rows.  A workgroup of four waves takes 128 rows, 32 to a wave, and a chunk of the prefix in
-// tiles of 32 positions that all its waves read from LDS: straight from the pool every wave would load 16 KB for the 2 x 0.5 MFLOP it does with a tile, more than the L1 delivers
-// beside the matrix instructions.  v_mfma_f32_32x32x16: half the instructions of 16x16x32 for the same product.
+// The shared prefix against many rows.  A workgroup of four waves takes 128 rows, 32 to a wave, and a chunk of the
+// prefix in tiles of 32 positions that all its waves read from LDS: straight from the pool every wave would load 16 KB
+// for the 2 x 0.5 MFLOP it does with a tile, more than the L1 delivers beside the matrix instructions.
+// v_mfma_f32_32x32x16: half the instructions of 16x16x32 for the same product.
 //   * 16-bit tiles go to LDS with global_load_lds, whole rows at a time, into rings of four, three tiles ahead; one barrier per
 //     tile.  The 16-byte pieces of a row are exchanged within it: K's so that the 32 rows of an operand fetch lie in
 //     different banks, V's so that the four rows that ds_read_b64_tr_b16 takes apart do (16 lanes read 4 positions x 16
@@ -966,8 +967,8 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_mixed_kernel(const 
         rows_body<TYPE, DP, EVEN>(a, blockIdx.x);
 }
 // Heads over 128: the queries and accumulators alone take more than half of a SIMD's registers and the ring 128 KB, one
-// workgroup to a CU, so the sequences' workgroups have a launch of their own.  16 heads of 256, 480 rows on 32768 positions of
-// fp16: 571 us (waves of their own 1315); bf16's third part spills 37 registers, 1024 (1347).
+// workgroup to a CU, so the sequences' workgroups have a launch of their own.  16 heads of 256, 480 rows on 32768
+// positions of fp16: 571 us (waves of their own 1315); bf16's third part spills 37 registers, 1024 (1347).
 template <int TYPE, bool EVEN>
 __global__ __launch_bounds__(64 * kPagedWaves, 1) void paged_prefix_kernel(const PagedAttnArgs a) {
     __shared__ __attribute__((aligned(16))) char ring[prefix_lds(TYPE, 256)];
