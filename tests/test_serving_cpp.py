@@ -12,7 +12,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(scope="module")
-def checker(tmp_path_factory):
+def program(tmp_path_factory):
     cxx = shutil.which("g++")
     if cxx is None:
         pytest.skip("g++ not found")
@@ -26,12 +26,12 @@ def checker(tmp_path_factory):
     return out
 
 
-def test_refusals_cpu(checker):
-    r = subprocess.run([checker, "cpu"], capture_output=True, text=True, timeout=60)
+def test_refusals_cpu(program):
+    r = subprocess.run([program, "cpu"], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
 
 
 @pytest.mark.gpu
-def test_one_token_gpu(checker):
-    r = subprocess.run([checker, "gpu"], capture_output=True, text=True, timeout=120)
+def test_one_token_gpu(program):
+    r = subprocess.run([program, "gpu"], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
