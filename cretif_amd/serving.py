@@ -187,11 +187,17 @@ class PagedBatch:
         self._dev = _device()
 
     def _for(self, n_rows):
-        c = self._by_rows.get(n_rows)  # descriptors differ in their row count alone: one per count, never changed
+        """The descriptor of batches of n_rows rows, never changed.  Only the reference that the caller holds keeps it
+        alive until its call is over: another thread may replace the kept one, or drop it when there are many."""
+        c = self._by_rows.get(n_rows)
         if c is None:
-            c = self._make(n_rows)
-            c = self._by_rows[n_rows] = (ctypes.addressof(c), c)
-        return c[0]
+            if len(self._by_rows) >= _KEPT:
+                self._by_rows.clear()
+            c = self._by_rows[n_rows] = self._make(n_rows)
+        return c
+
+
+_KEPT = 256  # row counts: a server's batches differ from step to step
 
 
 def qk_norm_rope(rot, q, k, q_out, k_out, positions, n_heads, n_kv_heads, head_dim, n_rows=None, stream=None):
@@ -231,7 +237,7 @@ def paged_append(cache, batch, rot, k, v, q=None, q_out=None, n_heads=0, n_rows=
         pq, lq, nq = _rows(q, n_heads * D, "q", dev)
         po, lo, no = _rows(q_out, n_heads * D, "q_out", dev)
     n = _same_rows(n_rows, ("k", nk), ("v", nv), ("q", nq), ("q_out", no))
-    st = L.cri_paged_append(cache._ref, batch._for(n), rot._ref, pq, lq, po, lo, n_heads, pk, lk, pv, lv,
+    st = L.cri_paged_append(cache._ref, ctypes.byref(batch._for(n)), rot._ref, pq, lq, po, lo, n_heads, pk, lk, pv, lv,
                             _on(stream, dev))
     if st:
         _check(st)
@@ -239,7 +245,7 @@ def paged_append(cache, batch, rot, k, v, q=None, q_out=None, n_heads=0, n_rows=
 
 def paged_attention_workspace_bytes(cache, batch, n_rows, n_heads, prefix_len=0):
     """Workspace bytes of paged_attention for batches of these host numbers."""
-    n = _torch().cri_paged_attention_workspace_bytes(cache._ref, batch._for(n_rows), prefix_len, n_heads)
+    n = _torch().cri_paged_attention_workspace_bytes(cache._ref, ctypes.byref(batch._for(n_rows)), prefix_len, n_heads)
     if n < 0:
         _check(int(n))
     return int(n)
@@ -266,8 +272,8 @@ def paged_attention(cache, batch, q, out, n_heads, scale, prefix_pages=None, pre
     if workspace is None:
         workspace = _new_room(paged_attention_workspace_bytes(cache, batch, n, n_heads, prefix_len), stream)
     pw, wb = _room(workspace, dev)
-    st = L.cri_paged_attention(cache._ref, batch._for(n), pp, prefix_len, pq, lq, po, lo, n_heads, scale, pw, wb,
-                               _on(stream, dev))
+    st = L.cri_paged_attention(cache._ref, ctypes.byref(batch._for(n)), pp, prefix_len, pq, lq, po, lo, n_heads, scale, pw,
+                               wb, _on(stream, dev))
     if st:
         _check(st)
 

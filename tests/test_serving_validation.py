@@ -1,6 +1,8 @@
 """The batched serving entry points refuse bad arguments before touching the GPU (so this runs without one), and
 the definitions the GPU tests use agree with what they claim."""
 import ctypes
+import threading
+import weakref
 
 import numpy as np
 import pytest
@@ -188,3 +190,54 @@ def test_definition_keeps_the_targets_distribution():
                 out, _ = ref.verify(np.stack([p, p]), np.stack([q, q]), [x, 0], u, d, [0, 2], [0, 0], [0])
                 share[out[0]] += q[x] / n / n
     assert np.abs(share - p).max() <= 1.0 / n
+
+
+def paged_batch(make):
+    """A PagedBatch whose descriptors `make` makes (its own need device tensors)."""
+    b = serving.PagedBatch.__new__(serving.PagedBatch)
+    b._make, b._by_rows, b._dev = make, {}, None
+    return b
+
+
+def paged_kv():
+    p = serving.PagedKV.__new__(serving.PagedKV)
+    p._c, p._dev = kv(), None
+    p._ref = ref_of(p._c)
+    return p
+
+
+def test_threads_that_share_a_batch_keep_their_descriptors(monkeypatch):
+    """Two threads meet a new row count together: each one's descriptor lives as long as its call."""
+    pytest.importorskip("torch")
+    both, made, alive = threading.Barrier(2, timeout=30), [], []
+
+    def make(rows):
+        c = batch(n_rows=rows)
+        made.append(weakref.ref(c))
+        both.wait()  # neither has been stored
+        return c
+
+    class Lib:
+        @staticmethod
+        def cri_paged_attention_workspace_bytes(*args):
+            both.wait()  # both have been stored, both calls run
+            alive.append([r() is not None for r in made])
+            both.wait()
+            return 0
+
+    monkeypatch.setattr(serving, "_torch", lambda: Lib)
+    b, p = paged_batch(make), paged_kv()
+    threads = [threading.Thread(target=cri.paged_attention_workspace_bytes, args=(p, b, 3, 4)) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert alive == [[True, True]] * 2
+
+
+def test_a_batch_keeps_a_bounded_number_of_descriptors():
+    pytest.importorskip("torch")
+    b, p = paged_batch(lambda rows: batch(n_rows=rows)), paged_kv()
+    want = [cri.paged_attention_workspace_bytes(p, b, n, 4) for n in range(1, 2000)]
+    assert len(b._by_rows) <= 1000 and sorted(set(want)) == sorted(want) and want[0] > 0
+    assert [cri.paged_attention_workspace_bytes(p, b, n, 4) for n in range(1, 2000)] == want
