@@ -78,7 +78,7 @@ def _rows(t, width, name, dev):
         n, w = sh
         ld, one = st
         if w == width and one == 1 and t.dtype is torch.float32 and t.get_device() == dev:
-            return t.data_ptr(), ld if n > 1 or ld > width else width, n  # (the stride of a single row says nothing)
+            return t.data_ptr(), ld if n > 1 else width, n  # (the stride of a single row says nothing)
     if t.dtype is not torch.float32:
         raise ValueError("%s must be float32, not %s" % (name, t.dtype))
     if len(sh) not in (2, 3):
@@ -88,7 +88,14 @@ def _rows(t, width, name, dev):
         raise ValueError("%s has rows of %d floats, not %d" % (name, wide, width))
     if (inner > 1 and st[-1] != 1) or (len(sh) == 3 and sh[1] > 1 and st[1] != inner):
         raise ValueError("%s: the elements of a row must be consecutive" % name)
-    return _on_device(t, name, dev), st[0] if sh[0] > 1 else max(st[0], width), sh[0]
+    return _on_device(t, name, dev), st[0] if sh[0] > 1 else width, sh[0]
+
+
+def _in_32_bits(*numbers):
+    """Host numbers that C takes as int: ctypes would cut them to 32 bits without a word.  (The calls of a step ask first
+    whether any has a bit from 31 on, 0.1 us; negative ones are C's to refuse.)"""
+    if max(numbers) > 0x7FFFFFFF or min(numbers) < -0x80000000:
+        raise ValueError("a size or a row stride does not fit 32 bits: %s" % (numbers,))
 
 
 def _same_rows(n_rows, *named):
@@ -138,6 +145,7 @@ class Rotation:
         for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
             if w is not None and (w.dtype is not torch.float32 or w.dim() != 1 or not w.is_contiguous()):
                 raise ValueError("%s must be a contiguous float32 tensor [head_dim]" % name)
+        _in_32_bits(rot_dim)
         self.q_norm, self.k_norm = q_norm, k_norm
         self._c = _Rotation(None if q_norm is None else _on_device(q_norm, "q_norm"),
                             None if k_norm is None else _on_device(k_norm, "k_norm"), eps, theta, rot_dim, PAIRS[pairs])
@@ -162,6 +170,7 @@ class PagedKV:
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride():
             raise ValueError("k and v must both be [n_pages, page_size, n_kv_heads, head_dim], with the same strides")
         n, ps, h, d = k.shape
+        _in_32_bits(n, ps, h, d)
         if n > 0 and not k[0].is_contiguous():
             raise ValueError("a page must be contiguous")
         self.k, self.v = k, v
@@ -181,6 +190,7 @@ class PagedBatch:
         n = lens.shape[0]
         if offsets.shape[0] != n + 1 or pages.shape[0] != n:
             raise ValueError("offsets must have n_seqs + 1 entries, lens and pages n_seqs")
+        _in_32_bits(n, pages.shape[1])
         self.offsets, self.lens, self.pages = offsets, lens, pages
         self._make = lambda rows: _PagedBatch(po, pl, pp, n, rows, pages.shape[1])
         self._by_rows = {}
@@ -216,6 +226,8 @@ def qk_norm_rope(rot, q, k, q_out, k_out, positions, n_heads, n_kv_heads, head_d
         px, lx, nx = _rows(k_out, n_kv_heads * head_dim, "k_out", dev)
     pp = _ints(positions, "positions", 1, dev)
     n = _same_rows(n_rows, ("positions", positions.shape[0]), ("q", nq), ("k", nk), ("q_out", no), ("k_out", nx))
+    if (lq | lo | lk | lx | n | n_heads | n_kv_heads | head_dim) >> 31:
+        _in_32_bits(lq, lo, lk, lx, n, n_heads, n_kv_heads, head_dim)
     st = L.cri_qk_norm_rope(rot._ref, pq, lq, pk, lk, po, lo, px, lx, pp, n, n_heads, n_kv_heads, head_dim,
                             _on(stream, dev))
     if st:
@@ -237,6 +249,8 @@ def paged_append(cache, batch, rot, k, v, q=None, q_out=None, n_heads=0, n_rows=
         pq, lq, nq = _rows(q, n_heads * D, "q", dev)
         po, lo, no = _rows(q_out, n_heads * D, "q_out", dev)
     n = _same_rows(n_rows, ("k", nk), ("v", nv), ("q", nq), ("q_out", no))
+    if (lq | lo | lk | lv | n | n_heads) >> 31:
+        _in_32_bits(lq, lo, lk, lv, n, n_heads)
     st = L.cri_paged_append(cache._ref, ctypes.byref(batch._for(n)), rot._ref, pq, lq, po, lo, n_heads, pk, lk, pv, lv,
                             _on(stream, dev))
     if st:
@@ -245,6 +259,7 @@ def paged_append(cache, batch, rot, k, v, q=None, q_out=None, n_heads=0, n_rows=
 
 def paged_attention_workspace_bytes(cache, batch, n_rows, n_heads, prefix_len=0):
     """Workspace bytes of paged_attention for batches of these host numbers."""
+    _in_32_bits(n_rows, n_heads, prefix_len)
     n = _torch().cri_paged_attention_workspace_bytes(cache._ref, ctypes.byref(batch._for(n_rows)), prefix_len, n_heads)
     if n < 0:
         _check(int(n))
@@ -262,6 +277,8 @@ def paged_attention(cache, batch, q, out, n_heads, scale, prefix_pages=None, pre
     pq, lq, nq = _rows(q, width, "q", dev)
     po, lo, no = _rows(out, width, "out", dev)
     n = _same_rows(n_rows, ("q", nq), ("out", no))
+    if (lq | lo | n | n_heads | prefix_len) >> 31:
+        _in_32_bits(lq, lo, n, n_heads, prefix_len)
     pp = 0
     if prefix_len > 0:
         if prefix_pages is None:
@@ -280,6 +297,7 @@ def paged_attention(cache, batch, q, out, n_heads, scale, prefix_pages=None, pre
 
 def verify_drafts_workspace_bytes(n_seqs, vocab):
     """Workspace bytes of verify_drafts."""
+    _in_32_bits(n_seqs, vocab)
     n = _torch().cri_verify_drafts_workspace_bytes(n_seqs, vocab)
     if n < 0:
         _check(int(n))
@@ -310,6 +328,8 @@ def verify_drafts(target, draft, draft_ids, uniforms, draws, offsets, out_ids, n
             raise ValueError("%s must be a contiguous float32 tensor [rows]" % name)
     if draft_ids.shape[0] != n or out_ids.shape[0] != n or offsets.shape[0] != B + 1:
         raise ValueError("draft_ids and out_ids must have target's rows, offsets n_seqs + 1 entries")
+    if (n | B | V) >> 31:
+        _in_32_bits(n, B, V)
     if workspace is None:
         workspace = _new_room(verify_drafts_workspace_bytes(B, V), stream)
     pw, wb = _room(workspace, dev)

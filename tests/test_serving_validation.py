@@ -202,6 +202,7 @@ def paged_batch(make):
 def paged_kv():
     p = serving.PagedKV.__new__(serving.PagedKV)
     p._c, p._dev = kv(), None
+    p.page_size, p.n_kv_heads, p.head_dim = p._c.page_size, p._c.n_kv_heads, p._c.head_dim
     p._ref = ref_of(p._c)
     return p
 
@@ -241,3 +242,117 @@ def test_a_batch_keeps_a_bounded_number_of_descriptors():
     want = [cri.paged_attention_workspace_bytes(p, b, n, 4) for n in range(1, 2000)]
     assert len(b._by_rows) <= 1000 and sorted(set(want)) == sorted(want) and want[0] > 0
     assert [cri.paged_attention_workspace_bytes(p, b, n, 4) for n in range(1, 2000)] == want
+
+
+class Recorder:
+    """Stands for the library: what reached it."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *args: self.calls.append((name, args)) or 0
+
+
+class Array:
+    """What the wrappers ask of a device tensor, with any shape and strides."""
+
+    def __init__(self, torch, *shape, strides=None, dtype=None, at=FAKE):
+        self.shape, self.dtype, self.device = torch.Size(shape), dtype or torch.int32, "cuda:0"
+        self._strides, self._at, self.nbytes = strides, at, 1 << 40
+
+    def stride(self, i=None):
+        return self._strides if i is None else self._strides[i]
+
+    def dim(self):
+        return len(self.shape)
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return 0
+
+    def data_ptr(self):
+        return self._at
+
+    def __getitem__(self, i):
+        return self
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    torch, lib = pytest.importorskip("torch"), Recorder()
+    monkeypatch.setattr(serving, "torch", torch)
+    monkeypatch.setattr(serving, "_torch", lambda: lib)
+    monkeypatch.setattr(serving, "_device", lambda: 0)
+    monkeypatch.setattr(serving, "_on", lambda stream, dev: 0)
+    return torch, lib
+
+
+FAR = [2 ** 31, 2 ** 32 + 256, 2 ** 32 + 2 ** 31 + 512, 2 ** 62]
+
+
+@pytest.mark.parametrize("ld", FAR)
+@pytest.mark.parametrize("as_tuple", [False, True])
+def test_row_strides_past_32_bits_are_refused(recorded, ld, as_tuple):
+    """C takes rows' strides as int, which ctypes would fill with the lower 32 bits."""
+    torch, lib = recorded
+
+    def rows(width, far, n=3):
+        if as_tuple:
+            return FAKE, ld if far else width
+        return Array(torch, n, width, strides=(ld if far else width, 1), dtype=torch.float32)
+
+    b, p, r = paged_batch(lambda n: batch(n_rows=n)), paged_kv(), cri.Rotation(1e4, 64)
+    pos, ws = Array(torch, 3), Array(torch, 1 << 40)
+    for i in range(4):
+        w = [rows(256, i == 0), rows(128, i == 1), rows(256, i == 2), rows(128, i == 3)]
+        with pytest.raises(ValueError, match="32 bits"):
+            cri.qk_norm_rope(r, *w, pos, 4, 2, 64)
+        w = [rows(128, i == 0), rows(128, i == 1), rows(256, i == 2), rows(256, i == 3)]
+        with pytest.raises(ValueError, match="32 bits"):
+            cri.paged_append(p, b, r, *w, n_heads=4, n_rows=3)
+        if i < 2:
+            with pytest.raises(ValueError, match="32 bits"):
+                cri.paged_attention(p, b, rows(256, i == 0), rows(256, i == 1), 4, 0.125, workspace=ws, n_rows=3)
+    assert lib.calls == []
+    if as_tuple:
+        return
+    # the stride of a single row says nothing, the verification's strides have 64 bits
+    cri.qk_norm_rope(r, rows(256, True, 1), None, rows(256, True, 1), None, Array(torch, 1), 4, 0, 64)
+    cri.paged_attention(p, b, rows(256, True, 1), rows(256, True, 1), 4, 0.125, workspace=ws)
+    assert lib.calls[0][1][2] == 256 and lib.calls[0][1][6] == 256 and lib.calls[1][1][5] == 256 and lib.calls[1][1][7] == 256
+    f = dict(dtype=torch.float32)
+    cri.verify_drafts(rows(100, True), None, Array(torch, 3), Array(torch, 3, **f), Array(torch, 3, **f), Array(torch, 2),
+                      Array(torch, 3), Array(torch, 1), ws)
+    assert lib.calls[2][1][1] == ld
+
+
+@pytest.mark.parametrize("far", [2 ** 31, 2 ** 32 + 64, -2 ** 32 + 64])
+def test_sizes_past_32_bits_are_refused(recorded, far):
+    torch, lib = recorded
+    b, p, r = paged_batch(lambda n: batch(n_rows=n)), paged_kv(), cri.Rotation(1e4, 64)
+    x, ws, wide = (FAKE, 256), Array(torch, 1 << 40), Array(torch, abs(far), 16, 2, 64, strides=(2048, 128, 64, 1), dtype=torch.float16)
+    f = dict(dtype=torch.float32)
+    calls = [
+        lambda: cri.Rotation(1e4, far),
+        lambda: cri.PagedKV(wide, wide),
+        lambda: cri.PagedBatch(Array(torch, 3), Array(torch, 2), Array(torch, 2, abs(far))),
+        lambda: cri.qk_norm_rope(r, x, None, x, None, Array(torch, 3), far, 0, 64),
+        lambda: cri.qk_norm_rope(r, x, None, x, None, Array(torch, abs(far)), 4, 0, 64),
+        lambda: cri.paged_append(p, b, r, x, x, n_rows=far),
+        lambda: cri.paged_append(p, b, r, x, x, x, x, n_heads=far, n_rows=3),
+        lambda: cri.paged_attention(p, b, x, x, far, 0.125, workspace=ws, n_rows=3),
+        lambda: cri.paged_attention(p, b, x, x, 4, 0.125, workspace=ws, n_rows=far),
+        lambda: cri.paged_attention(p, b, x, x, 4, 0.125, Array(torch, abs(far)), far, workspace=ws, n_rows=3),
+        lambda: cri.paged_attention_workspace_bytes(p, b, far, 4),
+        lambda: cri.paged_attention_workspace_bytes(p, b, 3, 4, far),
+        lambda: cri.verify_drafts_workspace_bytes(2, far),
+        lambda: cri.verify_drafts(Array(torch, 3, abs(far), strides=(abs(far), 1), **f), None, Array(torch, 3), Array(torch, 3, **f),
+                                  Array(torch, 3, **f), Array(torch, 2), Array(torch, 3), Array(torch, 1), ws),
+    ]
+    for call in calls:
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+    assert lib.calls == []
