@@ -12,6 +12,7 @@
 #include <cstdio>
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "internal.hpp"
@@ -724,6 +725,21 @@ bool in_pool(const cri::PagePool& pool, int type, const void* p, long bytes) {
     return overlaps(pool.k, size, p, bytes) || overlaps(pool.v, size, p, bytes);
 }
 
+// whether a buffer that is written meets one of those
+struct Span {
+    const void* p;
+    long bytes;
+};
+bool meets(Span out, std::initializer_list<Span> others) {
+    for (const Span& o : others)
+        if (overlaps(out.p, out.bytes, o.p, o.bytes)) return true;
+    return false;
+}
+// (and one of a batch's arrays)
+bool meets_batch(Span out, const cri::PageBatch& b) {
+    return meets(out, {{b.offsets, (b.n_seqs + 1L) * 4}, {b.lens, b.n_seqs * 4L}, {b.pages, b.n_seqs * 4L * b.max_pages}});
+}
+
 int check_rows(const float* p, int ld, long width, const char* name, const char* fn) {
     if (!p) return fail(CRI_ERR_INVALID_ARGUMENT, fn, std::string("null ") + name);
     if (!aligned(p, 4)) return fail(CRI_ERR_ALIGNMENT, fn, std::string(name) + " must be 4-byte aligned");
@@ -761,6 +777,10 @@ int cri_qk_norm_rope(const cri_rotation* rot, const float* q, int ldq, const flo
          (rows_overlap(q, wq, ldq, k_out, wk, ldk_out, M) || rows_overlap(k, wk, ldk, q_out, wq, ldq_out, M) ||
           rows_overlap(q_out, wq, ldq_out, k_out, wk, ldk_out, M))))
         return fail(CRI_ERR_INVALID_ARGUMENT, fn, "an output overlaps another buffer");
+    const std::initializer_list<Span> read = {{positions, M * 4L}, {R.q_norm, head_dim * 4L}, {R.k_norm, head_dim * 4L}};
+    if (meets({n_heads > 0 ? q_out : nullptr, span_bytes(M, wq, ldq_out)}, read) ||
+        meets({n_kv_heads > 0 ? k_out : nullptr, span_bytes(M, wk, ldk_out)}, read))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "an output overlaps the positions or the norm weights");
     clear_pending_error();
     if (cri::detail::launch_qk_norm_rope(R, q, ldq, k, ldk, q_out, ldq_out, k_out, ldk_out, positions, M, n_heads,
                                          n_kv_heads, head_dim, s) != 0)
@@ -795,6 +815,9 @@ int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const
         (wq > 0 && (in_pool(pool, type, q, span_bytes(b.n_rows, wq, ldq)) ||
                     in_pool(pool, type, q_out, span_bytes(b.n_rows, wq, ldq_out)))))
         return fail(CRI_ERR_INVALID_ARGUMENT, fn, "the pool overlaps q, k, v or q_out");
+    const Span written{wq > 0 ? q_out : nullptr, span_bytes(b.n_rows, wq, ldq_out)};
+    if (meets_batch(written, b) || meets(written, {{R.q_norm, pool.head_dim * 4L}, {R.k_norm, pool.head_dim * 4L}}))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "q_out overlaps the batch's arrays or the norm weights");
     clear_pending_error();
     if (cri::detail::launch_paged_append(pool, type, b, R, wq > 0 ? q : nullptr, ldq, q_out, ldq_out, n_heads, k, ldk, v,
                                          ldv, s) != 0)
@@ -803,6 +826,7 @@ int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const
 }
 
 namespace {
+constexpr char kTooManyChunks[] = "too many sequences x KV heads x chunks for one launch";
 int check_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, int prefix_len, int n_heads,
                           cri::PagePool* pool, cri::PageBatch* b, int* type, const char* fn) {
     if (const int st = check_paged(kv, batch, pool, b, type, fn)) return st;
@@ -826,7 +850,8 @@ long long cri_paged_attention_workspace_bytes(const cri_paged_kv* kv, const cri_
     int type;
     if (const int st = check_paged_attention(kv, batch, prefix_len, n_heads, &pool, &b, &type, fn)) return st;
     if (b.n_seqs == 0 || b.n_rows == 0 || n_heads == 0) return 0;
-    return cri::detail::paged_attention_workspace_bytes(pool, type, b, n_heads, prefix_len);
+    const long need = cri::detail::paged_attention_workspace_bytes(pool, type, b, n_heads, prefix_len);
+    return need < 0 ? fail(CRI_ERR_UNSUPPORTED, fn, kTooManyChunks) : need;
 }
 
 int cri_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, const int* prefix_pages, int prefix_len,
@@ -850,6 +875,7 @@ int cri_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, co
     if (in_pool(pool, type, out, out_bytes)) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out overlaps the pool");
     if (!std::isfinite(scale * 1.44269504f)) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "scale must be finite (and below 2^127)");
     const long need = cri::detail::paged_attention_workspace_bytes(pool, type, b, n_heads, prefix_len);
+    if (need < 0) return fail(CRI_ERR_UNSUPPORTED, fn, kTooManyChunks);
     if (need > 0) {
         if (!workspace) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null workspace");
         if (!aligned(workspace, 16)) return fail(CRI_ERR_ALIGNMENT, fn, "workspace must be 16-byte aligned");
@@ -860,10 +886,14 @@ int cri_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, co
     if (overlaps(workspace, need, out, out_bytes) || overlaps(workspace, need, q, span_bytes(b.n_rows, w, ldq)) ||
         in_pool(pool, type, workspace, need))
         return fail(CRI_ERR_INVALID_ARGUMENT, fn, "the workspace overlaps q, out or the pool");
+    const Span prefix{prefix_pages, prefix_len > 0 ? ((prefix_len - 1L) / pool.page_size + 1) * 4 : 0};
+    for (const Span& written : {Span{out, out_bytes}, Span{workspace, need}})
+        if (meets_batch(written, b) || meets(written, {prefix}))
+            return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out or the workspace overlaps the batch's arrays or prefix_pages");
     clear_pending_error();
     if (cri::detail::launch_paged_attention(pool, type, b, prefix_pages, prefix_len, q, ldq, out, ldo, n_heads, scale,
                                             static_cast<float*>(workspace), s) != 0)
-        return fail(CRI_ERR_UNSUPPORTED, fn, "too many sequences x KV heads x chunks for one launch");
+        return fail(CRI_ERR_UNSUPPORTED, fn, kTooManyChunks);
     return check_launch(fn);
 }
 
@@ -894,13 +924,19 @@ int cri_verify_drafts(const float* target, long long ldt, const float* draft, lo
     if (ldt > kMaxElems / std::max(n_rows, 1) || (draft && ldd > kMaxElems / std::max(n_rows, 1)))
         return fail(CRI_ERR_SHAPE, fn, "problem too large");
     const long ids = static_cast<long>(n_rows) * 4;
-    if (overlaps(out_ids, ids, draft_ids, ids)) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out_ids overlaps draft_ids");
     const long need = cri::detail::verify_workspace_bytes(n_seqs, vocab);
     if (!workspace) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null workspace");
     if (!aligned(workspace, 8)) return fail(CRI_ERR_ALIGNMENT, fn, "workspace must be 8-byte aligned");
     if (workspace_bytes < need)
         return fail(CRI_ERR_SHAPE, fn, "workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) +
                                            " needed");
+    const Span tokens{out_ids, ids}, counts{n_accepted, n_seqs * 4L}, room{workspace, need};
+    for (const Span& written : {tokens, counts, room})
+        if (meets(written, {{target, span_bytes(n_rows, vocab, ldt)}, {draft, span_bytes(n_rows, vocab, ldd)}, {draft_ids, ids},
+                            {uniforms, ids}, {draws, ids}, {offsets, (n_seqs + 1L) * 4}}))
+            return fail(CRI_ERR_INVALID_ARGUMENT, fn, "an output or the workspace overlaps an input");
+    if (meets(tokens, {counts, room}) || meets(counts, {room}))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out_ids, n_accepted and the workspace overlap");
     clear_pending_error();
     if (cri::detail::launch_verify_drafts(target, ldt, draft, ldd, draft_ids, uniforms, draws, offsets, n_seqs, n_rows, vocab,
                                           out_ids, n_accepted, static_cast<double*>(workspace), s) != 0)

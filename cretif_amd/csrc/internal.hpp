@@ -344,7 +344,8 @@ int launch_paged_append(const PagePool& P, int type, const PageBatch& B, const H
                         long ldv, hipStream_t stream);
 
 // attention of the batch's rows over the pages, positions below prefix_len through prefix_pages
-// (paged_attention.hip); ws: 16-byte aligned, paged_attention_workspace_bytes of it, written before it is read
+// (paged_attention.hip); ws: 16-byte aligned, paged_attention_workspace_bytes of it (negative: the call is declined),
+// written before it is read
 long paged_attention_workspace_bytes(const PagePool& P, int type, const PageBatch& B, int n_heads, int prefix_len);
 int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, const int* prefix_pages, int prefix_len,
                            const float* q, long ldq, float* out, long ldo, int n_heads, float scale, float* ws,

@@ -171,6 +171,8 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
     return c;
 }
 
+bool fits(const Cut& c) { return c.pre_blocks + c.own_blocks < 1L << 24; }  // 256 threads each: a launch's limit
+
 }  // namespace
 }  // namespace dev
 
@@ -178,6 +180,7 @@ namespace detail {
 
 long paged_attention_workspace_bytes(const PagePool& P, int type, const PageBatch& B, int n_heads, int prefix_len) {
     const dev::Cut c = dev::cut_of(P, type, B, n_heads, prefix_len);
+    if (!dev::fits(c)) return kDeclined;
     return c.nrec == 1 ? 0 : static_cast<long>(B.n_rows) * n_heads * c.nrec * (P.head_dim + 4) * 4;
 }
 
@@ -190,7 +193,7 @@ int launch_paged_attention(const PagePool& P, int type, const PageBatch& B, cons
     a.P = P, a.B = B;
     a.prefix_pages = prefix_pages, a.prefix_len = prefix_len;
     a.H = n_heads, a.G = n_heads / P.n_kv_heads, a.nrec = c.nrec;
-    if (c.pre_blocks + c.own_blocks >= 1L << 24) return kDeclined;  // 256 threads each: a launch's limit
+    if (!dev::fits(c)) return kDeclined;
     a.pre_tiles = c.pre_tiles, a.pre_chunks = c.pre_chunks, a.pre_per = c.pre_per, a.pre_blocks = c.pre_blocks;
     a.own_more = c.own_more, a.own_chunks = c.own_chunks, a.own_per = c.own_per;
     a.own_first = static_cast<int>(c.own_first);

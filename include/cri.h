@@ -395,7 +395,8 @@ typedef struct cri_rotation {
  * normed and rotated, row m at position positions[m] (device int32).  Rows are ldq, ldk, ldq_out and
  * ldk_out floats apart (at least their heads' width).  q_out may be q with ldq_out == ldq, k_out k
  * with ldk_out == ldk; no other overlap of an output with another buffer (outputs of columns of one
- * row are fine).  q or k may be left out with 0 heads.  Pointers 4-byte aligned. */
+ * row are fine; positions and norm weights count as buffers).  q or k may be left out with 0 heads.  Pointers 4-byte
+ * aligned. */
 int cri_qk_norm_rope(const cri_rotation* rot, const float* q, int ldq, const float* k, int ldk, float* q_out, int ldq_out,
                      float* k_out, int ldk_out, const int* positions, int M, int n_heads, int n_kv_heads, int head_dim,
                      hipStream_t stream);
@@ -403,7 +404,8 @@ int cri_qk_norm_rope(const cri_rotation* rot, const float* q, int ldq, const flo
  * pages, rounded to the cache's type (to nearest even); with q not null, its n_heads heads go to
  * q_out, normed and rotated, as by cri_qk_norm_rope.  A row whose position has no page (below 0,
  * past the table's max_pages, a page number outside the pool) is left out: its page and q_out row
- * stay as they were.  Pages that are written must belong to one sequence. */
+ * stay as they were.  Pages that are written must belong to one sequence.  q_out may be q with
+ * ldq_out == ldq; no other overlap of q_out or the pool with another buffer. */
 int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const cri_rotation* rot, const float* q, int ldq,
                      float* q_out, int ldq_out, int n_heads, const float* k, int ldk, const float* v, int ldv,
                      hipStream_t stream);
@@ -424,7 +426,7 @@ int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const
  * of n_kv_heads; n_rows * n_heads at most 2^24; scale finite.  q, out 4-byte aligned, workspace
  * 16-byte, cri_paged_attention_workspace_bytes of it (for the same kv, batch and prefix_len; only
  * their host numbers count, so one workspace serves every step with the same n_seqs, n_rows and
- * max_pages), not overlapping the others.  Sums, maxima and products are good to fp32 for every cache
+ * max_pages).  out and the workspace overlap no other buffer.  Sums, maxima and products are good to fp32 for every cache
  * type, in an order fixed by the host numbers and lens. */
 int cri_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, const int* prefix_pages, int prefix_len,
                         const float* q, int ldq, float* out, int ldo, int n_heads, float scale, void* workspace,
@@ -449,7 +451,7 @@ long long cri_paged_attention_workspace_bytes(const cri_paged_kv* kv, const cri_
  * sequence of no rows gets n_accepted 0.  A target probability that is NaN or negative counts as
  * zero; where a draft's is NaN its token is not accepted and has no weight.  Comparisons and sums
  * are in 64 bits and in a fixed order.
- * out_ids must not overlap draft_ids.  workspace: 8-byte aligned, cri_verify_drafts_workspace_bytes. */
+ * out_ids, n_accepted and the workspace overlap neither each other nor an input.  workspace: 8-byte aligned, cri_verify_drafts_workspace_bytes. */
 int cri_verify_drafts(const float* target, long long ldt, const float* draft, long long ldd, const int* draft_ids,
                       const float* uniforms, const float* draws, const int* offsets, int n_seqs, int n_rows,
                       int vocab, int* out_ids, int* n_accepted, void* workspace, long long workspace_bytes,

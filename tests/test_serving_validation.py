@@ -356,3 +356,43 @@ def test_sizes_past_32_bits_are_refused(recorded, far):
         with pytest.raises(ValueError, match="32 bits"):
             call()
     assert lib.calls == []
+
+
+def refused(st, word):
+    assert st == -1 and word in cri.lib().cri_last_error_string().decode(), (st, cri.lib().cri_last_error_string())
+
+
+def test_norm_rope_outputs_apart_from_what_it_reads():
+    far = rot(q_norm=WS, k_norm=WS + 256)
+    refused(norm_rope(pos=O + 2 * 1024 + 1020), "positions")  # the last of q_out's third row
+    refused(norm_rope(pos=O2 - 8), "positions")
+    refused(norm_rope(r=far, qo=WS + 252), "norm weights")
+    refused(norm_rope(r=far, ko=WS + 508), "norm weights")
+
+
+def test_append_query_rows_apart_from_the_batch():
+    p = kv(v=V << 8)
+    for b in (batch(offsets=O + 4 * 767, lens=WS, pages=WS), batch(offsets=WS, lens=O - 4, pages=WS), batch(offsets=WS, lens=WS, pages=O - 36)):
+        refused(append(p=p, b=b), "q_out overlaps the batch")
+    refused(append(p=p, b=batch(offsets=WS, lens=WS, pages=WS), r=rot(q_norm=O - 252)), "norm weights")
+
+
+def test_attention_outputs_apart_from_the_batch():
+    p = kv(k=Q << 8, v=Q << 8)  # (reading one page as both is fine)
+    for at in (O, WS):
+        for b in (batch(offsets=at - 8, lens=V, pages=V), batch(offsets=V, lens=at + 4, pages=V), batch(offsets=V, lens=V, pages=at - 36)):
+            refused(attend(p=p, b=b), "batch")
+        refused(attend(p=p, b=batch(offsets=V, lens=V, pages=V), pp=at - 4), "prefix_pages")
+
+
+def test_verify_outputs_apart_from_inputs_and_each_other():
+    far = Q << 8
+    ok = dict(t=far, d=far + (1 << 20), ids=far + (2 << 20), u=far + (3 << 20), dr=far + (3 << 20), off=far + (4 << 20))
+    for at in (dict(out=O), dict(acc=O), dict(ws=O, wsb=100)):
+        for name, back in (("t", 499), ("d", 499), ("ids", 4), ("u", 4), ("dr", 4), ("off", 2)):
+            kw = dict(ok)
+            kw[name] = O - back * 4  # its last element is the output's first
+            refused(verify(**{**dict(out=O2, acc=O2 + 4096, ws=WS), **at, **kw}), "an input")
+    refused(verify(**ok, out=O, acc=O + 16), "out_ids, n_accepted")
+    refused(verify(**ok, out=O + 24, ws=O, wsb=100), "out_ids, n_accepted")
+    refused(verify(**ok, acc=O2 + 24, ws=O2, wsb=100), "out_ids, n_accepted")
