@@ -740,6 +740,16 @@ bool meets_batch(Span out, const cri::PageBatch& b) {
     return meets(out, {{b.offsets, (b.n_seqs + 1L) * 4}, {b.lens, b.n_seqs * 4L}, {b.pages, b.n_seqs * 4L * b.max_pages}});
 }
 
+// Whether a page of K meets one of V: both pools have the same stride, so their pages' distances are one distance plus its
+// multiples.  (Pages of the one between those of the other are fine.)
+bool pages_meet(const cri::PagePool& pool, int type) {
+    const long e = type == cri::kKvF32 ? 4 : 2, stride = pool.stride * e;
+    const long page = static_cast<long>(pool.page_size) * pool.n_kv_heads * pool.head_dim * e;
+    const intptr_t d = reinterpret_cast<intptr_t>(pool.v) - reinterpret_cast<intptr_t>(pool.k), far = d < 0 ? -d : d;
+    const long pages = far / stride, rest = far % stride;  // a page of the one lies `rest` behind one of the other
+    return (pages < pool.n_pages && rest < page) || (pages + 1 < pool.n_pages && rest + page > stride);
+}
+
 int check_rows(const float* p, int ld, long width, const char* name, const char* fn) {
     if (!p) return fail(CRI_ERR_INVALID_ARGUMENT, fn, std::string("null ") + name);
     if (!aligned(p, 4)) return fail(CRI_ERR_ALIGNMENT, fn, std::string(name) + " must be 4-byte aligned");
@@ -815,6 +825,7 @@ int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const
         (wq > 0 && (in_pool(pool, type, q, span_bytes(b.n_rows, wq, ldq)) ||
                     in_pool(pool, type, q_out, span_bytes(b.n_rows, wq, ldq_out)))))
         return fail(CRI_ERR_INVALID_ARGUMENT, fn, "the pool overlaps q, k, v or q_out");
+    if (pages_meet(pool, type)) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "pages of k and v overlap");
     const Span written{wq > 0 ? q_out : nullptr, span_bytes(b.n_rows, wq, ldq_out)};
     if (meets_batch(written, b) || meets(written, {{R.q_norm, pool.head_dim * 4L}, {R.k_norm, pool.head_dim * 4L}}))
         return fail(CRI_ERR_INVALID_ARGUMENT, fn, "q_out overlaps the batch's arrays or the norm weights");

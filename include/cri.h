@@ -405,7 +405,8 @@ int cri_qk_norm_rope(const cri_rotation* rot, const float* q, int ldq, const flo
  * q_out, normed and rotated, as by cri_qk_norm_rope.  A row whose position has no page (below 0,
  * past the table's max_pages, a page number outside the pool) is left out: its page and q_out row
  * stay as they were.  Pages that are written must belong to one sequence.  q_out may be q with
- * ldq_out == ldq; no other overlap of q_out or the pool with another buffer. */
+ * ldq_out == ldq; no other overlap of q_out or the pool with another buffer, none of a page of k with one of v (pages of
+ * the one between those of the other are fine). */
 int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const cri_rotation* rot, const float* q, int ldq,
                      float* q_out, int ldq_out, int n_heads, const float* k, int ldk, const float* v, int ldv,
                      hipStream_t stream);

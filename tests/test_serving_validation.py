@@ -370,6 +370,23 @@ def test_norm_rope_outputs_apart_from_what_it_reads():
     refused(norm_rope(r=far, ko=WS + 508), "norm weights")
 
 
+@pytest.mark.parametrize("kind,e", [(6, 4), (5, 2), (7, 2)])
+def test_append_refuses_pages_of_keys_that_are_pages_of_values(kind, e):
+    page = 16 * 2 * 64
+    arrays = batch(offsets=O + 4, lens=Q << 8, pages=Q << 8)  # (q_out meets offsets: refused behind the pages' check)
+
+    def pool(v, stride):
+        return append(p=kv(type=kind, v=FAKE + v * e, page_stride=stride), b=arrays)
+
+    for v, stride in [(0, page), (8, page), (page - 8, page), (page, page), (3 * page, page), (-page, page), (0, 2 * page),
+                      (2 * page, 2 * page), (page - 8, 2 * page), (page + 8, 2 * page), (-page + 8, 2 * page), (6 * page, 2 * page),
+                      (5 * page + 8, 2 * page)]:
+        refused(pool(v, stride), "pages of k and v")
+    for v, stride in [(4 * page, page), (-4 * page, page), (page, 2 * page), (-page, 2 * page), (3 * page, 2 * page),
+                      (5 * page, 2 * page), (7 * page, 2 * page), (7 * page + 8, 2 * page), (page + 8, 3 * page), (8 * page, 2 * page)]:
+        refused(pool(v, stride), "q_out overlaps the batch")
+
+
 def test_append_query_rows_apart_from_the_batch():
     p = kv(v=V << 8)
     for b in (batch(offsets=O + 4 * 767, lens=WS, pages=WS), batch(offsets=WS, lens=O - 4, pages=WS), batch(offsets=WS, lens=WS, pages=O - 36)):
