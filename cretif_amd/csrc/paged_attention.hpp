@@ -16,7 +16,7 @@
 //     row loads (16-bit types: byte permutations; fp32: none are needed).
 //   * 16-bit caches, v_mfma_f32_16x16x32: cached numbers are exact operands.  The fp32 queries and probabilities
 //     are taken in parts whose sum is good to fp32: two fp16 parts (queries scaled per row into fp16's upper range,
-//     probabilities by 2^12), three bf16 parts.  fp32 caches: v_mfma_f32_16x16x4, which keeps up with memory.
+//     probabilities by 2^12; kSafe says what that leaves), three bf16 parts.  fp32 caches: v_mfma_f32_16x16x4, which keeps up with memory.
 //   * The running maximum is raised, and the accumulators rescaled, only when a score exceeds it by kSlack.
 //   * A tile that some column does not see as a whole is multiplied once per limit that its columns have, V zeroed
 //     from the limit on: what lies behind a row's last position (stale pages, infinities) never meets it, not even
@@ -79,6 +79,41 @@ struct PagedShape {
     static constexpr float kShift = TYPE == kKvF16 ? 12.0f : 0.0f;  // probabilities enter O times 2^kShift
     static constexpr float kSlack = 3.0f;  // 2^(12 + 3) is inside fp16
 };
+
+// Probabilities in two fp16 parts.  One of 2^-15 of the running maximum and more keeps 22 bits.  Below, the parts reach fp16's
+// smallest step, and what they leave is up to 2^-25 (in accumulators of 2^kShift times the sum) whatever the probability: over
+// n positions an accumulator is off by up to n 2^-25 of the largest value.  That counts where the result is small against
+// the values, as where a position of weight whose value is next to nothing stands before many others (an attention sink).  So
+// a wave keeps the largest value that a row sees, and a row whose accumulators all are below 2^kSafe of that bound is done again
+// with the probabilities as they are, by fp32 matrix instructions (rows_body with EXACT): it and no other row, or what
+// a row does not see would reach its bits.  Rows that pass
+// are within 2^-kSafe of their largest element, by this bound; as rounding goes they are at 2^-22.  Ordinary rows pass: a
+// position of weight 1 puts 2^12 of its value into them, and the bar is 2^6 of the largest value over 8192 positions.
+// Measured: the watch costs 1.5% (480 rows x 32 heads of 128 on 32768 positions 492 -> 500 us; 64 sequences of 1500 own
+// positions 64.4 -> 64.7), 3 to 4% where it is not EVEN, 11% of a prefix of heads of 256 (567 -> 628).  Where every row has such
+// a position in the prefix's first chunk, that chunk is done again by waves of their own: 496 -> 2228 us, 64 conversations
+// on 8192 positions 60 -> 216; own positions 52 -> 59.
+constexpr int kSafe = 18;
+struct Largest {  // of fp16 numbers of either sign; a NaN stays one
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    h2 top = {0, 0}, low = {0, 0};
+    __device__ __forceinline__ void add(uint32_t a, uint32_t b) {  // (two v_pk_maximum3 for four numbers)
+        const h2 x = __builtin_bit_cast(h2, a), y = __builtin_bit_cast(h2, b);
+        top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, x), y);
+        low = __builtin_elementwise_minimum(__builtin_elementwise_minimum(low, x), y);
+    }
+    // the wave's largest magnitude, infinity where there are NaN
+    __device__ __forceinline__ float of_wave() const {
+        const h2 m = __builtin_elementwise_maximum(top, -low);
+        const _Float16 most = __builtin_elementwise_maximum(m.x, m.y);
+        return wave_max(most == most ? static_cast<float>(most) : INFINITY);
+    }
+};
+// whether accumulators of largest magnitude `most` may be off by more than their share, n positions with values up to `value`
+__device__ __forceinline__ bool too_small(float most, int n, float value) {
+    constexpr float kStep = 1.0f / (1 << (25 - kSafe));
+    return !(most >= static_cast<float>(n) * kStep * value);
+}
 
 __device__ __forceinline__ f32x4 mma16(const u32x4& a, const u32x4& b, const f32x4& c, std::integral_constant<int, kKvF16>) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
@@ -209,15 +244,20 @@ __device__ __forceinline__ bool prefix_item(const PagedAttnArgs& a, int i, int H
 // workgroup b of n in the order of the XCDs that get them: b mod 8's first, n a multiple of 8
 __device__ __forceinline__ int by_xcd(int b, int n) { return b % kPagedXcds * (n / kPagedXcds) + b / kPagedXcds; }
 
-// EVEN: head_dim is DP and the page size a multiple of 16, so the 16 positions of a tile's row block lie in one page
-// (block: of pre_blocks workgroups of the prefix, then the sequences')
-template <int TYPE, int DP, bool EVEN>
-__device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int block) {
+constexpr int kPrefixRows = 128;  // rows of a workgroup of prefix_body
+
+// EVEN: head_dim is DP and the page size a multiple of 16, so the 16 positions of a tile's row block lie in one page.
+// block: of pre_blocks workgroups of the prefix, then the sequences'.  Returns the columns that have to be done again (bit c),
+// which are stored nowhere; EXACT (fp16) does columns `these` again with probabilities in fp32, of the item or of a half of
+// a wave's rows in prefix_body.
+template <int TYPE, int DP, bool EVEN, bool EXACT = false>
+__device__ __forceinline__ uint32_t rows_body(const PagedAttnArgs& a, const int block, const int half = 0, const uint32_t these = 0) {
     typedef PagedShape<TYPE, DP> S;
     typedef typename KvType<TYPE>::elem elem;
     typedef std::integral_constant<int, TYPE> Type;
     constexpr int kTile = S::kTile, kT = S::kT, kKs = S::kKs, kVe = S::kVe, kNh = S::kNh, kAcc = S::kAcc;
     constexpr int kEs = sizeof(elem), kNs = 4 * kT;  // scores of a lane
+    constexpr bool kWatch = TYPE == kKvF16 && !EXACT;
 
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -235,8 +275,10 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
     const int prefix_pages = (a.prefix_len + a.P.page_size - 1) / a.P.page_size;
     if (prefix) {
         int chunk, tile;
-        if (!prefix_item(a, 4 * by_xcd(block, a.pre_blocks) + w, Hkv, chunk, kvh, tile)) return;
-        row0 = tile * 16;
+        const int at = by_xcd(block, a.pre_blocks);
+        const bool shared = EXACT && a.staged;
+        if (!prefix_item(a, shared ? at : 4 * at + w, Hkv, chunk, kvh, tile)) return 0;
+        row0 = shared ? tile * kPrefixRows + 32 * w + 16 * half : tile * 16;
         nrows = a.B.n_rows * G;
         tok0 = 0;
         rec_at = chunk;
@@ -257,7 +299,7 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
             int more = item - rest * a.own_more;
             chunk = div_by(rest, a.by_Hkv);
             kvh = rest - chunk * Hkv;
-            if (chunk >= a.own_chunks) return;
+            if (chunk >= a.own_chunks) return 0;
             // the more-th of the tiles behind the sequences' first ones: 64 sequences' counts summed at a time
             seq = -1;
             for (int base = 0; base < a.B.n_seqs; base += 64) {
@@ -273,11 +315,11 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
                 }
                 more -= __builtin_amdgcn_readlane(sum, 63);
             }
-            if (seq < 0 || seq >= a.B.n_seqs) return;
+            if (seq < 0 || seq >= a.B.n_seqs) return 0;
         }
         tok0 = offsets[seq];
         const int n = min(max(offsets[seq + 1] - tok0, 0), a.B.n_rows);
-        if (n == 0) return;
+        if (n == 0) return 0;
         const int len = max(lens[seq], 0);
         row0 = tile * 16;
         nrows = n * G;
@@ -308,6 +350,7 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
             p = position_of(a.B, i0, min(div_by(row0 + 15, a.by_G), a.B.n_rows - 1) - i0 + 1, i - i0, found);
             ok = ok && found;
         }
+        if (EXACT) ok = ok && (these >> c & 1) != 0;
         if (ok) {
             tok = t;
             head = kvh * G + r - i * G;
@@ -318,7 +361,7 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
         if (g == 0 && tok >= 0)
             *reinterpret_cast<f32x2*>(a.rec + ((static_cast<long>(tok) * a.H + head) * a.nrec + rec_at) * (D + 4)) =
                 f32x2{-INFINITY, 0.0f};
-        return;
+        return 0;
     }
     // the query's row, under way while the first tile is looked up
     f32x4 raw[S::kWide ? kKs : 2 * kKs];
@@ -448,6 +491,8 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
 
     f32x4 acc[kAcc];
     float mx = -INFINITY, sum = 0.0f;
+    Largest values;      // of the tiles that every column sees as a whole
+    float value = 0.0f;  // of the others, as far as this column sees them
 #pragma unroll
     for (int i = 0; i < kAcc; ++i) acc[i] = f32x4{0, 0, 0, 0};
 
@@ -516,7 +561,21 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
                 sum += p[i];
             }
             u32x4 pb[S::kParts];
-            if constexpr (!S::kWide) split8<TYPE, S::kParts>(p, pb);
+            if constexpr (!S::kWide && !EXACT) split8<TYPE, S::kParts>(p, pb);
+            // the tile's values, if masked those of its positions [lo, hi)
+            auto watch = [&](auto masked, Largest& l, int lo, int hi) {
+#pragma unroll
+                for (int t = 0; t < kT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = 16 * t + 4 * g + i;
+                        const uint32_t on = !decltype(masked)::value || (at >= lo && at < hi) ? 0xFFFFFFFFu : 0u;
+#pragma unroll
+                        for (int h = 0; h < kNh; ++h)
+#pragma unroll
+                            for (int e = 0; e < kVe / 2; e += 2) l.add(v[t][i][h][e] & on, v[t][i][h][e + 1] & on);
+                    }
+            };
             // O^T += V^T P^T; `from` zeroes the positions from there on (an index into the tile) and those before p_lo
             auto multiply = [&](auto masked, int from, bool mine) {
                 constexpr bool kMask = decltype(masked)::value;
@@ -536,6 +595,19 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
                                 if (kMask && (4 * g + i < lo || 4 * g + i >= from)) u = 0.0f;
                                 x = __builtin_amdgcn_mfma_f32_16x16x4f32(u, p[i], x, 0, 0, 0);
                             }
+                        } else if constexpr (EXACT) {
+                            __builtin_amdgcn_sched_barrier(0);  // (registers before speed: one element of V at a time)
+#pragma unroll
+                            for (int t = 0; t < kT; ++t)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const int at = 16 * t + 4 * g + i;
+                                    const uint32_t r = v[t][i][h][e >> 1];
+                                    float u = static_cast<float>(
+                                        __builtin_bit_cast(_Float16, static_cast<uint16_t>(e & 1 ? r >> 16 : r)));
+                                    if (kMask && (at < lo || at >= from)) u = 0.0f;
+                                    x = __builtin_amdgcn_mfma_f32_16x16x4f32(u, p[4 * t + i], x, 0, 0, 0);
+                                }
                         } else {
                             // dim e of the lane's eight positions: halves of two rows' dwords
                             u32x4 f;
@@ -561,13 +633,24 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
                         }
                     }
             };
-            if (whole) {
+            if (!EXACT && whole) {
                 multiply(std::false_type{}, 0, true);
+                if constexpr (kWatch) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    watch(std::false_type{}, values, 0, 0);
+                }
             } else {  // once per limit that the tile's columns have
                 const int rel = min(max(min(p_hi, lim) - p0, 0), kTile);
                 for (unsigned long left = __ballot(rel > 0); left != 0;) {
                     const int from = __builtin_amdgcn_readlane(rel, __builtin_ctzl(left));
                     multiply(std::true_type{}, from, rel == from);
+                    if constexpr (kWatch) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        Largest some;
+                        watch(std::true_type{}, some, p_lo - p0, from);
+                        const float most = some.of_wave();
+                        if (rel == from) value = fmaxf(value, most);
+                    }
                     left &= ~__ballot(rel == from);
                 }
             }
@@ -580,9 +663,22 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
     }
 
     // ---- the record, or the output
+    uint32_t again = 0;
+    if constexpr (kWatch) {
+        float big = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kAcc; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(acc[i][e]));
+        big = col_max(big);
+        value = fmaxf(value, values.of_wave());
+        const int n = own_hi - own_lo + before_hi - before_lo;
+        again = __ballot(tok >= 0 && mx != -INFINITY && too_small(big, n, value)) & 0xFFFF;
+        if ((again >> c & 1) != 0) tok = -1;
+    }
     sum = col_sum(sum);
     if (sum != sum) mx = INFINITY;  // NaN scores leave no maximum: keep the record from being skipped
-    if (tok < 0) return;
+    if (tok < 0) return again;
     float* dst;
     float back = 1.0f;
     if (a.nrec == 1) {
@@ -592,7 +688,7 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
         dst = a.rec + ((static_cast<long>(tok) * a.H + head) * a.nrec + rec_at) * (D + 4);
         if (g == 0) *reinterpret_cast<f32x2*>(dst) = f32x2{mx, sum};
         dst += 4;
-        if (mx == -INFINITY) return;
+        if (mx == -INFINITY) return again;
     }
 #pragma unroll
     for (int h = 0; h < kNh; ++h)
@@ -606,6 +702,7 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
                         f32x4_a4{acc[h * kVe + e][i] * back, acc[h * kVe + e + 1][i] * back, acc[h * kVe + e + 2][i] * back,
                                  acc[h * kVe + e + 3][i] * back};
             }
+    return again;
 }
 
 // The shared prefix against many rows.  A workgroup of four waves takes 128 rows, 32 to a wave, and a chunk of the
@@ -626,7 +723,7 @@ __device__ __forceinline__ void rows_body(const PagedAttnArgs& a, const int bloc
 // TFLOP/s), the rest is the exponentials and parts, about 95 vector instructions and 16 exponentials per wave and tile to
 // 32 products.  Issuing the next tile's scores between them, and operands read ahead, were measured at 562 to 585 us against
 // 541: more registers, the same power.
-constexpr int kPrefixRows = 128, kPrefixTile = 32, kRing = 4;
+constexpr int kPrefixTile = 32, kRing = 4;
 constexpr int prefix_lds(int type, int dp) { return 2 * (type == kKvF32 ? 3 : kRing) * kPrefixTile * dp * 2; }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -667,8 +764,9 @@ __device__ __forceinline__ void wait_copies() {  // all but the last N copies of
 // the copy that needs it), pieces behind head_dim are the row's first one again (the query is zero there) and blocks of dims
 // behind it are not multiplied: 480 rows x 32 heads on 32768 positions, pages of 20 525 us (waves of their own 1407), heads of
 // 80 411 (1328), 40 299 (974).
+// Returns the wave's rows that have to be done again (bit i), which are stored nowhere.
 template <int TYPE, int DP, bool EVEN>
-__device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int block, char* const ring) {
+__device__ __forceinline__ uint32_t prefix_body(const PagedAttnArgs& a, const int block, char* const ring) {
     constexpr bool kWide = TYPE == kKvF32;                        // K and V, too, are taken in three bf16 parts
     constexpr int kMath = kWide ? kKvBF16 : TYPE, kKv = kWide ? 3 : 1;
     typedef PagedShape<kMath, DP> S;
@@ -684,7 +782,7 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
     constexpr int kEs = kWide ? 4 : 2;
     const uint32_t row_bytes = static_cast<uint32_t>(Hkv) * D * kEs;
     int chunk, kvh, tile;
-    if (!prefix_item(a, by_xcd(block, a.pre_blocks), Hkv, chunk, kvh, tile)) return;
+    if (!prefix_item(a, by_xcd(block, a.pre_blocks), Hkv, chunk, kvh, tile)) return 0;
     const int p_lo = chunk * a.pre_per, p_hi = min(p_lo + a.pre_per, a.prefix_len);
     const int ntiles = (p_hi - p_lo + kPrefixTile - 1) / kPrefixTile;
     const int table_len = (a.prefix_len + a.P.page_size - 1) / a.P.page_size;
@@ -869,6 +967,7 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
         return swap_max32(m, m) * kf;
     };
     // V^T's operand of dim block d and positions 16 b .. : two reads of 4 x 16
+    Largest values;  // of the wave's quarter of every tile
     const int v_row = 4 * h + ((lane >> 2) & 3), v_col = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);  // row, byte in 64
     for (int tl = 0; tl < ntiles; ++tl) {
         if constexpr (kWide) {
@@ -885,6 +984,15 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
             for (int x = threadIdx.x; x < (kPrefixTile - left) * kPieces; x += 256)
                 *reinterpret_cast<u32x4*>(ring + kValues + tl % kRing * kTileB + left * kRowB + 16 * x) = u32x4{0, 0, 0, 0};
             __syncthreads();
+        }
+        if constexpr (TYPE == kKvF16) {  // (a block of its own: among the products its reads cost 14 to 140 spilled registers)
+            const char* const at = ring + kValues + tl % kRing * kTileB + w * (kTileB / 4) + 16 * lane;
+#pragma unroll
+            for (int x = 0; x < kTileB / 4; x += 1024) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(at + x);
+                values.add(v[0], v[1]);
+                values.add(v[2], v[3]);
+            }
         }
         if (active) {
             f32x16 s;
@@ -935,25 +1043,60 @@ __device__ __forceinline__ void prefix_body(const PagedAttnArgs& a, const int bl
         if constexpr (kWide) __syncthreads();  // the parts have been read
     }
     if constexpr (!kWide) wait_copies<0>();
-
+    uint32_t again = 0;
+    if constexpr (TYPE == kKvF16) {
+        float big = 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDb; ++d)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) big = fmaxf(big, fabsf(o[d][v]));
+        big = swap_max32(big, big);
+        const float mine = values.of_wave();
+        float* const quarters = reinterpret_cast<float*>(ring);
+        __syncthreads();  // the ring has been read, and no copy is under way
+        if (lane == 0) quarters[w] = mine;
+        __syncthreads();
+        const float value = fmaxf(fmaxf(quarters[0], quarters[1]), fmaxf(quarters[2], quarters[3]));
+        again = static_cast<uint32_t>(__ballot(sees && mx != -INFINITY && too_small(big, p_hi - p_lo, value)));
+    }
     sum = swap_add32(sum, sum);
     if (sum != sum) mx = INFINITY;  // NaN scores leave no maximum: keep the record from being skipped
     if (!sees) mx = -INFINITY;
-    if (tok < 0) return;
+    if (tok < 0 || (again >> i & 1) != 0) return again;
     float* dst = a.rec + ((static_cast<long>(tok) * a.H + head) * a.nrec + chunk) * (D + 4);
     if (h == 0) *reinterpret_cast<f32x2*>(dst) = f32x2{mx, sees ? sum : 0.0f};
-    if (mx == -INFINITY) return;
+    if (mx == -INFINITY) return again;
 #pragma unroll
     for (int d = 0; d < kDb; ++d)
 #pragma unroll
         for (int v = 0; v < 16; v += 4)
             if (EVEN || 32 * d + 2 * v + 4 * h < D)
                 *reinterpret_cast<f32x4*>(dst + 4 + 32 * d + 2 * v + 4 * h) = f32x4{o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
+    return again;
+}
+
+// The columns that a body has left (rows of prefix_body: 16 and 16), with exact probabilities.
+// The kernel's arguments (its only one: a PagedAttnArgs) are loaded again, from where the compiler cannot know them: or it
+// would keep them, and what it computed of them, in registers over the bodies' loops for the sake of this rare path.
+template <int TYPE, int DP, bool EVEN>
+__device__ __forceinline__ void rows_again(const int block, const uint32_t left) {
+    if constexpr (TYPE == kKvF16) {
+        const uint32_t columns = __builtin_amdgcn_readfirstlane(left);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t these = columns >> 16 * half & 0xFFFF;
+            if (these == 0) continue;
+            auto args = (const __attribute__((address_space(4))) PagedAttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+            asm volatile("" : "+s"(args));
+            rows_body<TYPE, DP, EVEN, true>(*(const PagedAttnArgs*)args, block, half, these);
+        }
+    }
 }
 
 template <int TYPE, int DP, bool EVEN>
 __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_attn_kernel(const PagedAttnArgs a) {
-    rows_body<TYPE, DP, EVEN>(a, blockIdx.x + (a.staged ? a.pre_blocks : 0));
+    const int block = blockIdx.x + (a.staged ? a.pre_blocks : 0);
+    rows_again<TYPE, DP, EVEN>(block, rows_body<TYPE, DP, EVEN>(a, block));
 }
 // The prefix's workgroups and behind them the sequences', in one launch: the former are bound by the matrix instructions,
 // the latter by memory and by the trips to it before their first tile, and a CU holds one of each (64 conversations on
@@ -961,10 +1104,12 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
 template <int TYPE, int DP, bool EVEN>
 __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_mixed_kernel(const PagedAttnArgs a) {
     __shared__ __attribute__((aligned(16))) char ring[prefix_lds(TYPE, DP)];
+    uint32_t left;
     if (static_cast<int>(blockIdx.x) < a.pre_blocks)
-        prefix_body<TYPE, DP, EVEN>(a, blockIdx.x, ring);
+        left = prefix_body<TYPE, DP, EVEN>(a, blockIdx.x, ring);
     else
-        rows_body<TYPE, DP, EVEN>(a, blockIdx.x);
+        left = rows_body<TYPE, DP, EVEN>(a, blockIdx.x);
+    rows_again<TYPE, DP, EVEN>(blockIdx.x, left);
 }
 // Heads over 128: the queries and accumulators alone take more than half of a SIMD's registers and the ring 128 KB, one
 // workgroup to a CU, so the sequences' workgroups have a launch of their own.  16 heads of 256, 480 rows on 32768
@@ -972,7 +1117,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_mixed_kernel(const 
 template <int TYPE, bool EVEN>
 __global__ __launch_bounds__(64 * kPagedWaves, 1) void paged_prefix_kernel(const PagedAttnArgs a) {
     __shared__ __attribute__((aligned(16))) char ring[prefix_lds(TYPE, 256)];
-    prefix_body<TYPE, 256, EVEN>(a, blockIdx.x, ring);
+    rows_again<TYPE, 256, EVEN>(blockIdx.x, prefix_body<TYPE, 256, EVEN>(a, blockIdx.x, ring));
 }
 
 template <int TYPE, int DP, bool EVEN>

@@ -562,6 +562,99 @@ def test_fp32_numbers_far_apart(many):
         check_rows(out[:, part], want[:, part])
 
 
+def check_heads(got, want, H, bar=1e-5):
+    """Each head of a row against its own largest element."""
+    check_rows(got.reshape(len(want) * H, -1), want.reshape(len(want) * H, -1), bar)
+
+
+def sink(pool, place, q, H, scale, gap, spread, value, far, seed=0):
+    """Keys whose scores lie `gap` below those of position place(0): queries have 4 in dim 0, where that key alone has
+    something, and small numbers elsewhere; the others' scores differ by about `spread`.  The first value is `value` times the
+    others', or (far) they rise from 2^-8 to 1 over the heads' dims."""
+    Hkv, D = pool.k.shape[2:]
+    q.mul_(0.5 * spread / (D - 1) ** 0.5 / scale).view(len(q), H, D)[:, :, 0] = 4.0
+    pool.k[..., 0] = 0
+    if far:
+        pool.v.mul_(2.0 ** torch.linspace(-8, 0, D, device="cuda").to(pool.v.dtype))
+    pg, at = place(0)
+    pool.k[pg, at] = 0
+    pool.k[pg, at, :, 0] = gap / scale / 4.0
+    pool.v[pg, at] *= value
+
+
+# One position takes almost all weight and has (next to) no value: the others, far below it, are the result.  Bars as above:
+# the largest terms are the scores, up to 30 of 24 bits: 30 u in a probability's exponent.
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("gap,spread,value", [(12, 0.0, 0.0), (15, 0.0, 0.0), (15, 1.0, 0.0), (18, 0.0, 0.0), (18, 1.0, 0.0), (21, 0.0, 0.0),
+                                              (21, 1.0, 0.0), (18, 1.0, 2.0 ** -20), (18, 3.0, 2.0 ** -12), (26, 2.0, 0.0)])
+@pytest.mark.parametrize("shape", [
+    # counts, own, P, ps, H, Hkv, D: the position is the batch's first of the prefix, or each sequence's first
+    ([1], [1024], 0, 16, 4, 1, 128),                               # one chunk or several
+    ([1, 3], [31, 900], 0, 16, 8, 2, 64),
+    ([2, 1], [700, 33], 0, 9, 6, 2, 80),                            # other heads and pages
+    ([1, 2], [300, 500], 0, 16, 4, 1, 256),
+    ([1], [20], 0, 16, 2, 1, 64),                                   # one chunk, straight to out
+    ([1, 4], [30, 60], 700, 16, 8, 2, 128),                         # a prefix, waves of their own
+    ([2] * 60, [2 + i % 40 for i in range(60)], 1200, 16, 8, 2, 128),   # through LDS
+    ([2] * 70, [2 + i % 40 for i in range(70)], 1111, 20, 4, 2, 64),
+    ([1] * 66, [1 + i % 40 for i in range(66)], 1070, 7, 8, 2, 120),
+    ([2] * 40, [2 + i for i in range(40)], 8200, 16, 4, 2, 256),
+    ([2] * 36, [2 + i for i in range(36)], 7400, 12, 4, 1, 200),
+], ids=lambda s: "%dx%d_P%d_D%d" % (len(s[0]), s[0][0], s[2], s[6]))
+def test_a_position_of_weight_without_value(kind, gap, spread, value, shape):
+    counts, own, P, ps, H, Hkv, D = shape
+    scale = D ** -0.5
+    pool, off, held, rows, prefix, q = case(kind, counts, own, P, ps, H, Hkv, D, ahead=1, qscale=1.0)
+    first = [(prefix[0], 0)] if P else [(r[0], 0) for r in rows]
+    sink(pool, lambda i: first[i], q, H, scale, gap, spread, value, far=gap == 26)
+    for pg, at in first[1:]:  # (every sequence's own)
+        pool.k[pg, at], pool.v[pg, at] = pool.k[first[0]], pool.v[first[0]]
+    out = attend(pool, off, held, rows, q, H, scale, prefix, P)
+    want = ref.attention(q, pool.k, pool.v, off, held, rows, prefix, P, H, np.float64(np.float32(scale)), torch.full(q.shape, 7.0))
+    check_heads(out[1:], want[1:], H)
+    assert (out[0] == 7).all() and torch.equal(out, attend(pool, off, held, rows, q, H, scale, prefix, P))
+    # a row is done again for itself alone: other queries beside it leave its bits
+    other = q.clone()
+    other[1::2] *= -1
+    got = attend(pool, off, held, rows, other, H, scale, prefix, P)
+    assert torch.equal(got[2::2], out[2::2])
+    # what lies behind the rows still reaches none: those that are done again, too
+    used = torch.zeros(pool.k.shape[:2], dtype=torch.bool)
+    for s, n in enumerate(held):
+        for p in range(P, n):
+            used[rows[s][p // ps], p % ps] = True
+    for p in range(P):
+        used[prefix[p // ps], p % ps] = True
+    bad = ~used.cuda()
+    pool.k[bad], pool.v[bad] = float("nan"), float("inf")
+    assert torch.equal(out, attend(pool, off, held, rows, q, H, scale, prefix, P))
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("D,P,ps", [(64, 1000, 16), (128, 1000, 16), (256, 3900, 16), (80, 1000, 16), (128, 1000, 20), (200, 3900, 12),
+                                    (128, 200, 16)])
+def test_rows_inside_a_prefix_with_such_a_position(kind, D, P, ps):
+    """Rows that are done again beside rows that see a part of the prefix, or nothing; a NaN behind some of them."""
+    H, Hkv, scale = 4, 1, D ** -0.5
+    counts = [1] * 20 + [30, 6, 9, 1, 2, 1]
+    held = [P + 5 + i for i in range(20)] + [P + 10, 3, P - 60, 1, 0, 5000]
+    total, rows, _ = tables([P + 64] * len(held), ps)
+    rows = [r[:(P + 64) // ps] for r in rows]
+    pool = Pool(total, ps, Hkv, D, kind)
+    prefix = [int(x) for x in np.random.default_rng(1).permutation(total)[:-(-P // ps)]]
+    off = starts(counts)
+    q = randn(sum(counts), H * D, seed=2)
+    sink(pool, lambda i: (prefix[0], 0), q, H, scale, 18, 1.0, 0.0, False)
+    pos = np.array([p for _, _, p in ref.places(off, held, len(q))])
+    want = ref.attention(q, pool.k, pool.v, off, held[:-1] + [len(rows[0]) * ps], rows, prefix, P, H, np.float64(np.float32(scale)), torch.zeros(q.shape))
+    out = attend(pool, off, held, rows, q, H, scale, prefix, P)
+    check_heads(out, want, H)
+    assert (out[pos < 0] == 0).all() and (out[pos == 0] == 0).all() and (pos < 0).sum() == 5 and (pos == 0).sum() == 2
+    pool.v[prefix[150 // ps], 150 % ps] = float("nan")
+    got = attend(pool, off, held, rows, q, H, scale, prefix, P)
+    assert torch.equal(got[pos < 150], out[pos < 150]) and torch.isnan(got[pos >= 150]).all() and (pos >= 150).sum() > 50
+
+
 def test_strided_rows_and_a_given_workspace():
     H, Hkv, D, P, ps = 8, 2, 64, 40, 16
     pool, off, held, rows, prefix, q = case("fp16", [1, 4], [20, 100], P, ps, H, Hkv, D)
