@@ -99,6 +99,11 @@ struct Cut {
 };
 
 constexpr int kPreRecords = 64, kOwnRecords = 192;  // chunks at most
+// Bytes of records at most, as long as one chunk of the prefix and one of the sequences' positions fit: a prompt's rows are
+// many and their tables long, and 8192 rows of 32 heads of 128 under a table of 32768 positions had 17.7 GB.  So many rows
+// leave few idle places with fewer chunks: 8192 rows on as many positions 4046 -> 2753 us, 1100 rows under a table of 131072
+// 548 -> 180, 512 rows behind 130560 positions 5262 -> 5000.
+constexpr long kMaxRecordBytes = 1L << 30;
 constexpr int kSlots = 512;                         // workgroups on the GPU at a time: two per CU
 
 int round_up(int x, int to) { return (x + to - 1) / to * to; }
@@ -108,6 +113,7 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
     const int D = P.head_dim, G = n_heads / P.n_kv_heads;
     c.even = (D == 64 || D == 128 || D == 256) && P.page_size % 16 == 0;
     const long rows = static_cast<long>(B.n_rows) * G;  // of a KV head
+    const long most = kMaxRecordBytes / (rows * P.n_kv_heads * (D + 4) * 4);  // records of a row and head
     // Measured, heads of 128, 100 own positions, staged against waves of their own: 64 rows on 4096 positions 19.4 /
     // 19.9 us, 128 on 1024 18.2 / 17.8, on 4096 24.6 / 25.4, 512 on 512 23.8 / 27.5, on 2048 32.1 / 38.9, 2048 on 1024
     // 80 / 111 (fp32: 30.7 / 29.0, 25.9 / 23.0, 36 / 41, 38 / 45, 62 / 86, 138 / 210).
@@ -135,7 +141,7 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
         const int slots = D <= 128 ? kSlots : kSlots / 2;
         const double record_us = tile_rows * (D + 4) * 8 / 4.7e6;
         double best = 0.0;
-        for (int n = 1; n <= kPreRecords && n <= units; ++n) {
+        for (int n = 1; n <= kPreRecords && n <= units && (n == 1 || n < most); ++n) {
             const long items = streams * n, per = (units + n - 1) / n;
             double cost;
             if (c.staged) {
@@ -160,9 +166,9 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
     // positions, or less where the batch would leave waves idle.
     // sum of ceil(n G / 16) - 1 over the sequences that have rows: n G is a multiple of gcd(G, 16)
     c.own_more = static_cast<int>((rows - std::gcd(G, 16)) / 16);
-    const long streams = static_cast<long>(P.n_kv_heads) * std::min<long>(B.n_seqs + c.own_more, (rows + 15) / 16 + B.n_seqs);
+    const long streams = static_cast<long>(P.n_kv_heads) * std::min<long>(1L * B.n_seqs + c.own_more, (rows + 15) / 16 + B.n_seqs);
     const long fill = own * streams / (kPagedWaves * kSlots);  // positions of a wave that fill the GPU once
-    const long least = (own + kOwnRecords - 1) / kOwnRecords;
+    const long chunks = std::min<long>(kOwnRecords, std::max(most - c.pre_chunks, 1L)), least = (own + chunks - 1) / chunks;
     c.own_per = round_up(static_cast<int>(std::max({std::min(fill, 256L), least, 1L})), own_tile);
     c.own_chunks = static_cast<int>((own + c.own_per - 1) / c.own_per);
     c.own_first = static_cast<long>(c.own_chunks) * B.n_seqs * P.n_kv_heads;

@@ -427,7 +427,9 @@ int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const
  * of n_kv_heads; n_rows * n_heads at most 2^24; scale finite.  q, out 4-byte aligned, workspace
  * 16-byte, cri_paged_attention_workspace_bytes of it (for the same kv, batch and prefix_len; only
  * their host numbers count, so one workspace serves every step with the same n_seqs, n_rows and
- * max_pages).  out and the workspace overlap no other buffer.  Sums, maxima and products are good to fp32 for every cache
+ * max_pages).  It holds head_dim + 4 floats per row, head and chunk of positions, up to 1 GiB; where two of those for every
+ * row and head are more, as many (max_pages * page_size counts as the sequences' length: a table much wider than the
+ * sequences costs records and time).  out and the workspace overlap no other buffer.  Sums, maxima and products are good to fp32 for every cache
  * type, in an order fixed by the host numbers and lens (fp16, whose probabilities are taken in two parts: within 2^-18 of a
  * head's largest element in its row, whatever the values; rows that would not be are multiplied in fp32, which takes longer). */
 int cri_paged_attention(const cri_paged_kv* kv, const cri_paged_batch* batch, const int* prefix_pages, int prefix_len,

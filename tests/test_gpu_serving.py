@@ -676,6 +676,39 @@ def test_strided_rows_and_a_given_workspace():
         cri.paged_attention(pool.kv, b, q[:4], res[:, :H * D], H, 0.125)
 
 
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("n,past,P,ps,H,Hkv,D,positions", [
+    (1100, 0, 0, 16, 32, 8, 128, 131072),   # a prompt under a table of the longest context: the records' bound is met
+    (1030, 700, 0, 16, 8, 2, 64, 1792),
+    (1025, 90, 300, 20, 8, 1, 128, 1500),   # behind a shared prefix
+    (2049, 0, 0, 16, 4, 4, 128, 2064),
+])
+def test_a_prompts_rows(kind, n, past, P, ps, H, Hkv, D, positions):
+    """Many rows of one sequence (their causal limits run through all its tiles), and a workspace of no more than 1 GiB."""
+    held = P + past + n
+    need, first = -(-held // ps), -(-P // ps)
+    order = [int(x) for x in np.random.default_rng(3).permutation(need + first)]
+    rows, prefix = [order[:need] + [-1] * (-(-positions // ps) - need)], order[need:]
+    pool = Pool(need + first, ps, Hkv, D, kind, seed=4)
+    q = randn(n, H * D, seed=5, scale=2.0)
+    b = cri.PagedBatch(ints([0, n]), ints([held]), ints(rows))
+    room = cri.paged_attention_workspace_bytes(pool.kv, b, n, H, P)
+    assert room <= 1 << 30
+    ws = torch.full((room + 64,), 255, dtype=torch.uint8, device="cuda")  # NaNs
+    out = attend(pool, [0, n], [held], rows, q, H, D ** -0.5, prefix, P, workspace=ws[:room])
+    assert (ws[room:] == 255).all()
+    j = np.arange(held)
+    page = np.array([prefix[x // ps] if x < P else order[x // ps] for x in j])
+    k, v = ref.f64(pool.k)[page, j % ps], ref.f64(pool.v)[page, j % ps]
+    seen = j[None, :] <= (held - n + np.arange(n))[:, None]
+    got, x = ref.f64(out).reshape(n, H, D), ref.f64(q).reshape(n, H, D)
+    for h in range(0, H, 3):
+        s = np.where(seen, x[:, h] @ k[:, h * Hkv // H].T * D ** -0.5, -np.inf)
+        w = np.exp(s - s.max(-1, keepdims=True))
+        check_rows(got[:, h], (w / w.sum(-1, keepdims=True)) @ v[:, h * Hkv // H])
+    assert torch.equal(out, attend(pool, [0, n], [held], rows, q, H, D ** -0.5, prefix, P))
+
+
 # ---- verification ---------------------------------------------------------------------------------------------------
 
 

@@ -130,6 +130,26 @@ def test_attention_empty():
     assert f(None, ref_of(batch()), 20, 4) == -1
 
 
+@pytest.mark.parametrize("kind", [5, 6, 7])
+@pytest.mark.parametrize("D,ps", [(128, 16), (64, 20), (256, 16), (8, 1)])
+def test_attention_workspace_is_bounded(kind, D, ps):
+    """1 GiB, or a record of the prefix and one of the sequences' positions per row and head."""
+    f = cri.lib().cri_paged_attention_workspace_bytes
+    cache = kv(type=kind, head_dim=D, page_size=ps, n_kv_heads=4, page_stride=ps * 4 * D)
+    most = 0
+    for n_rows in (1, 7, 480, 1100, 2048, 8192, 1 << 17, 1 << 19):
+        for n_seqs in (1, 64, 1000):
+            for held in (500, 8192, 32768, 1 << 20):
+                for P in (0, 100, 8000, 32768):
+                    b = batch(n_seqs=n_seqs, n_rows=n_rows, max_pages=-(-held // ps))
+                    n = f(ref_of(cache), ref_of(b), P, 32)
+                    record = n_rows * 32 * (D + 4) * 4
+                    assert n == -5 or 0 <= n <= max(1 << 30, 2 * record if P else 0), (n_rows, n_seqs, held, P, n)
+                    assert n == -5 or n % record == 0
+                    most = max(most, n)
+    assert most > 1 << 29
+
+
 def verify(t=Q, ldt=100, d=K, ldd=100, ids=FAKE, u=V, dr=V, off=FAKE, B=2, n=5, vocab=100, out=O, acc=O2, ws=WS, wsb=1 << 40):
     return status("cri_verify_drafts", t, ldt, d, ldd, ids, u, dr, off, B, n, vocab, out, acc, ws, wsb, None)
 
