@@ -419,7 +419,8 @@ int cri_paged_append(const cri_paged_kv* kv, const cri_paged_batch* batch, const
  * prefix_len 0: every position through its sequence's table.  A row at a position below 0 (a
  * negative lens counts as 0) sees nothing and gets zeros; positions past the table (max_pages *
  * page_size) are not seen.  Nothing behind a row's last position reaches it, whatever its pages hold
- * there; a key or value that is not finite makes the rows that see it not finite.  Table entries of
+ * there; a NaN, or a value that is infinite, makes the rows that see it not finite; an infinite key does, or, where all
+ * its products are -infinity, has no weight (a row that sees nothing else then gets zeros).  Table entries of
  * positions that rows see must be inside the pool (others give unspecified numbers in their
  * sequence's rows).
  *

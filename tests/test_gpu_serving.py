@@ -510,6 +510,27 @@ def test_a_nan_reaches_the_rows_that_see_it(kind):
 
 
 @pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("many", [False, True])
+def test_an_infinite_key_has_no_weight_or_shows(kind, many):
+    """Keys of -infinity where the queries are positive: scores of -infinity.  A row is not finite, or as if those keys were
+    not there; one that sees nothing else gets zeros or is not finite."""
+    H, Hkv, D, P, ps = 8, 2, 128, 1000 if many else 40, 16
+    counts = [2] * 40 if many else [2, 1, 3]
+    pool, off, held, rows, prefix, q = case(kind, counts, [3 + i for i in range(len(counts))], P, ps, H, Hkv, D)
+    q.abs_()
+    pool.k[prefix[1], 5] = -float("inf")          # of all
+    pool.k[rows[0][(held[0] - 1) // ps], (held[0] - 1) % ps] = -float("inf")  # of the last row of sequence 0
+    out = attend(pool, off, held, rows, q, H, D ** -0.5, prefix, P)
+    big = torch.where(pool.k.isinf(), torch.tensor(-1e4, device="cuda").to(pool.k.dtype), pool.k)
+    want = ref.attention(q, big, pool.v, off, held, rows, prefix, P, H, D ** -0.5, torch.zeros(q.shape))
+    bad = ~torch.isfinite(out).all(-1)
+    check_rows(torch.where(bad[:, None], torch.from_numpy(want).float().cuda(), out), want)
+    pool.k.fill_(-float("inf"))
+    out = attend(pool, off, held, rows, q, H, D ** -0.5, prefix, P)
+    assert ((out == 0) | ~torch.isfinite(out)).all()
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
 @pytest.mark.parametrize("what", ["peak", "rising", "tiny_q", "huge_q", "large_v", "spread_q", "zero_q", "no_scale", "minus", "tiny_kv"])
 def test_attention_ranges(kind, what):
     H, Hkv, D, P, ps, scale = 8, 2, 128, 300, 16, 128 ** -0.5
