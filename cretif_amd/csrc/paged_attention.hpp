@@ -175,6 +175,23 @@ __device__ __forceinline__ void row_factors(float qscale, float m, float& f, flo
     kf = fmaxf(kf, kTiny);
     f = qscale == 0.0f ? 0.0f : __builtin_copysignf(f, qscale);
 }
+// A sum of many small terms beside a large one: in one float a chunk's 8192 weights of 2^-24 beside one of 1 are lost, each in
+// its rounding and all the same way, 1.5e-4 of the row as measured; so a tile's are added first, and what their addition
+// rounds away is kept beside the sum (2e-6; under 1% of the time, 3% with heads of 256).  The accumulators, which add 16 or more
+// terms at a time inside the matrix instructions, are left to fp32.
+struct Sum {
+    float hi = 0.0f, lo = 0.0f;
+    __device__ __forceinline__ void add(float t) {
+        const float s = hi + t;
+        lo += t - (s - hi);  // (exact where hi is the larger; else off by an ulp of t, once per rise of the maximum)
+        hi = s;
+    }
+    __device__ __forceinline__ void scale(float f) {
+        hi *= f;
+        lo *= f;
+    }
+    __device__ __forceinline__ float value() const { return hi + lo; }
+};
 __device__ __forceinline__ float col_max(float v) { return swap_max32(swap_max16(v, v), swap_max16(v, v)); }
 __device__ __forceinline__ float col_sum(float v) {
     const float s = swap_add16(v, v);
@@ -490,7 +507,8 @@ __device__ __forceinline__ uint32_t rows_body(const PagedAttnArgs& a, const int 
     }
 
     f32x4 acc[kAcc];
-    float mx = -INFINITY, sum = 0.0f;
+    float mx = -INFINITY;
+    Sum weights;
     Largest values;      // of the tiles that every column sees as a whole
     float value = 0.0f;  // of the others, as far as this column sees them
 #pragma unroll
@@ -549,17 +567,18 @@ __device__ __forceinline__ uint32_t rows_body(const PagedAttnArgs& a, const int 
             if (__ballot(raise) != 0) {
                 const float f = raise ? __builtin_amdgcn_exp2f(mx - m) : 1.0f;
                 if (raise) mx = m;
-                sum *= f;
+                weights.scale(f);
 #pragma unroll
                 for (int i = 0; i < kAcc; ++i) acc[i] *= f;
             }
             const float base = (mx == -INFINITY ? 0.0f : mx) - S::kShift;
-            float p[8] = {};
+            float p[8] = {}, tile_sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < kNs; ++i) {
                 p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], kf, -base));
-                sum += p[i];
+                tile_sum += p[i];
             }
+            weights.add(tile_sum);
             u32x4 pb[S::kParts];
             if constexpr (!S::kWide && !EXACT) split8<TYPE, S::kParts>(p, pb);
             // the tile's values, if masked those of its positions [lo, hi)
@@ -676,7 +695,7 @@ __device__ __forceinline__ uint32_t rows_body(const PagedAttnArgs& a, const int 
         again = __ballot(tok >= 0 && mx != -INFINITY && too_small(big, n, value)) & 0xFFFF;
         if ((again >> c & 1) != 0) tok = -1;
     }
-    sum = col_sum(sum);
+    const float sum = col_sum(weights.value());
     if (sum != sum) mx = INFINITY;  // NaN scores leave no maximum: keep the record from being skipped
     if (tok < 0) return again;
     float* dst;
@@ -931,7 +950,8 @@ __device__ __forceinline__ uint32_t prefix_body(const PagedAttnArgs& a, const in
     for (int d = 0; d < kDb; ++d)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
-    float mx = -INFINITY, sum = 0.0f;
+    float mx = -INFINITY;
+    Sum weights;
 
     // the raw scores of tile t, a lane's 16: positions 8 (v >> 2) + 4 h + (v & 3)
     const char* const k_at = ring + i * kRowB;
@@ -1002,22 +1022,24 @@ __device__ __forceinline__ uint32_t prefix_body(const PagedAttnArgs& a, const in
             if (__ballot(raise) != 0) {
                 const float f = raise ? __builtin_amdgcn_exp2f(mx - m) : 1.0f;
                 if (raise) mx = m;
-                sum *= f;
+                weights.scale(f);
 #pragma unroll
                 for (int d = 0; d < kDb; ++d) o[d] *= f;
             }
             const float base = (mx == -INFINITY ? 0.0f : mx) - S::kShift;
             u32x4 pb[2][kParts];
+            float tile_sum = 0.0f;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 float p[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * b + e], kf, -base));
-                    sum += p[e];
+                    tile_sum += p[e];
                 }
                 split8<kMath, kParts>(p, pb[b]);
             }
+            weights.add(tile_sum);
             const char* const vt = ring + kValues + (kWide ? 0 : tl % kRing * kTileB);
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -1059,6 +1081,7 @@ __device__ __forceinline__ uint32_t prefix_body(const PagedAttnArgs& a, const in
         const float value = fmaxf(fmaxf(quarters[0], quarters[1]), fmaxf(quarters[2], quarters[3]));
         again = static_cast<uint32_t>(__ballot(sees && mx != -INFINITY && too_small(big, p_hi - p_lo, value)));
     }
+    float sum = weights.value();
     sum = swap_add32(sum, sum);
     if (sum != sum) mx = INFINITY;  // NaN scores leave no maximum: keep the record from being skipped
     if (!sees) mx = -INFINITY;

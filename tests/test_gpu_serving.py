@@ -652,6 +652,32 @@ def test_a_position_of_weight_without_value(kind, gap, spread, value, shape):
 
 
 @pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("steps", [0.6, 1.3, 10.4])
+@pytest.mark.parametrize("shape", [
+    # counts, own, P, ps, H, Hkv, D, wider: table entries behind the sequences' (chunks are long under wide tables)
+    ([1] * 70, [1] * 70, 8192, 16, 8, 2, 128, 8000),  # through LDS
+    ([7] * 20, [9] * 20, 2000, 5, 8, 2, 120, 6000),
+    ([1], [2300], 0, 16, 8, 8, 64, 8000),
+    ([1], [9], 3000, 16, 8, 8, 128, 8000),            # a prefix, waves of their own
+], ids=["lds", "lds_other", "own", "prefix"])
+def test_many_small_weights_beside_a_large_one(kind, steps, shape):
+    """One position of weight 1 and thousands of `steps` half units in its last place: their sum counts, though each by itself
+    rounds off, all of them the same way."""
+    counts, own, P, ps, H, Hkv, D, wider = shape
+    scale = D ** -0.5
+    pool, off, held, rows, prefix, q = case(kind, counts, own, P, ps, H, Hkv, D)
+    rows = [r + [-1] * wider for r in rows]
+    place = (prefix[0], 0) if P else (rows[0][0], 0)
+    pool.k.zero_()
+    pool.k[place[0], place[1], :, 0] = 1.0
+    q.zero_().view(len(q), H, D)[:, :, 0] = -np.log(steps * U) / scale
+    out = attend(pool, off, held, rows, q, H, scale, prefix, P)
+    t = counts[0] - 1  # the first sequence's last row
+    want = ref.attention(q[t:t + 1], pool.k, pool.v, [0, 1], [P + own[0]], rows[:1], prefix, P, H, np.float64(np.float32(scale)), out[t:t + 1])
+    check_heads(out[t:t + 1], want, H)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
 @pytest.mark.parametrize("D,P,ps", [(64, 1000, 16), (128, 1000, 16), (256, 3900, 16), (80, 1000, 16), (128, 1000, 20), (200, 3900, 12),
                                     (128, 200, 16)])
 def test_rows_inside_a_prefix_with_such_a_position(kind, D, P, ps):
