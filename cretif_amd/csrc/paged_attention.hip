@@ -114,14 +114,10 @@ Cut cut_of(const PagePool& P, int type, const PageBatch& B, int n_heads, int pre
     c.even = (D == 64 || D == 128 || D == 256) && P.page_size % 16 == 0;
     const long rows = static_cast<long>(B.n_rows) * G;  // of a KV head
     const long most = kMaxRecordBytes / (rows * P.n_kv_heads * (D + 4) * 4);  // records of a row and head
-    // Measured, heads of 128, 100 own positions, staged against waves of their own: 64 rows on 4096 positions 19.4 /
-    // 19.9 us, 128 on 1024 18.2 / 17.8, on 4096 24.6 / 25.4, 512 on 512 23.8 / 27.5, on 2048 32.1 / 38.9, 2048 on 1024
-    // 80 / 111 (fp32: 30.7 / 29.0, 25.9 / 23.0, 36 / 41, 38 / 45, 62 / 86, 138 / 210).
-    // Other heads and pages of 20: 128 rows on 4096 positions 26.7 / 30.4 (heads of 128), 21.1 / 27.0 (80; fp32 31.2 /
-    // 48.2), 15.9 / 21.9 (40), 512 on 2048 34.3 / 47.7, 30.2 / 43.6 (49.5 / 87.9), 23.0 / 33.0, 1920 on 32768 518 /
-    // 1407, 411 / 1328 (1053 / 3651), 299 / 974.  Heads of 256, a workgroup to a CU: fp16 512 on 1024 47 / 44, 512 on
-    // 4096 63 / 72, 1920 on 32768 571 / 1315, bf16 512 on 4096 80 / 78, 1920 on 32768 1028 / 1347; fp32 was slower or
-    // equal everywhere.
+    // Where sharing the prefix through LDS begins to pay: at 2^18 rows x positions both ways take the same (64 rows on 4096
+    // positions 20.2 / 20.2 us, fp32 30.5 / 28.4), with twice as much it is ahead (128 on 4096 25.6 / 25.8, fp32 36.6 / 42.0) and
+    // stays so.  Heads over 128 have one workgroup to a CU: fp16 from 2^20 on (512 on 2048 55.2 / 54.7, on 4096 65.3 / 73.7),
+    // bf16 later (512 on 4096 79.6 / 79.5, 1920 on 32768 1048 / 1399), fp32 not at all (3334 either way).
     const int from = D <= 128 ? 18 : type == kKvF16 ? 20 : type == kKvBF16 ? 22 : 62;
     c.staged = rows > 32 && prefix_len >= 256 && rows * prefix_len >= 1L << from;
     const int own_tile = type == kKvF32 ? 16 : 32;

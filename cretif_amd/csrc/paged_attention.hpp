@@ -736,10 +736,10 @@ __device__ __forceinline__ uint32_t rows_body(const PagedAttnArgs& a, const int 
 //     of fp32's range); a product is the six of parts down to 2^-16, each exact in fp32.  v_mfma_f32_32x32x16_bf16 does 16
 //     times the multiply-adds per cycle of the fp32 instructions, so the six cost 0.38 of their cycles (512 rows of a KV
 //     head on 8192 positions 222 -> 115 us, 256 rows 118 -> 73), at the same distance from float64.
-// 480 rows x 32 heads of 128 on 32768 positions of fp16: 482 us, 1075 TFLOP/s of fp16 products, two for each of the
-// formula's, where a large library product runs at 1150 (bf16, three: 618 us, 1257 against 1207).  The matrix units are busy
+// 480 rows x 32 heads of 128 on 32768 positions of fp16: 493 us, 1045 TFLOP/s of fp16 products, two for each of the
+// formula's, where a large library product runs at 1150 (bf16, three: 620 us, 1247 against 1207).  The matrix units are busy
 // for half the cycles at 1.9 GHz (the clock under this load; nothing but these instructions on random numbers reach 1600
-// TFLOP/s), the rest is the exponentials and parts, about 95 vector instructions and 16 exponentials per wave and tile to
+// TFLOP/s), the rest is the exponentials and parts, about 110 vector instructions and 16 exponentials per wave and tile to
 // 32 products.  Issuing the next tile's scores between them, and operands read ahead, were measured at 562 to 585 us against
 // 541: more registers, the same power.
 constexpr int kPrefixTile = 32, kRing = 4;
@@ -781,8 +781,8 @@ __device__ __forceinline__ void wait_copies() {  // all but the last N copies of
 
 // EVEN: head_dim is DP and the page size a multiple of 16.  Else every lane looks up the page of its own row (a tile ahead of
 // the copy that needs it), pieces behind head_dim are the row's first one again (the query is zero there) and blocks of dims
-// behind it are not multiplied: 480 rows x 32 heads on 32768 positions, pages of 20 525 us (waves of their own 1407), heads of
-// 80 411 (1328), 40 299 (974).
+// behind it are not multiplied: 480 rows x 32 heads on 32768 positions, pages of 20 538 us (waves of their own 1437), heads of
+// 80 432 (1347), 40 309 (996).
 // Returns the wave's rows that have to be done again (bit i), which are stored nowhere.
 template <int TYPE, int DP, bool EVEN>
 __device__ __forceinline__ uint32_t prefix_body(const PagedAttnArgs& a, const int block, char* const ring) {
@@ -1123,7 +1123,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, DP <= 128 ? 2 : 1) void paged_att
 }
 // The prefix's workgroups and behind them the sequences', in one launch: the former are bound by the matrix instructions,
 // the latter by memory and by the trips to it before their first tile, and a CU holds one of each (64 conversations on
-// 8192 tokens: 67 us, 90 in two launches; 480 rows on 32768: 487 and 510).
+// 8192 tokens: 67 us, 90 in two launches; 480 rows on 32768: 487 and 510, both before kSafe's watch).
 template <int TYPE, int DP, bool EVEN>
 __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_mixed_kernel(const PagedAttnArgs a) {
     __shared__ __attribute__((aligned(16))) char ring[prefix_lds(TYPE, DP)];
@@ -1136,7 +1136,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_mixed_kernel(const 
 }
 // Heads over 128: the queries and accumulators alone take more than half of a SIMD's registers and the ring 128 KB, one
 // workgroup to a CU, so the sequences' workgroups have a launch of their own.  16 heads of 256, 480 rows on 32768
-// positions of fp16: 571 us (waves of their own 1315); bf16's third part spills 37 registers, 1024 (1347).
+// positions of fp16: 655 us (waves of their own 1316); bf16's third part spills 40 registers, 1048 (1399).
 template <int TYPE, bool EVEN>
 __global__ __launch_bounds__(64 * kPagedWaves, 1) void paged_prefix_kernel(const PagedAttnArgs a) {
     __shared__ __attribute__((aligned(16))) char ring[prefix_lds(TYPE, 256)];
