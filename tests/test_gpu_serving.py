@@ -985,6 +985,37 @@ def test_captured_attention_of_many_rows(kind):
         q.mul_(-0.9)
 
 
+@pytest.mark.parametrize("P,own", [(1000, 70), (0, 400)])
+def test_captured_rows_that_are_done_again(P, own):
+    """fp16 rows that are multiplied again (a position of weight without value) in a captured call, replayed while queries and
+    lengths change and eager calls run between: the eager bits."""
+    H, Hkv, D, ps = 8, 2, 128, 16
+    n = 70 if P else 5
+    pool, off, held, rows, prefix, q = case("fp16", [1] * n, [own + i % 30 for i in range(n)], P, ps, H, Hkv, D)
+    first = (prefix[0], 0) if P else (rows[0][0], 0)
+    sink(pool, lambda i: first, q, H, D ** -0.5, 20, 1.0, 0.0, False)
+    for r in rows:
+        pool.k[r[0], 0], pool.v[r[0], 0] = pool.k[first], pool.v[first]
+    lens, pp = ints([h - 60 for h in held]), ints(prefix) if P else None
+    b = cri.PagedBatch(ints(off), lens, ints(rows))
+    ws = torch.empty(cri.paged_attention_workspace_bytes(pool.kv, b, n, H, P), dtype=torch.uint8, device="cuda")
+    out, want = torch.zeros_like(q), torch.zeros_like(q)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        cri.paged_attention(pool.kv, b, q, out, H, D ** -0.5, pp, P, ws)
+    for i in range(5):
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        cri.paged_attention(pool.kv, b, q, want, H, D ** -0.5, pp, P, ws)
+        assert torch.equal(out, want)
+        check_heads(out, ref.attention(q, pool.k, pool.v, off, lens.tolist(), rows, prefix, P, H, np.float64(np.float32(D ** -0.5)), out), H)
+        lens += 11
+        q.mul_(0.97)
+
+
 def test_a_side_stream_orders_with_torch():
     want = Serving(2, "bf16")
     want.draw(1)
