@@ -62,6 +62,18 @@ __all__ = [
     "paged_attention_workspace_bytes",
     "verify_drafts",
     "verify_drafts_workspace_bytes",
+    "ExpertGroups",
+    "ExpertRouter",
+    "ExpertWeights",
+    "expert_combine",
+    "expert_combine_workspace_bytes",
+    "expert_matmul",
+    "expert_matmul_workspace_bytes",
+    "expert_swiglu",
+    "expert_swiglu_workspace_bytes",
+    "group_experts",
+    "route_experts",
+    "route_experts_workspace_bytes",
     "FORMAT_IDS",
     "ABI_SYMBOLS",
 ]
@@ -138,6 +150,17 @@ ABI_SYMBOLS = (
         "cri_paged_attention_workspace_bytes",
         "cri_verify_drafts",
         "cri_verify_drafts_workspace_bytes",
+        "cri_expert_packed_bytes",
+        "cri_expert_pack",
+        "cri_expert_route",
+        "cri_expert_group",
+        "cri_expert_group_workspace_bytes",
+        "cri_expert_matmul",
+        "cri_expert_matmul_workspace_bytes",
+        "cri_expert_swiglu",
+        "cri_expert_swiglu_workspace_bytes",
+        "cri_expert_combine",
+        "cri_expert_combine_workspace_bytes",
         "cri_stream_read",
         "cri_stream_read_ex",
         "cri_timestamp",
@@ -322,6 +345,7 @@ def lib():
     L.cri_block_elems.restype = i32
     L.cri_version.restype = i32
     serving.declare(L)
+    experts.declare(L)
     _lib = L
     return L
 
@@ -832,4 +856,19 @@ from .serving import (  # noqa: E402
     qk_norm_rope,
     verify_drafts,
     verify_drafts_workspace_bytes,
+)
+from . import experts  # noqa: E402
+from .experts import (  # noqa: E402
+    ExpertGroups,
+    ExpertRouter,
+    ExpertWeights,
+    expert_combine,
+    expert_combine_workspace_bytes,
+    expert_matmul,
+    expert_matmul_workspace_bytes,
+    expert_swiglu,
+    expert_swiglu_workspace_bytes,
+    group_experts,
+    route_experts,
+    route_experts_workspace_bytes,
 )

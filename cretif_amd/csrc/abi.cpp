@@ -955,6 +955,254 @@ int cri_verify_drafts(const float* target, long long ldt, const float* draft, lo
     return check_launch(fn);
 }
 
+// ---- a layer of experts -----------------------------------------------------
+
+namespace {
+
+constexpr int kMaxExperts = 1024, kMaxChoices = 64;
+constexpr long kMaxPairs = 1L << 23;  // a workgroup of 256 threads each: half of what a launch takes
+constexpr char kTooManyTiles[] = "too many tiles for one launch";
+
+int check_expert_sizes(int format, int n_experts, int N, int K, const char* fn) {
+    if (format < 0 || format > cri::kFmtF16) return fail(CRI_ERR_UNSUPPORTED, fn, "unknown format " + std::to_string(format));
+    if (n_experts < 0 || N < 0 || K < 0) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "negative dimension");
+    if (n_experts < 1 || n_experts > kMaxExperts)
+        return fail(CRI_ERR_SHAPE, fn, "n_experts=" + std::to_string(n_experts) + " must be in [1, " + std::to_string(kMaxExperts) + "]");
+    const int be = std::max(cri::block_elems(format), 32);
+    if (K < be || K % be != 0)
+        return fail(CRI_ERR_SHAPE, fn, "K=" + std::to_string(K) + " is not a positive multiple of " + std::to_string(be));
+    if (static_cast<long>(N) * K > kMaxElems / n_experts || K > (1 << 24) || N > (1 << 24) ||
+        cri::detail::expert_units(n_experts, N, K) > (1L << 25))
+        return fail(CRI_ERR_SHAPE, fn, "problem too large");
+    return CRI_OK;
+}
+
+int check_expert_groups(const cri_expert_groups* g, const char* fn) {
+    if (!g) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null groups");
+    if (g->n_tokens < 0 || g->top_k < 0 || g->n_experts < 0) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "negative dimension");
+    if (g->n_experts < 1 || g->n_experts > kMaxExperts)
+        return fail(CRI_ERR_SHAPE, fn, "n_experts=" + std::to_string(g->n_experts) + " must be in [1, " +
+                                           std::to_string(kMaxExperts) + "]");
+    if (g->top_k < 1 || g->top_k > kMaxChoices || g->top_k > g->n_experts)
+        return fail(CRI_ERR_SHAPE, fn, "top_k=" + std::to_string(g->top_k) + " must be in [1, " + std::to_string(kMaxChoices) +
+                                           "] and at most n_experts");
+    if (static_cast<long>(g->n_tokens) * g->top_k > kMaxPairs)
+        return fail(CRI_ERR_SHAPE, fn, "problem too large (more than 2^23 pairs of token and choice)");
+    return CRI_OK;
+}
+
+long pairs(const cri_expert_groups* g) { return static_cast<long>(g->n_tokens) * g->top_k; }
+
+int check_group_pointers(const cri_expert_groups* g, const char* fn) {
+    if (!g->offsets || (g->n_tokens > 0 && (!g->rows || !g->slots))) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null pointer in the groups");
+    if (!aligned(g->offsets, 4) || !aligned(g->rows, 4) || !aligned(g->slots, 4))
+        return fail(CRI_ERR_ALIGNMENT, fn, "offsets, rows and slots must be 4-byte aligned");
+    return CRI_OK;
+}
+
+Span offsets_of(const cri_expert_groups* g) { return {g->offsets, (g->n_experts + 1L) * 4}; }
+Span rows_of(const cri_expert_groups* g) { return {g->rows, pairs(g) * 4}; }
+Span slots_of(const cri_expert_groups* g) { return {g->slots, pairs(g) * 4}; }
+Span packed_of(const cri_expert_weights* w) {
+    return {w->data, cri::detail::expert_packed_bytes(w->format, w->n_experts, w->N, w->K)};
+}
+
+cri::ExpertRows rows_arg(const cri_expert_groups* g) { return {g->offsets, g->rows, g->slots, g->n_tokens, g->top_k}; }
+cri::ExpertMatrix matrix_arg(const cri_expert_weights* w) { return {w->data, w->format, w->n_experts, w->N, w->K}; }
+
+// the numbers of a product's matrix and groups
+int check_expert_product(const cri_expert_weights* w, const cri_expert_groups* g, const char* fn) {
+    if (!w) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null weights");
+    if (const int st = check_expert_sizes(w->format, w->n_experts, w->N, w->K, fn)) return st;
+    if (const int st = check_expert_groups(g, fn)) return st;
+    if (w->n_experts != g->n_experts)
+        return fail(CRI_ERR_SHAPE, fn, "weights of " + std::to_string(w->n_experts) + " experts, groups of " + std::to_string(g->n_experts));
+    return CRI_OK;
+}
+
+int check_packed(const cri_expert_weights* w, const char* fn) {
+    if (!w->data) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null weights");
+    if (!aligned(w->data, 16)) return fail(CRI_ERR_ALIGNMENT, fn, "laid out weights must be 16-byte aligned");
+    return CRI_OK;
+}
+
+int check_room(const void* workspace, long long bytes, long need, uintptr_t align, const char* fn) {
+    if (need == 0) return CRI_OK;
+    if (!workspace) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null workspace");
+    if (!aligned(workspace, align)) return fail(CRI_ERR_ALIGNMENT, fn, "workspace must be " + std::to_string(align) + "-byte aligned");
+    if (bytes < need)
+        return fail(CRI_ERR_SHAPE, fn, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
+    return CRI_OK;
+}
+
+// out = products of x's rows: cri_expert_matmul and, with up, cri_expert_swiglu
+int expert_product(const cri_expert_weights* w, const cri_expert_weights* up, const cri_expert_groups* g, const float* x, int ldx,
+                   bool gather, float* out, int ldo, void* workspace, long long workspace_bytes, hipStream_t s, const char* fn) {
+    int st;
+    if ((st = check_expert_product(w, g, fn))) return st;
+    if (up) {
+        if (up->format != w->format || up->n_experts != w->n_experts || up->N != w->N || up->K != w->K)
+            return fail(CRI_ERR_SHAPE, fn, "gate and up must have the same format and sizes");
+    }
+    if (g->n_tokens == 0 || w->N == 0) return CRI_OK;
+    if ((st = check_packed(w, fn)) || (up && (st = check_packed(up, fn)))) return st;
+    if ((st = check_group_pointers(g, fn))) return st;
+    const long R = pairs(g), rows = gather ? g->n_tokens : R;
+    if ((st = check_rows(x, ldx, w->K, "x", fn)) || (st = check_rows(out, ldo, w->N, "out", fn))) return st;
+    if (R * std::max(ldx, ldo) > kMaxElems) return fail(CRI_ERR_SHAPE, fn, "problem too large");
+    const long need = cri::detail::expert_product_workspace_bytes(matrix_arg(w), rows_arg(g), up != nullptr, gather);
+    if ((st = check_room(workspace, workspace_bytes, need, 16, fn))) return st;
+    const Span in{x, span_bytes(rows, w->K, ldx)}, to{out, span_bytes(R, w->N, ldo)}, room{workspace, need};
+    const Span second = up ? packed_of(up) : Span{nullptr, 0};
+    for (const Span& written : {to, room})
+        if (meets(written, {in, packed_of(w), second, offsets_of(g), rows_of(g), slots_of(g)}))
+            return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out or the workspace overlaps an input");
+    if (meets(to, {room})) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out overlaps the workspace");
+    clear_pending_error();
+    cri::ExpertMatrix second_arg{};
+    if (up) second_arg = matrix_arg(up);
+    const int rc = cri::detail::launch_expert_products(matrix_arg(w), up ? &second_arg : nullptr, rows_arg(g), x, ldx, gather, out, ldo,
+                                                       workspace, s);
+    if (rc == cri::detail::kDeclined) return fail(CRI_ERR_UNSUPPORTED, fn, kTooManyTiles);
+    return finish_matmul(rc, fn);
+}
+
+}  // namespace
+
+long long cri_expert_packed_bytes(int format, int n_experts, int N, int K) {
+    if (const int st = check_expert_sizes(format, n_experts, N, K, "cri_expert_packed_bytes")) return st;
+    return cri::detail::expert_packed_bytes(format, n_experts, N, K);
+}
+
+int cri_expert_pack(int format, const void* src, int n_experts, int N, int K, void* packed, hipStream_t s) {
+    const char* fn = "cri_expert_pack";
+    if (const int st = check_expert_sizes(format, n_experts, N, K, fn)) return st;
+    if (N == 0) return CRI_OK;
+    if (!src || !packed) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null pointer");
+    if (!aligned(packed, 16)) return fail(CRI_ERR_ALIGNMENT, fn, "laid out weights must be 16-byte aligned");
+    if (meets({packed, cri::detail::expert_packed_bytes(format, n_experts, N, K)},
+              {{src, static_cast<long>(n_experts) * N * cri::row_bytes(format, K)}}))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "packed overlaps src");
+    clear_pending_error();
+    cri::detail::launch_expert_pack(format, src, n_experts, N, K, packed, s);
+    return check_launch(fn);
+}
+
+long long cri_expert_group_workspace_bytes(const cri_expert_groups* g) {
+    if (const int st = check_expert_groups(g, "cri_expert_group_workspace_bytes")) return st;
+    return cri::detail::expert_group_workspace_bytes(g->n_tokens, g->top_k, g->n_experts);
+}
+
+int cri_expert_route(const cri_expert_router* r, const float* logits, int ldl, int* ids, float* weights,
+                     const cri_expert_groups* g, void* workspace, long long workspace_bytes, hipStream_t s) {
+    const char* fn = "cri_expert_route";
+    int st;
+    if (!r) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null router");
+    if (r->scoring != CRI_SCORE_SOFTMAX && r->scoring != CRI_SCORE_SIGMOID) return fail(CRI_ERR_UNSUPPORTED, fn, "unknown scoring");
+    if (!std::isfinite(r->scale)) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "scale must be finite");
+    if (!aligned(r->bias, 4)) return fail(CRI_ERR_ALIGNMENT, fn, "bias must be 4-byte aligned");
+    if ((st = check_expert_groups(g, fn)) || (st = check_group_pointers(g, fn))) return st;
+    const long P = pairs(g);
+    if (g->n_tokens > 0) {
+        if ((st = check_rows(logits, ldl, g->n_experts, "logits", fn))) return st;
+        if (!ids || !weights) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null ids or weights");
+        if (!aligned(ids, 4) || !aligned(weights, 4)) return fail(CRI_ERR_ALIGNMENT, fn, "ids and weights must be 4-byte aligned");
+    }
+    const long need = cri::detail::expert_group_workspace_bytes(g->n_tokens, g->top_k, g->n_experts);
+    if ((st = check_room(workspace, workspace_bytes, need, 4, fn))) return st;
+    const Span written[] = {{ids, P * 4}, {weights, P * 4}, offsets_of(g), rows_of(g), slots_of(g), {workspace, need}};
+    for (int i = 0; i < 6; ++i) {
+        if (meets(written[i], {{logits, span_bytes(g->n_tokens, g->n_experts, ldl)}, {r->bias, r->bias ? g->n_experts * 4L : 0}}))
+            return fail(CRI_ERR_INVALID_ARGUMENT, fn, "an output or the workspace overlaps an input");
+        for (int j = 0; j < i; ++j)
+            if (meets(written[i], {written[j]}))
+                return fail(CRI_ERR_INVALID_ARGUMENT, fn, "outputs, groups and the workspace must not overlap");
+    }
+    clear_pending_error();
+    cri::detail::launch_expert_route({r->bias, r->scale, r->scoring == CRI_SCORE_SIGMOID, r->normalize != 0}, logits, ldl, g->n_experts,
+                                     ids, weights, rows_arg(g), static_cast<int*>(workspace), s);
+    return check_launch(fn);
+}
+
+int cri_expert_group(const int* ids, const cri_expert_groups* g, void* workspace, long long workspace_bytes, hipStream_t s) {
+    const char* fn = "cri_expert_group";
+    int st;
+    if ((st = check_expert_groups(g, fn)) || (st = check_group_pointers(g, fn))) return st;
+    if (g->n_tokens > 0 && !ids) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null ids");
+    if (!aligned(ids, 4)) return fail(CRI_ERR_ALIGNMENT, fn, "ids must be 4-byte aligned");
+    const long need = cri::detail::expert_group_workspace_bytes(g->n_tokens, g->top_k, g->n_experts);
+    if ((st = check_room(workspace, workspace_bytes, need, 4, fn))) return st;
+    const Span written[] = {offsets_of(g), rows_of(g), slots_of(g), {workspace, need}};
+    for (int i = 0; i < 4; ++i) {
+        if (meets(written[i], {{ids, pairs(g) * 4}})) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "the groups or the workspace overlap ids");
+        for (int j = 0; j < i; ++j)
+            if (meets(written[i], {written[j]})) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "groups and the workspace must not overlap");
+    }
+    clear_pending_error();
+    cri::detail::launch_expert_group(ids, g->n_experts, rows_arg(g), static_cast<int*>(workspace), s);
+    return check_launch(fn);
+}
+
+long long cri_expert_matmul_workspace_bytes(const cri_expert_weights* w, const cri_expert_groups* g, int grouped) {
+    if (const int st = check_expert_product(w, g, "cri_expert_matmul_workspace_bytes")) return st;
+    if (g->n_tokens == 0 || w->N == 0) return 0;
+    return cri::detail::expert_product_workspace_bytes(matrix_arg(w), rows_arg(g), false, grouped == 0);
+}
+
+int cri_expert_matmul(const cri_expert_weights* w, const cri_expert_groups* g, const float* x, int ldx, int grouped, float* out,
+                      int ldo, void* workspace, long long workspace_bytes, hipStream_t s) {
+    return expert_product(w, nullptr, g, x, ldx, grouped == 0, out, ldo, workspace, workspace_bytes, s, "cri_expert_matmul");
+}
+
+long long cri_expert_swiglu_workspace_bytes(const cri_expert_weights* gate, const cri_expert_groups* g) {
+    if (const int st = check_expert_product(gate, g, "cri_expert_swiglu_workspace_bytes")) return st;
+    if (g->n_tokens == 0 || gate->N == 0) return 0;
+    return cri::detail::expert_product_workspace_bytes(matrix_arg(gate), rows_arg(g), true, true);
+}
+
+int cri_expert_swiglu(const cri_expert_weights* gate, const cri_expert_weights* up, const cri_expert_groups* g, const float* x,
+                      int ldx, float* out, int ldo, void* workspace, long long workspace_bytes, hipStream_t s) {
+    const char* fn = "cri_expert_swiglu";
+    if (!up) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null weights");
+    return expert_product(gate, up, g, x, ldx, true, out, ldo, workspace, workspace_bytes, s, fn);
+}
+
+long long cri_expert_combine_workspace_bytes(const cri_expert_weights* w, const cri_expert_groups* g) {
+    if (const int st = check_expert_product(w, g, "cri_expert_combine_workspace_bytes")) return st;
+    if (g->n_tokens == 0 || w->N == 0) return 0;
+    return cri::detail::expert_combine_workspace_bytes(matrix_arg(w), rows_arg(g));
+}
+
+int cri_expert_combine(const cri_expert_weights* w, const cri_expert_groups* g, const float* x, int ldx, const float* weights,
+                       const float* residual, int ldr, float* out, int ldo, void* workspace, long long workspace_bytes,
+                       hipStream_t s) {
+    const char* fn = "cri_expert_combine";
+    int st;
+    if ((st = check_expert_product(w, g, fn))) return st;
+    if (g->n_tokens == 0 || w->N == 0) return CRI_OK;
+    if ((st = check_packed(w, fn)) || (st = check_group_pointers(g, fn))) return st;
+    const long R = pairs(g);
+    if ((st = check_rows(x, ldx, w->K, "x", fn)) || (st = check_rows(out, ldo, w->N, "out", fn))) return st;
+    if (residual && (st = check_rows(residual, ldr, w->N, "residual", fn))) return st;
+    if (!weights) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null weights of the choices");
+    if (!aligned(weights, 4)) return fail(CRI_ERR_ALIGNMENT, fn, "weights must be 4-byte aligned");
+    if (R * std::max({ldx, ldo, residual ? ldr : 0}) > kMaxElems) return fail(CRI_ERR_SHAPE, fn, "problem too large");
+    const long need = cri::detail::expert_combine_workspace_bytes(matrix_arg(w), rows_arg(g));
+    if ((st = check_room(workspace, workspace_bytes, need, 16, fn))) return st;
+    const bool same = residual == out && ldr == ldo;
+    const Span to{out, span_bytes(g->n_tokens, w->N, ldo)}, room{workspace, need};
+    const Span from{residual, residual ? span_bytes(g->n_tokens, w->N, ldr) : 0};
+    for (const Span& written : {to, room})
+        if (meets(written, {{x, span_bytes(R, w->K, ldx)}, {weights, R * 4}, packed_of(w), offsets_of(g), rows_of(g), slots_of(g)}))
+            return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out or the workspace overlaps an input");
+    if (meets(room, {to, from}) || (residual && !same && rows_overlap(residual, w->N, ldr, out, w->N, ldo, g->n_tokens)))
+        return fail(CRI_ERR_INVALID_ARGUMENT, fn, "out, residual and the workspace overlap");
+    clear_pending_error();
+    const int rc = cri::detail::launch_expert_combine(matrix_arg(w), rows_arg(g), x, ldx, weights, residual, ldr, out, ldo, workspace, s);
+    if (rc == cri::detail::kDeclined) return fail(CRI_ERR_UNSUPPORTED, fn, kTooManyTiles);
+    return finish_matmul(rc, fn);
+}
+
 int cri_embedding_rows(int format, const void* table, const int* ids, float* out, int n_ids, int dim, int vocab,
                        hipStream_t s) {
     const char* fn = "cri_embedding_rows";

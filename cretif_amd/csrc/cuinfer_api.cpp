@@ -14,6 +14,7 @@
 #include "../../include/cuinfer/attention.h"
 #include "../../include/cuinfer/dispatch.h"
 #include "../../include/cuinfer/embedding.h"
+#include "../../include/cuinfer/experts.h"
 #include "../../include/cuinfer/hip_utils.h"
 #include "../../include/cuinfer/kernels/elementwise.h"
 #include "../../include/cuinfer/kernels/matmul_quant.h"
@@ -118,6 +119,46 @@ void verify_drafts(const float* target, long long ldt, const float* draft, long 
 }
 long long verify_drafts_workspace_bytes(int n_seqs, int vocab) {
     return checked_bytes(cri_verify_drafts_workspace_bytes(n_seqs, vocab));
+}
+
+// ---------------------------------------------------------------- a layer of experts
+long long expert_packed_bytes(int format, int n_experts, int N, int K) {
+    return checked_bytes(cri_expert_packed_bytes(format, n_experts, N, K));
+}
+void pack_experts(int format, const void* src, int n_experts, int N, int K, void* packed, hipStream_t s) {
+    CUINFER_CHECK_CRI(cri_expert_pack(format, src, n_experts, N, K, packed, s));
+}
+long long group_experts_workspace_bytes(const ExpertGroups& groups) {
+    return checked_bytes(cri_expert_group_workspace_bytes(&groups));
+}
+void route_experts(const ExpertRouter& router, const float* logits, int ldl, int* ids, float* weights,
+                   const ExpertGroups& groups, void* workspace, long long workspace_bytes, hipStream_t s) {
+    CUINFER_CHECK_CRI(cri_expert_route(&router, logits, ldl, ids, weights, &groups, workspace, workspace_bytes, s));
+}
+void group_experts(const int* ids, const ExpertGroups& groups, void* workspace, long long workspace_bytes, hipStream_t s) {
+    CUINFER_CHECK_CRI(cri_expert_group(ids, &groups, workspace, workspace_bytes, s));
+}
+long long expert_matmul_workspace_bytes(const ExpertWeights& w, const ExpertGroups& groups, bool grouped) {
+    return checked_bytes(cri_expert_matmul_workspace_bytes(&w, &groups, grouped));
+}
+void expert_matmul(const ExpertWeights& w, const ExpertGroups& groups, const float* x, int ldx, bool grouped, float* out,
+                   int ldo, void* workspace, long long workspace_bytes, hipStream_t s) {
+    CUINFER_CHECK_CRI(cri_expert_matmul(&w, &groups, x, ldx, grouped, out, ldo, workspace, workspace_bytes, s));
+}
+long long expert_swiglu_workspace_bytes(const ExpertWeights& gate, const ExpertGroups& groups) {
+    return checked_bytes(cri_expert_swiglu_workspace_bytes(&gate, &groups));
+}
+void expert_swiglu(const ExpertWeights& gate, const ExpertWeights& up, const ExpertGroups& groups, const float* x, int ldx,
+                   float* out, int ldo, void* workspace, long long workspace_bytes, hipStream_t s) {
+    CUINFER_CHECK_CRI(cri_expert_swiglu(&gate, &up, &groups, x, ldx, out, ldo, workspace, workspace_bytes, s));
+}
+long long expert_combine_workspace_bytes(const ExpertWeights& w, const ExpertGroups& groups) {
+    return checked_bytes(cri_expert_combine_workspace_bytes(&w, &groups));
+}
+void expert_combine(const ExpertWeights& w, const ExpertGroups& groups, const float* x, int ldx, const float* weights,
+                    const float* residual, int ldr, float* out, int ldo, void* workspace, long long workspace_bytes,
+                    hipStream_t s) {
+    CUINFER_CHECK_CRI(cri_expert_combine(&w, &groups, x, ldx, weights, residual, ldr, out, ldo, workspace, workspace_bytes, s));
 }
 
 // ---------------------------------------------------------------- dispatch

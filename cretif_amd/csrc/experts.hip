@@ -1,0 +1,254 @@
+// experts.hip -- a layer of experts: the activations as planes for the grouped products, the products' choice of kernel,
+// and the weighted sum of a token's experts.  The products are in experts_gemm.hpp, the routing in experts_route.hip.
+#include <algorithm>
+
+#include "experts.hpp"
+
+namespace cri {
+namespace dev {
+namespace {
+
+typedef _Float16 eh8 __attribute__((ext_vector_type(8)));
+
+// Activations as the products take them: row r is 2^exps[r] (hi + lo), |hi| up to 2^15, hi and lo to the nearest half, per 64
+// k 64 of hi and 64 of lo, zeros from K on; for Q4_K also the sums over 32 k times 2^-6 (32 terms below 2^15 then fit
+// fp16) in the same two parts.  A workgroup per row, read twice (the second time from the caches): K floats in, as many
+// bytes out; 4096 x 2048 takes 16 us.
+struct PlanesArgs {
+    const float* x;
+    long ldx;
+    const int* end;  // rows from *end on are not needed, or null
+    uint8_t* planes;
+    uint8_t* sums;  // null: not needed
+    int* exps;
+    int K, depth;
+};
+
+__global__ __launch_bounds__(256) void planes_kernel(const PlanesArgs a) {
+    __shared__ float most[4];
+    const int r = blockIdx.x, tid = threadIdx.x;
+    if (a.end != nullptr && r >= *a.end) return;
+    const float* x = a.x + r * a.ldx;
+    const int chunks = a.K >> 3, all = a.depth * 32;  // of 8
+    float mx = 0.0f;
+    for (int c = tid; c < chunks; c += 256) {
+        const f32x4 u = ld_f32x4(x + 8 * c), v = ld_f32x4(x + 8 * c + 4);
+        mx = fmaxf(mx, fmaxf(fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))),
+                             fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)))));
+    }
+    mx = wave_max(mx);
+    if ((tid & 63) == 0) most[tid >> 6] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    int ex = 0;
+    if (mx > 0.0f) {
+        frexpf(mx, &ex);
+        ex -= 15;
+    }
+    if (tid == 0) a.exps[r] = ex;
+    uint8_t* plane = a.planes + r * static_cast<long>(a.depth) * 1024;
+    for (int c = tid; c < all; c += 256) {  // (all is a multiple of 32, so lanes of a quad stay together)
+        f32x4 u = f32x4{0, 0, 0, 0}, v = u;
+        if (c < chunks) {
+            u = ld_f32x4(x + 8 * c);
+            v = ld_f32x4(x + 8 * c + 4);
+        }
+        eh8 hi, lo;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float y = ldexpf(i < 4 ? u[i] : v[i - 4], -ex);
+            sum += y;
+            hi[i] = static_cast<_Float16>(y);
+            lo[i] = static_cast<_Float16>(y - static_cast<float>(hi[i]));
+        }
+        uint8_t* to = plane + (c >> 3) * 256 + (c & 7) * 16;
+        *reinterpret_cast<eh8*>(to) = hi;
+        *reinterpret_cast<eh8*>(to + 128) = lo;
+        if (a.sums != nullptr) {
+            sum += dpp<kQuadPerm1032>(sum);
+            sum += dpp<kQuadPerm2301>(sum);
+            if ((c & 3) == 0) {
+                sum *= 0.015625f;
+                _Float16* o = reinterpret_cast<_Float16*>(a.sums + (r * static_cast<long>(a.depth) + (c >> 5)) * 32) + ((c >> 2) & 7);
+                o[0] = static_cast<_Float16>(sum);
+                o[8] = static_cast<_Float16>(sum - static_cast<float>(o[0]));
+            }
+        }
+    }
+}
+
+// out[t] = residual[t] + sum over the token's choices, in their order, of weight * p[slot]; choices without an expert are
+// left out, whatever their weight.  Bound by memory: k + 2 rows per token.
+struct CombineArgs {
+    const float* p;  // [R, ldp], 16-byte aligned rows
+    const float* weights;
+    const int* slots;
+    const float* residual;  // or null
+    float* out;
+    long ldp, ldr, ldo;
+    int N, k, R;
+};
+
+__global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
+    const int t = blockIdx.x, col = (blockIdx.y * 256 + threadIdx.x) * 4;
+    if (col >= a.N) return;
+    const int left = a.N - col;
+    const int* slots = a.slots + static_cast<long>(t) * a.k;
+    const float* weights = a.weights + static_cast<long>(t) * a.k;
+    const float* res = a.residual == nullptr ? nullptr : a.residual + t * a.ldr + col;
+    f32x4 first = f32x4{0, 0, 0, 0}, sum = first;
+    if (res != nullptr) {
+        if (left >= 4) {
+            first = ld_f32x4(res);
+        } else {
+            for (int i = 0; i < left; ++i) first[i] = res[i];
+        }
+    }
+    for (int j0 = 0; j0 < a.k; j0 += 4) {
+        f32x4 v[4];
+        float w[4];
+        bool there[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = min(j0 + i, a.k - 1), slot = slots[j];
+            there[i] = j0 + i < a.k && slot >= 0 && slot < a.R;
+            w[i] = weights[j];
+            v[i] = *reinterpret_cast<const f32x4*>(a.p + (there[i] ? slot : 0) * a.ldp + col);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (there[i]) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sum[c] = __builtin_fmaf(w[i], v[i][c], sum[c]);
+            }
+    }
+    sum += first;
+    float* out = a.out + t * a.ldo + col;
+    if (left >= 4) {
+        *reinterpret_cast<f32x4_a4*>(out) = f32x4_a4{sum.x, sum.y, sum.z, sum.w};
+    } else {
+        for (int i = 0; i < left; ++i) out[i] = sum[i];
+    }
+}
+
+}  // namespace
+}  // namespace dev
+
+namespace detail {
+namespace {
+
+// Which kernel, and how many rows a tile.
+struct Plan {
+    bool few;
+    int bm, waves;
+};
+
+Plan plan_products(const ExpertMatrix& w, const ExpertRows& g, bool swiglu) {
+    const int depth = (w.K + dev::kUnitK - 1) / dev::kUnitK;
+    const long R = static_cast<long>(g.n_tokens) * g.top_k;
+    (void)swiglu;
+    if (g.n_tokens <= 8) return {true, std::min(g.n_tokens, 16), std::min(depth, 8)};
+    const long each = R / w.n_experts;
+    return {false, each <= 12 ? 16 : each <= 40 ? 32 : 64, 0};
+}
+
+long up16(long bytes) { return (bytes + 15) & ~15L; }
+
+// bytes of the planes, sums and exponents of `rows` rows
+struct PlaneBytes {
+    long planes, sums, exps;
+    long all() const { return planes + sums + exps; }
+};
+PlaneBytes plane_bytes(const ExpertMatrix& w, long rows) {
+    const long depth = (w.K + dev::kUnitK - 1) / dev::kUnitK;
+    return {rows * depth * 1024, w.fmt == kFmtQ4_K ? rows * depth * 32 : 0, up16(rows * 4)};
+}
+
+// the product of w (and up: SiLU(x w^T) * (x up^T)) into out, rows in grouped order
+int launch_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertRows& g, const float* x, long ldx, bool gather,
+                    float* out, long ldo, void* ws, hipStream_t stream) {
+    const long R = static_cast<long>(g.n_tokens) * g.top_k;
+    const int depth = (w.K + dev::kUnitK - 1) / dev::kUnitK, tiles = (w.N + dev::kUnitCols - 1) / dev::kUnitCols;
+    const bool swiglu = up != nullptr;
+    const Plan plan = plan_products(w, g, swiglu);
+    dev::ProductArgs a{};
+    a.w[0] = static_cast<const uint8_t*>(w.data);
+    a.w[1] = static_cast<const uint8_t*>(swiglu ? up->data : w.data);
+    a.g = dev::Groups{g.offsets, g.rows, g.slots, w.n_experts, g.top_k, static_cast<int>(R)};
+    a.x = x;
+    a.ldx = ldx;
+    a.out = out;
+    a.ldo = ldo;
+    a.N = w.N;
+    a.K = w.K;
+    a.tiles = tiles;
+    a.depth = depth;
+    a.gather = gather;
+    const int blocks = plan.few ? tiles : swiglu ? (tiles + 3) / 4 : (tiles + 7) / 8;
+    const long groups = (dev::most_tiles(R, w.n_experts, plan.bm) * blocks + 7) / 8 * 8;
+    if (groups >= 1L << 23) return kDeclined;  // up to 512 threads each: a launch's limit
+    if (plan.few) {
+        switch (w.fmt) {
+            case kFmtQ8_0: return dev::expert_few<kFmtQ8_0>(a, swiglu, plan.bm, plan.waves, groups, stream);
+            case kFmtQ4_0: return dev::expert_few<kFmtQ4_0>(a, swiglu, plan.bm, plan.waves, groups, stream);
+            case kFmtQ5_0: return dev::expert_few<kFmtQ5_0>(a, swiglu, plan.bm, plan.waves, groups, stream);
+            case kFmtQ4_K: return dev::expert_few<kFmtQ4_K>(a, swiglu, plan.bm, plan.waves, groups, stream);
+            case kFmtQ6_K: return dev::expert_few<kFmtQ6_K>(a, swiglu, plan.bm, plan.waves, groups, stream);
+            default: return dev::expert_few<kFmtF16>(a, swiglu, plan.bm, plan.waves, groups, stream);
+        }
+    }
+    const long rows = gather ? g.n_tokens : R;
+    const PlaneBytes b = plane_bytes(w, rows);
+    uint8_t* const room = static_cast<uint8_t*>(ws);
+    const dev::PlanesArgs p{x, ldx, gather ? nullptr : g.offsets + w.n_experts, room, b.sums ? room + b.planes : nullptr,
+                            reinterpret_cast<int*>(room + b.planes + b.sums), w.K, depth};
+    hipLaunchKernelGGL(dev::planes_kernel, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, p);
+    a.planes = p.planes;
+    a.sums = p.sums;
+    a.exps = p.exps;
+    switch (w.fmt) {
+        case kFmtQ8_0: dev::expert_rows<kFmtQ8_0>(a, swiglu, plan.bm, groups, stream); break;
+        case kFmtQ4_0: dev::expert_rows<kFmtQ4_0>(a, swiglu, plan.bm, groups, stream); break;
+        case kFmtQ5_0: dev::expert_rows<kFmtQ5_0>(a, swiglu, plan.bm, groups, stream); break;
+        case kFmtQ4_K: dev::expert_rows<kFmtQ4_K>(a, swiglu, plan.bm, groups, stream); break;
+        case kFmtQ6_K: dev::expert_rows<kFmtQ6_K>(a, swiglu, plan.bm, groups, stream); break;
+        default: dev::expert_rows<kFmtF16>(a, swiglu, plan.bm, groups, stream);
+    }
+    return 0;
+}
+
+long product_columns(const ExpertMatrix& w) { return (w.N + 3L) & ~3L; }
+
+}  // namespace
+
+long expert_product_workspace_bytes(const ExpertMatrix& w, const ExpertRows& g, bool swiglu, bool gather) {
+    if (plan_products(w, g, swiglu).few) return 0;
+    return plane_bytes(w, gather ? g.n_tokens : static_cast<long>(g.n_tokens) * g.top_k).all();
+}
+
+int launch_expert_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertRows& g, const float* x, long ldx,
+                           bool gather, float* out, long ldo, void* ws, hipStream_t stream) {
+    return launch_products(w, up, g, x, ldx, gather, out, ldo, ws, stream);
+}
+
+// combine: the products of all rows, then what the products need
+long expert_combine_workspace_bytes(const ExpertMatrix& w, const ExpertRows& g) {
+    return up16(static_cast<long>(g.n_tokens) * g.top_k * product_columns(w) * 4) +
+           expert_product_workspace_bytes(w, g, false, false);
+}
+
+int launch_expert_combine(const ExpertMatrix& w, const ExpertRows& g, const float* h, long ldh, const float* weights,
+                          const float* residual, long ldr, float* out, long ldo, void* ws, hipStream_t stream) {
+    const long R = static_cast<long>(g.n_tokens) * g.top_k, ldp = product_columns(w);
+    float* const p = static_cast<float*>(ws);
+    const int rc = launch_products(w, nullptr, g, h, ldh, false, p, ldp, reinterpret_cast<uint8_t*>(p) + up16(R * ldp * 4), stream);
+    if (rc != 0) return rc;
+    const dev::CombineArgs c{p, weights, g.slots, residual, out, ldp, ldr, ldo, w.N, g.top_k, static_cast<int>(R)};
+    hipLaunchKernelGGL(dev::combine_kernel, dim3(static_cast<unsigned>(g.n_tokens), static_cast<unsigned>((w.N + 1023) / 1024)),
+                       dim3(256), 0, stream, c);
+    return 0;
+}
+
+}  // namespace detail
+}  // namespace cri

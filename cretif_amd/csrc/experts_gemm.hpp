@@ -1,0 +1,456 @@
+// experts_gemm.hpp -- products grouped by expert with ragged numbers of rows, on the matrix cores:
+//   C[r, :] = x[r] W[e]^T  or  C[r, :] = silu(x[r] G[e]^T) * (x[r] U[e]^T),  r in [offsets[e], offsets[e + 1]).
+//
+// The mathematics.  fp32 rows are taken as 2^e (hi + lo), two fp16 parts under a power of two per row (hi the nearest half,
+// lo the nearest half of the rest: 22 bits), weights as the exact integers of experts_formats.hpp, so the products are exact
+// in the fp32 accumulators and a result is as good as an fp32 product's.  Two MFMAs per operand pair instead of one, against
+// 16 times slower fp32 MFMAs.
+//
+// Two kernels, one file per weight format.
+//
+// rows_kernel: a workgroup of four waves takes MT * 32 rows of an expert (16 with PAIR) and, per wave, two tiles of 32
+// columns: two column tiles of W, or the same tile of G and U (SiLU * up is then arithmetic on a lane's own registers).
+//   * Rows come from the planes that planes_kernel leaves in the workspace (per 64 k: 64 hi, 64 lo), gathered by their
+//     token as they are copied to LDS (global_load_lds, one stage of 64 k ahead, one barrier a stage).  Chunk c of 16
+//     bytes of row r lies in slot c ^ (r & 15): the reads of 32 rows' operands meet no bank twice.
+//   * Weights go from memory to the registers of the one wave that multiplies them, a stage ahead, and are decoded there:
+//     nothing of a weight is shared between waves, so LDS would only cost.
+//   * Each decoded operand meets MT * 2 MFMAs and each operand read from LDS two.
+//   * PAIR (at most 16 rows): lane rows 0 .. 15 hold hi, 16 .. 31 lo of the same rows; one MFMA does both parts, and the
+//     two halves of the output are added at the end.
+// few_kernel: for calls of few tokens, where what counts is how many waves read weights at once: a workgroup takes up to 16
+// rows of an expert and one tile of 32 columns, its waves the units along k, each converting the activations of its own
+// units to an LDS area of its own (a power of two per row and unit), no barrier before the sum over the waves.
+#pragma once
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "act.hpp"
+#include "experts_formats.hpp"
+
+namespace cri {
+namespace dev {
+
+typedef _Float16 eh8 __attribute__((ext_vector_type(8)));
+typedef float ef16 __attribute__((ext_vector_type(16)));
+
+// first (most significant) operand A: 32 rows, B: 32 columns
+__device__ __forceinline__ ef16 e_mfma(eh8 a, const uint32_t (&b)[4], const ef16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, __builtin_bit_cast(eh8, u32x4{b[0], b[1], b[2], b[3]}), c, 0, 0, 0);
+}
+// 16 bytes per lane from global memory to LDS (lane l at byte 16 l of the wave-uniform lds; below 64 KB).  Not the builtin:
+// behind one of those the compiler has every read of LDS wait for the copy, whatever buffer it goes to.  Here the barrier of
+// a stage waits; the s_nop is the wait state after writing M0.
+__device__ __forceinline__ void e_dma16(const uint8_t* g, char* lds) {
+    typedef __attribute__((address_space(3))) char* Lds;
+    const uint32_t at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((Lds)lds)));
+    uint32_t m0;  // kept as the compiler has it
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "v"(g), "s"(at)
+                 : "memory");
+}
+
+// output row of register i for lanes below 32 (4 more above)
+__device__ __forceinline__ constexpr int e_row(int i) { return (i & 3) + 8 * (i >> 2); }
+
+// the source row of grouped row r
+__device__ __forceinline__ long source_row(const ProductArgs& a, int r) {
+    return a.gather ? clamp_int(a.g.rows[r], 0, a.g.R - 1) / a.g.k : r;
+}
+
+template <int I>
+using Int = std::integral_constant<int, I>;
+
+// One stage (64 k) of NT column tiles against MT row tiles of PARTS parts; a(step, part, mt) is an activation operand.
+// acc: kPerBlock and kNoScale the results, kPerUnit the unit's sum of integers.
+template <class F, int J, int NT, int MT, int PARTS, class A>
+__device__ __forceinline__ void multiply_stage(const typename F::Quant (&q)[NT], const typename F::Scale (&s)[NT],
+                                               ef16 (&acc)[NT][MT], A&& a) {
+    if constexpr (F::kScaled == kPerBlock) {
+        constexpr int B = F::kBlockSteps;
+        auto block = [&](auto blk) {
+            constexpr int I = decltype(blk)::value;  // of the stage
+            eh8 x[B][PARTS][MT];
+#pragma unroll
+            for (int i = 0; i < B; ++i)
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) x[i][p][m] = a(I * B + i, p, m);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                uint32_t b[B][4];
+                F::template operand<J, I * B>(q[n], s[n], b[0]);
+                if constexpr (B > 1) F::template operand<J, I * B + B - 1>(q[n], s[n], b[B - 1]);
+                const float d = F::template block_scale<J*(4 / B) + I>(s[n]);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    ef16 t = e_mfma(x[0][0][m], b[0], ef16{});
+                    if constexpr (PARTS > 1) t = e_mfma(x[0][1][m], b[0], t);
+                    if constexpr (B > 1) t = e_mfma(x[B - 1][0][m], b[B - 1], t);
+                    if constexpr (B > 1 && PARTS > 1) t = e_mfma(x[B - 1][1][m], b[B - 1], t);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[n][m][i] = __builtin_fmaf(d, t[i], acc[n][m][i]);
+                    asm volatile("" : "+v"(acc[n][m]));  // here, not where acc is used next: t would live until then
+                }
+            }
+        };
+        block(Int<0>{});
+        block(Int<1>{});
+        if constexpr (B == 1) {
+            block(Int<2>{});
+            block(Int<3>{});
+        }
+    } else {
+        auto step = [&](auto st) {
+            constexpr int S = decltype(st)::value;
+            eh8 x[PARTS][MT];
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) x[p][m] = a(S, p, m);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                uint32_t b[4];
+                F::template operand<J, S>(q[n], s[n], b);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) acc[n][m] = e_mfma(x[p][m], b, acc[n][m]);
+            }
+        };
+        step(Int<0>{});
+        step(Int<1>{});
+        step(Int<2>{});
+        step(Int<3>{});
+    }
+}
+
+// acc += d P - 64 dmin (minimums . sums), and P starts again; sums(mt) the operand of the rows' sums (Q4_K)
+template <int NT, int MT, class X>
+__device__ __forceinline__ void finish_unit(const typename ExpertFmt<kFmtQ4_K>::Scale (&s)[NT], ef16 (&P)[NT][MT],
+                                            ef16 (&acc)[NT][MT], X&& sums) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        uint32_t b[4];
+        ExpertFmt<kFmtQ4_K>::min_operand(s[n], b);
+        const float d = h_lo(s[n].d), dmin = -64.0f * h_hi(s[n].d);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const ef16 t = e_mfma(sums(m), b, ef16{});
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[n][m][i] = __builtin_fmaf(d, P[n][m][i], __builtin_fmaf(dmin, t[i], acc[n][m][i]));
+            P[n][m] = ef16{};
+        }
+    }
+}
+
+// this wave's loads and copies have arrived, what it read from LDS too, and every wave is here
+__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int FMT, int MT, bool PAIR, bool SWIGLU>
+__global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
+    typedef ExpertFmt<FMT> F;
+    constexpr int BM = PAIR ? 16 : 32 * MT, NT = 2, PARTS = PAIR ? 1 : 2;
+    constexpr int kStage = BM * 256, kCopies = BM / 16;  // bytes of a stage; copies of a wave for it
+    constexpr int kUnit = unit_bytes(FMT);
+    static_assert(!PAIR || MT == 1, "a pair is one tile");
+    __shared__ __attribute__((aligned(16))) char ring[2 * kStage];
+    __shared__ int exps[BM];
+
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int blocks = SWIGLU ? (a.tiles + 3) >> 2 : (a.tiles + 7) >> 3;
+    Tile t;
+    if (!find_tile(a.g, BM, blocks, blockIdx.x, t)) return;
+    if (threadIdx.x < BM) exps[threadIdx.x] = a.exps[source_row(a, t.first + min(static_cast<int>(threadIdx.x), t.count - 1))];
+
+    // this wave's column tiles; one past the last is computed again as the last and not stored
+    int tile[NT];
+    const uint8_t* unit[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        tile[n] = SWIGLU ? t.block * 4 + wave : t.block * 8 + wave * 2 + n;
+        unit[n] = a.w[SWIGLU ? n : 0] +
+                  (static_cast<long>(t.expert) * a.tiles + min(tile[n], a.tiles - 1)) * a.depth * static_cast<long>(kUnit);
+    }
+    const int stages = a.depth * 4;
+    // copies: lane l takes slot l & 15 of row l >> 4 of the four rows of a copy
+    const uint8_t* from[kCopies];
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+        const int r = wave * (BM / 4) + 4 * i + (lane >> 4);
+        from[i] = a.planes + source_row(a, t.first + min(r, t.count - 1)) * a.depth * 1024L + 16 * ((lane & 15) ^ (r & 15));
+    }
+    auto copy = [&](int stage) {  // (past the end: the last stage again, unused)
+        char* to = ring + (stage & 1) * kStage + wave * (BM / 4) * 256;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) e_dma16(from[i] + 256L * min(stage, stages - 1), to + 1024 * i);
+    };
+    // operands: lane row, and the slot of its chunk 2 step + h (hi) or 8 more (lo)
+    const int row = PAIR ? lane & 15 : lane & 31, part = PAIR ? 8 * ((lane >> 4) & 1) : 0;
+    const int rowx = row & 15;
+    auto reader = [&](int stage) {
+        const char* at = ring + (stage & 1) * kStage + row * 256;
+        return [=](int s, int p, int m) {
+            return *reinterpret_cast<const eh8*>(at + m * 32 * 256 + 16 * ((2 * s + h + part + 8 * p) ^ rowx));
+        };
+    };
+    const uint8_t* sums[MT];
+    if constexpr (FMT == kFmtQ4_K) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+            sums[m] = a.sums + source_row(a, t.first + min(32 * m + row, t.count - 1)) * a.depth * 32L + 16 * h;
+    }
+
+    ef16 acc[NT][MT] = {}, P[FMT == kFmtQ4_K ? NT : 1][FMT == kFmtQ4_K ? MT : 1] = {};
+    typename F::Quant q[2][NT];
+    typename F::Scale sc[2][NT];
+    auto load_quants = [&](typename F::Quant(&d)[NT], int stage) {
+        const int st = min(stage, stages - 1);  // (past the end: the last again, unused)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) F::load(d[n], unit[n] + (st >> 2) * static_cast<long>(kUnit), st & 3, lane);
+    };
+    auto load_scales = [&](typename F::Scale(&d)[NT], int u) {
+        const int at = min(u, a.depth - 1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) F::load(d[n], unit[n] + at * static_cast<long>(kUnit), lane);
+    };
+    load_quants(q[0], 0);
+    load_scales(sc[0], 0);
+    copy(0);
+
+    eh8 x[MT];  // the unit's sums
+    auto run = [&](auto pos, int u, const typename F::Scale(&s)[NT], typename F::Scale(&next)[NT]) {
+        constexpr int J = decltype(pos)::value;
+        const int stage = 4 * u + J;
+        stage_barrier();  // this stage is in LDS and in registers, and the other buffer free
+#pragma unroll
+        for (int n = 0; n < NT; ++n) q[J & 1][n].settle();  // the compiler's wait, before it would count the next loads
+        load_quants(q[(J + 1) & 1], stage + 1);
+        if constexpr (J == 0) load_scales(next, u + 1);
+        if constexpr (J == 2 && FMT == kFmtQ4_K) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) x[m] = *reinterpret_cast<const eh8*>(sums[m] + 32 * u);
+        }
+        copy(stage + 1);
+        if constexpr (FMT == kFmtQ4_K) multiply_stage<F, J, NT, MT, PARTS>(q[J & 1], s, P, reader(stage));
+        else multiply_stage<F, J, NT, MT, PARTS>(q[J & 1], s, acc, reader(stage));
+    };
+    auto unit_of = [&](int u, const typename F::Scale(&s)[NT], typename F::Scale(&next)[NT]) {
+        run(Int<0>{}, u, s, next);
+        run(Int<1>{}, u, s, next);
+        run(Int<2>{}, u, s, next);
+        run(Int<3>{}, u, s, next);
+        if constexpr (FMT == kFmtQ4_K) {
+            if (PAIR && part) x[0] = eh8{};  // both parts of the sums go with the rows of hi
+            finish_unit<NT, MT>(s, P, acc, [&](int m) { return x[m]; });
+        }
+    };
+    for (int u = 0; u < a.depth; u += 2) {
+        unit_of(u, sc[0], sc[1]);
+        if (u + 1 < a.depth) unit_of(u + 1, sc[1], sc[0]);
+    }
+
+    // nothing may arrive in LDS that is another workgroup's by then; exps was written before the first barrier
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int i = 0; i < (PAIR ? 8 : 16); ++i) {
+            const int r = 32 * m + e_row(i) + 4 * h;
+            if (r >= t.count) continue;
+            const int e = exps[r];
+            float* o = a.out + static_cast<long>(t.first + r) * a.ldo;
+            float v[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) v[n] = ldexpf(PAIR ? acc[n][m][i] + acc[n][m][i + 8] : acc[n][m][i], e);
+#pragma unroll
+            for (int n = 0; n < (SWIGLU ? 1 : NT); ++n) {
+                const int col = tile[n] * kUnitCols + (lane & 31);
+                if (col < a.N) o[col] = SWIGLU ? silu_f(v[0]) * v[1] : v[n];
+            }
+        }
+    }
+}
+
+// ---- few tokens ---------------------------------------------------------------
+
+constexpr int kFewWaves = 8;
+// LDS of a wave: rows of 1024 bytes (a unit's hi and lo, in the ring's order), 32 of sums and 4 of unscale
+__device__ __host__ inline int few_wave_bytes(int bm) { return bm * (1024 + 32) + 64; }
+
+// Eight activations of a row's unit (lane group of 32: one row) to their chunk of hi and lo, the row's sums over 32 and
+// its unscale; the whole wave calls it.
+__device__ __forceinline__ void few_convert(const f32x4& x, const f32x4& y, bool live, int r, char* area, char* sums, float* us) {
+    float mx = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
+                     fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+    mx = fmaxf(mx, dpp<kQuadPerm1032>(mx));
+    mx = fmaxf(mx, dpp<kQuadPerm2301>(mx));
+    mx = fmaxf(mx, dpp<kRowHalfMirror>(mx));
+    mx = fmaxf(mx, dpp<kRowMirror>(mx));
+    mx = fmaxf(mx, swizzle_xor16(mx));
+    int ex = 0;
+    if (mx > 0.0f) {
+        frexpf(mx, &ex);
+        ex -= 15;  // the largest just below 2^15
+    }
+    const int c = threadIdx.x & 31;  // chunk of the unit: 64-wide group c >> 3, chunk c & 7 of it
+    eh8 hi, lo;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = ldexpf(i < 4 ? x[i] : y[i - 4], -ex);
+        sum += v;
+        hi[i] = static_cast<_Float16>(v);
+        lo[i] = static_cast<_Float16>(v - static_cast<float>(hi[i]));
+    }
+    sum += dpp<kQuadPerm1032>(sum);
+    sum += dpp<kQuadPerm2301>(sum);
+    if (!live) return;
+    char* at = area + r * 1024 + 256 * (c >> 3);
+    *reinterpret_cast<eh8*>(at + 16 * ((c & 7) ^ (r & 15))) = hi;
+    *reinterpret_cast<eh8*>(at + 16 * (((c & 7) + 8) ^ (r & 15))) = lo;
+    if ((c & 3) == 0) {
+        sum *= 0.015625f;
+        const _Float16 s = static_cast<_Float16>(sum);
+        _Float16* o = reinterpret_cast<_Float16*>(sums + r * 32) + (c >> 2);
+        o[0] = s;
+        o[8] = static_cast<_Float16>(sum - static_cast<float>(s));
+    }
+    if (c == 0) us[r] = ldexpf(1.0f, ex);
+}
+
+// Workgroup of `waves` waves; wave w takes units w, w + waves, ...; bm rows a tile (1 .. 16).
+template <int FMT, bool SWIGLU>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const ProductArgs a, int bm, int waves) {
+    typedef ExpertFmt<FMT> F;
+    constexpr int NT = SWIGLU ? 2 : 1, kUnit = unit_bytes(FMT);
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Tile t;
+    if (!find_tile(a.g, bm, a.tiles, blockIdx.x, t)) return;
+    char* const area = lds + wave * few_wave_bytes(bm);
+    char* const sums = area + bm * 1024;
+    float* const us = reinterpret_cast<float*>(sums + bm * 32);
+    const uint8_t* base[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) base[n] = a.w[n] + (static_cast<long>(t.expert) * a.tiles + t.block) * a.depth * static_cast<long>(kUnit);
+
+    const int lrow = lane & 15, part = 8 * ((lane >> 4) & 1);
+    const int row = min(lrow, t.count - 1), rowx = row & 15;
+    ef16 acc[NT][1] = {};
+    for (int u = wave; u < a.depth; u += waves) {
+        typename F::Quant q[4][NT];
+        typename F::Scale sc[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint8_t* unit = base[n] + u * static_cast<long>(kUnit);
+            F::load(sc[n], unit, lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) F::load(q[j][n], unit, j, lane);
+        }
+        // a row for each half of the wave, eight activations a lane; values from K on are zero
+        const int k = u * kUnitK + 8 * (lane & 31);
+        for (int r0 = 0; r0 < t.count; r0 += 2) {
+            const int r = r0 + h;
+            const bool live = r < t.count;
+            f32x4 x = f32x4{0, 0, 0, 0}, y = x;
+            if (live && k < a.K) {
+                const float* p = a.x + source_row(a, t.first + r) * a.ldx + k;
+                x = ld_f32x4(p);
+                y = ld_f32x4(p + 4);
+            }
+            few_convert(x, y, live, r, area, sums, us);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        ef16 p[NT][1] = {};
+        auto reader = [&](int j) {
+            const char* at = area + row * 1024 + 256 * j;
+            return [=](int s, int, int) { return *reinterpret_cast<const eh8*>(at + 16 * ((2 * s + h + part) ^ rowx)); };
+        };
+        multiply_stage<F, 0, NT, 1, 1>(q[0], sc, p, reader(0));
+        multiply_stage<F, 1, NT, 1, 1>(q[1], sc, p, reader(1));
+        multiply_stage<F, 2, NT, 1, 1>(q[2], sc, p, reader(2));
+        multiply_stage<F, 3, NT, 1, 1>(q[3], sc, p, reader(3));
+        if constexpr (FMT == kFmtQ4_K) {
+            eh8 x = *reinterpret_cast<const eh8*>(sums + row * 32 + 16 * h);
+            if (part) x = eh8{};
+            ef16 r[NT][1] = {};
+            finish_unit<NT, 1>(sc, p, r, [&](int) { return x; });
+#pragma unroll
+            for (int n = 0; n < NT; ++n) p[n][0] = r[n][0];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = us[min(e_row(i) + 4 * h, t.count - 1)];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][0][i] = __builtin_fmaf(f, p[n][0][i] + p[n][0][i + 8], acc[n][0][i]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    // the waves' sums, in their order
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) red[((wave * NT + n) * 16 + e_row(i) + 4 * h) * 32 + (lane & 31)] = acc[n][0][i];
+    __syncthreads();
+    const int some = min(waves, a.depth);
+    for (int o = threadIdx.x; o < t.count * 32; o += 64 * waves) {
+        float v[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            v[n] = red[n * 512 + o];
+            for (int w = 1; w < some; ++w) v[n] += red[(w * NT + n) * 512 + o];
+        }
+        const int col = t.block * kUnitCols + (o & 31);
+        if (col < a.N) a.out[static_cast<long>(t.first + (o >> 5)) * a.ldo + col] = SWIGLU ? silu_f(v[0]) * v[NT - 1] : v[0];
+    }
+}
+
+template <int FMT>
+void expert_rows(const ProductArgs& a, bool swiglu, int bm, long workgroups, hipStream_t stream) {
+    const auto run = swiglu ? (bm == 16   ? rows_kernel<FMT, 1, true, true>
+                               : bm == 32 ? rows_kernel<FMT, 1, false, true>
+                                          : rows_kernel<FMT, 2, false, true>)
+                            : (bm == 16   ? rows_kernel<FMT, 1, true, false>
+                               : bm == 32 ? rows_kernel<FMT, 1, false, false>
+                                          : rows_kernel<FMT, 2, false, false>);
+    hipLaunchKernelGGL(run, dim3(static_cast<unsigned>(workgroups)), dim3(256), 0, stream, a);
+}
+
+template <int FMT, bool SWIGLU>
+int launch_few(const ProductArgs& a, int bm, int waves, long workgroups, hipStream_t stream) {
+    const int lds = std::max(waves * few_wave_bytes(bm), waves * (SWIGLU ? 2 : 1) * 2048);
+    if (lds > 65536) {  // past the default limit, raised once per kernel and device
+        constexpr int kMaxDevices = 64;
+        static std::atomic<bool> ready[kMaxDevices];
+        int device = 0;
+        if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= kMaxDevices) return detail::kFailed;
+        if (!ready[device].load(std::memory_order_acquire)) {
+            if (hipFuncSetAttribute(reinterpret_cast<const void*>(&few_kernel<FMT, SWIGLU>),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
+                return detail::kFailed;
+            ready[device].store(true, std::memory_order_release);
+        }
+    }
+    hipLaunchKernelGGL((few_kernel<FMT, SWIGLU>), dim3(static_cast<unsigned>(workgroups)), dim3(64 * waves), lds, stream, a, bm,
+                       waves);
+    return 0;
+}
+template <int FMT>
+int expert_few(const ProductArgs& a, bool swiglu, int bm, int waves, long workgroups, hipStream_t stream) {
+    return swiglu ? launch_few<FMT, true>(a, bm, waves, workgroups, stream)
+                  : launch_few<FMT, false>(a, bm, waves, workgroups, stream);
+}
+
+}  // namespace dev
+}  // namespace cri

@@ -1,0 +1,11 @@
+// experts_q8_0.hip -- the grouped products of experts_gemm.hpp for Q8_0 weights.
+#include "experts_gemm.hpp"
+
+namespace cri {
+namespace dev {
+
+template void expert_rows<kFmtQ8_0>(const ProductArgs&, bool, int, long, hipStream_t);
+template int expert_few<kFmtQ8_0>(const ProductArgs&, bool, int, int, long, hipStream_t);
+
+}  // namespace dev
+}  // namespace cri

@@ -116,6 +116,23 @@ struct HeadRotation {
     double log2_step;  // -2 log2(theta) / rot_dim: pair i turns by 2^(i log2_step) radians per position
 };
 
+// ---- a layer of experts, as the launchers take it (experts.hpp) ----
+struct ExpertMatrix {  // laid out by launch_expert_pack
+    const void* data;
+    int fmt, n_experts, N, K;
+};
+struct ExpertRows {
+    int* offsets;  // [n_experts + 1]: grouped rows of expert e are offsets[e] .. offsets[e + 1] - 1
+    int* rows;     // [n_tokens * top_k]: the pair token * top_k + choice of a grouped row, -1 behind the last
+    int* slots;    // [n_tokens * top_k]: a pair's grouped row, -1 without an expert
+    int n_tokens, top_k;
+};
+struct ExpertRouter {
+    const float* bias;  // [n_experts] or null
+    float scale;
+    bool sigmoid, normalize;
+};
+
 namespace detail {
 
 // Launcher status: 0 = enqueued; kDeclined = this kernel does not take the shape
@@ -355,6 +372,25 @@ long verify_workspace_bytes(int n_seqs, int vocab);
 int launch_verify_drafts(const float* target, long ldt, const float* draft, long ldd, const int* ids, const float* u,
                          const float* draws, const int* offsets, int n_seqs, int n_rows, int vocab, int* out, int* accepted, double* ws,
                          hipStream_t stream);
+
+// GGUF blocks [n_experts, N, K] laid out for the products below (experts_pack.hip): 32 columns x 256 k at a time
+long expert_units(int n_experts, int N, int K);
+long expert_packed_bytes(int fmt, int n_experts, int N, int K);
+int launch_expert_pack(int fmt, const void* src, int n_experts, int N, int K, void* dst, hipStream_t stream);
+// the router's logits to ids, weights and groups, or ids alone to groups (experts_route.hip); ws: 4-byte aligned,
+// expert_group_workspace_bytes of it, written before it is read
+long expert_group_workspace_bytes(int n_tokens, int top_k, int n_experts);
+int launch_expert_route(const ExpertRouter& r, const float* logits, long ldl, int n_experts, int* ids, float* weights,
+                        const ExpertRows& g, int* ws, hipStream_t stream);
+int launch_expert_group(const int* ids, int n_experts, const ExpertRows& g, int* ws, hipStream_t stream);
+// products of the grouped rows (experts.hip): x w^T, or silu(x w^T) * (x up^T) with up; x has a row per token (gather) or
+// per grouped row.  ws: 16-byte aligned, written before it is read
+long expert_product_workspace_bytes(const ExpertMatrix& w, const ExpertRows& g, bool swiglu, bool gather);
+int launch_expert_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertRows& g, const float* x, long ldx,
+                           bool gather, float* out, long ldo, void* ws, hipStream_t stream);
+long expert_combine_workspace_bytes(const ExpertMatrix& w, const ExpertRows& g);
+int launch_expert_combine(const ExpertMatrix& w, const ExpertRows& g, const float* h, long ldh, const float* weights,
+                          const float* residual, long ldr, float* out, long ldo, void* ws, hipStream_t stream);
 
 // rows per launch_prefill_attention call of the C ABI and the decode step (the scores workspace
 // holds n_heads x this many rows x the cache length)

@@ -463,6 +463,80 @@ int cri_verify_drafts(const float* target, long long ldt, const float* draft, lo
                       hipStream_t stream);
 long long cri_verify_drafts_workspace_bytes(int n_seqs, int vocab);
 
+/* ---- a layer of experts ------------------------------------------------------
+ * No counterpart in the reference, whose models have one FFN.  The FFN of such a layer is: the router's product (cri_matmul or
+ * cri_matmul_transposed_b: [E, dim] weights), cri_expert_route, cri_expert_swiglu, cri_expert_combine; cri_expert_matmul is for
+ * other activations.  Which rows meet which expert stays on the device: nothing synchronises, host numbers alone decide launches
+ * and workspaces, and a call may be captured in a HIP graph and replayed with other logits.  Results have the same bits at every
+ * call with the same sizes and contents.  Calls that share a workspace must be ordered on one stream.
+ *
+ * A matrix per expert, [n_experts, N, K] in GGUF blocks (ffn_gate_exps and the like), laid out once by cri_expert_pack: data
+ * is 16-byte aligned, cri_expert_packed_bytes long.  K a multiple of 32 (Q4_K, Q6_K: 256), at least one block; up to 1024
+ * experts. */
+typedef struct cri_expert_weights {
+    const void* data;
+    int format; /* cri_format */
+    int n_experts, N, K;
+} cri_expert_weights;
+long long cri_expert_packed_bytes(int format, int n_experts, int N, int K);
+/* packed = the blocks at src (raw GGUF bytes, any alignment) in the products' order: the same bits, padded to 32 rows and 256
+ * values (Q4_K 3% larger for its unpacked 6-bit scales).  src is not needed afterwards.  No overlap. */
+int cri_expert_pack(int format, const void* src, int n_experts, int N, int K, void* packed, hipStream_t stream);
+/* The pairs (token t, choice j), pair t * top_k + j, grouped by expert: the grouped rows of expert e are offsets[e] ..
+ * offsets[e + 1] - 1, in the order of their pairs; rows[r] is the pair of grouped row r (-1 from offsets[n_experts] on),
+ * slots[p] the grouped row of pair p (-1: it has no expert).  Written by cri_expert_route or cri_expert_group, read by the
+ * products, which take entries that do not fit (no sorted offsets, a pair or row out of range) without reading or writing out
+ * of bounds, the results being unspecified then.  top_k 1 .. 64 and at most n_experts, n_tokens * top_k at most 2^23. */
+typedef struct cri_expert_groups {
+    int* offsets; /* device [n_experts + 1] */
+    int* rows;    /* device [n_tokens * top_k] */
+    int* slots;   /* device [n_tokens * top_k] */
+    int n_tokens, top_k, n_experts;
+} cri_expert_groups;
+typedef enum cri_expert_scoring { CRI_SCORE_SOFTMAX = 0, CRI_SCORE_SIGMOID = 1 } cri_expert_scoring;
+typedef struct cri_expert_router {
+    const float* bias; /* device [n_experts], added to the scores for the choice alone; or null */
+    float scale;       /* of the weights */
+    int scoring;       /* cri_expert_scoring */
+    int normalize;     /* weights divided by their token's sum */
+} cri_expert_router;
+/* logits [n_tokens, n_experts], rows ldl floats apart -> ids and weights [n_tokens, top_k] and the groups.  A token's scores are
+ * the softmax or the sigmoid of its logits; its top_k experts are those of the largest score plus bias (without a bias: of the
+ * largest logit), in that order, the lowest number first where they are equal; their weights are the scores (without the
+ * bias), divided by their sum with normalize, times scale.  An expert whose logit is -infinity or NaN (or whose bias makes its sum
+ * so) is never chosen: a token left with fewer experts than top_k has id -1 and weight 0 in the choices behind, so a row of
+ * -infinity (a padded batch's) causes no work.  Scores and their order are computed in 64 bits.  workspace: 4-byte aligned,
+ * cri_expert_group_workspace_bytes. */
+int cri_expert_route(const cri_expert_router* router, const float* logits, int ldl, int* ids, float* weights,
+                     const cri_expert_groups* groups, void* workspace, long long workspace_bytes, hipStream_t stream);
+/* the groups of given ids [n_tokens, top_k]; ids outside [0, n_experts) are pairs without an expert (another GPU's, say), and a
+ * token may name an expert twice */
+int cri_expert_group(const int* ids, const cri_expert_groups* groups, void* workspace, long long workspace_bytes,
+                     hipStream_t stream);
+long long cri_expert_group_workspace_bytes(const cri_expert_groups* groups);
+/* out[r, :] = x[row(r), :] W[e]^T for the grouped rows r of every expert e; row(r) is rows[r] / top_k (x: [n_tokens, K], a row
+ * per token) or, with grouped, r (x: [n_tokens * top_k, K] in grouped order).  out [n_tokens * top_k, N]; its rows from
+ * offsets[n_experts] on stay as they were.  Rows ldx and ldo floats apart, 4-byte aligned.  fp32 results: weights are exact,
+ * activations have 22 bits of their row's (256 values' of their row's) largest magnitude; a row that is not finite makes its
+ * own results not finite.  out and the workspace (16-byte aligned) overlap no other buffer. */
+int cri_expert_matmul(const cri_expert_weights* w, const cri_expert_groups* groups, const float* x, int ldx, int grouped,
+                      float* out, int ldo, void* workspace, long long workspace_bytes, hipStream_t stream);
+long long cri_expert_matmul_workspace_bytes(const cri_expert_weights* w, const cri_expert_groups* groups, int grouped);
+/* out[r, :] = silu(x[row(r), :] gate[e]^T) * (x[row(r), :] up[e]^T), a row of x per token; gate and up have the same format and
+ * sizes.  Else as cri_expert_matmul. */
+int cri_expert_swiglu(const cri_expert_weights* gate, const cri_expert_weights* up, const cri_expert_groups* groups,
+                      const float* x, int ldx, float* out, int ldo, void* workspace, long long workspace_bytes,
+                      hipStream_t stream);
+long long cri_expert_swiglu_workspace_bytes(const cri_expert_weights* gate, const cri_expert_groups* groups);
+/* out[t, :] = residual[t, :] + sum_j weights[t, j] (x[slots[t top_k + j], :] W[e]^T), x [n_tokens * top_k, K] in grouped order (what
+ * cri_expert_swiglu leaves), weights [n_tokens, top_k]; choices without an expert are left out.  residual (rows ldr apart) may be
+ * null, or out itself with ldr == ldo; no other overlap of out or the workspace (16-byte aligned).  out [n_tokens, N] is written
+ * whole. */
+int cri_expert_combine(const cri_expert_weights* w, const cri_expert_groups* groups, const float* x, int ldx,
+                       const float* weights, const float* residual, int ldr, float* out, int ldo, void* workspace,
+                       long long workspace_bytes, hipStream_t stream);
+long long cri_expert_combine_workspace_bytes(const cri_expert_weights* w, const cri_expert_groups* groups);
+
 /* ---- diagnostics ---------------------------------------------------------- */
 
 /* Reads n_bytes (a multiple of 16) at src (16-byte aligned) once with 16-byte
