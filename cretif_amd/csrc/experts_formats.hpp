@@ -2,13 +2,14 @@
 // integers in fp16 (FP16: the weights themselves), and the scales that the fp32 partial sums take.
 //
 // ExpertFmt<FMT>: load(q, unit, stage) a lane's bytes of a stage of four steps (64 k), load(s, unit) those of the unit's
-// scales; operand<J, S>(q, s, b) the eight weights of step S of stage J, as four pairs.  kScaled says how scales are
-// applied: kNoScale not at all, kPerBlock the partial sum of kBlockSteps steps times block_scale<I>() (I: the unit's block),
-// kPerUnit (Q4_K) the whole unit's sum times d, less 64 dmin times that of the minimums and the activations' sums over 32
-// (staged times 2^-6): min_operand().
+// scales; operand<J, S>(q, s, b) the eight weights of step S of stage J, as four pairs.  kScaled says how scales are applied:
+// kNoScale not at all; kPerStep and kPerBlock the partial sum of a step (16 k) or of a block of two times part_scale<I>() (I: the
+// unit's step or block); kPerUnit (Q4_K) the whole unit's sum times unit_scale() less 64 dmin times that of the minimums,
+// min_operand(), and the activations' sums over 32, which are staged times 2^-6.
 //
-// Scales of a 32-weight block multiply a partial sum instead of the weights because d q has 19 bits, fp16 11; Q4_K's 6-bit
-// scale times 4-bit code has 10 and goes into the operand.
+// Scales multiply a partial sum instead of the weights because d q has 19 bits, fp16 11; Q4_K's 6-bit scale times 4-bit code
+// has 10 and goes into the operand.  Q6_K's scale times code has 12: as an operand's nearest half and its rest in a third MFMA
+// (no scaling before the unit's end) 4096 tokens' SwiGLU took 856 us, with scaled steps 790: the MFMAs' power counts.
 #pragma once
 
 #include "experts.hpp"
@@ -16,7 +17,7 @@
 namespace cri {
 namespace dev {
 
-enum : int { kNoScale = 0, kPerBlock = 1, kPerUnit = 2 };
+enum : int { kNoScale = 0, kPerStep = 1, kPerBlock = 2, kPerUnit = 3 };
 
 typedef _Float16 eh2 __attribute__((ext_vector_type(2)));
 
@@ -70,7 +71,7 @@ __device__ __forceinline__ uint32_t e_at(const u32x4& v, int i) { return v[i]; }
 
 template <>
 struct ExpertFmt<kFmtQ4_0> {
-    static constexpr int kScaled = kPerBlock, kBlockSteps = 2;
+    static constexpr int kScaled = kPerBlock;
     typedef NibbleQuant Quant;
     struct Scale {
         u32x4 d;
@@ -92,14 +93,14 @@ struct ExpertFmt<kFmtQ4_0> {
         b[3] = e_fma(t[3], kTenth, high);
     }
     template <int I>
-    static __device__ __forceinline__ float block_scale(const Scale& s) {
+    static __device__ __forceinline__ float part_scale(const Scale& s) {
         return e_half(s.d[I >> 1], I & 1);
     }
 };
 
 template <>
 struct ExpertFmt<kFmtQ8_0> {
-    static constexpr int kScaled = kPerBlock, kBlockSteps = 2;
+    static constexpr int kScaled = kPerBlock;
     struct Quant {
         u32x4 q[2];
         __device__ __forceinline__ void settle() { e_settle(q[0]), e_settle(q[1]); }
@@ -124,7 +125,7 @@ struct ExpertFmt<kFmtQ8_0> {
         b[3] = e_add(e_and_or(y >> 8, 0x00FF00FFu, kTop), zero);
     }
     template <int I>
-    static __device__ __forceinline__ float block_scale(const Scale& s) {
+    static __device__ __forceinline__ float part_scale(const Scale& s) {
         return e_half(s.d[I >> 1], I & 1);
     }
 };
@@ -134,7 +135,7 @@ __device__ __forceinline__ uint32_t e_move(uint32_t w, int from, int to) { retur
 
 template <>
 struct ExpertFmt<kFmtQ5_0> {
-    static constexpr int kScaled = kPerBlock, kBlockSteps = 2;
+    static constexpr int kScaled = kPerBlock;
     struct Quant {
         u32x4 q;
         uint32_t h;
@@ -161,14 +162,14 @@ struct ExpertFmt<kFmtQ5_0> {
         b[3] = e_fma(e_and_or(e_move(q.h, 4 * S + 3, 8), 0x01000100u, t[3]), kTenth, high);
     }
     template <int I>
-    static __device__ __forceinline__ float block_scale(const Scale& s) {
+    static __device__ __forceinline__ float part_scale(const Scale& s) {
         return e_half(s.d[I >> 1], I & 1);
     }
 };
 
 template <>
 struct ExpertFmt<kFmtQ6_K> {
-    static constexpr int kScaled = kPerBlock, kBlockSteps = 1;
+    static constexpr int kScaled = kPerStep;
     struct Quant {
         u32x4 q;
         uint32_t h[2];
@@ -202,14 +203,14 @@ struct ExpertFmt<kFmtQ6_K> {
         b[3] = e_fma(e_and_or(e_move(h, o + 6, 8), 0x03000300u, t[3]), kTenth, high);
     }
     template <int I>
-    static __device__ __forceinline__ float block_scale(const Scale& s) {
+    static __device__ __forceinline__ float part_scale(const Scale& s) {
         return h_lo(s.d) * sbyte(s.sc[I >> 2], I & 3);  // 19 bits: exact
     }
 };
 
 template <>
 struct ExpertFmt<kFmtQ4_K> {
-    static constexpr int kScaled = kPerUnit, kBlockSteps = 16;
+    static constexpr int kScaled = kPerUnit;
     typedef NibbleQuant Quant;
     struct Scale {
         u32x4 s;  // sc, mn
@@ -239,6 +240,7 @@ struct ExpertFmt<kFmtQ4_K> {
         b[2] = e_fma(t[2], sc, off);
         b[3] = e_fma(t[3], sc16, off16);
     }
+    static __device__ __forceinline__ float unit_scale(const Scale& s) { return h_lo(s.d); }
     static __device__ __forceinline__ void min_operand(const Scale& s, uint32_t (&b)[4]) {
         const uint32_t z = e_splat(-1024.0f);
         b[0] = e_add(__builtin_amdgcn_perm(kTop, s.s.z, 0x05010500u), z);
@@ -250,7 +252,7 @@ struct ExpertFmt<kFmtQ4_K> {
 
 template <>
 struct ExpertFmt<kFmtF16> {
-    static constexpr int kScaled = kNoScale, kBlockSteps = 0;
+    static constexpr int kScaled = kNoScale;
     struct Quant {
         u32x4 q[4];
         __device__ __forceinline__ void settle() { e_settle(q[0]), e_settle(q[1]), e_settle(q[2]), e_settle(q[3]); }

@@ -43,13 +43,11 @@ __device__ __forceinline__ ef16 e_mfma(eh8 a, const uint32_t (&b)[4], const ef16
 // 16 bytes per lane from global memory to LDS (lane l at byte 16 l of the wave-uniform lds; below 64 KB).  Not the builtin:
 // behind one of those the compiler has every read of LDS wait for the copy, whatever buffer it goes to.  Here the barrier of
 // a stage waits; the s_nop is the wait state after writing M0.
-__device__ __forceinline__ void e_dma16(const uint8_t* g, char* lds) {
-    typedef __attribute__((address_space(3))) char* Lds;
-    const uint32_t at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((Lds)lds)));
+__device__ __forceinline__ void e_dma16(const uint8_t* g, uint32_t lds) {
     uint32_t m0;  // kept as the compiler has it
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                  : "=&s"(m0)
-                 : "v"(g), "s"(at)
+                 : "v"(g), "s"(lds)
                  : "memory");
 }
 
@@ -64,80 +62,48 @@ __device__ __forceinline__ long source_row(const ProductArgs& a, int r) {
 template <int I>
 using Int = std::integral_constant<int, I>;
 
-// One stage (64 k) of NT column tiles against MT row tiles of PARTS parts; a(step, part, mt) is an activation operand.
-// acc: kPerBlock and kNoScale the results, kPerUnit the unit's sum of integers.
-template <class F, int J, int NT, int MT, int PARTS, class A>
+// One stage (64 k) of NT column tiles against a tile of paired rows; a(step) is an activation operand.  acc: the results, or with
+// kPerUnit the unit's sum of integers.
+template <class F, int J, int NT, class A>
 __device__ __forceinline__ void multiply_stage(const typename F::Quant (&q)[NT], const typename F::Scale (&s)[NT],
-                                               ef16 (&acc)[NT][MT], A&& a) {
-    if constexpr (F::kScaled == kPerBlock) {
-        constexpr int B = F::kBlockSteps;
-        auto block = [&](auto blk) {
-            constexpr int I = decltype(blk)::value;  // of the stage
-            eh8 x[B][PARTS][MT];
+                                               ef16 (&acc)[NT][1], A&& a) {
+    auto block = [&](auto blk) {
+        constexpr int I = decltype(blk)::value;  // of the stage
+        const eh8 x[2] = {a(2 * I), a(2 * I + 1)};
 #pragma unroll
-            for (int i = 0; i < B; ++i)
+        for (int n = 0; n < NT; ++n) {
+            uint32_t b[2][4];
+            F::template operand<J, 2 * I>(q[n], s[n], b[0]);
+            F::template operand<J, 2 * I + 1>(q[n], s[n], b[1]);
+            auto scale = [&](float d, const ef16& t) {
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) x[i][p][m] = a(I * B + i, p, m);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                uint32_t b[B][4];
-                F::template operand<J, I * B>(q[n], s[n], b[0]);
-                if constexpr (B > 1) F::template operand<J, I * B + B - 1>(q[n], s[n], b[B - 1]);
-                const float d = F::template block_scale<J*(4 / B) + I>(s[n]);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    ef16 t = e_mfma(x[0][0][m], b[0], ef16{});
-                    if constexpr (PARTS > 1) t = e_mfma(x[0][1][m], b[0], t);
-                    if constexpr (B > 1) t = e_mfma(x[B - 1][0][m], b[B - 1], t);
-                    if constexpr (B > 1 && PARTS > 1) t = e_mfma(x[B - 1][1][m], b[B - 1], t);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[n][m][i] = __builtin_fmaf(d, t[i], acc[n][m][i]);
-                    asm volatile("" : "+v"(acc[n][m]));  // here, not where acc is used next: t would live until then
-                }
+                for (int i = 0; i < 16; ++i) acc[n][0][i] = __builtin_fmaf(d, t[i], acc[n][0][i]);
+                asm volatile("" : "+v"(acc[n][0]));  // here, not where acc is used next: t would live until then
+            };
+            if constexpr (F::kScaled == kPerBlock) {
+                scale(F::template part_scale<2 * J + I>(s[n]), e_mfma(x[1], b[1], e_mfma(x[0], b[0], ef16{})));
+            } else if constexpr (F::kScaled == kPerStep) {
+                scale(F::template part_scale<4 * J + 2 * I>(s[n]), e_mfma(x[0], b[0], ef16{}));
+                scale(F::template part_scale<4 * J + 2 * I + 1>(s[n]), e_mfma(x[1], b[1], ef16{}));
+            } else {
+                acc[n][0] = e_mfma(x[1], b[1], e_mfma(x[0], b[0], acc[n][0]));
             }
-        };
-        block(Int<0>{});
-        block(Int<1>{});
-        if constexpr (B == 1) {
-            block(Int<2>{});
-            block(Int<3>{});
         }
-    } else {
-        auto step = [&](auto st) {
-            constexpr int S = decltype(st)::value;
-            eh8 x[PARTS][MT];
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                for (int m = 0; m < MT; ++m) x[p][m] = a(S, p, m);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                uint32_t b[4];
-                F::template operand<J, S>(q[n], s[n], b);
-#pragma unroll
-                for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) acc[n][m] = e_mfma(x[p][m], b, acc[n][m]);
-            }
-        };
-        step(Int<0>{});
-        step(Int<1>{});
-        step(Int<2>{});
-        step(Int<3>{});
-    }
+    };
+    block(Int<0>{});
+    block(Int<1>{});
 }
 
-// acc += d P - 64 dmin (minimums . sums), and P starts again; sums(mt) the operand of the rows' sums (Q4_K)
+// Q4_K: acc += d P - 64 dmin (minimums . sums), and P starts again; sums(m) the operand of the rows' sums
 template <int NT, int MT, class X>
 __device__ __forceinline__ void finish_unit(const typename ExpertFmt<kFmtQ4_K>::Scale (&s)[NT], ef16 (&P)[NT][MT],
                                             ef16 (&acc)[NT][MT], X&& sums) {
+    typedef ExpertFmt<kFmtQ4_K> F;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         uint32_t b[4];
-        ExpertFmt<kFmtQ4_K>::min_operand(s[n], b);
-        const float d = h_lo(s[n].d), dmin = -64.0f * h_hi(s[n].d);
+        F::min_operand(s[n], b);
+        const float d = F::unit_scale(s[n]), dmin = -64.0f * h_hi(s[n].d);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             const ef16 t = e_mfma(sums(m), b, ef16{});
@@ -148,25 +114,32 @@ __device__ __forceinline__ void finish_unit(const typename ExpertFmt<kFmtQ4_K>::
     }
 }
 
-// this wave's loads and copies have arrived, what it read from LDS too, and every wave is here
-__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// this wave's loads and copies have arrived, and every wave is here
+__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// The loop is laid out so that a wave alone keeps its matrix unit busy, two of them share a SIMD.  A block is two steps (32 k; Q6_K one);
+// its NT * MT tiles are slots of 4 MFMAs (half with PAIR and Q6_K), column tile by column tile, and beside the MFMAs of a slot run
+//   * the 16 scalings of the slot before, whose sums are whole by then;
+//   * decoding: the second column tile of this block in the first half of its slots, the first one of the next block in the other;
+//   * the reads of the next block's activations into the registers of a row tile that no later slot of this block needs (MT 2),
+//     or into a second set (MT 1).
+// The barrier of a stage stands before the last block of the stage before it, when this stage's copies and quants, asked for a
+// stage earlier, have arrived; four buffers of LDS make every buffer's place a constant.
 template <int FMT, int MT, bool PAIR, bool SWIGLU>
 __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
     typedef ExpertFmt<FMT> F;
     constexpr int BM = PAIR ? 16 : 32 * MT, NT = 2, PARTS = PAIR ? 1 : 2;
     constexpr int kStage = BM * 256, kCopies = BM / 16;  // bytes of a stage; copies of a wave for it
     constexpr int kUnit = unit_bytes(FMT);
+    constexpr bool kUnitSum = F::kScaled == kPerUnit;
     static_assert(!PAIR || MT == 1, "a pair is one tile");
-    __shared__ __attribute__((aligned(16))) char ring[2 * kStage];
-    __shared__ int exps[BM];
+    __shared__ __attribute__((aligned(16))) char ring[4 * kStage];
 
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int blocks = SWIGLU ? (a.tiles + 3) >> 2 : (a.tiles + 7) >> 3;
     Tile t;
     if (!find_tile(a.g, BM, blocks, blockIdx.x, t)) return;
-    if (threadIdx.x < BM) exps[threadIdx.x] = a.exps[source_row(a, t.first + min(static_cast<int>(threadIdx.x), t.count - 1))];
 
     // this wave's column tiles; one past the last is computed again as the last and not stored
     int tile[NT];
@@ -185,20 +158,20 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
         const int r = wave * (BM / 4) + 4 * i + (lane >> 4);
         from[i] = a.planes + source_row(a, t.first + min(r, t.count - 1)) * a.depth * 1024L + 16 * ((lane & 15) ^ (r & 15));
     }
+    typedef __attribute__((address_space(3))) char* Lds;
+    const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((Lds)ring)) + wave * (BM / 4) * 256;
     auto copy = [&](int stage) {  // (past the end: the last stage again, unused)
-        char* to = ring + (stage & 1) * kStage + wave * (BM / 4) * 256;
+        const long off = 256L * min(stage, stages - 1);
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) e_dma16(from[i] + 256L * min(stage, stages - 1), to + 1024 * i);
+        for (int i = 0; i < kCopies; ++i) e_dma16(from[i] + off, ring_at + (stage & 3) * kStage + 1024 * i);
     };
-    // operands: lane row, and the slot of its chunk 2 step + h (hi) or 8 more (lo)
+    // operands: lane row, and the place of its chunk 2 step + h (hi) or 8 more (lo)
     const int row = PAIR ? lane & 15 : lane & 31, part = PAIR ? 8 * ((lane >> 4) & 1) : 0;
-    const int rowx = row & 15;
-    auto reader = [&](int stage) {
-        const char* at = ring + (stage & 1) * kStage + row * 256;
-        return [=](int s, int p, int m) {
-            return *reinterpret_cast<const eh8*>(at + m * 32 * 256 + 16 * ((2 * s + h + part + 8 * p) ^ rowx));
-        };
-    };
+    const char* at[4][PARTS];
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) at[s][p] = ring + row * 256 + 16 * ((2 * s + h + part + 8 * p) ^ (row & 15));
     const uint8_t* sums[MT];
     if constexpr (FMT == kFmtQ4_K) {
 #pragma unroll
@@ -206,57 +179,145 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
             sums[m] = a.sums + source_row(a, t.first + min(32 * m + row, t.count - 1)) * a.depth * 32L + 16 * h;
     }
 
-    ef16 acc[NT][MT] = {}, P[FMT == kFmtQ4_K ? NT : 1][FMT == kFmtQ4_K ? MT : 1] = {};
+    ef16 acc[NT][MT] = {}, P[kUnitSum ? NT : 1][kUnitSum ? MT : 1] = {};
     typename F::Quant q[2][NT];
-    typename F::Scale sc[2][NT];
-    auto load_quants = [&](typename F::Quant(&d)[NT], int stage) {
-        const int st = min(stage, stages - 1);  // (past the end: the last again, unused)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) F::load(d[n], unit[n] + (st >> 2) * static_cast<long>(kUnit), st & 3, lane);
+    typename F::Scale sc[2][NT];  // this unit's and the next one's
+    auto load_quants = [&](typename F::Quant& d, int stage, int n) {
+        const int st = min(stage, stages - 1);
+        F::load(d, unit[n] + (st >> 2) * static_cast<long>(kUnit), st & 3, lane);
     };
     auto load_scales = [&](typename F::Scale(&d)[NT], int u) {
-        const int at = min(u, a.depth - 1);
+        const int v = min(u, a.depth - 1);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) F::load(d[n], unit[n] + at * static_cast<long>(kUnit), lane);
+        for (int n = 0; n < NT; ++n) F::load(d[n], unit[n] + v * static_cast<long>(kUnit), lane);
     };
-    load_quants(q[0], 0);
-    load_scales(sc[0], 0);
-    copy(0);
-
-    eh8 x[MT];  // the unit's sums
-    auto run = [&](auto pos, int u, const typename F::Scale(&s)[NT], typename F::Scale(&next)[NT]) {
-        constexpr int J = decltype(pos)::value;
-        const int stage = 4 * u + J;
-        stage_barrier();  // this stage is in LDS and in registers, and the other buffer free
+    constexpr int kSets = MT == 1 ? 2 : 1;
+    constexpr int STEPS = F::kScaled == kPerStep ? 1 : 2, BLOCKS = 4 / STEPS;  // of a block, of a stage
+    eh8 x[kSets][STEPS][PARTS][MT];  // activations: [set][step][part][row tile]
+    uint32_t b[NT][STEPS][4];
+    eh8 sum[MT];
+    // reads of block I of stage J (its buffer: J)
+    auto read = [&](auto stage, auto blk, int set, int m) {
+        constexpr int J = decltype(stage)::value, I = decltype(blk)::value;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) q[J & 1][n].settle();  // the compiler's wait, before it would count the next loads
-        load_quants(q[(J + 1) & 1], stage + 1);
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                x[set][s][p][m] = *reinterpret_cast<const eh8*>(at[STEPS * I + s][p] + J * kStage + m * 32 * 256);
+    };
+    auto decode = [&](auto stage, auto step, int n, const typename F::Scale(&scales)[NT]) {
+        constexpr int J = decltype(stage)::value, S = decltype(step)::value;
+        uint32_t(&to)[4] = b[n][S % STEPS];
+        F::template operand<J, S>(q[J & 1][n], scales[n], to);
+        asm volatile("" : "+v"(to[0]), "+v"(to[1]), "+v"(to[2]), "+v"(to[3]));
+    };
+    // step s of slot (n, m): its MFMAs onto d
+    auto multiply = [&](int set, int s, int n, int m, ef16& d) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) d = e_mfma(x[set][s][p][m], b[n][s], d);
+    };
+    // kPerBlock, kPerStep: this slot's sums and those of the one before, whose scale is scale_of
+    constexpr bool kParts = F::kScaled == kPerBlock || F::kScaled == kPerStep;
+    ef16 sums_of[2];
+    float scale_of = 0.0f;
+    auto scale = [&](int n, int m, const ef16& d) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[n][m][i] = __builtin_fmaf(scale_of, d[i], acc[n][m][i]);
+        asm volatile("" : "+v"(acc[n][m]));  // here, not where acc is used next: the sums would live until then
+    };
+    // block I of stage J; `next` the scales of the block after it
+    auto run_block = [&](auto stage, auto blk, int u, const typename F::Scale(&now)[NT], const typename F::Scale(&next)[NT]) {
+        constexpr int J = decltype(stage)::value, I = decltype(blk)::value;
+        constexpr int In = (I + 1) % BLOCKS, Jn = (J + (In == 0)) & 3;  // the next block
+        constexpr int set = MT == 1 ? I & 1 : 0, other = MT == 1 ? set ^ 1 : 0;
+        constexpr int SLOTS = NT * MT;
+#pragma unroll
+        for (int slot = 0; slot < SLOTS; ++slot) {
+            const int n = slot / MT, m = slot % MT;
+            __builtin_amdgcn_sched_barrier(0);
+            // a column tile's quants of this stage are decoded: those of the stage after the next one
+            if (I == BLOCKS - 1 && slot == 0) load_quants(q[J & 1][0], 4 * u + J + 2, 0);
+            if (I == BLOCKS - 1 && slot == SLOTS / 2) load_quants(q[J & 1][1], 4 * u + J + 2, 1);
+            // the next block's activations, or this one's of the last row tile
+            if constexpr (MT == 1) {
+                if (slot == 0) read(Int<Jn>{}, Int<In>{}, other, 0);
+            } else {
+                if (slot == 0) read(Int<J>{}, Int<I>{}, 0, 1);
+                if (slot == SLOTS - 1) read(Int<Jn>{}, Int<In>{}, 0, 0);
+            }
+            if constexpr (kParts) sums_of[slot & 1] = ef16{};
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) multiply(set, s, n, m, kParts ? sums_of[slot & 1] : kUnitSum ? P[n][m] : acc[n][m]);
+            // the second column tile of this block in the first half of the slots, the first one of the next block in the other
+            auto decode_block = [&](auto j, auto i, int tile, int share, const typename F::Scale(&scales)[NT]) {
+                constexpr int S0 = STEPS * decltype(i)::value;
+                if (MT == 1 || share == 0) decode(j, Int<S0>{}, tile, scales);
+                if constexpr (STEPS == 2)
+                    if (MT == 1 || share == 1) decode(j, Int<S0 + 1>{}, tile, scales);
+            };
+            if (slot < SLOTS / 2) decode_block(Int<J>{}, Int<I>{}, 1, slot, now);
+            else decode_block(Int<Jn>{}, Int<In>{}, 0, slot - SLOTS / 2, next);
+            if constexpr (kParts) {  // the slot before: this block's, or the last block's last
+                const int before = (slot + SLOTS - 1) % SLOTS;
+                scale(before / MT, before % MT, sums_of[before & 1]);
+                scale_of = F::template part_scale<BLOCKS * J + I>(now[n]);
+            }
+            if (MT == 1 ? slot == 0 : slot == 0 || slot == SLOTS - 1) __builtin_amdgcn_sched_group_barrier(0x100, STEPS * PARTS, 0);
+#pragma unroll
+            for (int i = 0; i < STEPS * PARTS; ++i) {  // an MFMA's time is eight instructions
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, STEPS == 1 ? 12 : 7, 0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto run_stage = [&](auto stage, int u, const typename F::Scale(&s)[NT], typename F::Scale(&next)[NT]) {
+        constexpr int J = decltype(stage)::value;
+        run_block(stage, Int<0>{}, u, s, s);
+        if constexpr (BLOCKS == 4) {
+            run_block(stage, Int<1>{}, u, s, s);
+            run_block(stage, Int<2>{}, u, s, s);
+        }
+        stage_barrier();  // the next stage is in LDS and in registers, and the buffer after it free
+#pragma unroll
+        for (int n = 0; n < NT; ++n) q[(J + 1) & 1][n].settle();  // the compiler's wait, before it would count the next loads
         if constexpr (J == 0) load_scales(next, u + 1);
         if constexpr (J == 2 && FMT == kFmtQ4_K) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) x[m] = *reinterpret_cast<const eh8*>(sums[m] + 32 * u);
+            for (int m = 0; m < MT; ++m) sum[m] = *reinterpret_cast<const eh8*>(sums[m] + 32 * u);
         }
-        copy(stage + 1);
-        if constexpr (FMT == kFmtQ4_K) multiply_stage<F, J, NT, MT, PARTS>(q[J & 1], s, P, reader(stage));
-        else multiply_stage<F, J, NT, MT, PARTS>(q[J & 1], s, acc, reader(stage));
+        copy(4 * u + J + 2);
+        run_block(stage, Int<BLOCKS - 1>{}, u, s, J == 3 ? next : s);
     };
-    auto unit_of = [&](int u, const typename F::Scale(&s)[NT], typename F::Scale(&next)[NT]) {
-        run(Int<0>{}, u, s, next);
-        run(Int<1>{}, u, s, next);
-        run(Int<2>{}, u, s, next);
-        run(Int<3>{}, u, s, next);
-        if constexpr (FMT == kFmtQ4_K) {
-            if (PAIR && part) x[0] = eh8{};  // both parts of the sums go with the rows of hi
-            finish_unit<NT, MT>(s, P, acc, [&](int m) { return x[m]; });
-        }
-    };
-    for (int u = 0; u < a.depth; u += 2) {
-        unit_of(u, sc[0], sc[1]);
-        if (u + 1 < a.depth) unit_of(u + 1, sc[1], sc[0]);
-    }
 
-    // nothing may arrive in LDS that is another workgroup's by then; exps was written before the first barrier
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    load_scales(sc[0], 0);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) load_quants(q[0][n], 0, n), load_quants(q[1][n], 1, n);
+    copy(0);
+    copy(1);
+    stage_barrier();
+    read(Int<0>{}, Int<0>{}, 0, 0);
+    decode(Int<0>{}, Int<0>{}, 0, sc[0]);
+    if constexpr (STEPS == 2) decode(Int<0>{}, Int<1>{}, 0, sc[0]);
+    sums_of[1] = ef16{};
+    for (int u = 0; u < a.depth; ++u) {
+        run_stage(Int<0>{}, u, sc[0], sc[1]);
+        run_stage(Int<1>{}, u, sc[0], sc[1]);
+        run_stage(Int<2>{}, u, sc[0], sc[1]);
+        run_stage(Int<3>{}, u, sc[0], sc[1]);
+        if constexpr (kUnitSum) {
+            if (PAIR && part) sum[0] = eh8{};  // both parts of the sums go with the rows of hi
+            finish_unit<NT, MT>(sc[0], P, acc, [&](int m) { return sum[m]; });
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sc[0][n] = sc[1][n];
+    }
+    if constexpr (kParts) scale(NT - 1, MT - 1, sums_of[(NT * MT - 1) & 1]);
+    stage_barrier();  // the last copies have arrived, too: the rows' exponents take their place
+    int* const exps = reinterpret_cast<int*>(ring);
+    if (threadIdx.x < BM) exps[threadIdx.x] = a.exps[source_row(a, t.first + min(static_cast<int>(threadIdx.x), t.count - 1))];
+    __syncthreads();
+
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -372,13 +433,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const ProductArgs a
         ef16 p[NT][1] = {};
         auto reader = [&](int j) {
             const char* at = area + row * 1024 + 256 * j;
-            return [=](int s, int, int) { return *reinterpret_cast<const eh8*>(at + 16 * ((2 * s + h + part) ^ rowx)); };
+            return [=](int s) { return *reinterpret_cast<const eh8*>(at + 16 * ((2 * s + h + part) ^ rowx)); };
         };
-        multiply_stage<F, 0, NT, 1, 1>(q[0], sc, p, reader(0));
-        multiply_stage<F, 1, NT, 1, 1>(q[1], sc, p, reader(1));
-        multiply_stage<F, 2, NT, 1, 1>(q[2], sc, p, reader(2));
-        multiply_stage<F, 3, NT, 1, 1>(q[3], sc, p, reader(3));
-        if constexpr (FMT == kFmtQ4_K) {
+        multiply_stage<F, 0, NT>(q[0], sc, p, reader(0));
+        multiply_stage<F, 1, NT>(q[1], sc, p, reader(1));
+        multiply_stage<F, 2, NT>(q[2], sc, p, reader(2));
+        multiply_stage<F, 3, NT>(q[3], sc, p, reader(3));
+        if constexpr (F::kScaled == kPerUnit) {
             eh8 x = *reinterpret_cast<const eh8*>(sums + row * 32 + 16 * h);
             if (part) x = eh8{};
             ef16 r[NT][1] = {};
