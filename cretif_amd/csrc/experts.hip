@@ -1,6 +1,7 @@
 // experts.hip -- a layer of experts: the activations as planes for the grouped products, the products' choice of kernel,
 // and the weighted sum of a token's experts.  The products are in experts_gemm.hpp, the routing in experts_route.hip.
 #include <algorithm>
+#include <cmath>
 
 #include "experts.hpp"
 
@@ -138,19 +139,48 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
 namespace detail {
 namespace {
 
-// Which kernel, and how many rows a tile.
+// Which kernel: few with tiles of 2^lg rows and so many waves, else rows with tiles of bm.
 struct Plan {
     bool few;
-    int bm, waves;
+    int bm, lg, waves;
 };
 
+// The one that a rough model of both gives the least time, in us; it knows only host numbers, so rows are taken to be spread
+// over the experts.  All read the weights of the experts that have rows at 5.5 TB/s at best.  few_kernel: 7 us, 0.52 ns for each
+// unit that a tile meets (that often as a 256th of the GPU) and 0.07 ns for each row of it.  rows_kernel: 10 us with the
+// planes' pass, then stages of 0.42, 0.5 or 0.78 us (16, 32, 64 rows) while a CU has one workgroup or less, 0.47, 0.57 or 1.0 us
+// each beyond.  `weight` is what decoding and scaling a format takes of either, beside Q4_0.
+// Measured, few (8 rows, 4 waves) / 16 / 32 / 64 rows, us: SwiGLU 2048 -> 1024 of 64 experts, 8 each, Q4_K: 4 tokens 16.0 / 24.9 /
+// 27.5 / 37.0, 16: 25.9 / 30.0 / 34.0 / 48.1, 64: 58.3 / 58.8 / 47.0 / 67.7, 256: 165.8 / 93.1 / 83.9 / 97.9, 512: 306 / 152 / 121 /
+// 125, 4096: - / 935 / 666 / 575; one expert each of 8, 8192 -> 2048 Q4_0: 16 tokens 26.7 / 71.5 / 76.8 / 105, 128: 57.3 / 72.2 /
+// 76.9 / 106, 512: 169 / 104 / 81 / 112.
 Plan plan_products(const ExpertMatrix& w, const ExpertRows& g, bool swiglu) {
-    const int depth = (w.K + dev::kUnitK - 1) / dev::kUnitK;
-    const long R = static_cast<long>(g.n_tokens) * g.top_k;
-    (void)swiglu;
-    if (g.n_tokens <= 8) return {true, std::min(g.n_tokens, 16), std::min(depth, 8)};
-    const long each = R / w.n_experts;
-    return {false, each <= 12 ? 16 : each <= 40 ? 32 : 64, 0};
+    const double few_weight[] = {1.2, 1.0, 1.8, 1.0, 2.0, 1.4}, rows_weight[] = {1.1, 1.0, 1.3, 1.1, 1.65, 1.0};  // by format
+    const int depth = (w.K + dev::kUnitK - 1) / dev::kUnitK, tiles = (w.N + dev::kUnitCols - 1) / dev::kUnitCols;
+    const double R = static_cast<double>(g.n_tokens) * g.top_k, E = w.n_experts;
+    const double used = E * (1.0 - std::pow(1.0 - 1.0 / E, R)), matrices = swiglu ? 2.0 : 1.0;
+    const auto row_tiles = [&](int bm) { return std::min(std::max(used, R / bm + used / 2), R); };
+    const double memory = used * tiles * depth * matrices * dev::unit_bytes(w.fmt) / 5.5e6;
+
+    const bool single = R < 1.15 * used;  // an expert's rows: hardly ever more than one
+    const int lg = single ? 0 : g.n_tokens <= 4 ? 2 : 3;
+    const double units = tiles * depth * matrices * 1e-3;
+    Plan best{true, 0, lg, std::min(depth, lg < 3 && (used * tiles <= 256 || depth >= 16) ? 8 : 4)};
+    double least = 7.0 + std::max(memory, units * (0.52 * few_weight[w.fmt] * row_tiles(1 << lg) + 0.07 * R));
+    const double blocks = swiglu ? (tiles + 3) / 4 : (tiles + 7) / 8;
+    const struct {
+        int bm;
+        double one, each;
+    } kinds[] = {{16, 0.42, 0.47}, {32, 0.5, 0.57}, {64, 0.78, 1.0}};
+    for (const auto& k : kinds) {
+        const double stage = std::max(k.one, k.each * row_tiles(k.bm) * blocks / 256) * rows_weight[w.fmt];
+        const double us = 10.0 + std::max(memory, 4 * depth * stage);
+        if (us < least) {
+            least = us;
+            best = Plan{false, k.bm, 0, 0};
+        }
+    }
+    return best;
 }
 
 long up16(long bytes) { return (bytes + 15) & ~15L; }
@@ -165,6 +195,23 @@ PlaneBytes plane_bytes(const ExpertMatrix& w, long rows) {
     return {rows * depth * 1024, w.fmt == kFmtQ4_K ? rows * depth * 32 : 0, up16(rows * 4)};
 }
 
+dev::ProductArgs product_args(const ExpertMatrix& w, const ExpertRows& g, const float* x, long ldx, bool gather, float* out,
+                              long ldo) {
+    dev::ProductArgs a{};
+    a.w[0] = a.w[1] = static_cast<const uint8_t*>(w.data);
+    a.g = dev::Groups{g.offsets, g.rows, g.slots, w.n_experts, g.top_k, g.n_tokens * g.top_k};
+    a.x = x;
+    a.ldx = ldx;
+    a.out = out;
+    a.ldo = ldo;
+    a.N = w.N;
+    a.K = w.K;
+    a.tiles = (w.N + dev::kUnitCols - 1) / dev::kUnitCols;
+    a.depth = (w.K + dev::kUnitK - 1) / dev::kUnitK;
+    a.gather = gather;
+    return a;
+}
+
 // the product of w (and up: SiLU(x w^T) * (x up^T)) into out, rows in grouped order
 int launch_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertRows& g, const float* x, long ldx, bool gather,
                     float* out, long ldo, void* ws, hipStream_t stream) {
@@ -172,31 +219,21 @@ int launch_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertR
     const int depth = (w.K + dev::kUnitK - 1) / dev::kUnitK, tiles = (w.N + dev::kUnitCols - 1) / dev::kUnitCols;
     const bool swiglu = up != nullptr;
     const Plan plan = plan_products(w, g, swiglu);
-    dev::ProductArgs a{};
-    a.w[0] = static_cast<const uint8_t*>(w.data);
-    a.w[1] = static_cast<const uint8_t*>(swiglu ? up->data : w.data);
-    a.g = dev::Groups{g.offsets, g.rows, g.slots, w.n_experts, g.top_k, static_cast<int>(R)};
-    a.x = x;
-    a.ldx = ldx;
-    a.out = out;
-    a.ldo = ldo;
-    a.N = w.N;
-    a.K = w.K;
-    a.tiles = tiles;
-    a.depth = depth;
-    a.gather = gather;
+    dev::ProductArgs a = product_args(w, g, x, ldx, gather, out, ldo);
+    if (swiglu) a.w[1] = static_cast<const uint8_t*>(up->data);
     const int blocks = plan.few ? tiles : swiglu ? (tiles + 3) / 4 : (tiles + 7) / 8;
-    const long groups = (dev::most_tiles(R, w.n_experts, plan.bm) * blocks + 7) / 8 * 8;
+    const long groups = (dev::most_tiles(R, w.n_experts, plan.few ? 1 << plan.lg : plan.bm) * blocks + 7) / 8 * 8;
     if (groups >= 1L << 23) return kDeclined;  // up to 512 threads each: a launch's limit
     if (plan.few) {
         switch (w.fmt) {
-            case kFmtQ8_0: return dev::expert_few<kFmtQ8_0>(a, swiglu, plan.bm, plan.waves, groups, stream);
-            case kFmtQ4_0: return dev::expert_few<kFmtQ4_0>(a, swiglu, plan.bm, plan.waves, groups, stream);
-            case kFmtQ5_0: return dev::expert_few<kFmtQ5_0>(a, swiglu, plan.bm, plan.waves, groups, stream);
-            case kFmtQ4_K: return dev::expert_few<kFmtQ4_K>(a, swiglu, plan.bm, plan.waves, groups, stream);
-            case kFmtQ6_K: return dev::expert_few<kFmtQ6_K>(a, swiglu, plan.bm, plan.waves, groups, stream);
-            default: return dev::expert_few<kFmtF16>(a, swiglu, plan.bm, plan.waves, groups, stream);
+            case kFmtQ8_0: dev::expert_few<kFmtQ8_0>(a, swiglu, plan.lg, plan.waves, groups, stream); break;
+            case kFmtQ4_0: dev::expert_few<kFmtQ4_0>(a, swiglu, plan.lg, plan.waves, groups, stream); break;
+            case kFmtQ5_0: dev::expert_few<kFmtQ5_0>(a, swiglu, plan.lg, plan.waves, groups, stream); break;
+            case kFmtQ4_K: dev::expert_few<kFmtQ4_K>(a, swiglu, plan.lg, plan.waves, groups, stream); break;
+            case kFmtQ6_K: dev::expert_few<kFmtQ6_K>(a, swiglu, plan.lg, plan.waves, groups, stream); break;
+            default: dev::expert_few<kFmtF16>(a, swiglu, plan.lg, plan.waves, groups, stream);
         }
+        return 0;
     }
     const long rows = gather ? g.n_tokens : R;
     const PlaneBytes b = plane_bytes(w, rows);
@@ -218,6 +255,14 @@ int launch_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertR
     return 0;
 }
 
+// Whether a call's weighted sums are taken in one launch, a workgroup per token and column tile, which reads an expert's
+// weights for every token that has it: where that is a round of workgroups or little more.  Us, two launches / one: 1024 -> 2048
+// Q4_K, 8 of 64 experts each: 1 token 12.3 / 9.1, 4 14.3 / 10.7, 8 18.0 / 17.9, 16 23.4 / 32.1; 1536 -> 576 Q8_0, 4 of 32: 8 tokens
+// 12.5 / 8.8.
+bool token_takes(const ExpertMatrix& w, const ExpertRows& g) {
+    return static_cast<long>(g.n_tokens) * ((w.N + dev::kUnitCols - 1) / dev::kUnitCols) <= 320;
+}
+
 long product_columns(const ExpertMatrix& w) { return (w.N + 3L) & ~3L; }
 
 }  // namespace
@@ -234,12 +279,26 @@ int launch_expert_products(const ExpertMatrix& w, const ExpertMatrix* up, const 
 
 // combine: the products of all rows, then what the products need
 long expert_combine_workspace_bytes(const ExpertMatrix& w, const ExpertRows& g) {
+    if (token_takes(w, g)) return 0;
     return up16(static_cast<long>(g.n_tokens) * g.top_k * product_columns(w) * 4) +
            expert_product_workspace_bytes(w, g, false, false);
 }
 
 int launch_expert_combine(const ExpertMatrix& w, const ExpertRows& g, const float* h, long ldh, const float* weights,
                           const float* residual, long ldr, float* out, long ldo, void* ws, hipStream_t stream) {
+    if (token_takes(w, g)) {
+        const dev::ProductArgs a = product_args(w, g, h, ldh, false, out, ldo);
+        const dev::TokenArgs b{weights, residual, ldr};
+        switch (w.fmt) {
+            case kFmtQ8_0: dev::expert_token<kFmtQ8_0>(a, b, g.n_tokens, stream); break;
+            case kFmtQ4_0: dev::expert_token<kFmtQ4_0>(a, b, g.n_tokens, stream); break;
+            case kFmtQ5_0: dev::expert_token<kFmtQ5_0>(a, b, g.n_tokens, stream); break;
+            case kFmtQ4_K: dev::expert_token<kFmtQ4_K>(a, b, g.n_tokens, stream); break;
+            case kFmtQ6_K: dev::expert_token<kFmtQ6_K>(a, b, g.n_tokens, stream); break;
+            default: dev::expert_token<kFmtF16>(a, b, g.n_tokens, stream);
+        }
+        return 0;
+    }
     const long R = static_cast<long>(g.n_tokens) * g.top_k, ldp = product_columns(w);
     float* const p = static_cast<float*>(ws);
     const int rc = launch_products(w, nullptr, g, h, ldh, false, p, ldp, reinterpret_cast<uint8_t*>(p) + up16(R * ldp * 4), stream);

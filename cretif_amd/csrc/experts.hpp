@@ -42,67 +42,90 @@ struct Groups {
     int E, k, R;         // R = tokens * k
 };
 
-// Rows [first, first + count) of an expert, a tile of at most BM of them, and its block of columns.
+// Rows [first, first + count) of an expert, a tile of them, and its block of columns.
 struct Tile {
     int expert, first, count, block;
 };
 
 __device__ __forceinline__ int wave_scan_add(int v) {  // inclusive sum over the lanes below
-    const int lane = __lane_id();
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __builtin_amdgcn_ds_bpermute((lane - d) << 2, v);
-        v += lane >= d ? o : 0;
-    }
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8 within 16 lanes
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
     return v;
 }
 
 __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+// tiles of 2^lg rows
+__device__ __forceinline__ int tiles_of(int lo, int hi, int lg) { return (max(hi - lo, 0) + (1 << lg) - 1) >> lg; }
 
-// Work item number of workgroup b, out of every expert's ceil(rows / BM) tiles x blocks, or no such item.  Experts come in
+// Work item number of workgroup b, out of every expert's tiles of up to 2^lg rows x blocks, or no such item.  Experts come in
 // order, then blocks, then tiles: the tiles that share an expert's block of weights are neighbours, and each of the eight
-// XCDs (workgroup b runs on XCD b mod 8, with an L2 of its own) gets consecutive items.  The whole wave calls it.
-__device__ __forceinline__ bool find_tile(const Groups& g, int bm, int blocks, int b, Tile& t) {
-    const int lane = __lane_id(), per = (g.E + 63) >> 6;
-    const int e0 = lane * per, e1 = min(e0 + per, g.E);
-    int tiles = 0;
-    if (per == 1) {
-        if (e0 < g.E) {
-            const int lo = clamp_int(g.offsets[e0], 0, g.R), hi = clamp_int(g.offsets[e0 + 1], 0, g.R);
-            tiles = hi > lo ? (hi - lo + bm - 1) / bm : 0;
+// XCDs (workgroup b runs on XCD b mod 8, with an L2 of its own) gets consecutive items.  The whole wave calls it.  Up to 256
+// experts a lane holds four in registers: one trip to memory, then a few dozen instructions.
+__device__ __forceinline__ bool find_tile(const Groups& g, int lg, int blocks, int b, Tile& t) {
+    constexpr int HELD = 4;
+    const int lane = __lane_id(), per = g.E <= 64 ? 1 : g.E <= 64 * HELD ? HELD : (g.E + 63) >> 6;
+    const int e0 = lane * per;
+    int off[HELD + 1], n[HELD], tiles = 0;
+    if (per <= HELD) {
+#pragma unroll
+        for (int i = 0; i <= HELD; ++i) off[i] = g.offsets[min(e0 + i, g.E)];  // (all asked for at once)
+#pragma unroll
+        for (int i = 0; i <= HELD; ++i) off[i] = clamp_int(off[i], 0, g.R);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            n[i] = i < per ? tiles_of(off[i], off[i + 1], lg) : 0;  // (past the last expert nothing: the same offset)
+            tiles += n[i];
         }
     } else {
-        int lo = e0 < g.E ? clamp_int(g.offsets[e0], 0, g.R) : 0;
-        for (int e = e0; e < e1; ++e) {
-            const int hi = clamp_int(g.offsets[e + 1], 0, g.R);
-            tiles += hi > lo ? (hi - lo + bm - 1) / bm : 0;
-            lo = hi;
-        }
+        for (int e = e0; e < min(e0 + per, g.E); ++e)
+            tiles += tiles_of(clamp_int(g.offsets[e], 0, g.R), clamp_int(g.offsets[e + 1], 0, g.R), lg);
     }
     const int up = wave_scan_add(tiles);
     const long total = static_cast<long>(__builtin_amdgcn_readlane(up, 63)) * blocks;
     const long share = (total + 7) >> 3;
     const long item = (b & 7) * share + (b >> 3);
     if ((b >> 3) >= share || item >= total) return false;
-    const unsigned long hit = __ballot(static_cast<long>(up) * blocks > item);
-    const int who = __builtin_ctzl(hit);
-    int before = __builtin_amdgcn_readlane(up - tiles, who), e = who * per;
-    if (per > 1) {  // which of that lane's experts: one of them a lane
-        const int mine = min(e + lane, g.E - 1);
-        const int lo = clamp_int(g.offsets[mine], 0, g.R), hi = clamp_int(g.offsets[mine + 1], 0, g.R);
-        const int n = lane < per && e + lane < g.E && hi > lo ? (hi - lo + bm - 1) / bm : 0;
-        const int sum = wave_scan_add(n);
-        const int at = __builtin_ctzl(__ballot(static_cast<long>(before + sum) * blocks > item));
-        before += __builtin_amdgcn_readlane(sum - n, at);
-        e = min(e + at, g.E - 1);  // (as it was found, unless the offsets change meanwhile)
+    const int who = __builtin_ctzl(__ballot(static_cast<long>(up) * blocks > item));
+    long before = static_cast<long>(__builtin_amdgcn_readlane(up - tiles, who)) * blocks;
+    int lo = 0, hi = 0, count = 0;
+    t.expert = who * per;
+    if (per <= HELD) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int ni = __builtin_amdgcn_readlane(n[i], who);
+            if (count == 0 && item < before + static_cast<long>(ni) * blocks) {
+                count = ni;
+                lo = __builtin_amdgcn_readlane(off[i], who);
+                hi = __builtin_amdgcn_readlane(off[i + 1], who);
+                t.expert += i;
+            } else if (count == 0) {
+                before += static_cast<long>(ni) * blocks;
+            }
+        }
+    } else {  // one of that lane's experts to a lane
+        const int mine = min(t.expert + lane, g.E - 1);
+        const int from = clamp_int(g.offsets[mine], 0, g.R), to = clamp_int(g.offsets[mine + 1], 0, g.R);
+        const int some = lane < per && t.expert + lane < g.E ? tiles_of(from, to, lg) : 0;
+        const int sum = wave_scan_add(some);
+        const unsigned long hit = __ballot(before + static_cast<long>(sum) * blocks > item);
+        if (hit == 0) return false;  // (the offsets changed meanwhile)
+        const int at = __builtin_ctzl(hit);
+        before += static_cast<long>(__builtin_amdgcn_readlane(sum - some, at)) * blocks;
+        count = __builtin_amdgcn_readlane(some, at);
+        lo = __builtin_amdgcn_readlane(from, at);
+        hi = __builtin_amdgcn_readlane(to, at);
+        t.expert += at;
     }
-    const int lo = clamp_int(g.offsets[e], 0, g.R), hi = clamp_int(g.offsets[e + 1], 0, g.R);
-    const int n = max((hi - lo + bm - 1) / bm, 1), rest = static_cast<int>(item - static_cast<long>(before) * blocks);
-    t.expert = e;
-    t.block = rest / n;
-    t.first = lo + (rest - t.block * n) * bm;
-    t.count = min(bm, hi - t.first);
-    return t.count > 0 && t.block < blocks;
+    if (count == 0) return false;
+    const int rest = static_cast<int>(item - before);
+    t.block = count == 1 ? rest : rest / count;
+    t.first = lo + ((rest - t.block * count) << lg);
+    t.count = min(1 << lg, hi - t.first);
+    return true;
 }
 
 // workgroups that find_tile needs whatever the groups hold: an expert's tiles are at most its rows, and all but one of
@@ -127,12 +150,21 @@ struct ProductArgs {
     bool gather;             // the row of grouped row r is rows[r] / k, else r
 };
 
-// the kernels of experts_gemm.hpp, instantiated in one file per format (experts_q4_k.hip, ...).  bm: rows of a tile, 16, 32
-// or 64 for expert_rows, 1 .. 16 for expert_few, whose workgroups have `waves` waves; expert_few returns a launcher status
+struct TokenArgs {
+    const float* weights;   // [tokens, k]
+    const float* residual;  // or null
+    long ldr;
+};
+
+// the kernels of experts_gemm.hpp, instantiated in one file per format (experts_q4_k.hip, ...).  expert_rows: tiles of bm = 16, 32
+// or 64 rows; expert_few: tiles of up to 2^lg rows, lg 0 .. 3, workgroups of `waves` waves, up to 8 (and few_lds(lg, waves) within
+// 64 KB); expert_token: the weighted sums of so many tokens, x in grouped order
 template <int FMT>
 void expert_rows(const ProductArgs& a, bool swiglu, int bm, long workgroups, hipStream_t stream);
 template <int FMT>
-int expert_few(const ProductArgs& a, bool swiglu, int bm, int waves, long workgroups, hipStream_t stream);
+void expert_few(const ProductArgs& a, bool swiglu, int lg, int waves, long workgroups, hipStream_t stream);
+template <int FMT>
+void expert_token(const ProductArgs& a, const TokenArgs& b, int tokens, hipStream_t stream);
 
 }  // namespace dev
 }  // namespace cri

@@ -4,12 +4,13 @@
 // ExpertFmt<FMT>: load(q, unit, stage) a lane's bytes of a stage of four steps (64 k), load(s, unit) those of the unit's
 // scales; operand<J, S>(q, s, b) the eight weights of step S of stage J, as four pairs.  kScaled says how scales are applied:
 // kNoScale not at all; kPerStep and kPerBlock the partial sum of a step (16 k) or of a block of two times part_scale<I>() (I: the
-// unit's step or block); kPerUnit (Q4_K) the whole unit's sum times unit_scale() less 64 dmin times that of the minimums,
-// min_operand(), and the activations' sums over 32, which are staged times 2^-6.
+// unit's step or block).  Q4_K's minimums meet the activations' sums over 32, which are staged times 2^-6, once per unit:
+// min_operand(), min_scale().
 //
-// Scales multiply a partial sum instead of the weights because d q has 19 bits, fp16 11; Q4_K's 6-bit scale times 4-bit code
-// has 10 and goes into the operand.  Q6_K's scale times code has 12: as an operand's nearest half and its rest in a third MFMA
-// (no scaling before the unit's end) 4096 tokens' SwiGLU took 856 us, with scaled steps 790: the MFMAs' power counts.
+// Scales multiply a partial sum instead of the weights because d q has 19 bits, fp16 11.  Other forms that fit: Q4_K's 6-bit
+// scale times 4-bit code (10 bits) in the operand, d per unit, half the scalings: its 64 registers of unit sums spill, 4096
+// tokens' SwiGLU 630 us against 591 as Q4_0 does it; Q6_K's scale times code (12 bits) as an operand's nearest half and its rest
+// in a third MFMA, no scalings before the unit's end: 856 us against 790, the MFMAs' power counts.
 #pragma once
 
 #include "experts.hpp"
@@ -17,7 +18,7 @@
 namespace cri {
 namespace dev {
 
-enum : int { kNoScale = 0, kPerStep = 1, kPerBlock = 2, kPerUnit = 3 };
+enum : int { kNoScale = 0, kPerStep = 1, kPerBlock = 2 };
 
 typedef _Float16 eh2 __attribute__((ext_vector_type(2)));
 
@@ -35,16 +36,18 @@ __device__ __forceinline__ uint32_t e_add(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t e_mul(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(eh2, a) * __builtin_bit_cast(eh2, b));
 }
-// (v & m) | o as one instruction: the mask in an SGPR, the constant in a VGPR
+// (v & m) | o as one v_and_or_b32: the constants are kept from the compiler, which would take two instructions with literals.
+// (Not as an instruction in asm: the compiler does not see that one write registers that an MFMA is still to write.)
 __device__ __forceinline__ uint32_t e_and_or(uint32_t v, uint32_t m, uint32_t o) {
-    uint32_t r;
-    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(v), "s"(m), "v"(o));
-    return r;
+    asm("" : "+s"(m));
+    asm("" : "+v"(o));
+    return (v & m) | o;
 }
 constexpr uint32_t kTop = 0x64006400u;     // 1024 in both halves
 constexpr uint32_t kTenth = 0x2C002C00u;   // 1/16 in both halves
 
-__device__ __forceinline__ u32x4 e_load16(const uint8_t* p) { return *reinterpret_cast<const u32x4*>(p); }
+// 16 bytes at a wave-uniform address and the lane's offset (one SGPR pair, one VGPR)
+__device__ __forceinline__ u32x4 e_load16(const uint8_t* p, uint32_t off) { return *reinterpret_cast<const u32x4*>(p + off); }
 __device__ __forceinline__ float e_half(uint32_t w, bool high) { return high ? h_hi(w) : h_lo(w); }
 
 // The compiler waits for v's loads here.
@@ -76,11 +79,11 @@ struct ExpertFmt<kFmtQ4_0> {
     struct Scale {
         u32x4 d;
     };
-    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, int lane) {
-        q.q = e_load16(unit + 1024 * stage + 16 * lane);
+    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, uint32_t lane) {
+        q.q = e_load16(unit + 1024 * stage, 16 * lane);
     }
-    static __device__ __forceinline__ void load(Scale& s, const uint8_t* unit, int lane) {
-        s.d = e_load16(unit + 4096 + 16 * (lane & 31));
+    static __device__ __forceinline__ void load(Scale& s, const uint8_t* unit, uint32_t lane) {
+        s.d = e_load16(unit + 4096, 16 * (lane & 31));
     }
     template <int J, int S>
     static __device__ __forceinline__ void operand(const Quant& q, const Scale&, uint32_t (&b)[4]) {
@@ -108,12 +111,12 @@ struct ExpertFmt<kFmtQ8_0> {
     struct Scale {
         u32x4 d;
     };
-    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, int lane) {
-        q.q[0] = e_load16(unit + 2048 * stage + 16 * lane);
-        q.q[1] = e_load16(unit + 2048 * stage + 1024 + 16 * lane);
+    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, uint32_t lane) {
+        q.q[0] = e_load16(unit + 2048 * stage, 16 * lane);
+        q.q[1] = e_load16(unit + 2048 * stage + 1024, 16 * lane);
     }
-    static __device__ __forceinline__ void load(Scale& s, const uint8_t* unit, int lane) {
-        s.d = e_load16(unit + 8192 + 16 * (lane & 31));
+    static __device__ __forceinline__ void load(Scale& s, const uint8_t* unit, uint32_t lane) {
+        s.d = e_load16(unit + 8192, 16 * (lane & 31));
     }
     template <int J, int S>
     static __device__ __forceinline__ void operand(const Quant& q, const Scale&, uint32_t (&b)[4]) {
@@ -144,12 +147,12 @@ struct ExpertFmt<kFmtQ5_0> {
     struct Scale {
         u32x4 d;
     };
-    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, int lane) {
-        q.q = e_load16(unit + 1024 * stage + 16 * lane);
-        q.h = *reinterpret_cast<const uint32_t*>(unit + 4096 + 16 * lane + 4 * stage);
+    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, uint32_t lane) {
+        q.q = e_load16(unit + 1024 * stage, 16 * lane);
+        q.h = *reinterpret_cast<const uint32_t*>(unit + (4096 + 4 * stage) + 16 * lane);
     }
-    static __device__ __forceinline__ void load(Scale& s, const uint8_t* unit, int lane) {
-        s.d = e_load16(unit + 5120 + 16 * (lane & 31));
+    static __device__ __forceinline__ void load(Scale& s, const uint8_t* unit, uint32_t lane) {
+        s.d = e_load16(unit + 5120, 16 * (lane & 31));
     }
     template <int J, int S>
     static __device__ __forceinline__ void operand(const Quant& q, const Scale&, uint32_t (&b)[4]) {
@@ -179,15 +182,15 @@ struct ExpertFmt<kFmtQ6_K> {
         u32x4 sc;
         uint32_t d;
     };
-    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, int lane) {
+    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, uint32_t lane) {
         typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-        q.q = e_load16(unit + 1024 * stage + 16 * lane);
-        const u2 h = *reinterpret_cast<const u2*>(unit + 4096 + 1024 * (stage >> 1) + 16 * lane + 8 * (stage & 1));
+        q.q = e_load16(unit + 1024 * stage, 16 * lane);
+        const u2 h = *reinterpret_cast<const u2*>(unit + (4096 + 1024 * (stage >> 1) + 8 * (stage & 1)) + 16 * lane);
         q.h[0] = h.x;
         q.h[1] = h.y;
     }
-    static __device__ __forceinline__ void load(Scale& s, const uint8_t* unit, int lane) {
-        s.sc = e_load16(unit + 6144 + 16 * (lane & 31));
+    static __device__ __forceinline__ void load(Scale& s, const uint8_t* unit, uint32_t lane) {
+        s.sc = e_load16(unit + 6144, 16 * (lane & 31));
         s.d = *reinterpret_cast<const uint16_t*>(unit + 6656 + 2 * (lane & 31));
     }
     template <int J, int S>
@@ -210,37 +213,34 @@ struct ExpertFmt<kFmtQ6_K> {
 
 template <>
 struct ExpertFmt<kFmtQ4_K> {
-    static constexpr int kScaled = kPerUnit;
+    static constexpr int kScaled = kPerBlock;
     typedef NibbleQuant Quant;
     struct Scale {
         u32x4 s;  // sc, mn
         uint32_t d;
     };
-    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, int lane) {
-        q.q = e_load16(unit + 1024 * stage + 16 * lane);
+    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, uint32_t lane) {
+        q.q = e_load16(unit + 1024 * stage, 16 * lane);
     }
-    static __device__ __forceinline__ void load(Scale& s, const uint8_t* unit, int lane) {
-        s.s = e_load16(unit + 4096 + 16 * (lane & 31));
+    static __device__ __forceinline__ void load(Scale& s, const uint8_t* unit, uint32_t lane) {
+        s.s = e_load16(unit + 4096, 16 * (lane & 31));
         s.d = *reinterpret_cast<const uint32_t*>(unit + 4608 + 4 * (lane & 31));
     }
-    // byte P of w in both halves, in fp16
-    template <int P>
-    static __device__ __forceinline__ uint32_t both(uint32_t w) {
-        return e_add(__builtin_amdgcn_perm(kTop, w, 0x05000500u | (P << 16) | P), e_splat(-1024.0f));
-    }
     template <int J, int S>
-    static __device__ __forceinline__ void operand(const Quant& q, const Scale& s, uint32_t (&b)[4]) {
+    static __device__ __forceinline__ void operand(const Quant& q, const Scale&, uint32_t (&b)[4]) {
         uint32_t t[4];
         e_nibbles(e_at(q.q, S), t);
-        constexpr int i = 2 * J + (S >> 1);  // the sub-block of 32
-        const uint32_t sc = both<(i & 3)>(i < 4 ? s.s.x : s.s.y);
-        const uint32_t off = e_mul(sc, e_splat(-1024.0f)), sc16 = e_mul(sc, kTenth), off16 = e_mul(sc, e_splat(-64.0f));
-        b[0] = e_fma(t[0], sc, off);  // (1024 + q) sc - 1024 sc = q sc <= 945, exactly
-        b[1] = e_fma(t[1], sc16, off16);
-        b[2] = e_fma(t[2], sc, off);
-        b[3] = e_fma(t[3], sc16, off16);
+        const uint32_t low = e_splat(-1024.0f), high = e_splat(-64.0f);
+        b[0] = e_add(t[0], low);
+        b[1] = e_fma(t[1], kTenth, high);
+        b[2] = e_add(t[2], low);
+        b[3] = e_fma(t[3], kTenth, high);
     }
-    static __device__ __forceinline__ float unit_scale(const Scale& s) { return h_lo(s.d); }
+    template <int I>
+    static __device__ __forceinline__ float part_scale(const Scale& s) {
+        return h_lo(s.d) * ubyte(I < 4 ? s.s.x : s.s.y, I & 3);  // 17 bits: exact
+    }
+    // the unit's minimums as an operand that meets the activations' sums, and what their product is multiplied by
     static __device__ __forceinline__ void min_operand(const Scale& s, uint32_t (&b)[4]) {
         const uint32_t z = e_splat(-1024.0f);
         b[0] = e_add(__builtin_amdgcn_perm(kTop, s.s.z, 0x05010500u), z);
@@ -248,6 +248,7 @@ struct ExpertFmt<kFmtQ4_K> {
         b[2] = e_add(__builtin_amdgcn_perm(kTop, s.s.w, 0x05010500u), z);
         b[3] = e_add(__builtin_amdgcn_perm(kTop, s.s.w, 0x05030502u), z);
     }
+    static __device__ __forceinline__ float min_scale(const Scale& s) { return -64.0f * h_hi(s.d); }
 };
 
 template <>
@@ -258,11 +259,11 @@ struct ExpertFmt<kFmtF16> {
         __device__ __forceinline__ void settle() { e_settle(q[0]), e_settle(q[1]), e_settle(q[2]), e_settle(q[3]); }
     };
     struct Scale {};
-    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, int lane) {
+    static __device__ __forceinline__ void load(Quant& q, const uint8_t* unit, int stage, uint32_t lane) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q.q[i] = e_load16(unit + 4096 * stage + 1024 * i + 16 * lane);
+        for (int i = 0; i < 4; ++i) q.q[i] = e_load16(unit + 4096 * stage + 1024 * i, 16 * lane);
     }
-    static __device__ __forceinline__ void load(Scale&, const uint8_t*, int) {}
+    static __device__ __forceinline__ void load(Scale&, const uint8_t*, uint32_t) {}
     template <int J, int S>
     static __device__ __forceinline__ void operand(const Quant& q, const Scale&, uint32_t (&b)[4]) {
 #pragma unroll

@@ -5,7 +5,8 @@ namespace cri {
 namespace dev {
 
 template void expert_rows<kFmtF16>(const ProductArgs&, bool, int, long, hipStream_t);
-template int expert_few<kFmtF16>(const ProductArgs&, bool, int, int, long, hipStream_t);
+template void expert_few<kFmtF16>(const ProductArgs&, bool, int, int, long, hipStream_t);
+template void expert_token<kFmtF16>(const ProductArgs&, const TokenArgs&, int, hipStream_t);
 
 }  // namespace dev
 }  // namespace cri

@@ -18,13 +18,12 @@
 //   * Each decoded operand meets MT * 2 MFMAs and each operand read from LDS two.
 //   * PAIR (at most 16 rows): lane rows 0 .. 15 hold hi, 16 .. 31 lo of the same rows; one MFMA does both parts, and the
 //     two halves of the output are added at the end.
-// few_kernel: for calls of few tokens, where what counts is how many waves read weights at once: a workgroup takes up to 16
+// few_kernel: for calls of few tokens, where what counts is how many waves read weights at once: a workgroup takes up to 8
 // rows of an expert and one tile of 32 columns, its waves the units along k, each converting the activations of its own
 // units to an LDS area of its own (a power of two per row and unit), no barrier before the sum over the waves.
 #pragma once
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "act.hpp"
@@ -51,6 +50,9 @@ __device__ __forceinline__ void e_dma16(const uint8_t* g, uint32_t lds) {
                  : "memory");
 }
 
+typedef __attribute__((address_space(3))) char* Lds;
+typedef __attribute__((address_space(3))) const eh8* LdsEight;
+
 // output row of register i for lanes below 32 (4 more above)
 __device__ __forceinline__ constexpr int e_row(int i) { return (i & 3) + 8 * (i >> 2); }
 
@@ -62,54 +64,22 @@ __device__ __forceinline__ long source_row(const ProductArgs& a, int r) {
 template <int I>
 using Int = std::integral_constant<int, I>;
 
-// One stage (64 k) of NT column tiles against a tile of paired rows; a(step) is an activation operand.  acc: the results, or with
-// kPerUnit the unit's sum of integers.
-template <class F, int J, int NT, class A>
-__device__ __forceinline__ void multiply_stage(const typename F::Quant (&q)[NT], const typename F::Scale (&s)[NT],
-                                               ef16 (&acc)[NT][1], A&& a) {
-    auto block = [&](auto blk) {
-        constexpr int I = decltype(blk)::value;  // of the stage
-        const eh8 x[2] = {a(2 * I), a(2 * I + 1)};
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            uint32_t b[2][4];
-            F::template operand<J, 2 * I>(q[n], s[n], b[0]);
-            F::template operand<J, 2 * I + 1>(q[n], s[n], b[1]);
-            auto scale = [&](float d, const ef16& t) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[n][0][i] = __builtin_fmaf(d, t[i], acc[n][0][i]);
-                asm volatile("" : "+v"(acc[n][0]));  // here, not where acc is used next: t would live until then
-            };
-            if constexpr (F::kScaled == kPerBlock) {
-                scale(F::template part_scale<2 * J + I>(s[n]), e_mfma(x[1], b[1], e_mfma(x[0], b[0], ef16{})));
-            } else if constexpr (F::kScaled == kPerStep) {
-                scale(F::template part_scale<4 * J + 2 * I>(s[n]), e_mfma(x[0], b[0], ef16{}));
-                scale(F::template part_scale<4 * J + 2 * I + 1>(s[n]), e_mfma(x[1], b[1], ef16{}));
-            } else {
-                acc[n][0] = e_mfma(x[1], b[1], e_mfma(x[0], b[0], acc[n][0]));
-            }
-        }
-    };
-    block(Int<0>{});
-    block(Int<1>{});
-}
-
-// Q4_K: acc += d P - 64 dmin (minimums . sums), and P starts again; sums(m) the operand of the rows' sums
+// Q4_K: acc -= 64 dmin (minimums . sums); sums(m) the operand of the rows' sums
 template <int NT, int MT, class X>
-__device__ __forceinline__ void finish_unit(const typename ExpertFmt<kFmtQ4_K>::Scale (&s)[NT], ef16 (&P)[NT][MT],
-                                            ef16 (&acc)[NT][MT], X&& sums) {
+__device__ __forceinline__ void subtract_minimums(const typename ExpertFmt<kFmtQ4_K>::Scale (&s)[NT], ef16 (&acc)[NT][MT],
+                                                  X&& sums) {
     typedef ExpertFmt<kFmtQ4_K> F;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         uint32_t b[4];
         F::min_operand(s[n], b);
-        const float d = F::unit_scale(s[n]), dmin = -64.0f * h_hi(s[n].d);
+        const float dmin = F::min_scale(s[n]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             const ef16 t = e_mfma(sums(m), b, ef16{});
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[n][m][i] = __builtin_fmaf(d, P[n][m][i], __builtin_fmaf(dmin, t[i], acc[n][m][i]));
-            P[n][m] = ef16{};
+            for (int i = 0; i < 16; ++i) acc[n][m][i] = __builtin_fmaf(dmin, t[i], acc[n][m][i]);
+            asm volatile("" : "+v"(acc[n][m]));
         }
     }
 }
@@ -128,18 +98,17 @@ __device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(
 template <int FMT, int MT, bool PAIR, bool SWIGLU>
 __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
     typedef ExpertFmt<FMT> F;
-    constexpr int BM = PAIR ? 16 : 32 * MT, NT = 2, PARTS = PAIR ? 1 : 2;
+    constexpr int BM = PAIR ? 16 : 32 * MT, LG = PAIR ? 4 : MT == 1 ? 5 : 6, NT = 2, PARTS = PAIR ? 1 : 2;
     constexpr int kStage = BM * 256, kCopies = BM / 16;  // bytes of a stage; copies of a wave for it
     constexpr int kUnit = unit_bytes(FMT);
-    constexpr bool kUnitSum = F::kScaled == kPerUnit;
     static_assert(!PAIR || MT == 1, "a pair is one tile");
-    __shared__ __attribute__((aligned(16))) char ring[4 * kStage];
+    __shared__ __attribute__((aligned(256))) char ring[4 * kStage];
 
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int blocks = SWIGLU ? (a.tiles + 3) >> 2 : (a.tiles + 7) >> 3;
     Tile t;
-    if (!find_tile(a.g, BM, blocks, blockIdx.x, t)) return;
+    if (!find_tile(a.g, LG, blocks, blockIdx.x, t)) return;
 
     // this wave's column tiles; one past the last is computed again as the last and not stored
     int tile[NT];
@@ -152,34 +121,35 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
     }
     const int stages = a.depth * 4;
     // copies: lane l takes slot l & 15 of row l >> 4 of the four rows of a copy
-    const uint8_t* from[kCopies];
+    uint32_t from[kCopies];  // the rows
+    const uint32_t row_bytes = a.depth * 1024;
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-        const int r = wave * (BM / 4) + 4 * i + (lane >> 4);
-        from[i] = a.planes + source_row(a, t.first + min(r, t.count - 1)) * a.depth * 1024L + 16 * ((lane & 15) ^ (r & 15));
-    }
-    typedef __attribute__((address_space(3))) char* Lds;
-    const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((Lds)ring)) + wave * (BM / 4) * 256;
+    for (int i = 0; i < kCopies; ++i)
+        from[i] = source_row(a, t.first + min(wave * (BM / 4) + 4 * i + (lane >> 4), t.count - 1));
+    const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((Lds)ring));
     auto copy = [&](int stage) {  // (past the end: the last stage again, unused)
-        const long off = 256L * min(stage, stages - 1);
+        const uint8_t* at = a.planes + 256L * min(stage, stages - 1);
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) e_dma16(from[i] + off, ring_at + (stage & 3) * kStage + 1024 * i);
+        for (int i = 0; i < kCopies; ++i) {
+            const int r = wave * (BM / 4) + 4 * i + (lane >> 4);
+            uint32_t row = from[i];
+            asm volatile("" : "+v"(row));  // the address is made here: kept for all rows it would take twice the registers
+            e_dma16(at + static_cast<uint64_t>(row) * row_bytes + 16 * ((lane & 15) ^ (r & 15)),
+                    ring_at + (stage & 3) * kStage + wave * (BM / 4) * 256 + 1024 * i);
+        }
     };
     // operands: lane row, and the place of its chunk 2 step + h (hi) or 8 more (lo)
     const int row = PAIR ? lane & 15 : lane & 31, part = PAIR ? 8 * ((lane >> 4) & 1) : 0;
-    const char* at[4][PARTS];
+    uint32_t at[4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) at[s][p] = ring + row * 256 + 16 * ((2 * s + h + part + 8 * p) ^ (row & 15));
-    const uint8_t* sums[MT];
+    for (int s = 0; s < 4; ++s) at[s] = ring_at + row * 256 + 16 * ((2 * s + h + part) ^ (row & 15));
+    uint32_t sums[MT];  // the rows' sums: row * depth
     if constexpr (FMT == kFmtQ4_K) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-            sums[m] = a.sums + source_row(a, t.first + min(32 * m + row, t.count - 1)) * a.depth * 32L + 16 * h;
+        for (int m = 0; m < MT; ++m) sums[m] = source_row(a, t.first + min(32 * m + row, t.count - 1)) * a.depth;
     }
 
-    ef16 acc[NT][MT] = {}, P[kUnitSum ? NT : 1][kUnitSum ? MT : 1] = {};
+    ef16 acc[NT][MT] = {};
     typename F::Quant q[2][NT];
     typename F::Scale sc[2][NT];  // this unit's and the next one's
     auto load_quants = [&](typename F::Quant& d, int stage, int n) {
@@ -203,7 +173,7 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
         for (int s = 0; s < STEPS; ++s)
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
-                x[set][s][p][m] = *reinterpret_cast<const eh8*>(at[STEPS * I + s][p] + J * kStage + m * 32 * 256);
+                x[set][s][p][m] = *reinterpret_cast<LdsEight>((at[STEPS * I + s] ^ (128 * p)) + J * kStage + m * 32 * 256);
     };
     auto decode = [&](auto stage, auto step, int n, const typename F::Scale(&scales)[NT]) {
         constexpr int J = decltype(stage)::value, S = decltype(step)::value;
@@ -247,7 +217,7 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
             }
             if constexpr (kParts) sums_of[slot & 1] = ef16{};
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) multiply(set, s, n, m, kParts ? sums_of[slot & 1] : kUnitSum ? P[n][m] : acc[n][m]);
+            for (int s = 0; s < STEPS; ++s) multiply(set, s, n, m, kParts ? sums_of[slot & 1] : acc[n][m]);
             // the second column tile of this block in the first half of the slots, the first one of the next block in the other
             auto decode_block = [&](auto j, auto i, int tile, int share, const typename F::Scale(&scales)[NT]) {
                 constexpr int S0 = STEPS * decltype(i)::value;
@@ -284,7 +254,11 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
         if constexpr (J == 0) load_scales(next, u + 1);
         if constexpr (J == 2 && FMT == kFmtQ4_K) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) sum[m] = *reinterpret_cast<const eh8*>(sums[m] + 32 * u);
+            for (int m = 0; m < MT; ++m) {
+                uint32_t row = sums[m];
+                asm volatile("" : "+v"(row));
+                sum[m] = *reinterpret_cast<const eh8*>(a.sums + 32 * static_cast<uint64_t>(row + u) + 16 * h);
+            }
         }
         copy(4 * u + J + 2);
         run_block(stage, Int<BLOCKS - 1>{}, u, s, J == 3 ? next : s);
@@ -305,9 +279,9 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
         run_stage(Int<1>{}, u, sc[0], sc[1]);
         run_stage(Int<2>{}, u, sc[0], sc[1]);
         run_stage(Int<3>{}, u, sc[0], sc[1]);
-        if constexpr (kUnitSum) {
+        if constexpr (FMT == kFmtQ4_K) {
             if (PAIR && part) sum[0] = eh8{};  // both parts of the sums go with the rows of hi
-            finish_unit<NT, MT>(sc[0], P, acc, [&](int m) { return sum[m]; });
+            subtract_minimums<NT, MT>(sc[0], acc, [&](int m) { return sum[m]; });
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) sc[0][n] = sc[1][n];
@@ -341,8 +315,14 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
 // ---- few tokens ---------------------------------------------------------------
 
 constexpr int kFewWaves = 8;
+// what few_kernel needs after its first loads
+struct FewRest {
+    float* out;
+    long ldx, ldo;
+    int N, K;
+};
 // LDS of a wave: rows of 1024 bytes (a unit's hi and lo, in the ring's order), 32 of sums and 4 of unscale
-__device__ __host__ inline int few_wave_bytes(int bm) { return bm * (1024 + 32) + 64; }
+__device__ __host__ constexpr int few_wave_bytes(int bm) { return bm * (1024 + 32) + 64; }
 
 // Eight activations of a row's unit (lane group of 32: one row) to their chunk of hi and lo, the row's sums over 32 and
 // its unscale; the whole wave calls it.
@@ -385,76 +365,156 @@ __device__ __forceinline__ void few_convert(const f32x4& x, const f32x4& y, bool
     if (c == 0) us[r] = ldexpf(1.0f, ex);
 }
 
-// Workgroup of `waves` waves; wave w takes units w, w + waves, ...; bm rows a tile (1 .. 16).
-template <int FMT, bool SWIGLU>
-__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const ProductArgs a, int bm, int waves) {
+// A stage (64 k) of NT column tiles against paired rows, of which lanes keep the first KEEP of registers 0 .. 3 (rows e_row(i) + 4 h;
+// the second part's are 8 registers on): r += the scaled sums, with kNoScale t += the sums.  a(step): an activation operand.
+template <class F, int J, int NT, int KEEP, class A>
+__device__ __forceinline__ void few_stage(const typename F::Quant (&q)[NT], const typename F::Scale (&s)[NT], float (&r)[NT][KEEP],
+                                          ef16 (&whole)[NT], A&& a) {
+    auto block = [&](auto blk) {
+        constexpr int I = decltype(blk)::value;  // of the stage
+        const eh8 x[2] = {a(2 * I), a(2 * I + 1)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            uint32_t b[2][4];
+            F::template operand<J, 2 * I>(q[n], s[n], b[0]);
+            F::template operand<J, 2 * I + 1>(q[n], s[n], b[1]);
+            auto scale = [&](float d, const ef16& t) {
+#pragma unroll
+                for (int i = 0; i < KEEP; ++i) r[n][i] = __builtin_fmaf(d, t[i] + t[i + 8], r[n][i]);
+            };
+            if constexpr (F::kScaled == kPerBlock) {
+                scale(F::template part_scale<2 * J + I>(s[n]), e_mfma(x[1], b[1], e_mfma(x[0], b[0], ef16{})));
+            } else if constexpr (F::kScaled == kPerStep) {
+                scale(F::template part_scale<4 * J + 2 * I>(s[n]), e_mfma(x[0], b[0], ef16{}));
+                scale(F::template part_scale<4 * J + 2 * I + 1>(s[n]), e_mfma(x[1], b[1], ef16{}));
+            } else {
+                whole[n] = e_mfma(x[1], b[1], e_mfma(x[0], b[0], whole[n]));
+            }
+        }
+    };
+    block(Int<0>{});
+    block(Int<1>{});
+}
+
+// A unit of NT column tiles times the rows that few_convert has left in the wave's area, up to 8 (lane rows from `count` on: the
+// last again, unused): r[n][i], times the row's unscale, is the product of row i + 4 h.
+template <int FMT, int NT, int KEEP>
+__device__ __forceinline__ void few_multiply(const typename ExpertFmt<FMT>::Quant (&q)[4][NT],
+                                             const typename ExpertFmt<FMT>::Scale (&sc)[NT], const char* area,
+                                             const char* sums, int count, float (&r)[NT][KEEP]) {
+    typedef ExpertFmt<FMT> F;
+    const int lane = threadIdx.x & 63, h = lane >> 5, part = 8 * ((lane >> 4) & 1), row = min(lane & 15, count - 1);
+    auto reader = [&](int j) {
+        const char* at = area + row * 1024 + 256 * j;
+        return [=](int s) { return *reinterpret_cast<const eh8*>(at + 16 * ((2 * s + h + part) ^ (row & 15))); };
+    };
+    ef16 whole[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        if constexpr (F::kScaled == kNoScale) whole[n] = ef16{};
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) r[n][i] = 0.0f;
+    }
+    few_stage<F, 0, NT, KEEP>(q[0], sc, r, whole, reader(0));
+    few_stage<F, 1, NT, KEEP>(q[1], sc, r, whole, reader(1));
+    few_stage<F, 2, NT, KEEP>(q[2], sc, r, whole, reader(2));
+    few_stage<F, 3, NT, KEEP>(q[3], sc, r, whole, reader(3));
+    if constexpr (F::kScaled == kNoScale) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i) r[n][i] = whole[n][i] + whole[n][i + 8];
+    }
+    if constexpr (FMT == kFmtQ4_K) {
+        eh8 x = *reinterpret_cast<const eh8*>(sums + row * 32 + 16 * h);
+        if (part) x = eh8{};  // both parts of the sums go with the rows of hi
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            uint32_t b[4];
+            F::min_operand(sc[n], b);
+            const ef16 t = e_mfma(x, b, ef16{});
+            const float dmin = F::min_scale(sc[n]);
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i) r[n][i] = __builtin_fmaf(dmin, t[i], r[n][i]);
+        }
+    }
+}
+
+// what one lane wrote to the wave's LDS, others read: in order, and not to be reordered
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Workgroup of `waves` waves; wave w takes units w, w + waves, ...; up to 2^lg rows a tile (KEEP 1:
+// one, 4: 1 .. 8).  The arguments that the
+// first loads need come first and plain: those are preloaded into SGPRs.
+template <int FMT, bool SWIGLU, int KEEP>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const int* offsets, const int* rows, const uint8_t* w0, const uint8_t* w1,
+                                                             const float* x, int E, int R, int k, int lg_waves, int tiles, int depth,
+                                                             const FewRest rest) {
     typedef ExpertFmt<FMT> F;
     constexpr int NT = SWIGLU ? 2 : 1, kUnit = unit_bytes(FMT);
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int lane = threadIdx.x & 63, h = lane >> 5, lg = lg_waves & 3, waves = lg_waves >> 2;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Tile t;
-    if (!find_tile(a.g, bm, a.tiles, blockIdx.x, t)) return;
-    char* const area = lds + wave * few_wave_bytes(bm);
-    char* const sums = area + bm * 1024;
-    float* const us = reinterpret_cast<float*>(sums + bm * 32);
-    const uint8_t* base[NT];
+    if (!find_tile(Groups{offsets, nullptr, nullptr, E, k, R}, lg, tiles, blockIdx.x, t)) return;
+    // a row for each half of the wave and pass, eight of its activations a lane
+    constexpr int PASSES = KEEP;
+    int source[PASSES];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) base[n] = a.w[n] + (static_cast<long>(t.expert) * a.tiles + t.block) * a.depth * static_cast<long>(kUnit);
-
-    const int lrow = lane & 15, part = 8 * ((lane >> 4) & 1);
-    const int row = min(lrow, t.count - 1), rowx = row & 15;
-    ef16 acc[NT][1] = {};
-    for (int u = wave; u < a.depth; u += waves) {
+    for (int i = 0; i < PASSES; ++i) {
+        const int r = t.first + min(2 * i + h, t.count - 1);
+        source[i] = k > 0 ? rows[r] : r;  // (k 0: rows of x in grouped order)
+    }
+    const long first_unit = (static_cast<long>(t.expert) * tiles + t.block) * depth;
+    char* const area = lds + wave * few_wave_bytes(1 << lg);
+    char* const sums = area + (1024 << lg);
+    float* const us = reinterpret_cast<float*>(sums + (32 << lg));
+    float acc[NT][KEEP] = {};
+    for (int u = wave; u < depth; u += waves) {
+        // Loads arrive in order: half of the weights, the activations (whose rows had to be looked up), the other half, so that
+        // the activations are converted while weights are on their way.
         typename F::Quant q[4][NT];
         typename F::Scale sc[NT];
+        f32x4 lo[PASSES], hi[PASSES];
+        const uint8_t* const unit[2] = {w0 + (first_unit + u) * kUnit, w1 + (first_unit + u) * kUnit};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const uint8_t* unit = base[n] + u * static_cast<long>(kUnit);
-            F::load(sc[n], unit, lane);
+        for (int n = 0; n < NT; ++n) F::load(sc[n], unit[n], lane);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) F::load(q[j][n], unit, j, lane);
-        }
-        // a row for each half of the wave, eight activations a lane; values from K on are zero
-        const int k = u * kUnitK + 8 * (lane & 31);
-        for (int r0 = 0; r0 < t.count; r0 += 2) {
-            const int r = r0 + h;
-            const bool live = r < t.count;
-            f32x4 x = f32x4{0, 0, 0, 0}, y = x;
-            if (live && k < a.K) {
-                const float* p = a.x + source_row(a, t.first + r) * a.ldx + k;
-                x = ld_f32x4(p);
-                y = ld_f32x4(p + 4);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) F::load(q[j][n], unit[n], j, lane);
+        const int c = u * kUnitK + 8 * (lane & 31);
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            lo[i] = hi[i] = f32x4{0, 0, 0, 0};
+            if (2 * i < t.count && c < rest.K) {
+                const float* p = x + (k > 0 ? clamp_int(source[i], 0, R - 1) / k : source[i]) * rest.ldx + c;
+                lo[i] = ld_f32x4(p);
+                hi[i] = ld_f32x4(p + 4);
             }
-            few_convert(x, y, live, r, area, sums, us);
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        ef16 p[NT][1] = {};
-        auto reader = [&](int j) {
-            const char* at = area + row * 1024 + 256 * j;
-            return [=](int s) { return *reinterpret_cast<const eh8*>(at + 16 * ((2 * s + h + part) ^ rowx)); };
-        };
-        multiply_stage<F, 0, NT>(q[0], sc, p, reader(0));
-        multiply_stage<F, 1, NT>(q[1], sc, p, reader(1));
-        multiply_stage<F, 2, NT>(q[2], sc, p, reader(2));
-        multiply_stage<F, 3, NT>(q[3], sc, p, reader(3));
-        if constexpr (F::kScaled == kPerUnit) {
-            eh8 x = *reinterpret_cast<const eh8*>(sums + row * 32 + 16 * h);
-            if (part) x = eh8{};
-            ef16 r[NT][1] = {};
-            finish_unit<NT, 1>(sc, p, r, [&](int) { return x; });
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) p[n][0] = r[n][0];
+        for (int j = 2; j < 4; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) F::load(q[j][n], unit[n], j, lane);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i)
+            if (2 * i < t.count) few_convert(lo[i], hi[i], 2 * i + h < t.count, 2 * i + h, area, sums, us);
+        wave_order();
+        float p[NT][KEEP];
+        few_multiply<FMT, NT, KEEP>(q, sc, area, sums, t.count, p);
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) {
+            const float f = us[min(i + 4 * h, t.count - 1)];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][i] = __builtin_fmaf(f, p[n][i], acc[n][i]);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float f = us[min(e_row(i) + 4 * h, t.count - 1)];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][0][i] = __builtin_fmaf(f, p[n][0][i] + p[n][0][i + 8], acc[n][0][i]);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
     }
     // the waves' sums, in their order
     __syncthreads();
@@ -462,18 +522,71 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const ProductArgs a
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) red[((wave * NT + n) * 16 + e_row(i) + 4 * h) * 32 + (lane & 31)] = acc[n][0][i];
+        for (int i = 0; i < KEEP; ++i) red[((wave * NT + n) * 8 + i + 4 * h) * 32 + (lane & 31)] = acc[n][i];
     __syncthreads();
-    const int some = min(waves, a.depth);
     for (int o = threadIdx.x; o < t.count * 32; o += 64 * waves) {
         float v[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            v[n] = red[n * 512 + o];
-            for (int w = 1; w < some; ++w) v[n] += red[(w * NT + n) * 512 + o];
+            v[n] = red[n * 256 + o];
+            for (int w = 1; w < waves; ++w) v[n] += red[(w * NT + n) * 256 + o];
         }
         const int col = t.block * kUnitCols + (o & 31);
-        if (col < a.N) a.out[static_cast<long>(t.first + (o >> 5)) * a.ldo + col] = SWIGLU ? silu_f(v[0]) * v[NT - 1] : v[0];
+        if (col < rest.N) rest.out[static_cast<long>(t.first + (o >> 5)) * rest.ldo + col] = SWIGLU ? silu_f(v[0]) * v[NT - 1] : v[0];
+    }
+}
+
+// The weighted sum for a token or two in one launch: a workgroup of 16 waves takes a token and a tile of 32 columns, its waves
+// the units of all of the token's choices (unit i: choice i / depth), each unit's products times the choice's weight.
+template <int FMT>
+__global__ __launch_bounds__(1024) void token_kernel(const ProductArgs a, const TokenArgs b) {
+    typedef ExpertFmt<FMT> F;
+    constexpr int WAVES = 16, kUnit = unit_bytes(FMT);
+    __shared__ __attribute__((aligned(16))) char lds[WAVES * few_wave_bytes(1)];
+    __shared__ float red[WAVES][32];
+    const int lane = threadIdx.x & 63, h = lane >> 5, k = a.g.k;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tile = blockIdx.x, t = blockIdx.y;
+    char* const area = lds + wave * few_wave_bytes(1);
+    char* const sums = area + 1024;
+    float* const us = reinterpret_cast<float*>(sums + 32);
+    float acc = 0.0f;  // lanes below 32: column tile * 32 + lane
+    for (int i = wave; i < k * a.depth; i += WAVES) {
+        const int j = i / a.depth, u = i - j * a.depth;
+        const int slot = __builtin_amdgcn_readfirstlane(a.g.slots[t * k + j]);
+        if (slot < 0 || slot >= a.g.R) continue;
+        int e = 0;  // the slot's expert: how many end at or before it
+        for (int e0 = 0; e0 < a.g.E; e0 += 64) e += __popcll(__ballot(e0 + lane < a.g.E && a.g.offsets[e0 + lane + 1] <= slot));
+        e = min(e, a.g.E - 1);
+        const uint8_t* unit = a.w[0] + ((static_cast<long>(e) * a.tiles + tile) * a.depth + u) * static_cast<long>(kUnit);
+        typename F::Quant q[4][1];
+        typename F::Scale sc[1];
+        const int c = u * kUnitK + 8 * (lane & 31);
+        f32x4 lo = f32x4{0, 0, 0, 0}, hi = lo;
+        if (c < a.K) {
+            const float* p = a.x + slot * a.ldx + c;
+            lo = ld_f32x4(p);
+            hi = ld_f32x4(p + 4);
+        }
+        F::load(sc[0], unit, lane);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) F::load(q[s][0], unit, s, lane);
+        few_convert(lo, hi, h == 0, 0, area, sums, us);
+        wave_order();
+        float p[1][1];
+        few_multiply<FMT, 1, 1>(q, sc, area, sums, 1, p);
+        acc = __builtin_fmaf(b.weights[t * k + j] * us[0], p[0][0], acc);
+        wave_order();
+    }
+    if (h == 0) red[wave][lane] = acc;
+    __syncthreads();
+    const int col = tile * kUnitCols + threadIdx.x;
+    if (threadIdx.x < 32 && col < a.N) {
+        float v = red[0][threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v += red[w][threadIdx.x];
+        if (b.residual != nullptr) v += b.residual[t * b.ldr + col];
+        a.out[t * a.ldo + col] = v;
     }
 }
 
@@ -488,29 +601,20 @@ void expert_rows(const ProductArgs& a, bool swiglu, int bm, long workgroups, hip
     hipLaunchKernelGGL(run, dim3(static_cast<unsigned>(workgroups)), dim3(256), 0, stream, a);
 }
 
-template <int FMT, bool SWIGLU>
-int launch_few(const ProductArgs& a, int bm, int waves, long workgroups, hipStream_t stream) {
-    const int lds = std::max(waves * few_wave_bytes(bm), waves * (SWIGLU ? 2 : 1) * 2048);
-    if (lds > 65536) {  // past the default limit, raised once per kernel and device
-        constexpr int kMaxDevices = 64;
-        static std::atomic<bool> ready[kMaxDevices];
-        int device = 0;
-        if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= kMaxDevices) return detail::kFailed;
-        if (!ready[device].load(std::memory_order_acquire)) {
-            if (hipFuncSetAttribute(reinterpret_cast<const void*>(&few_kernel<FMT, SWIGLU>),
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
-                return detail::kFailed;
-            ready[device].store(true, std::memory_order_release);
-        }
-    }
-    hipLaunchKernelGGL((few_kernel<FMT, SWIGLU>), dim3(static_cast<unsigned>(workgroups)), dim3(64 * waves), lds, stream, a, bm,
-                       waves);
-    return 0;
-}
 template <int FMT>
-int expert_few(const ProductArgs& a, bool swiglu, int bm, int waves, long workgroups, hipStream_t stream) {
-    return swiglu ? launch_few<FMT, true>(a, bm, waves, workgroups, stream)
-                  : launch_few<FMT, false>(a, bm, waves, workgroups, stream);
+void expert_few(const ProductArgs& a, bool swiglu, int lg, int waves, long workgroups, hipStream_t stream) {
+    const int lds = std::max(waves * few_wave_bytes(1 << lg), waves * (swiglu ? 2 : 1) * 1024);
+    const FewRest rest{a.out, a.ldx, a.ldo, a.N, a.K};
+    const auto run = swiglu ? (lg == 0 ? few_kernel<FMT, true, 1> : few_kernel<FMT, true, 4>)
+                            : (lg == 0 ? few_kernel<FMT, false, 1> : few_kernel<FMT, false, 4>);
+    hipLaunchKernelGGL(run, dim3(static_cast<unsigned>(workgroups)),
+                       dim3(64 * waves), lds, stream, a.g.offsets, a.g.rows, a.w[0], a.w[1], a.x, a.g.E, a.g.R,
+                       a.gather ? a.g.k : 0, lg | waves << 2, a.tiles, a.depth, rest);
+}
+
+template <int FMT>
+void expert_token(const ProductArgs& a, const TokenArgs& b, int tokens, hipStream_t stream) {
+    hipLaunchKernelGGL(token_kernel<FMT>, dim3(a.tiles, tokens), dim3(1024), 0, stream, a, b);
 }
 
 }  // namespace dev

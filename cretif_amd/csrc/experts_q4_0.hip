@@ -5,7 +5,8 @@ namespace cri {
 namespace dev {
 
 template void expert_rows<kFmtQ4_0>(const ProductArgs&, bool, int, long, hipStream_t);
-template int expert_few<kFmtQ4_0>(const ProductArgs&, bool, int, int, long, hipStream_t);
+template void expert_few<kFmtQ4_0>(const ProductArgs&, bool, int, int, long, hipStream_t);
+template void expert_token<kFmtQ4_0>(const ProductArgs&, const TokenArgs&, int, hipStream_t);
 
 }  // namespace dev
 }  // namespace cri
