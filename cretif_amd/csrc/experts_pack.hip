@@ -1,6 +1,6 @@
 // experts_pack.hip -- GGUF blocks [E, N, K] laid out once for the products of a layer of experts (experts.hpp says how),
 // each weight's own bits moved to where the lane that multiplies it finds them; rows from N on and values from K on are
-// weights of zero.  Runs once per matrix: 64 x 1024 x 2048 Q4_K (75 MB) takes 0.2 ms.
+// weights of zero.  Runs once per matrix.
 #include "decode.hpp"
 #include "experts.hpp"
 
@@ -44,21 +44,44 @@ __device__ __forceinline__ uint32_t code(const uint8_t* row, int k) {
 // nibble j of a step's dword (experts.hpp)
 __device__ constexpr int kNibbleAt[8] = {0, 16, 4, 20, 8, 24, 12, 28};
 
-// A wave per unit: lane (n, h) writes its own quants, lanes below 32 the scales of column n.
+constexpr int run_bytes(int fmt) { return kUnitK / (fmt == kFmtQ4_K || fmt == kFmtQ6_K ? 256 : fmt == kFmtF16 ? 1 : 32) * (fmt == kFmtQ8_0 ? 34 : fmt == kFmtQ4_0 ? 18 : fmt == kFmtQ5_0 ? 22 : fmt == kFmtQ4_K ? 144 : fmt == kFmtQ6_K ? 210 : 2); }
+
+// A wave per unit: its 32 rows' bytes go to LDS, two at a time over consecutive lanes (a block begins at any even address), then
+// lane (n, h) writes its own quants, lanes below 32 the scales of column n.
 template <int FMT>
 __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
-    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
-    const long u = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (u >= a.units) return;
-    const long per = static_cast<long>(a.tiles) * a.depth, e = u / per, in = u - e * per;
+    constexpr int kRun = run_bytes(FMT);  // bytes of a row in a unit
+    __shared__ __attribute__((aligned(4))) uint8_t lds[4][FMT == kFmtF16 ? 4 : kUnitCols * kRun];  // (FP16: straight from memory)
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, wave = threadIdx.x >> 6;
+    const long u = static_cast<long>(blockIdx.x) * 4 + wave;
+    const bool there = u < a.units;
+    const long per = static_cast<long>(a.tiles) * a.depth, e = there ? u / per : 0, in = there ? u - e * per : 0;
     const int tile = static_cast<int>(in / a.depth), k0 = static_cast<int>(in - static_cast<long>(tile) * a.depth) * kUnitK;
-    const int col = tile * kUnitCols + n;
-    const bool real = col < a.N;
-    const uint8_t* row = a.src + (e * a.N + (real ? col : 0)) * a.row_bytes;
+    const long start = static_cast<long>(k0 / kUnitK) * kRun;
+    const int rows = min(kUnitCols, a.N - tile * kUnitCols), bytes = static_cast<int>(min(static_cast<long>(kRun), a.row_bytes - start));
+    const uint8_t* from = a.src + (e * a.N + static_cast<long>(tile) * kUnitCols) * a.row_bytes + start;
+    if (there && FMT != kFmtF16) {
+        if ((reinterpret_cast<uintptr_t>(a.src) & 1) == 0) {  // (row_bytes is even)
+#pragma unroll 8
+            for (int i = lane; i < rows * (kRun / 2); i += 64) {
+                const int r = i / (kRun / 2), c = 2 * (i - r * (kRun / 2));
+                if (c < bytes) *reinterpret_cast<uint16_t*>(&lds[wave][r * kRun + c]) = *reinterpret_cast<const uint16_t*>(from + r * a.row_bytes + c);
+            }
+        } else {
+            for (int i = lane; i < rows * kRun; i += 64) {
+                const int r = i / kRun, c = i - r * kRun;
+                if (c < bytes) lds[wave][i] = from[r * a.row_bytes + c];
+            }
+        }
+    }
+    __syncthreads();
+    if (!there) return;
+    const bool real = n < rows;
+    const uint8_t* row = FMT == kFmtF16 ? from + (real ? n : 0) * a.row_bytes : &lds[wave][(real ? n : 0) * kRun];
     uint8_t* unit = a.dst + u * unit_bytes(FMT);
     auto at = [&](int i, int j) -> uint32_t {  // weight j of the lane's step i
-        const int k = k0 + 16 * i + 8 * h + j;
-        return real && k < a.K ? code<FMT>(row, k) : 0u;
+        const int k = 16 * i + 8 * h + j;
+        return real && k0 + k < a.K ? code<FMT>(row, k) : 0u;
     };
     if constexpr (FMT == kFmtF16) {
         for (int i = 0; i < 16; ++i) {
@@ -103,10 +126,10 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
         constexpr int size = FMT == kFmtQ8_0 ? 34 : FMT == kFmtQ4_0 ? 18 : 22;
         u32x4 d = u32x4{0, 0, 0, 0};
         for (int i = 0; i < 8; ++i)
-            if (real && k0 + 32 * i < a.K) d[i >> 1] |= half(row + ((k0 >> 5) + i) * size) << (16 * (i & 1));
+            if (real && k0 + 32 * i < a.K) d[i >> 1] |= half(row + i * size) << (16 * (i & 1));
         *reinterpret_cast<u32x4*>(unit + unit_bytes(FMT) - 512 + 16 * n) = d;
     } else if constexpr (FMT == kFmtQ4_K) {
-        const uint8_t* b = row + (k0 >> 8) * 144;
+        const uint8_t* b = row;
         u32x4 s = u32x4{0, 0, 0, 0};
         for (int i = 0; i < 8 && real; ++i) {
             const uint8_t* c = b + 4;
@@ -118,7 +141,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs a) {
         *reinterpret_cast<u32x4*>(unit + 4096 + 16 * n) = s;
         *reinterpret_cast<uint32_t*>(unit + 4608 + 4 * n) = real ? half(b) | (half(b + 2) << 16) : 0u;
     } else {
-        const uint8_t* b = row + (k0 >> 8) * 210;
+        const uint8_t* b = row;
         u32x4 s = u32x4{0, 0, 0, 0};
         for (int i = 0; i < 16 && real; ++i) s[i >> 2] |= static_cast<uint32_t>(b[192 + i]) << (8 * (i & 3));
         *reinterpret_cast<u32x4*>(unit + 6144 + 16 * n) = s;
