@@ -10,7 +10,8 @@
 // 64 at a time (the lanes of a wave with the same expert by one ballot per bit of its number).  Up to kSingle tokens one
 // workgroup does it all; more take two launches, the counts of at most kBlocks blocks between them, which every block of
 // the second adds up for itself.
-// Bound by the chain of launches, loads and reductions: one token of 128 experts, 8 chosen, 7 us; 8192 x 256 with a bias 34.
+// Bound by the chain of launches, loads and reductions: one token of 128 experts, 8 chosen, 4.9 us; 8192 of
+// 256 with a bias 17.2 us and 10.5 for the second launch.
 #include <algorithm>
 
 #include "common.hpp"
@@ -48,21 +49,74 @@ struct Shared {
     int totals[kWaves];
 };
 
-__device__ __forceinline__ double wave_max64(double v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = fmax(v, __shfl_xor(v, d));
-    return v;
+// v of the lane that a DPP control names, 0 where there is none
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lower(uint32_t v) {
+    return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false);
+}
+// The largest of the wave; into lane 63 over 1, 2, 4 and 8 lanes of a row, then row after row.
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+    v = max(v, lower<0x111, 0xF>(v));
+    v = max(v, lower<0x112, 0xF>(v));
+    v = max(v, lower<0x114, 0xF>(v));
+    v = max(v, lower<0x118, 0xF>(v));
+    v = max(v, lower<0x142, 0xA>(v));
+    v = max(v, lower<0x143, 0xC>(v));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double lower64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(lower<CTRL, ROWS>(static_cast<uint32_t>(u))) |
+                                          static_cast<uint64_t>(lower<CTRL, ROWS>(static_cast<uint32_t>(u >> 32))) << 32);
 }
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
+    v += lower64<0x111, 0xF>(v);
+    v += lower64<0x112, 0xF>(v);
+    v += lower64<0x114, 0xF>(v);
+    v += lower64<0x118, 0xF>(v);
+    v += lower64<0x142, 0xA>(v);
+    v += lower64<0x143, 0xC>(v);
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u), 63))) |
+                                          static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u >> 32), 63)))
+                                              << 32);
 }
-__device__ __forceinline__ float top_of(float v) { return wave_max(v); }
-__device__ __forceinline__ double top_of(double v) { return wave_max64(v); }
 
-// The choices of token t, by one wave; lane j returns choice j's expert, or -1.
-template <int C, class Key>
+// Numbers as unsigned integers of the same order, all above 0, which stands for what is never chosen.  (+0 and -0 are one.)
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v + 0.0f);
+    return u ^ (u >> 31 ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ uint64_t ordered(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
+    return u ^ (u >> 63 ? ~0ull : 1ull << 63);
+}
+
+// e^y to about 2^-52: y = n ln 2 + r with ln 2 in two parts, the series of e^r up to r^13 / 13! (|r| <= ln 2 / 2: the rest is below
+// 2^-57), times 2^n.  Fewer instructions than the library's exp, whose range reduction and special cases are not needed here.
+__device__ __forceinline__ double exp64(double y) {
+    y = fmin(fmax(y, -800.0), 800.0);  // beyond: 0 or infinity all the same
+    const double n = rint(y * 1.4426950408889634);
+    const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, y));
+    constexpr double kOver[] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320, 1.0 / 362880,
+                                1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600, 1.0 / 6227020800.0};
+    double p = kOver[13];
+#pragma unroll
+    for (int i = 12; i >= 0; --i) p = fma(p, r, kOver[i]);
+    return ldexp(p, static_cast<int>(n));
+}
+// 1 / d for d >= 1: the hardware's reciprocal and two steps of Newton's (past their range, and for infinity, a division)
+__device__ __forceinline__ double reciprocal(double d) {
+    if (d > 1e150) return 1.0 / d;
+    double r = __builtin_amdgcn_rcp(d);
+    r = fma(fma(-d, r, 1.0), r, r);
+    return fma(fma(-d, r, 1.0), r, r);
+}
+
+// The choices of token t, by one wave; lane j returns choice j's expert, or -1.  WIDE: with a bias, by scores of 64 bits, whose
+// upper halves are compared first and the lower ones only between equal upper ones.
+template <int C, bool WIDE>
 __device__ __forceinline__ int choose(const RouteArgs& a, int t) {
     const int lane = __lane_id();
     const float* z = a.logits + t * a.ldl;
@@ -78,52 +132,89 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int t) {
     for (int i = 1; i < C; ++i) best = fmaxf(best, x[i]);
     const float most = wave_max(best);
     // of all experts: softmax's sum, where anything needs it
-    const bool biased = sizeof(Key) == 8;
-    auto part = [&](float v) { return v == most ? 1.0 : exp(static_cast<double>(v) - most); };
+    auto part = [&](float v) { return v == most ? 1.0 : exp64(static_cast<double>(v) - most); };
     double all = 1.0;
-    if (!a.sigmoid && (biased || !a.normalize) && most > -INFINITY) {
+    if (!a.sigmoid && (WIDE || !a.normalize) && most > -INFINITY) {
         all = 0.0;
 #pragma unroll
         for (int i = 0; i < C; ++i) all += part(x[i]);
         all = wave_sum64(all);
     }
-    auto score = [&](float v) { return a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(v))) : part(v) / all; };
-    Key key[C];
+    const double over = 1.0 / all;
+    auto score = [&](float v) { return a.sigmoid ? reciprocal(1.0 + exp64(-static_cast<double>(v))) : part(v) * over; };
+    uint32_t high[C], low[WIDE ? C : 1] = {};
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-        if constexpr (sizeof(Key) == 8) {
-            const int e = lane * C + i;
-            const double s = x[i] > -INFINITY ? score(x[i]) + a.bias[e] : -INFINITY;
-            key[i] = s == s ? s : -INFINITY;
+        if constexpr (WIDE) {
+            const int e = min(lane * C + i, a.E - 1);
+            const double s = score(x[i]) + a.bias[e];
+            const uint64_t u = x[i] > -INFINITY && s > -INFINITY ? ordered(s) : 0;  // (NaN is not above)
+            high[i] = static_cast<uint32_t>(u >> 32);
+            low[i] = static_cast<uint32_t>(u);
         } else {
-            key[i] = x[i];
+            high[i] = x[i] > -INFINITY ? ordered(x[i]) : 0;
+        }
+    }
+    // Up to four a lane are sorted once (neighbours exchanged where the later one is larger, so equal ones keep their order):
+    // the lane's largest is then always the first, and a chosen one leaves by a shift.  More are searched each time.
+    constexpr bool SORTED = C <= 4;
+    int place[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) place[i] = i;
+    if constexpr (SORTED) {
+#pragma unroll
+        for (int round = 0; round < C; ++round) {
+#pragma unroll
+            for (int i = round & 1; i + 1 < C; i += 2) {
+                const bool more = high[i + 1] > high[i] || (WIDE && high[i + 1] == high[i] && low[WIDE ? i + 1 : 0] > low[WIDE ? i : 0]);
+                const auto exchange = [&](auto& p, auto& q) {
+                    const auto was = p;
+                    p = more ? q : p;
+                    q = more ? was : q;
+                };
+                exchange(high[i], high[i + 1]);
+                exchange(place[i], place[i + 1]);
+                if constexpr (WIDE) exchange(low[i], low[i + 1]);
+            }
         }
     }
     int mine = -1;
-    float value = 0.0f;
     for (int j = 0; j < a.k; ++j) {
-        Key b = key[0];
-        int at = 0;
-        float v = x[0];
+        uint32_t h = high[0], l = low[0];
+        int at = place[0];
+        if constexpr (!SORTED) {
 #pragma unroll
-        for (int i = 1; i < C; ++i) {
-            const bool more = key[i] > b;
-            b = more ? key[i] : b;
-            at = more ? i : at;
-            v = more ? x[i] : v;
+            for (int i = 1; i < C; ++i) {
+                const bool more = high[i] > h || (WIDE && high[i] == h && low[WIDE ? i : 0] > l);
+                h = more ? high[i] : h;
+                if (WIDE) l = more ? low[WIDE ? i : 0] : l;
+                at = more ? i : at;
+            }
         }
-        const Key top = top_of(b);
-        if (!(top > static_cast<Key>(-INFINITY))) break;
-        const int who = __builtin_ctzl(__ballot(b == top));
+        const uint32_t top = wave_top(h);
+        if (top == 0) break;
+        unsigned long same = __ballot(h == top);
+        if (WIDE && (same & (same - 1)) != 0) {
+            const uint32_t rest = wave_top(h == top ? l : 0);
+            same = __ballot(h == top && l == rest);
+        }
+        const int who = __builtin_ctzl(same);
         const int expert = who * C + __builtin_amdgcn_readlane(at, who);
-        const float logit = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), who));
-        if (lane == j) {
-            mine = expert;
-            value = logit;
-        }
+        mine = lane == j ? expert : mine;
+        const bool gone = lane == who;
+        if constexpr (SORTED) {
 #pragma unroll
-        for (int i = 0; i < C; ++i) key[i] = lane == who && i == at ? static_cast<Key>(-INFINITY) : key[i];
+            for (int i = 0; i < C; ++i) {
+                high[i] = gone ? (i + 1 < C ? high[i + 1 < C ? i + 1 : i] : 0) : high[i];
+                if (i + 1 < C) place[i] = gone ? place[i + 1 < C ? i + 1 : i] : place[i];
+                if (WIDE && i + 1 < C) low[WIDE ? i : 0] = gone ? low[WIDE && i + 1 < C ? i + 1 : 0] : low[WIDE ? i : 0];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < C; ++i) high[i] = gone && i == at ? 0 : high[i];
+        }
     }
+    const float value = mine >= 0 ? z[mine] : 0.0f;
     double w = mine >= 0 ? score(value) : 0.0;
     if (a.normalize) {
         const double sum = wave_sum64(w);
@@ -209,7 +300,7 @@ __device__ __forceinline__ void write_rest(const RouteArgs& a, int all, int bloc
 }
 
 // Chooses (with logits) and counts the block's pairs; a single block groups them, too.
-template <int C, class Key>
+template <int C, bool WIDE>
 __global__ __launch_bounds__(kThreads) void route_kernel(const RouteArgs a) {
     __shared__ Shared s;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -218,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteArgs a) {
     const int t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.M);
     if (a.logits != nullptr) {
         for (int t = t0 + wave; t < t1; t += kWaves) {
-            const int e = choose<C, Key>(a, t);
+            const int e = choose<C, WIDE>(a, t);
             if (lane < a.k && e >= 0) atomicAdd(&s.count[e], 1);
         }
     } else {
@@ -255,10 +346,15 @@ __global__ __launch_bounds__(kThreads) void group_kernel(const RouteArgs a, int 
     const int each = (blocks + shares - 1) / shares, b0 = share * each, b1 = min(b0 + each, blocks);
     int total = 0, before = 0;
     if (e < a.E) {
-        for (int b = b0; b < b1; ++b) {
-            const int n = a.counts[static_cast<long>(b) * a.E + e];
-            total += n;
-            before += b < block ? n : 0;
+        for (int b = b0; b < b1; b += 16) {
+            int n[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) n[i] = a.counts[static_cast<long>(min(b + i, b1 - 1)) * a.E + e];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                total += b + i < b1 ? n[i] : 0;
+                before += b + i < min(b1, block) ? n[i] : 0;
+            }
         }
     }
     s.parts[0][tid] = total;
@@ -291,17 +387,17 @@ void launch(RouteArgs a, hipStream_t stream) {
     const int blocks = std::max((a.M + a.per - 1) / a.per, 1);
     const bool biased = a.logits != nullptr && a.bias != nullptr;
     const int c = (a.E + 63) / 64;
-    const auto run = a.logits == nullptr ? route_kernel<1, float>
-                     : biased            ? (c == 1   ? route_kernel<1, double>
-                                            : c == 2 ? route_kernel<2, double>
-                                            : c <= 4 ? route_kernel<4, double>
-                                            : c <= 8 ? route_kernel<8, double>
-                                                     : route_kernel<16, double>)
-                                         : (c == 1   ? route_kernel<1, float>
-                                            : c == 2 ? route_kernel<2, float>
-                                            : c <= 4 ? route_kernel<4, float>
-                                            : c <= 8 ? route_kernel<8, float>
-                                                     : route_kernel<16, float>);
+    const auto run = a.logits == nullptr ? route_kernel<1, false>
+                     : biased            ? (c == 1   ? route_kernel<1, true>
+                                            : c == 2 ? route_kernel<2, true>
+                                            : c <= 4 ? route_kernel<4, true>
+                                            : c <= 8 ? route_kernel<8, true>
+                                                     : route_kernel<16, true>)
+                                         : (c == 1   ? route_kernel<1, false>
+                                            : c == 2 ? route_kernel<2, false>
+                                            : c <= 4 ? route_kernel<4, false>
+                                            : c <= 8 ? route_kernel<8, false>
+                                                     : route_kernel<16, false>);
     hipLaunchKernelGGL(run, dim3(blocks), dim3(kThreads), 0, stream, a);
     if (blocks > 1) hipLaunchKernelGGL(group_kernel, dim3(blocks), dim3(kThreads), 0, stream, a, blocks);
 }
