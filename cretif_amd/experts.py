@@ -57,9 +57,9 @@ def _bytes(n):
 
 class ExpertWeights:
     """A matrix per expert, laid out once for the products: raw, a uint8 device tensor that holds the
-    GGUF blocks of [n_experts, N, K] (not needed afterwards).  Runs on stream, by default the current one."""
+    GGUF blocks of [n_experts, N, K] (not needed afterwards).  Runs on the current stream, to which its memory belongs."""
 
-    def __init__(self, fmt, raw, n_experts, N, K, stream=None):
+    def __init__(self, fmt, raw, n_experts, N, K):
         L, dev = _torch(), _device()
         _in_32_bits(n_experts, N, K)
         need = _bytes(L.cri_expert_packed_bytes(FORMAT_IDS[fmt], n_experts, N, K))
@@ -68,7 +68,7 @@ class ExpertWeights:
         src = _on_device(raw, "raw", dev)
         self.data = torch.empty(need, dtype=torch.uint8, device=raw.device)
         self.format, self.n_experts, self.N, self.K = fmt, n_experts, N, K
-        _check(L.cri_expert_pack(FORMAT_IDS[fmt], src, n_experts, N, K, self.data.data_ptr(), _on(stream, dev)))
+        _check(L.cri_expert_pack(FORMAT_IDS[fmt], src, n_experts, N, K, self.data.data_ptr(), _on(None, dev)))
         self._c = _ExpertWeights(self.data.data_ptr(), FORMAT_IDS[fmt], n_experts, N, K)
         self._ref = ctypes.addressof(self._c)
         self._dev = dev

@@ -474,3 +474,77 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for layer, want in zip(layers, alone):
         assert torch.equal(layer.out, want)
+
+
+def test_python_refusals():
+    """What the tensors say before the library is called."""
+    E, N, K, M, k = 4, 32, 256, 3, 2
+    w = packed("q4_k", E, N, K)
+    raw = dev(matrix("q4_k", E, N, K)[0])
+    g = cri.ExpertGroups(M, k, E)
+    f = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    x, h, out, rows, ids, wts = f(M, K), f(M * k, K), f(M, N), f(M * k, N), i(M, k), f(M, k)
+    ws = torch.empty(1 << 16, dtype=torch.uint8, device="cuda")
+    with pytest.raises(KeyError):
+        cri.ExpertWeights("q3_k", raw, E, N, K)
+    with pytest.raises(KeyError):
+        cri.ExpertRouter("relu")
+    bad = [
+        lambda: cri.ExpertWeights("q4_k", raw[:-1], E, N, K),
+        lambda: cri.ExpertWeights("q4_k", raw.view(torch.int8), E, N, K),
+        lambda: cri.ExpertWeights("q4_k", raw.cpu(), E, N, K),
+        lambda: cri.ExpertWeights("q4_k", raw, E, N, 1 << 40),
+        lambda: cri.ExpertGroups(M, k, E, offsets=i(E)),
+        lambda: cri.ExpertGroups(M, k, E, rows=i(M * k).long()),
+        lambda: cri.ExpertGroups(M, k, E, slots=i(M * k).cpu()),
+        lambda: cri.ExpertGroups(-1, k, E),
+        lambda: cri.ExpertRouter(bias=f(E).half()),
+        lambda: cri.ExpertRouter(bias=f(2 * E)[::2]),
+        lambda: cri.route_experts(cri.ExpertRouter(bias=f(E + 1)), f(M, E), ids, wts, g),
+        lambda: cri.route_experts(cri.ExpertRouter(), f(M, E + 1), ids, wts, g),
+        lambda: cri.route_experts(cri.ExpertRouter(), f(M, E).half(), ids, wts, g),
+        lambda: cri.route_experts(cri.ExpertRouter(), f(M, E), ids.long(), wts, g),
+        lambda: cri.route_experts(cri.ExpertRouter(), f(M, E), ids, f(k, M).t(), g),
+        lambda: cri.group_experts(i(M, k + 1), g),
+        lambda: cri.group_experts(ids.cpu(), g),
+        lambda: cri.expert_matmul(w, g, h, rows),
+        lambda: cri.expert_matmul(w, g, x, rows, grouped=True),
+        lambda: cri.expert_matmul(w, g, x, out),
+        lambda: cri.expert_matmul(w, g, x, f(M * k, N + 1)),
+        lambda: cri.expert_matmul(w, g, x.cpu(), rows),
+        lambda: cri.expert_matmul(w, g, x, rows, ws[::2]),
+        lambda: cri.expert_swiglu(w, w, g, x.double(), rows),
+        lambda: cri.expert_combine(w, g, h, wts[:-1], out),
+        lambda: cri.expert_combine(w, g, h, wts, out, residual=f(M + 1, N)),
+        lambda: cri.expert_combine(w, g, x, wts, out),
+    ]
+    for n, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail("call %d was not refused" % n)
+    with pytest.raises(RuntimeError):
+        cri.expert_matmul(w, cri.ExpertGroups(M, k, E + 1), x, rows)
+    with pytest.raises(RuntimeError):
+        cri.expert_swiglu(w, packed("q8_0", E, N, K), g, x, rows)
+    with pytest.raises(RuntimeError):
+        cri.expert_combine(w, g, h, wts, out, residual=f(M + 1, N)[1:].as_strided((M, N), (0, 1)))
+
+
+def test_layer_of_a_padded_batch():
+    """Rows of logits -infinity are nobody's: no work, weights 0, the residual alone comes out."""
+    layer = Layer(40)
+    x = randn(layer.M, layer.dim, seed=3)
+    layer.x.copy_(dev(x))
+    layer.run()
+    full, slots = layer.out.clone(), layer.g.slots.clone()
+    pad = torch.arange(layer.M, device="cuda") % 4 == 3
+    layer.logits[pad] = float("-inf")
+    cri.route_experts(layer.router, layer.logits, layer.ids, layer.weights, layer.g, layer.ws)
+    assert int(layer.g.offsets[-1]) == 30 * layer.k
+    layer.h.fill_(float("nan"))  # rows behind the last are neither written nor read
+    cri.expert_swiglu(layer.w[0], layer.w[1], layer.g, layer.x, layer.h, layer.ws)
+    assert torch.isnan(layer.h[30 * layer.k:]).all() and not torch.isnan(layer.h[:30 * layer.k]).any()
+    cri.expert_combine(layer.w[2], layer.g, layer.h, layer.weights, layer.out, layer.x, layer.ws)
+    assert torch.equal(layer.out[pad], layer.x[pad])
+    assert torch.equal(layer.out[~pad], full[~pad])
