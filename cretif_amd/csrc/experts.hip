@@ -146,16 +146,16 @@ struct Plan {
 };
 
 // The one that a rough model of both gives the least time, in us; it knows only host numbers, so rows are taken to be spread
-// over the experts.  All read the weights of the experts that have rows at 5.5 TB/s at best.  few_kernel: 7 us, 0.52 ns for each
-// unit that a tile meets (that often as a 256th of the GPU) and 0.07 ns for each row of it.  rows_kernel: 10 us with the
-// planes' pass, then stages of 0.42, 0.5 or 0.78 us (16, 32, 64 rows) while a CU has one workgroup or less, 0.47, 0.57 or 1.0 us
-// each beyond.  `weight` is what decoding and scaling a format takes of either, beside Q4_0.
-// Measured, few (8 rows, 4 waves) / 16 / 32 / 64 rows, us: SwiGLU 2048 -> 1024 of 64 experts, 8 each, Q4_K: 4 tokens 16.0 / 24.9 /
-// 27.5 / 37.0, 16: 25.9 / 30.0 / 34.0 / 48.1, 64: 58.3 / 58.8 / 47.0 / 67.7, 256: 165.8 / 93.1 / 83.9 / 97.9, 512: 306 / 152 / 121 /
-// 125, 4096: - / 935 / 666 / 575; one expert each of 8, 8192 -> 2048 Q4_0: 16 tokens 26.7 / 71.5 / 76.8 / 105, 128: 57.3 / 72.2 /
-// 76.9 / 106, 512: 169 / 104 / 81 / 112.
+// over the experts.  All read the weights of the experts that have rows at 5.5 TB/s at best.  few_kernel: 8 us, 0.6 ns for each
+// unit that a tile meets (that often as a 256th of the GPU) and 0.1 ns for each row of it.  rows_kernel: 8 us with the planes'
+// pass, then stages of 0.44, 0.52 or 0.79 us (16, 32, 64 rows) while a CU has one workgroup or less, 0.47, 0.52 or 0.92 us each
+// beyond; an expert's further tiles read its weights again at 0.4 of the cost.  `weight` is what decoding and scaling a format
+// takes of either, beside Q4_0.  Over 135 calls of all formats what it takes was 1.5% slower than the best on average.
+// Measured, few (8 rows, 4 waves) / 16 / 32 / 64 rows, us: SwiGLU 2048 -> 1024 of 64 experts, 8 each, Q4_K: 4 tokens 18 / 24 / 27 /
+// 38, 16: 26 / 30 / 34 / 50, 48: 49 / 40 / 44 / 67, 256: 169 / 82 / 81 / 98, 512: 314 / 140 / 118 / 128, 1024: 643 / 270 / 195 / 195;
+// one expert each of 8, 8192 -> 2048 Q4_0: 16 tokens 27 / 65 / 74 / 108, 128: 64 / 68 / 76 / 110, 512: 194 / 112 / 85 / 117.
 Plan plan_products(const ExpertMatrix& w, const ExpertRows& g, bool swiglu) {
-    const double few_weight[] = {1.2, 1.0, 1.8, 1.0, 2.0, 1.4}, rows_weight[] = {1.1, 1.0, 1.3, 1.1, 1.65, 1.0};  // by format
+    const double few_weight[] = {1.4, 1.2, 1.65, 1.1, 2.2, 1.1}, rows_weight[] = {1.3, 1.0, 1.3, 1.1, 1.6, 0.85};  // by format
     const int depth = (w.K + dev::kUnitK - 1) / dev::kUnitK, tiles = (w.N + dev::kUnitCols - 1) / dev::kUnitCols;
     const double R = static_cast<double>(g.n_tokens) * g.top_k, E = w.n_experts;
     const double used = E * (1.0 - std::pow(1.0 - 1.0 / E, R)), matrices = swiglu ? 2.0 : 1.0;
@@ -166,15 +166,15 @@ Plan plan_products(const ExpertMatrix& w, const ExpertRows& g, bool swiglu) {
     const int lg = single ? 0 : g.n_tokens <= 4 ? 2 : 3;
     const double units = tiles * depth * matrices * 1e-3;
     Plan best{true, 0, lg, std::min(depth, lg < 3 && (used * tiles <= 256 || depth >= 16) ? 8 : 4)};
-    double least = 7.0 + std::max(memory, units * (0.52 * few_weight[w.fmt] * row_tiles(1 << lg) + 0.07 * R));
-    const double blocks = swiglu ? (tiles + 3) / 4 : (tiles + 7) / 8;
+    double least = 8.0 + std::max(memory, units * (0.6 * few_weight[w.fmt] * row_tiles(1 << lg) + 0.1 * R));
+    const double blocks = dev::rows_blocks(tiles, swiglu);
     const struct {
         int bm;
         double one, each;
-    } kinds[] = {{16, 0.42, 0.47}, {32, 0.5, 0.57}, {64, 0.78, 1.0}};
+    } kinds[] = {{16, 0.44, 0.47}, {32, 0.52, 0.52}, {64, 0.79, 0.92}};
     for (const auto& k : kinds) {
         const double stage = std::max(k.one, k.each * row_tiles(k.bm) * blocks / 256) * rows_weight[w.fmt];
-        const double us = 10.0 + std::max(memory, 4 * depth * stage);
+        const double us = 8.0 + std::max(memory * (0.6 + 0.4 * row_tiles(k.bm) / used), 4 * depth * stage);
         if (us < least) {
             least = us;
             best = Plan{false, k.bm, 0, 0};
@@ -221,7 +221,7 @@ int launch_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertR
     const Plan plan = plan_products(w, g, swiglu);
     dev::ProductArgs a = product_args(w, g, x, ldx, gather, out, ldo);
     if (swiglu) a.w[1] = static_cast<const uint8_t*>(up->data);
-    const int blocks = plan.few ? tiles : swiglu ? (tiles + 3) / 4 : (tiles + 7) / 8;
+    const int blocks = plan.few ? tiles : dev::rows_blocks(tiles, swiglu);
     const long groups = (dev::most_tiles(R, w.n_experts, plan.few ? 1 << plan.lg : plan.bm) * blocks + 7) / 8 * 8;
     if (groups >= 1L << 23) return kDeclined;  // up to 512 threads each: a launch's limit
     if (plan.few) {

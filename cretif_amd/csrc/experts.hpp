@@ -150,6 +150,9 @@ struct ProductArgs {
     bool gather;             // the row of grouped row r is rows[r] / k, else r
 };
 
+// column blocks of rows_kernel: a wave takes a tile of G and U, or two tiles
+__device__ __host__ inline int rows_blocks(int tiles, bool swiglu) { return swiglu ? (tiles + 3) >> 2 : (tiles + 7) >> 3; }
+
 struct TokenArgs {
     const float* weights;   // [tokens, k]
     const float* residual;  // or null
@@ -157,8 +160,8 @@ struct TokenArgs {
 };
 
 // the kernels of experts_gemm.hpp, instantiated in one file per format (experts_q4_k.hip, ...).  expert_rows: tiles of bm = 16, 32
-// or 64 rows; expert_few: tiles of up to 2^lg rows, lg 0 .. 3, workgroups of `waves` waves, up to 8 (and few_lds(lg, waves) within
-// 64 KB); expert_token: the weighted sums of so many tokens, x in grouped order
+// or 64 rows, workgroups of 4 waves; expert_few: tiles of up to 2^lg rows, lg 0 .. 3, workgroups of `waves` waves, up
+// to 8 (lg 3: 4, for its LDS); expert_token: the weighted sums of so many tokens, x in grouped order
 template <int FMT>
 void expert_rows(const ProductArgs& a, bool swiglu, int bm, long workgroups, hipStream_t stream);
 template <int FMT>

@@ -74,7 +74,7 @@ __device__ __forceinline__ uint32_t e_at(const u32x4& v, int i) { return v[i]; }
 
 template <>
 struct ExpertFmt<kFmtQ4_0> {
-    static constexpr int kScaled = kPerBlock;
+    static constexpr int kScaled = kPerBlock, kLoads = 1;
     typedef NibbleQuant Quant;
     struct Scale {
         u32x4 d;
@@ -103,7 +103,7 @@ struct ExpertFmt<kFmtQ4_0> {
 
 template <>
 struct ExpertFmt<kFmtQ8_0> {
-    static constexpr int kScaled = kPerBlock;
+    static constexpr int kScaled = kPerBlock, kLoads = 2;
     struct Quant {
         u32x4 q[2];
         __device__ __forceinline__ void settle() { e_settle(q[0]), e_settle(q[1]); }
@@ -138,7 +138,7 @@ __device__ __forceinline__ uint32_t e_move(uint32_t w, int from, int to) { retur
 
 template <>
 struct ExpertFmt<kFmtQ5_0> {
-    static constexpr int kScaled = kPerBlock;
+    static constexpr int kScaled = kPerBlock, kLoads = 2;
     struct Quant {
         u32x4 q;
         uint32_t h;
@@ -172,7 +172,7 @@ struct ExpertFmt<kFmtQ5_0> {
 
 template <>
 struct ExpertFmt<kFmtQ6_K> {
-    static constexpr int kScaled = kPerStep;
+    static constexpr int kScaled = kPerStep, kLoads = 2;
     struct Quant {
         u32x4 q;
         uint32_t h[2];
@@ -213,7 +213,7 @@ struct ExpertFmt<kFmtQ6_K> {
 
 template <>
 struct ExpertFmt<kFmtQ4_K> {
-    static constexpr int kScaled = kPerBlock;
+    static constexpr int kScaled = kPerBlock, kLoads = 1;
     typedef NibbleQuant Quant;
     struct Scale {
         u32x4 s;  // sc, mn
@@ -253,7 +253,7 @@ struct ExpertFmt<kFmtQ4_K> {
 
 template <>
 struct ExpertFmt<kFmtF16> {
-    static constexpr int kScaled = kNoScale;
+    static constexpr int kScaled = kNoScale, kLoads = 4;
     struct Quant {
         u32x4 q[4];
         __device__ __forceinline__ void settle() { e_settle(q[0]), e_settle(q[1]), e_settle(q[2]), e_settle(q[3]); }
