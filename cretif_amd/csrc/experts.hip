@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "act.hpp"
 #include "experts.hpp"
 
 namespace cri {
@@ -82,13 +83,13 @@ __global__ __launch_bounds__(256) void planes_kernel(const PlanesArgs a) {
 // out[t] = residual[t] + sum over the token's choices, in their order, of weight * p[slot]; choices without an expert are
 // left out, whatever their weight.  Bound by memory: k + 2 rows per token.
 struct CombineArgs {
-    const float* p;  // [R, ldp], 16-byte aligned rows
+    const float* p;  // [splits][R, ldp], 16-byte aligned rows, to be added up
     const float* weights;
     const int* slots;
     const float* residual;  // or null
     float* out;
     long ldp, ldr, ldo;
-    int N, k, R;
+    int N, k, R, splits;
 };
 
 __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
@@ -115,7 +116,9 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
             const int j = min(j0 + i, a.k - 1), slot = slots[j];
             there[i] = j0 + i < a.k && slot >= 0 && slot < a.R;
             w[i] = weights[j];
-            v[i] = *reinterpret_cast<const f32x4*>(a.p + (there[i] ? slot : 0) * a.ldp + col);
+            const float* p = a.p + (there[i] ? slot : 0) * a.ldp + col;
+            v[i] = *reinterpret_cast<const f32x4*>(p);
+            for (int s = 1; s < a.splits; ++s) v[i] += *reinterpret_cast<const f32x4*>(p + s * (a.R * a.ldp));
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -133,29 +136,68 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
     }
 }
 
+// The parts of k of a product (SwiGLU: of both) added up in order: out[r], for the rows that have an expert.
+struct JoinArgs {
+    const float* p;  // [splits][matrices][R, ldp], 16-byte aligned rows
+    const int* end;
+    float* out;
+    long ldp, ldo;
+    int N, R, splits;
+};
+
+template <bool SWIGLU>
+__global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
+    constexpr int NT = SWIGLU ? 2 : 1;
+    const int r = blockIdx.x, col = (blockIdx.y * 256 + threadIdx.x) * 4;
+    if (col >= a.N || r >= *a.end) return;
+    const long part = a.R * a.ldp;
+    const float* p = a.p + r * a.ldp + col;
+    f32x4 v[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) v[n] = *reinterpret_cast<const f32x4*>(p + n * part);
+    for (int s = 1; s < a.splits; ++s)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) v[n] += *reinterpret_cast<const f32x4*>(p + (s * NT + n) * part);
+    if constexpr (SWIGLU) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[0][c] = silu_f(v[0][c]) * v[1][c];
+    }
+    float* out = a.out + r * a.ldo + col;
+    if (a.N - col >= 4) {
+        *reinterpret_cast<f32x4_a4*>(out) = f32x4_a4{v[0].x, v[0].y, v[0].z, v[0].w};
+    } else {
+        for (int i = 0; i < a.N - col; ++i) out[i] = v[0][i];
+    }
+}
+
 }  // namespace
 }  // namespace dev
 
 namespace detail {
 namespace {
 
-// Which kernel: few with tiles of 2^lg rows and so many waves, else rows with tiles of bm.
+// Which kernel: few with tiles of 2^lg rows and so many waves, else rows with tiles of bm and k in so many parts.
 struct Plan {
     bool few;
-    int bm, lg, waves;
+    int bm, lg, waves, splits;
 };
+// what is made of the products
+enum class Use { kMatmul, kSwiglu, kCombine };
 
 // The one that a rough model of both gives the least time, in us; it knows only host numbers, so rows are taken to be spread
 // over the experts.  All read the weights of the experts that have rows at 5.5 TB/s at best.  few_kernel: 8 us, 0.6 ns for each
-// unit that a tile meets (that often as a 256th of the GPU) and 0.1 ns for each row of it.  rows_kernel: 8 us with the planes'
-// pass, then stages of 0.44, 0.52 or 0.79 us (16, 32, 64 rows) while a CU has one workgroup or less, 0.47, 0.52 or 0.92 us each
-// beyond; an expert's further tiles read its weights again at 0.4 of the cost.  `weight` is what decoding and scaling a format
-// takes of either, beside Q4_0.  Over 135 calls of all formats what it takes was 1.5% slower than the best on average.
+// unit that a tile meets (that often as a 256th of the GPU) and 0.1 ns for each row of it.  rows_kernel: 8.8 us with the planes'
+// pass, then stages of 64 k at 0.42, 0.52 or 0.88 us (16, 32, 64 rows) while a CU has one workgroup or less, 0.47, 0.52 or 0.96 us
+// for each beyond, some of a last round that is not full; an expert's further tiles read its weights again at 0.28 of the
+// cost.  k in several parts costs their sums a way to memory and back at 3.8 TB/s and a launch (the combination adds them up
+// itself).  `weight` is what decoding and scaling a format takes of either, beside Q4_0.  Over 189 calls of all formats what it
+// takes was 1.5% slower than the best on average, 29% at most.
 // Measured, few (8 rows, 4 waves) / 16 / 32 / 64 rows, us: SwiGLU 2048 -> 1024 of 64 experts, 8 each, Q4_K: 4 tokens 18 / 24 / 27 /
-// 38, 16: 26 / 30 / 34 / 50, 48: 49 / 40 / 44 / 67, 256: 169 / 82 / 81 / 98, 512: 314 / 140 / 118 / 128, 1024: 643 / 270 / 195 / 195;
-// one expert each of 8, 8192 -> 2048 Q4_0: 16 tokens 27 / 65 / 74 / 108, 128: 64 / 68 / 76 / 110, 512: 194 / 112 / 85 / 117.
-Plan plan_products(const ExpertMatrix& w, const ExpertRows& g, bool swiglu) {
-    const double few_weight[] = {1.4, 1.2, 1.65, 1.1, 2.2, 1.1}, rows_weight[] = {1.3, 1.0, 1.3, 1.1, 1.6, 0.85};  // by format
+// 38, 16: 26 / 30 / 34 / 50, 48: 49 / 40 / 44 / 67, 256: 169 / 82 / 81 / 98, 512: 314 / 140 / 118 / 128, 1024: 643 / 270 / 195 / 195.
+// 8192 -> 2048 Q4_0, one of 8 experts each, 128 tokens: 61 / 66 / 74 / 106, k in two parts - / 42 / 47 / 64, in four - / 39 / 44 / 45.
+Plan plan_products(const ExpertMatrix& w, const ExpertRows& g, Use use) {
+    const bool swiglu = use == Use::kSwiglu;
+    const double few_weight[] = {1.35, 1.2, 1.65, 1.1, 1.75, 1.55}, rows_weight[] = {1.7, 1.0, 1.2, 1.1, 1.2, 1.3};  // by format
     const int depth = (w.K + dev::kUnitK - 1) / dev::kUnitK, tiles = (w.N + dev::kUnitCols - 1) / dev::kUnitCols;
     const double R = static_cast<double>(g.n_tokens) * g.top_k, E = w.n_experts;
     const double used = E * (1.0 - std::pow(1.0 - 1.0 / E, R)), matrices = swiglu ? 2.0 : 1.0;
@@ -165,19 +207,26 @@ Plan plan_products(const ExpertMatrix& w, const ExpertRows& g, bool swiglu) {
     const bool single = R < 1.15 * used;  // an expert's rows: hardly ever more than one
     const int lg = single ? 0 : g.n_tokens <= 4 ? 2 : 3;
     const double units = tiles * depth * matrices * 1e-3;
-    Plan best{true, 0, lg, std::min(depth, lg < 3 && (used * tiles <= 256 || depth >= 16) ? 8 : 4)};
+    Plan best{true, 0, lg, std::min(depth, lg < 3 && (used * tiles <= 256 || depth >= 16) ? 8 : 4), 1};
     double least = 8.0 + std::max(memory, units * (0.6 * few_weight[w.fmt] * row_tiles(1 << lg) + 0.1 * R));
     const double blocks = dev::rows_blocks(tiles, swiglu);
+    const double part = R * w.N * matrices * 4e-6;  // MB
     const struct {
         int bm;
         double one, each;
-    } kinds[] = {{16, 0.44, 0.47}, {32, 0.52, 0.52}, {64, 0.79, 0.92}};
+    } kinds[] = {{16, 0.42, 0.47}, {32, 0.52, 0.52}, {64, 0.88, 0.96}};
     for (const auto& k : kinds) {
-        const double stage = std::max(k.one, k.each * row_tiles(k.bm) * blocks / 256) * rows_weight[w.fmt];
-        const double us = 8.0 + std::max(memory * (0.6 + 0.4 * row_tiles(k.bm) / used), 4 * depth * stage);
-        if (us < least) {
-            least = us;
-            best = Plan{false, k.bm, 0, 0};
+        for (int splits = 1; splits <= std::min(depth, 8) && (splits == 1 || part * splits <= 256); splits *= 2) {
+            double load = row_tiles(k.bm) * blocks * splits / 256;  // workgroups of a CU
+            if (load > 1.0) load += 0.38 * (std::ceil(load) - load);
+            const double stage = std::max(k.one, k.each * load) * rows_weight[w.fmt];
+            const int stages = splits == 1 ? (w.K + 63) / 64 : 4 * ((depth + splits - 1) / splits);
+            const double join = splits == 1 ? 0.0 : use == Use::kCombine ? part * 2 * (splits - 1) / 3.8 : 2.3 + part * 2 * splits / 3.8;
+            const double us = 8.8 + join + std::max(memory * (0.72 + 0.28 * row_tiles(k.bm) / used), stages * stage);
+            if (us < least) {
+                least = us;
+                best = Plan{false, k.bm, 0, 0, splits};
+            }
         }
     }
     return best;
@@ -212,16 +261,23 @@ dev::ProductArgs product_args(const ExpertMatrix& w, const ExpertRows& g, const 
     return a;
 }
 
-// the product of w (and up: SiLU(x w^T) * (x up^T)) into out, rows in grouped order
-int launch_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertRows& g, const float* x, long ldx, bool gather,
-                    float* out, long ldo, void* ws, hipStream_t stream) {
+long product_columns(const ExpertMatrix& w) { return (w.N + 3L) & ~3L; }
+
+// bytes of the parts of k that are to be added up
+long part_bytes(const ExpertMatrix& w, long rows, const Plan& plan, bool swiglu) {
+    return plan.few || plan.splits == 1 ? 0 : up16(plan.splits * (swiglu ? 2 : 1) * rows * product_columns(w) * 4);
+}
+
+// The product of w (and up: SiLU(x w^T) * (x up^T)) into out, rows in grouped order; for Use::kCombine out is
+// [plan.splits][R][ldo].
+int launch_products(const Plan& plan, Use use, const ExpertMatrix& w, const ExpertMatrix* up, const ExpertRows& g, const float* x,
+                    long ldx, bool gather, float* out, long ldo, void* ws, hipStream_t stream) {
     const long R = static_cast<long>(g.n_tokens) * g.top_k;
     const int depth = (w.K + dev::kUnitK - 1) / dev::kUnitK, tiles = (w.N + dev::kUnitCols - 1) / dev::kUnitCols;
     const bool swiglu = up != nullptr;
-    const Plan plan = plan_products(w, g, swiglu);
     dev::ProductArgs a = product_args(w, g, x, ldx, gather, out, ldo);
     if (swiglu) a.w[1] = static_cast<const uint8_t*>(up->data);
-    const int blocks = plan.few ? tiles : dev::rows_blocks(tiles, swiglu);
+    const int blocks = plan.few ? tiles : dev::rows_blocks(tiles, swiglu) * plan.splits;
     const long groups = (dev::most_tiles(R, w.n_experts, plan.few ? 1 << plan.lg : plan.bm) * blocks + 7) / 8 * 8;
     if (groups >= 1L << 23) return kDeclined;  // up to 512 threads each: a launch's limit
     if (plan.few) {
@@ -244,6 +300,12 @@ int launch_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertR
     a.planes = p.planes;
     a.sums = p.sums;
     a.exps = p.exps;
+    a.splits = plan.splits;
+    const bool join = plan.splits > 1 && use != Use::kCombine;
+    if (join) {
+        a.out = reinterpret_cast<float*>(room + b.all());
+        a.ldo = product_columns(w);
+    }
     switch (w.fmt) {
         case kFmtQ8_0: dev::expert_rows<kFmtQ8_0>(a, swiglu, plan.bm, groups, stream); break;
         case kFmtQ4_0: dev::expert_rows<kFmtQ4_0>(a, swiglu, plan.bm, groups, stream); break;
@@ -251,6 +313,11 @@ int launch_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertR
         case kFmtQ4_K: dev::expert_rows<kFmtQ4_K>(a, swiglu, plan.bm, groups, stream); break;
         case kFmtQ6_K: dev::expert_rows<kFmtQ6_K>(a, swiglu, plan.bm, groups, stream); break;
         default: dev::expert_rows<kFmtF16>(a, swiglu, plan.bm, groups, stream);
+    }
+    if (join) {
+        const dev::JoinArgs j{a.out, g.offsets + w.n_experts, out, a.ldo, ldo, w.N, static_cast<int>(R), plan.splits};
+        hipLaunchKernelGGL(swiglu ? dev::join_kernel<true> : dev::join_kernel<false>,
+                           dim3(static_cast<unsigned>(R), static_cast<unsigned>((w.N + 1023) / 1024)), dim3(256), 0, stream, j);
     }
     return 0;
 }
@@ -263,25 +330,26 @@ bool token_takes(const ExpertMatrix& w, const ExpertRows& g) {
     return static_cast<long>(g.n_tokens) * ((w.N + dev::kUnitCols - 1) / dev::kUnitCols) <= 320;
 }
 
-long product_columns(const ExpertMatrix& w) { return (w.N + 3L) & ~3L; }
-
 }  // namespace
 
 long expert_product_workspace_bytes(const ExpertMatrix& w, const ExpertRows& g, bool swiglu, bool gather) {
-    if (plan_products(w, g, swiglu).few) return 0;
-    return plane_bytes(w, gather ? g.n_tokens : static_cast<long>(g.n_tokens) * g.top_k).all();
+    const Plan plan = plan_products(w, g, swiglu ? Use::kSwiglu : Use::kMatmul);
+    const long R = static_cast<long>(g.n_tokens) * g.top_k;
+    return plan.few ? 0 : plane_bytes(w, gather ? g.n_tokens : R).all() + part_bytes(w, R, plan, swiglu);
 }
 
 int launch_expert_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertRows& g, const float* x, long ldx,
                            bool gather, float* out, long ldo, void* ws, hipStream_t stream) {
-    return launch_products(w, up, g, x, ldx, gather, out, ldo, ws, stream);
+    const Use use = up != nullptr ? Use::kSwiglu : Use::kMatmul;
+    return launch_products(plan_products(w, g, use), use, w, up, g, x, ldx, gather, out, ldo, ws, stream);
 }
 
 // combine: the products of all rows, then what the products need
 long expert_combine_workspace_bytes(const ExpertMatrix& w, const ExpertRows& g) {
     if (token_takes(w, g)) return 0;
-    return up16(static_cast<long>(g.n_tokens) * g.top_k * product_columns(w) * 4) +
-           expert_product_workspace_bytes(w, g, false, false);
+    const Plan plan = plan_products(w, g, Use::kCombine);
+    const long R = static_cast<long>(g.n_tokens) * g.top_k;
+    return up16(plan.splits * R * product_columns(w) * 4) + (plan.few ? 0 : plane_bytes(w, R).all());
 }
 
 int launch_expert_combine(const ExpertMatrix& w, const ExpertRows& g, const float* h, long ldh, const float* weights,
@@ -301,9 +369,11 @@ int launch_expert_combine(const ExpertMatrix& w, const ExpertRows& g, const floa
     }
     const long R = static_cast<long>(g.n_tokens) * g.top_k, ldp = product_columns(w);
     float* const p = static_cast<float*>(ws);
-    const int rc = launch_products(w, nullptr, g, h, ldh, false, p, ldp, reinterpret_cast<uint8_t*>(p) + up16(R * ldp * 4), stream);
+    const Plan plan = plan_products(w, g, Use::kCombine);
+    const int rc = launch_products(plan, Use::kCombine, w, nullptr, g, h, ldh, false, p, ldp,
+                                   reinterpret_cast<uint8_t*>(p) + up16(plan.splits * R * ldp * 4), stream);
     if (rc != 0) return rc;
-    const dev::CombineArgs c{p, weights, g.slots, residual, out, ldp, ldr, ldo, w.N, g.top_k, static_cast<int>(R)};
+    const dev::CombineArgs c{p, weights, g.slots, residual, out, ldp, ldr, ldo, w.N, g.top_k, static_cast<int>(R), plan.splits};
     hipLaunchKernelGGL(dev::combine_kernel, dim3(static_cast<unsigned>(g.n_tokens), static_cast<unsigned>((w.N + 1023) / 1024)),
                        dim3(256), 0, stream, c);
     return 0;

@@ -148,6 +148,7 @@ struct ProductArgs {
     long ldo;
     int N, K, tiles, depth;  // tiles: columns / 32, depth: k / 256
     bool gather;             // the row of grouped row r is rows[r] / k, else r
+    int splits;              // rows_kernel: parts of k; with more than one, out is [splits][R][ldo] (SwiGLU: [splits][2][R][ldo])
 };
 
 // column blocks of rows_kernel: a wave takes a tile of G and U, or two tiles

@@ -18,6 +18,7 @@
 //   * Each decoded operand meets MT * 2 MFMAs and each operand read from LDS two.
 //   * PAIR (at most 16 rows): lane rows 0 .. 15 hold hi, 16 .. 31 lo of the same rows; one MFMA does both parts, and the
 //     two halves of the output are added at the end.
+//   * Where workgroups are few and k is long, k goes to several of them, whose products are added up in order afterwards.
 // few_kernel: for calls of few tokens, where what counts is how many waves read weights at once: a workgroup takes up to 8
 // rows of an expert and one tile of 32 columns, its waves the units along k, each converting the activations of its own
 // units to an LDS area of its own (a power of two per row and unit), no barrier before the sum over the waves.
@@ -111,16 +112,17 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
 
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int blocks = rows_blocks(a.tiles, SWIGLU);
     Tile t;
-    if (!find_tile(a.g, LG, blocks, blockIdx.x, t)) return;
+    if (!find_tile(a.g, LG, rows_blocks(a.tiles, SWIGLU) * a.splits, blockIdx.x, t)) return;
+    const int block = a.splits == 1 ? t.block : t.block / a.splits, split = t.block - block * a.splits;
+    const int u0 = a.splits == 1 ? 0 : split * a.depth / a.splits, u1 = a.splits == 1 ? a.depth : (split + 1) * a.depth / a.splits;
 
     // this wave's column tiles; one past the last is computed again as the last and not stored
     int tile[NT];
     const uint8_t* unit[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        tile[n] = SWIGLU ? t.block * 4 + wave : t.block * 8 + wave * 2 + n;
+        tile[n] = SWIGLU ? block * 4 + wave : block * 8 + wave * 2 + n;
         unit[n] = a.w[SWIGLU ? n : 0] +
                   (static_cast<long>(t.expert) * a.tiles + min(tile[n], a.tiles - 1)) * a.depth * static_cast<long>(kUnit);
     }
@@ -287,14 +289,14 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
         run_block(stage, Int<BLOCKS - 1>{}, tail, u, s, J == 3 ? next : s);
     };
 
-    load_scales(sc[0], 0);
+    load_scales(sc[0], u0);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) load_quants(q[0][n], 0, n), load_quants(q[1][n], 1, n);
-    copy(0);
-    copy(1);
+    for (int n = 0; n < NT; ++n) load_quants(q[0][n], 4 * u0, n), load_quants(q[1][n], 4 * u0 + 1, n);
+    copy(4 * u0);
+    copy(4 * u0 + 1);
     if constexpr (RING == 4) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) load_quants(q[2][n], 2, n);
+        for (int n = 0; n < NT; ++n) load_quants(q[2][n], 4 * u0 + 2, n);
     }
     if (threadIdx.x < BM) exps[threadIdx.x] = my_exp;  // (seen behind the stages' barriers)
     stage_barrier<kLater>();
@@ -302,9 +304,9 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
     decode(Int<0>{}, Int<0>{}, 0, sc[0]);
     if constexpr (STEPS == 2) decode(Int<0>{}, Int<1>{}, 0, sc[0]);
     sums_of[1] = ef16{};
-    const int whole = kRagged ? stages >> 2 : a.depth;
+    const int whole = kRagged ? min(stages >> 2, u1) : u1;
 #pragma unroll 1  // (a last round of its own would leave out loads that the barriers count on)
-    for (int u = 0; u < whole; ++u) {
+    for (int u = u0; u < whole; ++u) {
         run_stage(Int<0>{}, Int<0>{}, u, sc[0], sc[1]);
         run_stage(Int<1>{}, Int<0>{}, u, sc[0], sc[1]);
         run_stage(Int<2>{}, Int<0>{}, u, sc[0], sc[1]);
@@ -317,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
         for (int n = 0; n < NT; ++n) sc[0][n] = sc[1][n];
     }
     if constexpr (kRagged) {
-        const int rest = stages & 3;
+        const int rest = whole < u1 ? stages & 3 : 0;
         if (rest > 0) {
             run_stage(Int<0>{}, Int<1>{}, whole, sc[0], sc[1]);
             if (rest > 1) {
@@ -336,10 +338,19 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
             const int r = 32 * m + e_row(i) + 4 * h;
             if (r >= t.count) continue;
             const int e = exps[r];
-            float* o = a.out + static_cast<long>(t.first + r) * a.ldo;
             float v[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) v[n] = ldexpf(PAIR ? acc[n][m][i] + acc[n][m][i + 8] : acc[n][m][i], e);
+            if (SWIGLU && a.splits > 1) {
+                float* o = a.out + ((static_cast<long>(split) * 2) * a.g.R + t.first + r) * a.ldo;
+                const int col = tile[0] * kUnitCols + (lane & 31);
+                if (col < a.N) {
+                    o[col] = v[0];
+                    o[a.g.R * a.ldo + col] = v[NT - 1];
+                }
+                continue;
+            }
+            float* o = a.out + (static_cast<long>(split) * a.g.R + t.first + r) * a.ldo;
 #pragma unroll
             for (int n = 0; n < (SWIGLU ? 1 : NT); ++n) {
                 const int col = tile[n] * kUnitCols + (lane & 31);

@@ -289,50 +289,69 @@ def test_combine(fmt, M, E, k, N, K, kind):
     assert torch.equal(out, second)
 
 
-WIDE = [0, 1, 30, 31, 32, 63, 64, 255, 256, 300, 1023, 1024, 2047, 2049, 3333, 4095, 4096, 4098, 4099]  # columns that are checked
+COLUMNS = [0, 1, 30, 31, 32, 63, 64, 255, 256, 300, 511, 512, 515, 1023, 1024, 2047, 2049, 3333, 4095, 4096, 4098, 4099]  # the checked ones
 
 
 @functools.lru_cache(maxsize=8)
 def wide(fmt, E, N, K, seed):
-    """A matrix's blocks, and the values and magnitudes of the columns WIDE alone."""
+    """A matrix's blocks, and the values and magnitudes of some columns alone."""
     raw = quant.synthetic_weights(fmt, E * N, K, seed)
-    some = np.ascontiguousarray(np.asarray(raw).reshape(E, N, -1)[:, WIDE]).reshape(-1)
-    return raw, ref.weights(fmt, some, E, len(WIDE), K)
+    some = np.asarray(raw).reshape(E, N, -1)[:, [c for c in COLUMNS if c < N]]
+    return raw, ref.weights(fmt, np.ascontiguousarray(some).reshape(-1), E, some.shape[1], K)
 
 
-@pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("M", [24, 48, 200, 400])
-@pytest.mark.parametrize("K", [32, 160, 416, 544, 640, 768, 1056])
-def test_wide_matrices(fmt, M, K):
-    """Steps and prompts that take tiles of 16, 32 and 64 rows; K that ends inside 256 values after each number of 64, and
-    inside 64."""
-    if K % BLOCK.get(fmt, 32):
-        pytest.skip("no such K in this format")
-    E, k, N = 5, 2, 4100
+def check_large(fmt, M, E, k, N, K):
+    """All three products of a call, at some columns; a token without experts and every column finite."""
+    cols = [c for c in COLUMNS if c < N]
     ids = route_ids(M, E, k, "spread", seed=M)
     ids[1] = -1
     g, off, rows, slots = grouped(ids, E)
     raws, refs = zip(*(wide(fmt, E, N, K, seed) for seed in (1, 2)))
     gate, up = (cri.ExpertWeights(fmt, dev(r), E, N, K) for r in raws)
     (gv, gm), (uv, um) = refs
-    if M >= 48:
-        assert cri.expert_matmul_workspace_bytes(gate, g) > 0  # the rows are split once for all tiles
     x = randn(M, K, seed=M + 1)
     tok = np.maximum(rows, 0) // k
-    out = torch.full((M * k, N), 7.0, device="cuda")
-    cols = torch.tensor(WIDE, device="cuda")
+    whole, out = strided(M * k, N, 3)
+    at = torch.tensor(cols, device="cuda")
     cri.expert_matmul(gate, g, dev(x), out)
-    check_experts(out[:, cols], lambda e, lo, hi: ref.Product(x[tok[lo:hi]], gv[e], gm[e]), off)
+    check_experts(out[:, at], lambda e, lo, hi: ref.Product(x[tok[lo:hi]], gv[e], gm[e]), off)
     assert (out[off[-1]:] == 7).all() and torch.isfinite(out).all()
-    out.fill_(7.0)
+    whole.fill_(7.0)
     cri.expert_swiglu(gate, up, g, dev(x), out)
-    check_experts(out[:, cols], lambda e, lo, hi: ref.Swiglu(x[tok[lo:hi]], (gv[e], gm[e]), (uv[e], um[e])), off)
+    check_experts(out[:, at], lambda e, lo, hi: ref.Swiglu(x[tok[lo:hi]], (gv[e], gm[e]), (uv[e], um[e])), off)
     assert (out[off[-1]:] == 7).all() and torch.isfinite(out).all()
+    assert (whole[:, 0] == 7).all() and (whole[:, 1 + N:] == 7).all()
     h, weights, res = randn(M * k, K, seed=M + 2), randn(M, k, seed=M + 3), randn(M, N, seed=M + 4)
-    got = torch.empty(M, N, device="cuda")
+    h[off[-1]:] = np.nan
+    whole, got = strided(M, N, 2)
     cri.expert_combine(gate, g, dev(h), dev(weights), got, dev(res))
-    ref.check(got[:, cols], combined(h, gv, gm, ids, slots, weights, res[:, WIDE]))
+    ref.check(got[:, at], combined(h, gv, gm, ids, slots, weights, res[:, cols]))
     assert torch.equal(got[1], dev(res)[1]) and torch.isfinite(got).all()
+    assert (whole[:, 0] == 7).all() and (whole[:, 1 + N:] == 7).all()
+    return gate, g
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M", [24, 48, 96, 200, 400])
+@pytest.mark.parametrize("K", [32, 160, 416, 544, 640, 768, 1056])
+def test_wide_matrices(fmt, M, K):
+    """Steps and prompts that take tiles of 16, 32 and 64 rows; K that ends inside 256 values after each number of 64, and
+    inside 64."""
+    if K % BLOCK.get(fmt, 32):
+        pytest.skip("no such K in this format")
+    w, g = check_large(fmt, M, 5, 2, 4100, K)
+    if M >= 200:
+        assert cri.expert_matmul_workspace_bytes(w, g) > 0  # the rows are split into their parts once for all tiles
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M", [40, 120, 300, 700])
+def test_long_rows(fmt, M):
+    """Few tiles of long rows: K is shared between workgroups, the last of them with less than the others."""
+    K = 4352 if fmt in BLOCK else 4000
+    w, g = check_large(fmt, M, 4, 2, 516, K)
+    if M == 120:  # more than the rows' parts
+        assert cri.expert_matmul_workspace_bytes(w, g) > M * (K + 255) // 256 * 256 * 4 + 2 * M * 516 * 4
 
 
 @pytest.mark.parametrize("fmt", ["q4_k", "q6_k", "q8_0"])
