@@ -93,6 +93,7 @@ class ExpertGroups:
         self.offsets, self.rows, self.slots = made
         self.n_tokens, self.top_k, self.n_experts = n_tokens, top_k, n_experts
         self.n_rows = n_tokens * top_k
+        self._shape = (n_tokens, top_k)
         self._c = _ExpertGroups(*(t.data_ptr() for t in made), n_tokens, top_k, n_experts)
         self._ref = ctypes.addressof(self._c)
         self._dev = _device()
@@ -112,14 +113,19 @@ class ExpertRouter:
         self._dev = None if bias is None else _device()
 
 
+# A step's calls cost the host about as much as the GPU, so each check below has a short way for the usual case first.
+
+
 def _on_it(dev, *descriptors):
     for d in descriptors:
-        if d._dev is not None and d._dev != dev:
+        if d._dev != dev and d._dev is not None:
             raise ValueError("the tensors of a %s are on cuda:%d, not on the current device" % (type(d).__name__, d._dev))
 
 
 def _floats(t, rows, width, name, dev):
     """(address, floats from row to row) of a row buffer."""
+    if type(t) is not tuple and t.dtype is _f32t and t.is_contiguous() and t.shape == (rows, width) and t.get_device() == dev:
+        return t.data_ptr(), width
     p, ld, n = _rows(t, width, name, dev)
     if n is not None and n != rows:
         raise ValueError("%s has %d rows, not %d" % (name, n, rows))
@@ -130,18 +136,20 @@ def _floats(t, rows, width, name, dev):
 
 def _choices(t, kind, groups, name, dev):
     """The address of a contiguous [n_tokens, top_k] tensor."""
-    if t.dtype is not kind or t.shape != (groups.n_tokens, groups.top_k) or not t.is_contiguous():
+    if t.dtype is not kind or t.shape != groups._shape or not t.is_contiguous():
         raise ValueError("%s must be a contiguous %s tensor [n_tokens, top_k]" % (name, kind))
-    return _on_device(t, name, dev)
+    return t.data_ptr() if t.get_device() == dev else _on_device(t, name, dev)
 
 
-def _workspace(workspace, need, stream, dev):
-    """(address, bytes); one is allocated when None and something is needed."""
+def _workspace(workspace, stream, dev, need, *args):
+    """(address, bytes, the tensor); one is allocated when None and something is needed."""
     if workspace is None:
-        n = _bytes(need())
+        n = _bytes(need(*args))
         if n == 0:
             return None, 0, None
         workspace = _new_room(n, stream)
+    elif workspace.is_contiguous() and workspace.get_device() == dev:
+        return workspace.data_ptr(), workspace.nbytes, workspace
     p, n = _room(workspace, dev)
     return p, n, workspace
 
@@ -154,14 +162,14 @@ def route_experts_workspace_bytes(groups):
 def route_experts(router, logits, ids, weights, groups, workspace=None, stream=None):
     """Logits [n_tokens, n_experts] -> ids (int32) and weights (float32) [n_tokens, top_k], and the groups.
     workspace: a device tensor of route_experts_workspace_bytes (one is allocated when None)."""
-    L, dev = _torch(), _device()
+    L, dev = _loaded or _torch(), _device()
     _on_it(dev, router, groups)
     if router.bias is not None and router.bias.shape[0] != groups.n_experts:
         raise ValueError("the bias has %d entries, not %d" % (router.bias.shape[0], groups.n_experts))
     pl, ldl = _floats(logits, groups.n_tokens, groups.n_experts, "logits", dev)
     pi = _choices(ids, torch.int32, groups, "ids", dev)
     pw = _choices(weights, torch.float32, groups, "weights", dev)
-    ws, n, held = _workspace(workspace, lambda: L.cri_expert_group_workspace_bytes(groups._ref), stream, dev)
+    ws, n, held = _workspace(workspace, stream, dev, L.cri_expert_group_workspace_bytes, groups._ref)
     st = L.cri_expert_route(router._ref, pl, ldl, pi, pw, groups._ref, ws, n, _on(stream, dev))
     if st:
         _check(st)
@@ -169,10 +177,10 @@ def route_experts(router, logits, ids, weights, groups, workspace=None, stream=N
 
 def group_experts(ids, groups, workspace=None, stream=None):
     """The groups of given ids (int32 [n_tokens, top_k]; outside [0, n_experts): no expert)."""
-    L, dev = _torch(), _device()
+    L, dev = _loaded or _torch(), _device()
     _on_it(dev, groups)
     pi = _choices(ids, torch.int32, groups, "ids", dev)
-    ws, n, held = _workspace(workspace, lambda: L.cri_expert_group_workspace_bytes(groups._ref), stream, dev)
+    ws, n, held = _workspace(workspace, stream, dev, L.cri_expert_group_workspace_bytes, groups._ref)
     st = L.cri_expert_group(pi, groups._ref, ws, n, _on(stream, dev))
     if st:
         _check(st)
@@ -187,11 +195,11 @@ def expert_matmul(w, groups, x, out, workspace=None, grouped=False, stream=None)
     """out[r] = x[token of r] W[e]^T for the grouped rows r of every expert e: x [n_tokens, K] (with grouped,
     [n_tokens * top_k, K] in grouped order), out [n_tokens * top_k, N].  workspace: a device tensor of
     expert_matmul_workspace_bytes (one is allocated when None)."""
-    L, dev = _torch(), _device()
+    L, dev = _loaded or _torch(), _device()
     _on_it(dev, w, groups)
     px, ldx = _floats(x, groups.n_rows if grouped else groups.n_tokens, w.K, "x", dev)
     po, ldo = _floats(out, groups.n_rows, w.N, "out", dev)
-    ws, n, held = _workspace(workspace, lambda: L.cri_expert_matmul_workspace_bytes(w._ref, groups._ref, 1 if grouped else 0), stream, dev)
+    ws, n, held = _workspace(workspace, stream, dev, L.cri_expert_matmul_workspace_bytes, w._ref, groups._ref, 1 if grouped else 0)
     st = L.cri_expert_matmul(w._ref, groups._ref, px, ldx, 1 if grouped else 0, po, ldo, ws, n, _on(stream, dev))
     if st:
         _check(st)
@@ -204,11 +212,11 @@ def expert_swiglu_workspace_bytes(gate, groups):
 
 def expert_swiglu(gate, up, groups, x, out, workspace=None, stream=None):
     """out[r] = silu(x[token of r] gate[e]^T) * (x[token of r] up[e]^T): x [n_tokens, K], out [n_tokens * top_k, N]."""
-    L, dev = _torch(), _device()
+    L, dev = _loaded or _torch(), _device()
     _on_it(dev, gate, up, groups)
     px, ldx = _floats(x, groups.n_tokens, gate.K, "x", dev)
     po, ldo = _floats(out, groups.n_rows, gate.N, "out", dev)
-    ws, n, held = _workspace(workspace, lambda: L.cri_expert_swiglu_workspace_bytes(gate._ref, groups._ref), stream, dev)
+    ws, n, held = _workspace(workspace, stream, dev, L.cri_expert_swiglu_workspace_bytes, gate._ref, groups._ref)
     st = L.cri_expert_swiglu(gate._ref, up._ref, groups._ref, px, ldx, po, ldo, ws, n, _on(stream, dev))
     if st:
         _check(st)
@@ -222,27 +230,29 @@ def expert_combine_workspace_bytes(w, groups):
 def expert_combine(w, groups, x, weights, out, residual=None, workspace=None, stream=None):
     """out[t] = residual[t] + the sum over t's choices of weight * (x[grouped row] W[e]^T): x [n_tokens * top_k, K] in
     grouped order, weights [n_tokens, top_k], out and residual (may be None, or out) [n_tokens, N]."""
-    L, dev = _torch(), _device()
+    L, dev = _loaded or _torch(), _device()
     _on_it(dev, w, groups)
     px, ldx = _floats(x, groups.n_rows, w.K, "x", dev)
     pw = _choices(weights, torch.float32, groups, "weights", dev)
     po, ldo = _floats(out, groups.n_tokens, w.N, "out", dev)
     pr, ldr = (None, 0) if residual is None else _floats(residual, groups.n_tokens, w.N, "residual", dev)
-    ws, n, held = _workspace(workspace, lambda: L.cri_expert_combine_workspace_bytes(w._ref, groups._ref), stream, dev)
+    ws, n, held = _workspace(workspace, stream, dev, L.cri_expert_combine_workspace_bytes, w._ref, groups._ref)
     st = L.cri_expert_combine(w._ref, groups._ref, px, ldx, pw, pr, ldr, po, ldo, ws, n, _on(stream, dev))
     if st:
         _check(st)
 
 
-torch = _loaded = None
+torch = _loaded = _f32t = None
 
 
 def _torch():
     """torch and the library are loaded by the first call, not by importing the package."""
-    global torch, _loaded
+    global torch, _loaded, _f32t
     if _loaded is None:
-        _loaded = serving._torch()
+        lib = serving._torch()
         torch = serving.torch
+        _f32t = torch.float32
+        _loaded = lib
     return _loaded
 
 
