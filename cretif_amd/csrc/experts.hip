@@ -322,12 +322,12 @@ int launch_products(const Plan& plan, Use use, const ExpertMatrix& w, const Expe
     return 0;
 }
 
-// Whether a call's weighted sums are taken in one launch, a workgroup per token and column tile, which reads an expert's
-// weights for every token that has it: where that is a round of workgroups or little more.  Us, two launches / one: 1024 -> 2048
-// Q4_K, 8 of 64 experts each: 1 token 12.3 / 9.1, 4 14.3 / 10.7, 8 18.0 / 17.9, 16 23.4 / 32.1; 1536 -> 576 Q8_0, 4 of 32: 8 tokens
-// 12.5 / 8.8.
+// Whether a call's weighted sums are taken in one launch, two workgroups per token and column tile, which read an expert's
+// weights for every token that has it: where those are two rounds of workgroups at most.  Us, two launches / one: 1024 -> 2048
+// Q6_K, 8 of 64 experts each: 1 token 11.1 / 8.0, 4 16.2 / 15.0, 5 18.5 / 19.8, 8 21.5 / 26.1; 1536 -> 576 Q8_0, 4 of 32: 12 tokens
+// 12.7 / 11.7.
 bool token_takes(const ExpertMatrix& w, const ExpertRows& g) {
-    return static_cast<long>(g.n_tokens) * ((w.N + dev::kUnitCols - 1) / dev::kUnitCols) <= 320;
+    return static_cast<long>(g.n_tokens) * ((w.N + dev::kUnitCols - 1) / dev::kUnitCols) <= 256;
 }
 
 }  // namespace

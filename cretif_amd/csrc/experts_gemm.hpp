@@ -429,6 +429,7 @@ __device__ __forceinline__ void few_stage(const typename F::Quant (&q)[NT], cons
             auto scale = [&](float d, const ef16& t) {
 #pragma unroll
                 for (int i = 0; i < KEEP; ++i) r[n][i] = __builtin_fmaf(d, t[i] + t[i + 8], r[n][i]);
+                if constexpr (KEEP == 1) asm volatile("" : "+v"(r[n][0]));  // the next step's sums not before: together they spill
             };
             if constexpr (F::kScaled == kPerBlock) {
                 scale(F::template part_scale<2 * J + I>(s[n]), e_mfma(x[1], b[1], e_mfma(x[0], b[0], ef16{})));
@@ -584,67 +585,86 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const int* offsets,
     }
 }
 
-// The weighted sums of few tokens in one launch: a workgroup of 16 waves takes a token and a tile of 32 columns, its waves
-// the units of all of the token's choices (unit i: choice i / depth), each unit's products times the choice's weight.  All that
-// lookups need is asked for at once and kept.  Decoding bounds it: 8 waves for 16 columns each, on twice as many CUs but with
-// every unit decoded twice, took 16.0 us instead of 10.6 (a token of 8 experts, 1024 -> 2048 Q6_K).
+// The weighted sums of few tokens in one launch: a workgroup of 16 waves takes a token and 16 columns, its waves the units of
+// all of the token's choices (unit i: choice i / depth), each unit's products times the choice's weight.  Decoding is what
+// counts, and a multiplication has 32 columns: a wave takes two units at once, lanes 0 .. 15 and 32 .. 47 the first one's 16
+// columns, the others the second one's, against two rows of activations; of the four blocks of the result two are used.  (One
+// unit of 32 columns a wave, on half as many CUs: 10.6 us instead of 7.6 for a token of 8 experts, 1024 -> 2048 Q6_K.)  All that
+// lookups need is asked for at once and kept.
 template <int FMT>
 __global__ __launch_bounds__(1024) void token_kernel(const ProductArgs a, const TokenArgs b) {
     typedef ExpertFmt<FMT> F;
-    constexpr int WAVES = 16, kUnit = unit_bytes(FMT), HELD = 4;
-    __shared__ __attribute__((aligned(16))) char lds[WAVES * few_wave_bytes(1)];
+    constexpr int WAVES = 16, HELD = 4;
+    constexpr long kUnit = unit_bytes(FMT);
+    __shared__ __attribute__((aligned(16))) char lds[WAVES * few_wave_bytes(2)];
     __shared__ float red[WAVES][32];
     const int lane = threadIdx.x & 63, h = lane >> 5, k = a.g.k, E = a.g.E;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = blockIdx.x, t = blockIdx.y;
+    const int tile = blockIdx.x >> 1, t = blockIdx.y;
+    const bool second = (lane & 16) != 0;                                  // whose weights the lane multiplies
+    const uint32_t from = (lane & 47) | (blockIdx.x & 1) << 4;             // and which of a unit's lanes they were laid out for
     const int choice = t * k + min(lane, k - 1);
     const int slots = a.g.slots[choice];
     const float weights = b.weights[choice];
     int ends[HELD];  // of experts lane, 64 + lane, ...
 #pragma unroll
     for (int i = 0; i < HELD; ++i) ends[i] = a.g.offsets[min(64 * i + lane + 1, E)];
-    const int col = tile * kUnitCols + (threadIdx.x & 31);
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15);
     float first = 0.0f;
-    if (b.residual != nullptr && threadIdx.x < 32 && col < a.N) first = b.residual[t * b.ldr + col];
-    char* const area = lds + wave * few_wave_bytes(1);
-    char* const sums = area + 1024;
-    float* const us = reinterpret_cast<float*>(sums + 32);
-    float acc = 0.0f;  // lanes below 32: column tile * 32 + lane
-    for (int i = wave; i < k * a.depth; i += WAVES) {
-        const int j = i / a.depth, u = i - j * a.depth;
-        const int slot = __builtin_amdgcn_readlane(slots, j);
-        if (slot < 0 || slot >= a.g.R) continue;
-        int e = 0;  // the slot's expert: how many end at or before it
+    if (b.residual != nullptr && threadIdx.x < 16 && col < a.N) first = b.residual[t * b.ldr + col];
+    char* const area = lds + wave * few_wave_bytes(2);
+    char* const sums = area + 2 * 1024;
+    float* const us = reinterpret_cast<float*>(sums + 2 * 32);
+    float acc = 0.0f;  // lanes 0 .. 15 of the first units, lanes 48 .. 63 of the second ones
+    const int units = k * a.depth;
+    for (int i0 = wave; i0 < units; i0 += 2 * WAVES) {
+        bool live[2];
+        int slot[2], u[2];
+        float weight[2];
+        long at[2];  // the unit's place
 #pragma unroll
-        for (int m = 0; m < HELD; ++m) e += __popcll(__ballot(64 * m + lane < E && ends[m] <= slot));
-        for (int e0 = 64 * HELD; e0 < E; e0 += 64) e += __popcll(__ballot(e0 + lane < E && a.g.offsets[e0 + lane + 1] <= slot));
-        const uint8_t* unit = a.w[0] + ((static_cast<long>(min(e, E - 1)) * a.tiles + tile) * a.depth + u) * static_cast<long>(kUnit);
-        typename F::Quant q[4][1];
-        typename F::Scale sc[1];
-        const int c = u * kUnitK + 8 * (lane & 31);
+        for (int n = 0; n < 2; ++n) {
+            const int i = min(i0 + n * WAVES, units - 1), j = i / a.depth;
+            u[n] = i - j * a.depth;
+            slot[n] = __builtin_amdgcn_readlane(slots, j);
+            weight[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weights), j));
+            live[n] = i0 + n * WAVES < units && slot[n] >= 0 && slot[n] < a.g.R;
+            slot[n] = clamp_int(slot[n], 0, a.g.R - 1);
+            int e = 0;  // the slot's expert: how many end at or before it
+#pragma unroll
+            for (int m = 0; m < HELD; ++m) e += __popcll(__ballot(64 * m + lane < E && ends[m] <= slot[n]));
+            for (int e0 = 64 * HELD; e0 < E; e0 += 64) e += __popcll(__ballot(e0 + lane < E && a.g.offsets[e0 + lane + 1] <= slot[n]));
+            at[n] = ((static_cast<long>(min(e, E - 1)) * a.tiles + tile) * a.depth + u[n]) * kUnit;
+        }
+        if (!live[0] && !live[1]) continue;
+        if (!live[1]) slot[1] = slot[0], u[1] = u[0], at[1] = at[0];  // read twice, used once
+        if (!live[0]) slot[0] = slot[1], u[0] = u[1], at[0] = at[1];
+        const int c = (h ? u[1] : u[0]) * kUnitK + 8 * (lane & 31);
         f32x4 lo = f32x4{0, 0, 0, 0}, hi = lo;
         if (c < a.K) {
-            const float* p = a.x + slot * a.ldx + c;
+            const float* p = a.x + (h ? slot[1] : slot[0]) * a.ldx + c;
             lo = ld_f32x4(p);
             hi = ld_f32x4(p + 4);
         }
-        F::load(sc[0], unit, lane);
+        const uint8_t* const unit = a.w[0] + (second ? at[1] : at[0]);
+        typename F::Quant q[4][1];
+        typename F::Scale sc[1];
+        F::load(sc[0], unit, from);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) F::load(q[s][0], unit, s, lane);
-        few_convert(lo, hi, h == 0, 0, area, sums, us);
+        for (int s = 0; s < 4; ++s) F::load(q[s][0], unit, s, from);
+        few_convert(lo, hi, true, h, area, sums, us);
         wave_order();
-        float p[1][1];
-        few_multiply<FMT, 1, 1>(q, sc, area, sums, 1, p);
-        const float weight = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weights), j));
-        acc = __builtin_fmaf(weight * us[0], p[0][0], acc);
+        float p[1][1];  // of row 0, or row 4: the last one again, the second unit's
+        few_multiply<FMT, 1, 1>(q, sc, area, sums, 2, p);
+        if (h ? live[1] : live[0]) acc = __builtin_fmaf((h ? weight[1] : weight[0]) * us[h], p[0][0], acc);
         wave_order();
     }
-    if (h == 0) red[wave][lane] = acc;
+    if (second == (h != 0)) red[wave][lane & 31] = acc;  // (lanes 0 .. 15, and 48 .. 63 as 16 .. 31)
     __syncthreads();
-    if (threadIdx.x < 32 && col < a.N) {
-        float v = red[0][threadIdx.x];
+    if (threadIdx.x < 16 && col < a.N) {
+        float v = 0.0f;
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) v += red[w][threadIdx.x];
+        for (int w = 0; w < WAVES; ++w) v += red[w][threadIdx.x] + red[w][threadIdx.x + 16];
         a.out[t * a.ldo + col] = v + first;
     }
 }
@@ -673,7 +693,7 @@ void expert_few(const ProductArgs& a, bool swiglu, int lg, int waves, long workg
 
 template <int FMT>
 void expert_token(const ProductArgs& a, const TokenArgs& b, int tokens, hipStream_t stream) {
-    hipLaunchKernelGGL(token_kernel<FMT>, dim3(a.tiles, tokens), dim3(1024), 0, stream, a, b);
+    hipLaunchKernelGGL(token_kernel<FMT>, dim3(2 * a.tiles, tokens), dim3(1024), 0, stream, a, b);
 }
 
 }  // namespace dev
