@@ -1,16 +1,17 @@
 // experts_formats.hpp -- from a laid out unit's bytes (experts.hpp) to the B operands of v_mfma_f32_32x32x16_f16: exact
 // integers in fp16 (FP16: the weights themselves), and the scales that the fp32 partial sums take.
 //
-// ExpertFmt<FMT>: load(q, unit, stage) a lane's bytes of a stage of four steps (64 k), load(s, unit) those of the unit's
-// scales; operand<J, S>(q, s, b) the eight weights of step S of stage J, as four pairs.  kScaled says how scales are applied:
-// kNoScale not at all; kPerStep and kPerBlock the partial sum of a step (16 k) or of a block of two times part_scale<I>() (I: the
+// ExpertFmt<FMT>: load(q, unit, stage) a lane's bytes of a stage of four steps (64 k), in kLoads loads, load(s, unit) those of
+// the unit's scales; operand<J, S>(q, s, b) the eight weights of step S of stage J, as four pairs.  kScaled says how scales are
+// applied: kNoScale not at all; kPerStep and kPerBlock the partial sum of a step (16 k) or of a block of two times part_scale<I>() (I: the
 // unit's step or block).  Q4_K's minimums meet the activations' sums over 32, which are staged times 2^-6, once per unit:
 // min_operand(), min_scale().
 //
 // Scales multiply a partial sum instead of the weights because d q has 19 bits, fp16 11.  Other forms that fit: Q4_K's 6-bit
 // scale times 4-bit code (10 bits) in the operand, d per unit, half the scalings: its 64 registers of unit sums spill, 4096
 // tokens' SwiGLU 630 us against 591 as Q4_0 does it; Q6_K's scale times code (12 bits) as an operand's nearest half and its rest
-// in a third MFMA, no scalings before the unit's end: 856 us against 790, the MFMAs' power counts.
+// in a third MFMA, no scalings before the unit's end: 856 us against 790, the MFMAs' power counts; Q4_K's codes as fp16's
+// smallest numbers, masked alone: 555 us against 581, but the products lose bits, errors of 1e-5 instead of 3e-7.
 #pragma once
 
 #include "experts.hpp"
