@@ -107,8 +107,8 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
     // a stage's barrier leaves on their way
     constexpr int RING = FMT == kFmtQ8_0 && MT == 2 ? 2 : 4, kLater = RING == 2 ? 0 : NT * F::kLoads;
     static_assert(!PAIR || MT == 1, "a pair is one tile");
-    __shared__ __attribute__((aligned(256))) char ring[4 * kStage];
-    __shared__ int exps[BM];
+    __shared__ __attribute__((aligned(256))) char ring[4 * kStage + 4 * BM];  // the copies' buffers first: they are below 64 KB
+    int* const exps = reinterpret_cast<int*>(ring + 4 * kStage);
 
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

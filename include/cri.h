@@ -503,7 +503,7 @@ typedef struct cri_expert_router {
 /* logits [n_tokens, n_experts], rows ldl floats apart -> ids and weights [n_tokens, top_k] and the groups.  A token's scores are
  * the softmax or the sigmoid of its logits; its top_k experts are those of the largest score plus bias (without a bias: of the
  * largest logit), in that order, the lowest number first where they are equal; their weights are the scores (without the
- * bias), divided by their sum with normalize, times scale.  An expert whose logit is -infinity or NaN (or whose bias makes its sum
+ * bias), divided by their sum with normalize (a sum of 0 leaves them 0), times scale.  An expert whose logit is -infinity or NaN (or whose bias makes its sum
  * so) is never chosen: a token left with fewer experts than top_k has id -1 and weight 0 in the choices behind, so a row of
  * -infinity (a padded batch's) causes no work.  Scores and their order are computed in 64 bits.  workspace: 4-byte aligned,
  * cri_expert_group_workspace_bytes. */

@@ -331,14 +331,11 @@ def check_large(fmt, M, E, k, N, K):
     return gate, g
 
 
-@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("fmt,K", [(f, K) for f in FORMATS for K in (32, 160, 416, 544, 640, 768, 1056) if K % BLOCK.get(f, 32) == 0])
 @pytest.mark.parametrize("M", [24, 48, 96, 200, 400])
-@pytest.mark.parametrize("K", [32, 160, 416, 544, 640, 768, 1056])
 def test_wide_matrices(fmt, M, K):
     """Steps and prompts that take tiles of 16, 32 and 64 rows; K that ends inside 256 values after each number of 64, and
     inside 64."""
-    if K % BLOCK.get(fmt, 32):
-        pytest.skip("no such K in this format")
     w, g = check_large(fmt, M, 5, 2, 4100, K)
     if M >= 200:
         assert cri.expert_matmul_workspace_bytes(w, g) > 0  # the rows are split into their parts once for all tiles
@@ -381,6 +378,55 @@ def test_rows_of_any_magnitude(fmt, M):
             assert not torch.isfinite(bad[r[t]]).any()
         else:
             assert torch.equal(bad[r[t]], out[r[t]])
+
+
+@pytest.mark.parametrize("E,k,M", [(300, 4, 1000), (520, 2, 3000)])
+def test_many_experts_of_many_rows(E, k, M):
+    """More experts than a wave holds offsets of, tiles shared by many rows."""
+    w, g = check_large("q4_0", M, E, k, 1028, 256)
+    assert cri.expert_matmul_workspace_bytes(w, g) > 0
+
+
+def test_rows_that_are_not_finite_in_a_wide_call():
+    """As above, where the rows are split into their parts first and tiles are shared by many rows."""
+    E, k, N, K, M = 3, 1, 4100, 768, 200
+    for fmt in ("q4_k", "q5_0", "fp16"):
+        w = cri.ExpertWeights(fmt, dev(wide(fmt, E, N, K, 1)[0]), E, N, K)
+        g, _, _, slots = grouped(np.arange(M)[:, None] % E, E)
+        x = randn(M, K, seed=8)
+        x[5] *= 1e-35
+        x[6] *= 1e30
+        out, bad = torch.empty(M, N, device="cuda"), torch.empty(M, N, device="cuda")
+        cri.expert_matmul(w, g, dev(x), out)
+        assert torch.isfinite(out).all() and (out[slots[5]].abs() > 0).any()
+        x[0, 3], x[70, 700], x[131, 0] = np.inf, np.nan, -np.inf
+        cri.expert_matmul(w, g, dev(x), bad)
+        hit = torch.tensor(slots[[0, 70, 131]], device="cuda").long()
+        assert not torch.isfinite(bad[hit]).any()
+        keep = torch.ones(M, dtype=torch.bool, device="cuda")
+        keep[hit] = False
+        assert torch.equal(bad[keep], out[keep])
+
+
+@pytest.mark.parametrize("E,k,M", [(256, 8, 3), (257, 3, 5), (600, 9, 40), (1024, 64, 2), (1024, 2, 700)])
+def test_many_experts(E, k, M):
+    """More experts than a wave holds offsets of: every kernel's way to its rows."""
+    N, K = 70, 256
+    ids = route_ids(M, E, k, "spread", seed=E)
+    ids[-1, 0] = E - 1
+    ids[-1, 1:] = np.arange(k - 1)
+    g, off, rows, slots = grouped(ids, E)
+    w = packed("q4_0", E, N, K)
+    v, mag = matrix("q4_0", E, N, K)[1]
+    x = randn(M, K, seed=1)
+    tok = np.maximum(rows, 0) // k
+    out = torch.empty(M * k, N, device="cuda")
+    cri.expert_matmul(w, g, dev(x), out)
+    check_experts(out, lambda e, lo, hi: ref.Product(x[tok[lo:hi]], v[e], mag[e]), off)
+    h, weights = randn(M * k, K, seed=2), randn(M, k, seed=3)
+    got = torch.empty(M, N, device="cuda")
+    cri.expert_combine(w, g, dev(h), dev(weights), got)
+    ref.check(got, combined(h, v, mag, ids, slots, weights, None))
 
 
 def test_any_alignment_of_the_blocks():
@@ -432,6 +478,16 @@ def test_groups_that_do_not_fit_stay_in_bounds():
         cri.expert_combine(w, g, dev(randn(M * k, K)), dev(randn(M, k)), whole[1:1 + M])
         few = cri.ExpertGroups(2, k, E, g.offsets, wild(2 * k), wild(2 * k))
         cri.expert_matmul(w, few, x[:2], whole[1:1 + 2 * k])
+        assert (whole[0] == 7).all() and (whole[-1] == 7).all()
+    N, M = 4100, 300
+    w = packed("q4_k", E, N, K)
+    for seed in range(3):
+        wild = lambda n: ints(rng.choice([-2 ** 31, -5, 0, 3, 17, 200, M * k, 2 ** 31 - 1, 1000], n))  # noqa: E731
+        g = cri.ExpertGroups(M, k, E, wild(E + 1), wild(M * k), wild(M * k))
+        whole = torch.full((M * k + 2, N), 7.0, device="cuda")
+        cri.expert_matmul(w, g, dev(randn(M, K)), whole[1:-1])
+        cri.expert_swiglu(w, w, g, dev(randn(M, K)), whole[1:-1])
+        cri.expert_combine(w, g, dev(randn(M * k, K)), dev(randn(M, k)), whole[1:1 + M])
         assert (whole[0] == 7).all() and (whole[-1] == 7).all()
 
 
@@ -520,6 +576,53 @@ def test_layer_captured(M):
         torch.cuda.synchronize()
         assert torch.equal(layer.out, eager)
         layer.check(x)
+
+
+@pytest.mark.parametrize("M,N,K", [(120, 516, 4352), (300, 516, 4352), (200, 4100, 768), (2, 516, 4352)])
+def test_large_calls_captured(M, N, K):
+    """Rows split into their parts, K shared between workgroups: a graph over one workspace, replayed with other activations and
+    other choices, gives the eager calls' bits."""
+    E, k = 4, 2
+    w, up = (cri.ExpertWeights("q4_k", dev(wide("q4_k", E, N, K, seed)[0]), E, N, K) for seed in (1, 2))
+    g = cri.ExpertGroups(M, k, E)
+    f = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    x, h, weights, a, b, c = f(M, K), f(M * k, K), f(M, k), f(M * k, N), f(M * k, N), f(M, N)
+    ids = torch.zeros(M, k, dtype=torch.int32, device="cuda")
+    need = max(cri.expert_matmul_workspace_bytes(w, g), cri.expert_swiglu_workspace_bytes(w, g), cri.expert_combine_workspace_bytes(w, g),
+               cri.route_experts_workspace_bytes(g), 16)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+
+    def calls():
+        cri.group_experts(ids, g, ws)
+        cri.expert_matmul(w, g, x, a, ws)
+        cri.expert_swiglu(w, up, g, x, b, ws)
+        cri.expert_combine(w, g, h, weights, c, None, ws)
+
+    def fill(seed):
+        x.copy_(dev(randn(M, K, seed=seed)))
+        h.copy_(dev(randn(M * k, K, seed=seed + 1)))
+        weights.copy_(dev(randn(M, k, seed=seed + 2)))
+        ids.copy_(ints(route_ids(M, E, k, "spread" if seed % 2 else "one", seed=seed)))
+
+    s = torch.cuda.Stream()
+    fill(0)
+    with torch.cuda.stream(s):
+        calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        calls()
+    for seed in (1, 2, 3, 1):
+        fill(seed)
+        calls()
+        eager = [t.clone() for t in (a, b, c)]
+        for t in (a, b, c):
+            t.zero_()
+        ws.fill_(0xFF)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip((a, b, c), eager):
+            assert torch.equal(got, want) and torch.isfinite(got).all()
 
 
 def test_two_streams_at_once():
