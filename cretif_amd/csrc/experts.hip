@@ -258,6 +258,7 @@ dev::ProductArgs product_args(const ExpertMatrix& w, const ExpertRows& g, const 
     a.tiles = (w.N + dev::kUnitCols - 1) / dev::kUnitCols;
     a.depth = (w.K + dev::kUnitK - 1) / dev::kUnitK;
     a.gather = gather;
+    a.over_k = ((1u << 31) + g.top_k - 1) / g.top_k;
     return a;
 }
 

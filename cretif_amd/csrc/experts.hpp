@@ -136,6 +136,12 @@ __host__ inline long most_tiles(long R, int E, int bm) {
     return bound < R ? bound : R;
 }
 
+// pair / k: over_k is 2^31 / k rounded up, off by less than 1, so the product by less than 2^-7 (pairs are below 2^23), and a quotient
+// is at least 1 / 64 below the next whole number
+__device__ __forceinline__ int token_of(int pair, uint32_t over_k) {
+    return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(pair), over_k));
+}
+
 struct ProductArgs {
     const uint8_t* w[2];  // W, or G and U
     Groups g;
@@ -148,6 +154,7 @@ struct ProductArgs {
     long ldo;
     int N, K, tiles, depth;  // tiles: columns / 32, depth: k / 256
     bool gather;             // the row of grouped row r is rows[r] / k, else r
+    uint32_t over_k;         // of token_of
     int splits;              // rows_kernel: parts of k; with more than one, out is [splits][R][ldo] (SwiGLU: [splits][2][R][ldo])
 };
 

@@ -59,7 +59,7 @@ __device__ __forceinline__ constexpr int e_row(int i) { return (i & 3) + 8 * (i 
 
 // the source row of grouped row r
 __device__ __forceinline__ long source_row(const ProductArgs& a, int r) {
-    return a.gather ? clamp_int(a.g.rows[r], 0, a.g.R - 1) / a.g.k : r;
+    return a.gather ? token_of(clamp_int(a.g.rows[r], 0, a.g.R - 1), a.over_k) : r;
 }
 
 template <int I>
@@ -133,8 +133,6 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
 #pragma unroll
     for (int i = 0; i < kCopies; ++i)
         from[i] = source_row(a, t.first + min(wave * kShare + 4 * i + (lane >> 4), t.count - 1));
-    int my_exp = 0;
-    if (threadIdx.x < BM) my_exp = a.exps[source_row(a, t.first + min(static_cast<int>(threadIdx.x), t.count - 1))];
     const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((Lds)ring));
     auto copy = [&](int stage) {  // (past the end: the last stage again, unused)
         const uint8_t* at = a.planes + 256L * min(stage, stages - 1);
@@ -292,6 +290,7 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
     load_scales(sc[0], u0);
 #pragma unroll
     for (int n = 0; n < NT; ++n) load_quants(q[0][n], 4 * u0, n), load_quants(q[1][n], 4 * u0 + 1, n);
+    const int my_exp = a.exps[source_row(a, t.first + min(static_cast<int>(threadIdx.x), t.count - 1))];
     copy(4 * u0);
     copy(4 * u0 + 1);
     if constexpr (RING == 4) {
@@ -500,7 +499,7 @@ __device__ __forceinline__ void wave_order() {
 // first loads need come first and plain: those are preloaded into SGPRs.
 template <int FMT, bool SWIGLU, int KEEP>
 __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const int* offsets, const int* rows, const uint8_t* w0, const uint8_t* w1,
-                                                             const float* x, int E, int R, int k, int lg_waves, int tiles, int depth,
+                                                             const float* x, int E, int R, uint32_t over_k, int lg_waves, int tiles, int depth,
                                                              const FewRest rest) {
     typedef ExpertFmt<FMT> F;
     constexpr int NT = SWIGLU ? 2 : 1, kUnit = unit_bytes(FMT);
@@ -508,14 +507,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const int* offsets,
     const int lane = threadIdx.x & 63, h = lane >> 5, lg = lg_waves & 3, waves = lg_waves >> 2;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Tile t;
-    if (!find_tile(Groups{offsets, nullptr, nullptr, E, k, R}, lg, tiles, blockIdx.x, t)) return;
+    if (!find_tile(Groups{offsets, nullptr, nullptr, E, 1, R}, lg, tiles, blockIdx.x, t)) return;
     // a row for each half of the wave and pass, eight of its activations a lane
     constexpr int PASSES = KEEP;
     int source[PASSES];
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         const int r = t.first + min(2 * i + h, t.count - 1);
-        source[i] = k > 0 ? rows[r] : r;  // (k 0: rows of x in grouped order)
+        source[i] = over_k != 0 ? rows[r] : r;  // (0: rows of x in grouped order)
     }
     const long first_unit = (static_cast<long>(t.expert) * tiles + t.block) * depth;
     char* const area = lds + wave * few_wave_bytes(1 << lg);
@@ -540,7 +539,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const int* offsets,
         for (int i = 0; i < PASSES; ++i) {
             lo[i] = hi[i] = f32x4{0, 0, 0, 0};
             if (2 * i < t.count && c < rest.K) {
-                const float* p = x + (k > 0 ? clamp_int(source[i], 0, R - 1) / k : source[i]) * rest.ldx + c;
+                const float* p = x + (over_k != 0 ? token_of(clamp_int(source[i], 0, R - 1), over_k) : source[i]) * rest.ldx + c;
                 lo[i] = ld_f32x4(p);
                 hi[i] = ld_f32x4(p + 4);
             }
@@ -688,7 +687,7 @@ void expert_few(const ProductArgs& a, bool swiglu, int lg, int waves, long workg
                             : (lg == 0 ? few_kernel<FMT, false, 1> : few_kernel<FMT, false, 4>);
     hipLaunchKernelGGL(run, dim3(static_cast<unsigned>(workgroups)),
                        dim3(64 * waves), lds, stream, a.g.offsets, a.g.rows, a.w[0], a.w[1], a.x, a.g.E, a.g.R,
-                       a.gather ? a.g.k : 0, lg | waves << 2, a.tiles, a.depth, rest);
+                       a.gather ? a.over_k : 0u, lg | waves << 2, a.tiles, a.depth, rest);
 }
 
 template <int FMT>
