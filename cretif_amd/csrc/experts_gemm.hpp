@@ -330,30 +330,38 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const ProductArgs a) {
     if constexpr (kParts) scale(NT - 1, MT - 1, sums_of[(NT * MT - 1) & 1]);
     stage_barrier<0>();  // the last copies have arrived
 
+    // lanes of a half have rows 32 m + e_row(i) + 4 h; what is the same in all lanes of these is kept out of the addresses
+    const int col = tile[0] * kUnitCols + (lane & 31), rows = t.count - 4 * h;
+    const bool parts = SWIGLU && a.splits > 1;  // SwiGLU's two products apart
+    float* const first = a.out + (static_cast<long>(split) * (parts ? 2 : 1) * a.g.R + t.first + 4 * h) * a.ldo + col;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
-        for (int i = 0; i < (PAIR ? 8 : 16); ++i) {
-            const int r = 32 * m + e_row(i) + 4 * h;
-            if (r >= t.count) continue;
-            const int e = exps[r];
-            float v[NT];
+        for (int q4 = 0; q4 < (PAIR ? 2 : 4); ++q4) {
+            typedef int int4_t __attribute__((ext_vector_type(4)));
+            const int4_t e = *reinterpret_cast<const int4_t*>(exps + 32 * m + 8 * q4 + 4 * h);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) v[n] = ldexpf(PAIR ? acc[n][m][i] + acc[n][m][i + 8] : acc[n][m][i], e);
-            if (SWIGLU && a.splits > 1) {
-                float* o = a.out + ((static_cast<long>(split) * 2) * a.g.R + t.first + r) * a.ldo;
-                const int col = tile[0] * kUnitCols + (lane & 31);
-                if (col < a.N) {
-                    o[col] = v[0];
-                    o[a.g.R * a.ldo + col] = v[NT - 1];
+            for (int j = 0; j < 4; ++j) {
+                const int i = 4 * q4 + j, r = 32 * m + e_row(i);
+                float v[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) v[n] = ldexpf(PAIR ? acc[n][m][i] + acc[n][m][i + 8] : acc[n][m][i], e[j]);
+                if (r >= rows) continue;
+                float* const o = first + r * a.ldo;
+                if constexpr (SWIGLU) {
+                    if (col < a.N) {
+                        if (parts) {
+                            o[0] = v[0];
+                            o[a.g.R * a.ldo] = v[NT - 1];
+                        } else {
+                            o[0] = silu_f(v[0]) * v[NT - 1];
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        if (col + n * kUnitCols < a.N) o[n * kUnitCols] = v[n];
                 }
-                continue;
-            }
-            float* o = a.out + (static_cast<long>(split) * a.g.R + t.first + r) * a.ldo;
-#pragma unroll
-            for (int n = 0; n < (SWIGLU ? 1 : NT); ++n) {
-                const int col = tile[n] * kUnitCols + (lane & 31);
-                if (col < a.N) o[col] = SWIGLU ? silu_f(v[0]) * v[1] : v[n];
             }
         }
     }
