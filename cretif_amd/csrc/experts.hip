@@ -190,7 +190,8 @@ enum class Use { kMatmul, kSwiglu, kCombine };
 // pass, then stages of 64 k at 0.42, 0.52 or 0.88 us (16, 32, 64 rows) while a CU has one workgroup or less, 0.47, 0.52 or 0.96 us
 // for each beyond, some of a last round that is not full; an expert's further tiles read its weights again at 0.28 of the
 // cost.  k in several parts costs their sums a way to memory and back at 3.8 TB/s and a launch (the combination adds them up
-// itself).  `weight` is what decoding and scaling a format takes of either, beside Q4_0.  Over 189 calls of all formats what it
+// itself).  `weight` is what decoding and scaling a format takes of either, beside Q4_0; Q6_K, whose decoding is the longest, gains
+// most by 64 rows that share it (1000 tokens, 2 of 16, 2048 -> 2048: 80.5 us against 82.9 with 32).  Over 189 calls of all formats what it
 // takes was 1.5% slower than the best on average, 29% at most.
 // Measured, few (8 rows, 4 waves) / 16 / 32 / 64 rows, us: SwiGLU 2048 -> 1024 of 64 experts, 8 each, Q4_K: 4 tokens 18 / 24 / 27 /
 // 38, 16: 26 / 30 / 34 / 50, 48: 49 / 40 / 44 / 67, 256: 169 / 82 / 81 / 98, 512: 314 / 140 / 118 / 128, 1024: 643 / 270 / 195 / 195.
@@ -219,7 +220,8 @@ Plan plan_products(const ExpertMatrix& w, const ExpertRows& g, Use use) {
         for (int splits = 1; splits <= std::min(depth, 8) && (splits == 1 || part * splits <= 256); splits *= 2) {
             double load = row_tiles(k.bm) * blocks * splits / 256;  // workgroups of a CU
             if (load > 1.0) load += 0.38 * (std::ceil(load) - load);
-            const double stage = std::max(k.one, k.each * load) * rows_weight[w.fmt];
+            const double shared = w.fmt == kFmtQ6_K && k.bm == 64 ? 0.87 : 1.0;
+            const double stage = std::max(k.one, k.each * load) * rows_weight[w.fmt] * shared;
             const int stages = splits == 1 ? (w.K + 63) / 64 : 4 * ((depth + splits - 1) / splits);
             const double join = splits == 1 ? 0.0 : use == Use::kCombine ? part * 2 * (splits - 1) / 3.8 : 2.3 + part * 2 * splits / 3.8;
             const double us = 8.8 + join + std::max(memory * (0.72 + 0.28 * row_tiles(k.bm) / used), stages * stage);
