@@ -13,6 +13,7 @@
 // Bound by the chain of launches, loads and reductions: one token of 128 experts, 8 chosen, 4.9 us; 8192 of
 // 256 with a bias 17.2 us and 10.5 for the second launch.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "internal.hpp"
@@ -37,15 +38,21 @@ struct RouteArgs {
     int* offsets;
     int* rows;
     int* slots;
-    int* counts;  // [blocks][E]
+    int* counts;  // [blocks][padded(E)]
     int M, E, k, per;  // per: tokens of a block
 };
+
+__host__ __device__ inline int padded(int E) { return (E + 3) & ~3; }
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 struct Shared {
     int run[kMaxExperts];                    // a block's next place of each expert
     int count[kMaxExperts];
-    int parts[2][kThreads];
-    uint16_t wave[kWaves][kMaxExperts];      // pairs of each expert in a wave's 64, then before them in the chunk
+    union {
+        uint16_t wave[kWaves][kMaxExperts];  // pairs of each expert in a wave's 64, then before them in the chunk
+        i32x4 parts[2][kThreads];            // of four experts in a run of blocks, and of those before this one
+    };
     int totals[kWaves];
 };
 
@@ -54,15 +61,24 @@ template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t lower(uint32_t v) {
     return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false);
 }
-// The largest of the wave; into lane 63 over 1, 2, 4 and 8 lanes of a row, then row after row.
-__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
-    v = max(v, lower<0x111, 0xF>(v));
-    v = max(v, lower<0x112, 0xF>(v));
-    v = max(v, lower<0x114, 0xF>(v));
-    v = max(v, lower<0x118, 0xF>(v));
-    v = max(v, lower<0x142, 0xA>(v));
-    v = max(v, lower<0x143, 0xC>(v));
-    return __builtin_amdgcn_readlane(v, 63);
+// The largest of the wave, of T numbers side by side; into lane 63 over 1, 2, 4 and 8 lanes of a row, then row after row.
+template <int T>
+__device__ __forceinline__ void wave_tops(const uint32_t (&from)[T], uint32_t (&top)[T]) {
+    uint32_t v[T];
+    auto step = [&](auto&& moved) {
+#pragma unroll
+        for (int n = 0; n < T; ++n) v[n] = max(v[n], moved(v[n]));
+    };
+#pragma unroll
+    for (int n = 0; n < T; ++n) v[n] = from[n];
+    step([](uint32_t u) { return lower<0x111, 0xF>(u); });
+    step([](uint32_t u) { return lower<0x112, 0xF>(u); });
+    step([](uint32_t u) { return lower<0x114, 0xF>(u); });
+    step([](uint32_t u) { return lower<0x118, 0xF>(u); });
+    step([](uint32_t u) { return lower<0x142, 0xA>(u); });
+    step([](uint32_t u) { return lower<0x143, 0xC>(u); });
+#pragma unroll
+    for (int n = 0; n < T; ++n) top[n] = __builtin_amdgcn_readlane(v[n], 63);
 }
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double lower64(double v) {
@@ -114,117 +130,154 @@ __device__ __forceinline__ double reciprocal(double d) {
     return fma(fma(-d, r, 1.0), r, r);
 }
 
-// The choices of token t, by one wave; lane j returns choice j's expert, or -1.  WIDE: with a bias, by scores of 64 bits, whose
-// upper halves are compared first and the lower ones only between equal upper ones.
-template <int C, bool WIDE>
-__device__ __forceinline__ int choose(const RouteArgs& a, int t) {
+// The choices of T tokens t, t + step, ... by one wave, side by side (a chain of maxima each); lane j returns choice j's expert, or
+// -1.  WIDE: with a bias, by scores of 64 bits, whose upper halves are compared first and the lower ones only between equal
+// upper ones.
+template <int C, bool WIDE, int T>
+__device__ __forceinline__ void choose(const RouteArgs& a, int t, int step, int (&mine)[T]) {
     const int lane = __lane_id();
-    const float* z = a.logits + t * a.ldl;
-    float x[C];
+    const float* z[T];
+    float x[T][C], most[T];
+    uint32_t high[T][C], low[T][WIDE ? C : 1] = {};
+    double all[T], over[T];
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        const int e = lane * C + i;
-        const float v = e < a.E ? z[e] : -INFINITY;
-        x[i] = v == v ? v : -INFINITY;
+    for (int n = 0; n < T; ++n) {
+        z[n] = a.logits + (t + n * step) * a.ldl;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int e = lane * C + i;
+            const float v = e < a.E ? z[n][e] : -INFINITY;
+            x[n][i] = v == v ? v : -INFINITY;
+        }
     }
-    float best = x[0];
-#pragma unroll
-    for (int i = 1; i < C; ++i) best = fmaxf(best, x[i]);
-    const float most = wave_max(best);
     // of all experts: softmax's sum, where anything needs it
-    auto part = [&](float v) { return v == most ? 1.0 : exp64(static_cast<double>(v) - most); };
-    double all = 1.0;
-    if (!a.sigmoid && (WIDE || !a.normalize) && most > -INFINITY) {
-        all = 0.0;
+    auto part = [&](int n, float v) { return v == most[n] ? 1.0 : exp64(static_cast<double>(v) - most[n]); };
+    auto score = [&](int n, float v) { return a.sigmoid ? reciprocal(1.0 + exp64(-static_cast<double>(v))) : part(n, v) * over[n]; };
 #pragma unroll
-        for (int i = 0; i < C; ++i) all += part(x[i]);
-        all = wave_sum64(all);
+    for (int n = 0; n < T; ++n) {
+        mine[n] = -1;
+        all[n] = 1.0;
+        if (a.sigmoid) continue;
+        float best = x[n][0];
+#pragma unroll
+        for (int i = 1; i < C; ++i) best = fmaxf(best, x[n][i]);
+        most[n] = wave_max(best);
+        if ((WIDE || !a.normalize) && most[n] > -INFINITY) {
+            all[n] = 0.0;
+#pragma unroll
+            for (int i = 0; i < C; ++i) all[n] += part(n, x[n][i]);
+            all[n] = wave_sum64(all[n]);
+        }
     }
-    const double over = 1.0 / all;
-    auto score = [&](float v) { return a.sigmoid ? reciprocal(1.0 + exp64(-static_cast<double>(v))) : part(v) * over; };
-    uint32_t high[C], low[WIDE ? C : 1] = {};
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        if constexpr (WIDE) {
-            const int e = min(lane * C + i, a.E - 1);
-            const double s = score(x[i]) + a.bias[e];
-            const uint64_t u = x[i] > -INFINITY && s > -INFINITY ? ordered(s) : 0;  // (NaN is not above)
-            high[i] = static_cast<uint32_t>(u >> 32);
-            low[i] = static_cast<uint32_t>(u);
-        } else {
-            high[i] = x[i] > -INFINITY ? ordered(x[i]) : 0;
+    for (int n = 0; n < T; ++n) {
+        over[n] = 1.0 / all[n];
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            if constexpr (WIDE) {
+                const int e = min(lane * C + i, a.E - 1);
+                const double s = score(n, x[n][i]) + a.bias[e];
+                const uint64_t u = x[n][i] > -INFINITY && s > -INFINITY ? ordered(s) : 0;  // (NaN is not above)
+                high[n][i] = static_cast<uint32_t>(u >> 32);
+                low[n][i] = static_cast<uint32_t>(u);
+            } else {
+                high[n][i] = x[n][i] > -INFINITY ? ordered(x[n][i]) : 0;
+            }
         }
     }
     // Up to four a lane are sorted once (neighbours exchanged where the later one is larger, so equal ones keep their order):
     // the lane's largest is then always the first, and a chosen one leaves by a shift.  More are searched each time.
     constexpr bool SORTED = C <= 4;
-    int place[C];
+    int place[T][C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) place[i] = i;
-    if constexpr (SORTED) {
+    for (int n = 0; n < T; ++n) {
 #pragma unroll
-        for (int round = 0; round < C; ++round) {
-#pragma unroll
-            for (int i = round & 1; i + 1 < C; i += 2) {
-                const bool more = high[i + 1] > high[i] || (WIDE && high[i + 1] == high[i] && low[WIDE ? i + 1 : 0] > low[WIDE ? i : 0]);
-                const auto exchange = [&](auto& p, auto& q) {
-                    const auto was = p;
-                    p = more ? q : p;
-                    q = more ? was : q;
-                };
-                exchange(high[i], high[i + 1]);
-                exchange(place[i], place[i + 1]);
-                if constexpr (WIDE) exchange(low[i], low[i + 1]);
-            }
-        }
-    }
-    int mine = -1;
-    for (int j = 0; j < a.k; ++j) {
-        uint32_t h = high[0], l = low[0];
-        int at = place[0];
-        if constexpr (!SORTED) {
-#pragma unroll
-            for (int i = 1; i < C; ++i) {
-                const bool more = high[i] > h || (WIDE && high[i] == h && low[WIDE ? i : 0] > l);
-                h = more ? high[i] : h;
-                if (WIDE) l = more ? low[WIDE ? i : 0] : l;
-                at = more ? i : at;
-            }
-        }
-        const uint32_t top = wave_top(h);
-        if (top == 0) break;
-        unsigned long same = __ballot(h == top);
-        if (WIDE && (same & (same - 1)) != 0) {
-            const uint32_t rest = wave_top(h == top ? l : 0);
-            same = __ballot(h == top && l == rest);
-        }
-        const int who = __builtin_ctzl(same);
-        const int expert = who * C + __builtin_amdgcn_readlane(at, who);
-        mine = lane == j ? expert : mine;
-        const bool gone = lane == who;
+        for (int i = 0; i < C; ++i) place[n][i] = i;
         if constexpr (SORTED) {
 #pragma unroll
-            for (int i = 0; i < C; ++i) {
-                high[i] = gone ? (i + 1 < C ? high[i + 1 < C ? i + 1 : i] : 0) : high[i];
-                if (i + 1 < C) place[i] = gone ? place[i + 1 < C ? i + 1 : i] : place[i];
-                if (WIDE && i + 1 < C) low[WIDE ? i : 0] = gone ? low[WIDE && i + 1 < C ? i + 1 : 0] : low[WIDE ? i : 0];
-            }
-        } else {
+            for (int round = 0; round < C; ++round) {
 #pragma unroll
-            for (int i = 0; i < C; ++i) high[i] = gone && i == at ? 0 : high[i];
+                for (int i = round & 1; i + 1 < C; i += 2) {
+                    const bool more = high[n][i + 1] > high[n][i] ||
+                                      (WIDE && high[n][i + 1] == high[n][i] && low[n][WIDE ? i + 1 : 0] > low[n][WIDE ? i : 0]);
+                    const auto exchange = [&](auto& p, auto& q) {
+                        const auto was = p;
+                        p = more ? q : p;
+                        q = more ? was : q;
+                    };
+                    exchange(high[n][i], high[n][i + 1]);
+                    exchange(place[n][i], place[n][i + 1]);
+                    if constexpr (WIDE) exchange(low[n][i], low[n][i + 1]);
+                }
+            }
         }
     }
-    const float value = mine >= 0 ? z[mine] : 0.0f;
-    double w = mine >= 0 ? score(value) : 0.0;
-    if (a.normalize) {
-        const double sum = wave_sum64(w);
-        w = sum > 0.0 ? w / sum : 0.0;
+    for (int j = 0; j < a.k; ++j) {
+        uint32_t h[T], l[T], top[T];
+        int at[T];
+#pragma unroll
+        for (int n = 0; n < T; ++n) {
+            h[n] = high[n][0];
+            l[n] = low[n][0];
+            at[n] = place[n][0];
+            if constexpr (!SORTED) {
+#pragma unroll
+                for (int i = 1; i < C; ++i) {
+                    const bool more = high[n][i] > h[n] || (WIDE && high[n][i] == h[n] && low[n][WIDE ? i : 0] > l[n]);
+                    h[n] = more ? high[n][i] : h[n];
+                    if (WIDE) l[n] = more ? low[n][WIDE ? i : 0] : l[n];
+                    at[n] = more ? i : at[n];
+                }
+            }
+        }
+        wave_tops(h, top);
+        uint32_t any = 0;
+#pragma unroll
+        for (int n = 0; n < T; ++n) any |= top[n];
+        if (any == 0) break;
+#pragma unroll
+        for (int n = 0; n < T; ++n) {
+            unsigned long same = __ballot(h[n] == top[n]);
+            if (WIDE && (same & (same - 1)) != 0 && top[n] != 0) {
+                uint32_t low_half[1] = {h[n] == top[n] ? l[n] : 0}, rest[1];
+                wave_tops(low_half, rest);
+                same = __ballot(h[n] == top[n] && l[n] == rest[0]);
+            }
+            const int who = __builtin_ctzl(same);
+            const int expert = who * C + __builtin_amdgcn_readlane(at[n], who);
+            mine[n] = lane == j && top[n] != 0 ? expert : mine[n];
+            const bool gone = lane == who;  // (with nothing left everything is 0 already)
+            if constexpr (SORTED) {
+#pragma unroll
+                for (int i = 0; i < C; ++i) {
+                    high[n][i] = gone ? (i + 1 < C ? high[n][i + 1 < C ? i + 1 : i] : 0) : high[n][i];
+                    if (i + 1 < C) place[n][i] = gone ? place[n][i + 1 < C ? i + 1 : i] : place[n][i];
+                    if (WIDE && i + 1 < C) low[n][WIDE ? i : 0] = gone ? low[n][WIDE && i + 1 < C ? i + 1 : 0] : low[n][WIDE ? i : 0];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < C; ++i) high[n][i] = gone && i == at[n] ? 0 : high[n][i];
+            }
+        }
     }
-    if (lane < a.k) {
-        a.ids[static_cast<long>(t) * a.k + lane] = mine;
-        a.weights[static_cast<long>(t) * a.k + lane] = static_cast<float>(w * a.scale);
+    double w[T];
+#pragma unroll
+    for (int n = 0; n < T; ++n) {
+        const float value = mine[n] >= 0 ? z[n][mine[n]] : 0.0f;
+        w[n] = mine[n] >= 0 ? score(n, value) : 0.0;
     }
-    return mine;
+#pragma unroll
+    for (int n = 0; n < T; ++n) {
+        if (a.normalize) {
+            const double sum = wave_sum64(w[n]);
+            w[n] = sum > 0.0 ? w[n] / sum : 0.0;
+        }
+        if (lane < a.k) {
+            const long p = static_cast<long>(t + n * step) * a.k + lane;
+            a.ids[p] = mine[n];
+            a.weights[p] = static_cast<float>(w[n] * a.scale);
+        }
+    }
 }
 
 // exclusive sums of v over the workgroup's threads; the total in `all`
@@ -255,8 +308,8 @@ __device__ __forceinline__ int expert_of(const RouteArgs& a, long p) {
     return e >= 0 && e < a.E ? e : a.E;
 }
 
-// The block's pairs to their places: run[e] is where its first pair of expert e goes.
-__device__ __forceinline__ void place(const RouteArgs& a, Shared& s, long p0, long p1) {
+// The block's pairs to their places: run[e] is where its first pair of expert e goes.  `first`: the expert of the thread's first pair.
+__device__ __forceinline__ void place(const RouteArgs& a, Shared& s, long p0, long p1, int first) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int bits = 32 - __builtin_clz(a.E);
     for (long base = p0; base < p1; base += kThreads) {
@@ -264,7 +317,7 @@ __device__ __forceinline__ void place(const RouteArgs& a, Shared& s, long p0, lo
             if (tid < a.E) s.wave[w][tid] = 0;
         __syncthreads();
         const long p = base + tid;
-        const int e = p < p1 ? expert_of(a, p) : a.E;
+        const int e = base == p0 ? first : p < p1 ? expert_of(a, p) : a.E;
         unsigned long same = ~0ul;
         for (int i = 0; i < bits; ++i) {
             const unsigned long set = __ballot((e >> i) & 1);
@@ -300,7 +353,7 @@ __device__ __forceinline__ void write_rest(const RouteArgs& a, int all, int bloc
 }
 
 // Chooses (with logits) and counts the block's pairs; a single block groups them, too.
-template <int C, bool WIDE>
+template <int C, bool WIDE, int T>
 __global__ __launch_bounds__(kThreads) void route_kernel(const RouteArgs a) {
     __shared__ Shared s;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -308,10 +361,16 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteArgs a) {
     __syncthreads();
     const int t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.M);
     if (a.logits != nullptr) {
-        for (int t = t0 + wave; t < t1; t += kWaves) {
-            const int e = choose<C, WIDE>(a, t);
-            if (lane < a.k && e >= 0) atomicAdd(&s.count[e], 1);
-        }
+        const auto take = [&](auto tokens, int t) {
+            int e[decltype(tokens)::value];
+            choose<C, WIDE>(a, t, kWaves, e);
+            for (int n : e)
+                if (lane < a.k && n >= 0) atomicAdd(&s.count[n], 1);
+        };
+        int t = t0 + wave;
+        if constexpr (T == 2)
+            for (; t + kWaves < t1; t += 2 * kWaves) take(std::integral_constant<int, 2>{}, t);
+        for (; t < t1; t += kWaves) take(std::integral_constant<int, 1>{}, t);
     } else {
         for (long p = static_cast<long>(t0) * a.k + tid; p < static_cast<long>(t1) * a.k; p += kThreads) {
             const int e = expert_of(a, p);
@@ -321,7 +380,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteArgs a) {
     __syncthreads();  // (the ids of this block are read again below: written by this workgroup)
     const int n = tid < a.E ? s.count[tid] : 0;
     if (gridDim.x > 1) {
-        if (tid < a.E) a.counts[static_cast<long>(blockIdx.x) * a.E + tid] = n;
+        if (tid < padded(a.E)) a.counts[static_cast<long>(blockIdx.x) * padded(a.E) + tid] = n;
         return;
     }
     int all;
@@ -331,7 +390,8 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteArgs a) {
         a.offsets[tid] = before;
     }
     if (tid == 0) a.offsets[a.E] = all;
-    place(a, s, 0, static_cast<long>(a.M) * a.k);
+    const long pairs = static_cast<long>(a.M) * a.k;
+    place(a, s, 0, pairs, tid < pairs ? expert_of(a, tid) : a.E);
     write_rest(a, all, 0, 1);
 }
 
@@ -339,32 +399,36 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteArgs a) {
 __global__ __launch_bounds__(kThreads) void group_kernel(const RouteArgs a, int blocks) {
     __shared__ Shared s;
     const int tid = threadIdx.x, block = blockIdx.x;
-    // the counts of an expert by several threads, a run of blocks each
-    int width = 64;
-    while (width < a.E) width <<= 1;
-    const int shares = kThreads / width, e = tid & (width - 1), share = tid / width;
+    const int t0 = block * a.per, t1 = min(t0 + a.per, a.M);
+    const long p0 = static_cast<long>(t0) * a.k, p1 = static_cast<long>(t1) * a.k;
+    const int first = p0 + tid < p1 ? expert_of(a, p0 + tid) : a.E;  // (asked for with the counts)
+    // the counts of four experts by several threads, a run of blocks each
+    const int row = padded(a.E), quads = row >> 2;
+    int width = 16;
+    while (width < quads) width <<= 1;
+    const int shares = kThreads / width, q = tid & (width - 1), share = tid / width;
     const int each = (blocks + shares - 1) / shares, b0 = share * each, b1 = min(b0 + each, blocks);
-    int total = 0, before = 0;
-    if (e < a.E) {
+    i32x4 sum = {0, 0, 0, 0}, earlier = sum;
+    if (q < quads) {
         for (int b = b0; b < b1; b += 16) {
-            int n[16];
+            i32x4_a4 n[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) n[i] = a.counts[static_cast<long>(min(b + i, b1 - 1)) * a.E + e];
+            for (int i = 0; i < 16; ++i) n[i] = *reinterpret_cast<const i32x4_a4*>(a.counts + static_cast<long>(min(b + i, b1 - 1)) * row + 4 * q);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                total += b + i < b1 ? n[i] : 0;
-                before += b + i < min(b1, block) ? n[i] : 0;
+                sum += b + i < b1 ? n[i] : i32x4{0, 0, 0, 0};
+                earlier += b + i < min(b1, block) ? n[i] : i32x4{0, 0, 0, 0};
             }
         }
     }
-    s.parts[0][tid] = total;
-    s.parts[1][tid] = before;
+    s.parts[0][tid] = sum;
+    s.parts[1][tid] = earlier;
     __syncthreads();
-    total = before = 0;
+    int total = 0, before = 0;
     if (tid < a.E) {
         for (int i = 0; i < shares; ++i) {
-            total += s.parts[0][i * width + tid];
-            before += s.parts[1][i * width + tid];
+            total += s.parts[0][i * width + (tid >> 2)][tid & 3];
+            before += s.parts[1][i * width + (tid >> 2)][tid & 3];
         }
     }
     int all;
@@ -374,8 +438,7 @@ __global__ __launch_bounds__(kThreads) void group_kernel(const RouteArgs a, int 
         if (block == 0) a.offsets[tid] = start;
     }
     if (block == 0 && tid == 0) a.offsets[a.E] = all;
-    const int t0 = block * a.per, t1 = min(t0 + a.per, a.M);
-    place(a, s, static_cast<long>(t0) * a.k, static_cast<long>(t1) * a.k);
+    place(a, s, p0, p1, first);
     write_rest(a, all, block, blocks);
 }
 
@@ -385,19 +448,12 @@ int block_tokens(int M) { return M <= kSingle ? std::max(M, 1) : std::max((M + k
 void launch(RouteArgs a, hipStream_t stream) {
     a.per = block_tokens(a.M);
     const int blocks = std::max((a.M + a.per - 1) / a.per, 1);
-    const bool biased = a.logits != nullptr && a.bias != nullptr;
-    const int c = (a.E + 63) / 64;
-    const auto run = a.logits == nullptr ? route_kernel<1, false>
-                     : biased            ? (c == 1   ? route_kernel<1, true>
-                                            : c == 2 ? route_kernel<2, true>
-                                            : c <= 4 ? route_kernel<4, true>
-                                            : c <= 8 ? route_kernel<8, true>
-                                                     : route_kernel<16, true>)
-                                         : (c == 1   ? route_kernel<1, false>
-                                            : c == 2 ? route_kernel<2, false>
-                                            : c <= 4 ? route_kernel<4, false>
-                                            : c <= 8 ? route_kernel<8, false>
-                                                     : route_kernel<16, false>);
+    const bool biased = a.logits != nullptr && a.bias != nullptr, pairs = a.per > kWaves;
+    const int c = a.logits == nullptr ? 1 : (a.E + 63) / 64;
+#define CRI_ROUTE(C) \
+    (biased ? (pairs && C < 16 ? route_kernel<C, true, C < 16 ? 2 : 1> : route_kernel<C, true, 1>) : (pairs ? route_kernel<C, false, 2> : route_kernel<C, false, 1>))
+    const auto run = c == 1 ? CRI_ROUTE(1) : c == 2 ? CRI_ROUTE(2) : c <= 4 ? CRI_ROUTE(4) : c <= 8 ? CRI_ROUTE(8) : CRI_ROUTE(16);
+#undef CRI_ROUTE
     hipLaunchKernelGGL(run, dim3(blocks), dim3(kThreads), 0, stream, a);
     if (blocks > 1) hipLaunchKernelGGL(group_kernel, dim3(blocks), dim3(kThreads), 0, stream, a, blocks);
 }
@@ -410,7 +466,7 @@ namespace detail {
 long expert_group_workspace_bytes(int n_tokens, int, int n_experts) {
     if (n_tokens <= dev::kSingle) return 0;
     const int per = dev::block_tokens(n_tokens);
-    return static_cast<long>((n_tokens + per - 1) / per) * n_experts * 4;
+    return static_cast<long>((n_tokens + per - 1) / per) * dev::padded(n_experts) * 4;
 }
 
 int launch_expert_route(const ExpertRouter& r, const float* logits, long ldl, int n_experts, int* ids, float* weights,
