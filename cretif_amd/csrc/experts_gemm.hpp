@@ -690,12 +690,13 @@ void expert_rows(const ProductArgs& a, bool swiglu, int bm, long workgroups, hip
 template <int FMT>
 void expert_few(const ProductArgs& a, bool swiglu, int lg, int waves, long workgroups, hipStream_t stream) {
     const int lds = std::max(waves * few_wave_bytes(1 << lg), waves * (swiglu ? 2 : 1) * 1024);
-    const FewRest rest{a.out, a.ldx, a.ldo, a.N, a.K};
+    const bool one = a.gather && a.g.R == a.g.k;  // one token: whatever a row's number is, x has that row
+    const FewRest rest{a.out, one ? 0 : a.ldx, a.ldo, a.N, a.K};
     const auto run = swiglu ? (lg == 0 ? few_kernel<FMT, true, 1> : few_kernel<FMT, true, 4>)
                             : (lg == 0 ? few_kernel<FMT, false, 1> : few_kernel<FMT, false, 4>);
     hipLaunchKernelGGL(run, dim3(static_cast<unsigned>(workgroups)),
                        dim3(64 * waves), lds, stream, a.g.offsets, a.g.rows, a.w[0], a.w[1], a.x, a.g.E, a.g.R,
-                       a.gather ? a.over_k : 0u, lg | waves << 2, a.tiles, a.depth, rest);
+                       a.gather && !one ? a.over_k : 0u, lg | waves << 2, a.tiles, a.depth, rest);
 }
 
 template <int FMT>
