@@ -248,3 +248,13 @@ def test_error_text_names_the_call():
 def test_python_refuses(call):
     with pytest.raises(KeyError):
         call()
+
+
+def test_too_many_tiles():
+    """More tiles than a launch takes are refused before anything is launched."""
+    far = [i << 44 for i in range(1, 8)]
+    w = weights(data=far[0], N=1 << 16)
+    g = groups(offsets=far[1], rows=far[2], slots=far[3], n_tokens=1 << 20, top_k=8)
+    got = status("cri_expert_matmul", ref(w), ref(g), far[4], 256, 0, far[5], 1 << 16, far[6], 1 << 42, None)
+    assert got == UNSUPPORTED
+    assert "tiles" in cri.lib().cri_last_error_string().decode()
