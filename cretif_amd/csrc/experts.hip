@@ -15,7 +15,7 @@ typedef _Float16 eh8 __attribute__((ext_vector_type(8)));
 // Activations as the products take them: row r is 2^exps[r] (hi + lo), |hi| up to 2^15, hi and lo to the nearest half, per 64
 // k 64 of hi and 64 of lo, zeros from K on; for Q4_K also the sums over 32 k times 2^-6 (32 terms below 2^15 then fit
 // fp16) in the same two parts.  A workgroup per row, read twice (the second time from the caches): K floats in, as many
-// bytes out; 4096 x 2048 takes 16 us.
+// bytes out; 4096 x 2048 takes 15 us, 32768 x 1024 45 (5.9 TB/s).
 struct PlanesArgs {
     const float* x;
     long ldx;
