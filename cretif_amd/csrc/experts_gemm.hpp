@@ -376,12 +376,12 @@ struct FewRest {
     long ldx, ldo;
     int N, K;
 };
-// LDS of a wave: rows of 1024 bytes (a unit's hi and lo, in the ring's order), 32 of sums and 4 of unscale
+// LDS of a wave: rows of 1024 bytes (a unit's hi and lo, in the ring's order), 32 of sums and 4 of exponent
 __device__ __host__ constexpr int few_wave_bytes(int bm) { return bm * (1024 + 32) + 64; }
 
 // Eight activations of a row's unit (lane group of 32: one row) to their chunk of hi and lo, the row's sums over 32 and
-// its unscale; the whole wave calls it.
-__device__ __forceinline__ void few_convert(const f32x4& x, const f32x4& y, bool live, int r, char* area, char* sums, float* us) {
+// its exponent (not the power of two itself, which fp32 may not hold: down to 2^-163); the whole wave calls it.
+__device__ __forceinline__ void few_convert(const f32x4& x, const f32x4& y, bool live, int r, char* area, char* sums, int* exps) {
     float mx = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
                      fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
     mx = fmaxf(mx, dpp<kQuadPerm1032>(mx));
@@ -417,7 +417,7 @@ __device__ __forceinline__ void few_convert(const f32x4& x, const f32x4& y, bool
         o[0] = s;
         o[8] = static_cast<_Float16>(sum - static_cast<float>(s));
     }
-    if (c == 0) us[r] = ldexpf(1.0f, ex);
+    if (c == 0) exps[r] = ex;
 }
 
 // A stage (64 k) of NT column tiles against paired rows, of which lanes keep the first KEEP of registers 0 .. 3 (rows e_row(i) + 4 h;
@@ -453,7 +453,7 @@ __device__ __forceinline__ void few_stage(const typename F::Quant (&q)[NT], cons
 }
 
 // A unit of NT column tiles times the rows that few_convert has left in the wave's area, up to 8 (lane rows from `count` on: the
-// last again, unused): r[n][i], times the row's unscale, is the product of row i + 4 h.
+// last again, unused): r[n][i], times two to the row's exponent, is the product of row i + 4 h.
 template <int FMT, int NT, int KEEP>
 __device__ __forceinline__ void few_multiply(const typename ExpertFmt<FMT>::Quant (&q)[4][NT],
                                              const typename ExpertFmt<FMT>::Scale (&sc)[NT], const char* area,
@@ -527,7 +527,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const int* offsets,
     const long first_unit = (static_cast<long>(t.expert) * tiles + t.block) * depth;
     char* const area = lds + wave * few_wave_bytes(1 << lg);
     char* const sums = area + (1024 << lg);
-    float* const us = reinterpret_cast<float*>(sums + (32 << lg));
+    int* const exps = reinterpret_cast<int*>(sums + (32 << lg));
     float acc[NT][KEEP] = {};
     for (int u = wave; u < depth; u += waves) {
         // Loads arrive in order: half of the weights, the activations (whose rows had to be looked up), the other half, so that
@@ -560,15 +560,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const int* offsets,
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i)
-            if (2 * i < t.count) few_convert(lo[i], hi[i], 2 * i + h < t.count, 2 * i + h, area, sums, us);
+            if (2 * i < t.count) few_convert(lo[i], hi[i], 2 * i + h < t.count, 2 * i + h, area, sums, exps);
         wave_order();
         float p[NT][KEEP];
         few_multiply<FMT, NT, KEEP>(q, sc, area, sums, t.count, p);
 #pragma unroll
         for (int i = 0; i < KEEP; ++i) {
-            const float f = us[min(i + 4 * h, t.count - 1)];
+            const int e = exps[min(i + 4 * h, t.count - 1)];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][i] = __builtin_fmaf(f, p[n][i], acc[n][i]);
+            for (int n = 0; n < NT; ++n) acc[n][i] += ldexpf(p[n][i], e);
         }
         wave_order();
     }
@@ -621,7 +621,7 @@ __global__ __launch_bounds__(1024) void token_kernel(const ProductArgs a, const 
     if (b.residual != nullptr && threadIdx.x < 16 && col < a.N) first = b.residual[t * b.ldr + col];
     char* const area = lds + wave * few_wave_bytes(2);
     char* const sums = area + 2 * 1024;
-    float* const us = reinterpret_cast<float*>(sums + 2 * 32);
+    int* const exps = reinterpret_cast<int*>(sums + 2 * 32);
     float acc = 0.0f;  // lanes 0 .. 15 of the first units, lanes 48 .. 63 of the second ones
     const int units = k * a.depth;
     for (int i0 = wave; i0 < units; i0 += 2 * WAVES) {
@@ -659,11 +659,12 @@ __global__ __launch_bounds__(1024) void token_kernel(const ProductArgs a, const 
         F::load(sc[0], unit, from);
 #pragma unroll
         for (int s = 0; s < 4; ++s) F::load(q[s][0], unit, s, from);
-        few_convert(lo, hi, true, h, area, sums, us);
+        few_convert(lo, hi, true, h, area, sums, exps);
         wave_order();
         float p[1][1];  // of row 0, or row 4: the last one again, the second unit's
         few_multiply<FMT, 1, 1>(q, sc, area, sums, 2, p);
-        if (h ? live[1] : live[0]) acc = __builtin_fmaf((h ? weight[1] : weight[0]) * us[h], p[0][0], acc);
+        // the weight meets the product, not the power of two: their product may leave fp32's range where the result does not
+        if (h ? live[1] : live[0]) acc = __builtin_fmaf(h ? weight[1] : weight[0], ldexpf(p[0][0], exps[h]), acc);
         wave_order();
     }
     if (second == (h != 0)) red[wave][lane & 31] = acc;  // (lanes 0 .. 15, and 48 .. 63 as 16 .. 31)
