@@ -309,6 +309,8 @@ __device__ __forceinline__ int expert_of(const RouteArgs& a, long p) {
 }
 
 // The block's pairs to their places: run[e] is where its first pair of expert e goes.  `first`: the expert of the thread's first pair.
+// run comes from counts that another call may have written over (a workspace shared by calls that are not ordered, ids that
+// change meanwhile): a place that is no row is not followed.
 __device__ __forceinline__ void place(const RouteArgs& a, Shared& s, long p0, long p1, int first) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int bits = 32 - __builtin_clz(a.E);
@@ -339,7 +341,7 @@ __device__ __forceinline__ void place(const RouteArgs& a, Shared& s, long p0, lo
         if (p < p1) {
             const int to = e < a.E ? s.run[e] + s.wave[wave][e] + rank : -1;
             a.slots[p] = to;
-            if (to >= 0) a.rows[to] = static_cast<int>(p);
+            if (to >= 0 && to < a.M * a.k) a.rows[to] = static_cast<int>(p);
         }
         __syncthreads();
         if (tid < a.E) s.run[tid] += more;
@@ -348,7 +350,7 @@ __device__ __forceinline__ void place(const RouteArgs& a, Shared& s, long p0, lo
 
 __device__ __forceinline__ void write_rest(const RouteArgs& a, int all, int block, int blocks) {
     const long R = static_cast<long>(a.M) * a.k;
-    for (long r = all + block * static_cast<long>(kThreads) + threadIdx.x; r < R; r += static_cast<long>(blocks) * kThreads)
+    for (long r = max(all, 0) + block * static_cast<long>(kThreads) + threadIdx.x; r < R; r += static_cast<long>(blocks) * kThreads)
         a.rows[r] = -1;
 }
 

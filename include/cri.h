@@ -468,7 +468,8 @@ long long cri_verify_drafts_workspace_bytes(int n_seqs, int vocab);
  * cri_matmul_transposed_b: [E, dim] weights), cri_expert_route, cri_expert_swiglu, cri_expert_combine; cri_expert_matmul is for
  * other activations.  Which rows meet which expert stays on the device: nothing synchronises, host numbers alone decide launches
  * and workspaces, and a call may be captured in a HIP graph and replayed with other logits.  Results have the same bits at every
- * call with the same sizes and contents.  Calls that share a workspace must be ordered on one stream.
+ * call with the same sizes and contents.  Calls that share a workspace must be ordered on one stream: if two run at once, both
+ * results are unspecified, but nothing is read or written outside of their buffers.
  *
  * A matrix per expert, [n_experts, N, K] in GGUF blocks (ffn_gate_exps and the like), laid out once by cri_expert_pack: data
  * is 16-byte aligned, cri_expert_packed_bytes long.  K a multiple of 32 (Q4_K, Q6_K: 256), at least one block; up to 1024
