@@ -161,6 +161,7 @@ ABI_SYMBOLS = (
         "cri_expert_swiglu_workspace_bytes",
         "cri_expert_combine",
         "cri_expert_combine_workspace_bytes",
+        "cri_expert_plan",
         "cri_stream_read",
         "cri_stream_read_ex",
         "cri_timestamp",

@@ -1167,6 +1167,17 @@ int cri_expert_swiglu(const cri_expert_weights* gate, const cri_expert_weights* 
     return expert_product(gate, up, g, x, ldx, true, out, ldo, workspace, workspace_bytes, s, fn);
 }
 
+int cri_expert_plan(const cri_expert_weights* w, const cri_expert_groups* g, int op, int* plan) {
+    const char* fn = "cri_expert_plan";
+    if (op != CRI_EXPERT_MATMUL && op != CRI_EXPERT_SWIGLU && op != CRI_EXPERT_COMBINE) return fail(CRI_ERR_UNSUPPORTED, fn, "unknown operator");
+    if (!plan) return fail(CRI_ERR_INVALID_ARGUMENT, fn, "null plan");
+    if (const int st = check_expert_product(w, g, fn)) return st;
+    int p[3] = {0, 0, 0};
+    if (g->n_tokens > 0 && w->N > 0) cri::detail::expert_plan(matrix_arg(w), rows_arg(g), op, p);
+    std::copy(p, p + 3, plan);
+    return CRI_OK;
+}
+
 long long cri_expert_combine_workspace_bytes(const cri_expert_weights* w, const cri_expert_groups* g) {
     if (const int st = check_expert_product(w, g, "cri_expert_combine_workspace_bytes")) return st;
     if (g->n_tokens == 0 || w->N == 0) return 0;

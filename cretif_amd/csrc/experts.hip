@@ -181,7 +181,7 @@ struct Plan {
     bool few;
     int bm, lg, waves, splits;
 };
-// what is made of the products
+// what is made of the products (cri_expert_op)
 enum class Use { kMatmul, kSwiglu, kCombine };
 
 // The one that a rough model of both gives the least time, in us; it knows only host numbers, so rows are taken to be spread
@@ -334,6 +334,14 @@ bool token_takes(const ExpertMatrix& w, const ExpertRows& g) {
 }
 
 }  // namespace
+
+void expert_plan(const ExpertMatrix& w, const ExpertRows& g, int op, int (&plan)[3]) {
+    const bool one = op == static_cast<int>(Use::kCombine) && token_takes(w, g);
+    const Plan p = plan_products(w, g, static_cast<Use>(op));
+    plan[0] = one ? 0 : p.few ? 1 << p.lg : p.bm;
+    plan[1] = one ? 1 : p.splits;
+    plan[2] = one ? 16 : p.few ? p.waves : 4;
+}
 
 long expert_product_workspace_bytes(const ExpertMatrix& w, const ExpertRows& g, bool swiglu, bool gather) {
     const Plan plan = plan_products(w, g, swiglu ? Use::kSwiglu : Use::kMatmul);

@@ -389,6 +389,8 @@ long expert_product_workspace_bytes(const ExpertMatrix& w, const ExpertRows& g, 
 int launch_expert_products(const ExpertMatrix& w, const ExpertMatrix* up, const ExpertRows& g, const float* x, long ldx,
                            bool gather, float* out, long ldo, void* ws, hipStream_t stream);
 long expert_combine_workspace_bytes(const ExpertMatrix& w, const ExpertRows& g);
+// what the products of such a call (a cri_expert_op) take: rows of a tile, parts of k, waves of a workgroup (cri_expert_plan)
+void expert_plan(const ExpertMatrix& w, const ExpertRows& g, int op, int (&plan)[3]);
 int launch_expert_combine(const ExpertMatrix& w, const ExpertRows& g, const float* h, long ldh, const float* weights,
                           const float* residual, long ldr, float* out, long ldo, void* ws, hipStream_t stream);
 

@@ -39,6 +39,7 @@ SYMBOLS = {
     "cri_expert_swiglu_workspace_bytes": ([_vp, _vp], _i64),
     "cri_expert_swiglu": ([_vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _i64, _vp], _i32),
     "cri_expert_combine_workspace_bytes": ([_vp, _vp], _i64),
+    "cri_expert_plan": ([_vp, _vp, _i32, _vp], _i32),
     "cri_expert_combine": ([_vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i32, _vp, _i64, _vp], _i32),
 }
 

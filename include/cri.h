@@ -538,6 +538,12 @@ int cri_expert_combine(const cri_expert_weights* w, const cri_expert_groups* gro
                        const float* weights, const float* residual, int ldr, float* out, int ldo, void* workspace,
                        long long workspace_bytes, hipStream_t stream);
 long long cri_expert_combine_workspace_bytes(const cri_expert_weights* w, const cri_expert_groups* groups);
+/* How a call of these sizes multiplies, which the numbers alone decide: plan[0] the rows of a tile (1, 4, 8: few rows, converted by
+ * the workgroup that multiplies them; 16, 32, 64: many; 0: the combination in one launch), plan[1] the parts that K is shared in,
+ * plan[2] the waves of a workgroup; 0, 0, 0 where there is nothing to do.  w: gate's for CRI_EXPERT_SWIGLU.  For tests and
+ * measurements; touches no GPU. */
+typedef enum cri_expert_op { CRI_EXPERT_MATMUL = 0, CRI_EXPERT_SWIGLU = 1, CRI_EXPERT_COMBINE = 2 } cri_expert_op;
+int cri_expert_plan(const cri_expert_weights* w, const cri_expert_groups* groups, int op, int* plan);
 
 /* ---- diagnostics ---------------------------------------------------------- */
 
