@@ -1,9 +1,11 @@
 // experts_route.hip -- each token's experts from the router's logits, and the pairs (token, choice) grouped by expert.
 //
-// A wave takes a token (two side by side where a block has more than 16): lane l holds the logits of experts l C .. l C + C - 1 in registers, and k times the largest is found
-// (the lane's own, a maximum over the wave, the first lane that has it: ties go to the lowest index) and struck out.  The
-// order is the logits' own; only with a bias are scores computed first, in 64 bits, where different ones stay different.
-// The weights of the k chosen, too, are computed in 64 bits, a lane each.
+// A wave takes a token (two side by side where a block has more than 16): lane l holds the logits of experts
+// l C .. l C + C - 1 in registers, and k times the largest is found (the lane's own, a maximum over the wave, the first lane that
+// has it: ties go to the lowest index) and struck out.  The order is the logits' own; only with a bias are scores computed first,
+// in 64 bits: sums of score and bias that differ by less than a few 2^-53 of themselves (saturated scores, or tiny ones under a bias
+// that is not) may be the same number, whichever logit is larger.  The weights of the k chosen, too, are computed in 64 bits, a
+// lane each.
 //
 // Grouping is a counting sort, stable and without an order left to chance: counts per block of tokens (integer atomics in
 // LDS, whose order does not matter), offsets from their sums, and the place of a pair from the pairs before it in its block,

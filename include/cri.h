@@ -506,8 +506,10 @@ typedef struct cri_expert_router {
  * largest logit), in that order, the lowest number first where they are equal; their weights are the scores (without the
  * bias), divided by their sum with normalize (a sum of 0 leaves them 0), times scale.  An expert whose logit is -infinity or NaN (or whose bias makes its sum
  * so) is never chosen: a token left with fewer experts than top_k has id -1 and weight 0 in the choices behind, so a row of
- * -infinity (a padded batch's) causes no work.  Scores and their order are computed in 64 bits.  workspace: 4-byte aligned,
- * cri_expert_group_workspace_bytes. */
+ * -infinity (a padded batch's) causes no work.  Without a bias the order is exactly the logits'.  With one, score plus bias is
+ * computed in 64 bits: sums that differ by less than about 2^-51 of themselves may count as equal or come in either order (the
+ * sigmoids of 40 and 50 under one bias are equal, and so are scores of e^-50 and e^-49 beside a bias of 0.1).  workspace: 4-byte
+ * aligned, cri_expert_group_workspace_bytes. */
 int cri_expert_route(const cri_expert_router* router, const float* logits, int ldl, int* ids, float* weights,
                      const cri_expert_groups* groups, void* workspace, long long workspace_bytes, hipStream_t stream);
 /* the groups of given ids [n_tokens, top_k]; ids outside [0, n_experts) are pairs without an expert (another GPU's, say), and a
