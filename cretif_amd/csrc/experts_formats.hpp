@@ -34,9 +34,6 @@ __device__ __forceinline__ uint32_t e_fma(uint32_t a, uint32_t b, uint32_t c) {
 __device__ __forceinline__ uint32_t e_add(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(eh2, a) + __builtin_bit_cast(eh2, b));
 }
-__device__ __forceinline__ uint32_t e_mul(uint32_t a, uint32_t b) {
-    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(eh2, a) * __builtin_bit_cast(eh2, b));
-}
 // (v & m) | o as one v_and_or_b32: the constants are kept from the compiler, which would take two instructions with literals.
 // (Not as an instruction in asm: the compiler does not see that one write registers that an MFMA is still to write.)
 __device__ __forceinline__ uint32_t e_and_or(uint32_t v, uint32_t m, uint32_t o) {
