@@ -58,7 +58,8 @@ def _bytes(n):
 
 class ExpertWeights:
     """A matrix per expert, laid out once for the products: raw, a uint8 device tensor that holds the
-    GGUF blocks of [n_experts, N, K] (not needed afterwards).  Runs on the current stream, to which its memory belongs."""
+    GGUF blocks of [n_experts, N, K] (not needed afterwards; Q4_0 with element i in byte i / 2, as everywhere in the
+    library, not in upstream GGML's order).  Runs on the current stream, to which its memory belongs."""
 
     def __init__(self, fmt, raw, n_experts, N, K):
         L, dev = _torch(), _device()

@@ -481,7 +481,9 @@ typedef struct cri_expert_weights {
 } cri_expert_weights;
 long long cri_expert_packed_bytes(int format, int n_experts, int N, int K);
 /* packed = the blocks at src (raw GGUF bytes, any alignment) in the products' order: the same bits, padded to 32 rows and 256
- * values (Q4_K 3% larger for its unpacked 6-bit scales).  src is not needed afterwards.  No overlap. */
+ * values (Q4_K 3% larger for its unpacked 6-bit scales).  src is not needed afterwards.  No overlap.  Q4_0 blocks have the element
+ * order of cri_matmul_q4_0 (element i in byte i / 2); upstream GGML's files have another one (elements i and i + 16 in byte i), which
+ * cannot be told apart here and has to be reordered first. */
 int cri_expert_pack(int format, const void* src, int n_experts, int N, int K, void* packed, hipStream_t stream);
 /* The pairs (token t, choice j), pair t * top_k + j, grouped by expert: the grouped rows of expert e are offsets[e] ..
  * offsets[e + 1] - 1, in the order of their pairs; rows[r] is the pair of grouped row r (-1 from offsets[n_experts] on),

@@ -14,7 +14,8 @@ using ExpertWeights = cri_expert_weights;
 using ExpertGroups = cri_expert_groups;
 using ExpertRouter = cri_expert_router;
 
-// GGUF blocks [n_experts, N, K] laid out once: expert_packed_bytes of device memory.
+// GGUF blocks [n_experts, N, K] laid out once: expert_packed_bytes of device memory.  (Q4_0: element i in byte i / 2, as in
+// matmul_q4_0, not upstream GGML's order.)
 long long expert_packed_bytes(int format, int n_experts, int N, int K);
 void pack_experts(int format, const void* src, int n_experts, int N, int K, void* packed, hipStream_t stream = 0);
 

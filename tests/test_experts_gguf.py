@@ -1,4 +1,5 @@
-"""The matrices of a layer of experts from GGUF files: 3-D tensors through the Python and the C++ reader."""
+"""The matrices of a layer of experts from GGUF files: 3-D tensors through the Python and the C++ reader, and the element order of
+Q4_0 blocks."""
 import os
 import shutil
 import subprocess
@@ -60,6 +61,38 @@ def test_products_of_a_file(model):
             v, mag = ref.weights(f, raws[f], E, N, K)
             for e in range(E):
                 ref.check(out[off[e]:off[e + 1]], ref.Product(x[pairs[off[e]:off[e + 1]] // k], v[e], mag[e]), f)
+
+
+def reordered(b):
+    """Blocks [..., 18] of upstream's order (elements i and i + 16 in byte i) in the library's."""
+    b = b.copy()
+    q = np.concatenate([b[..., 2:] & 15, b[..., 2:] >> 4], -1)
+    b[..., 2:] = q[..., 0::2] | q[..., 1::2] << 4
+    return b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("upstream", [False, True])
+def test_order_of_q4_0(upstream):
+    """One-hot rows read single weights: element i from byte i / 2, and upstream's blocks once they are reordered."""
+    e_, n_, k_ = 2, 3, 64
+    rng = np.random.default_rng(5)
+    blocks = rng.integers(0, 256, (e_, n_, k_ // 32, 18)).astype(np.uint8)
+    blocks[..., :2] = np.array([1.0, 0.5], np.float16).view(np.uint8).reshape(2, 2)[rng.integers(0, 2, blocks.shape[:3])]
+    d = np.ascontiguousarray(blocks[..., :2]).view(np.float16)[..., 0].astype(np.float64)
+    b = blocks[..., 2:].astype(np.int64)
+    if upstream:
+        q = np.concatenate([b & 15, b >> 4], -1)
+        blocks = reordered(blocks)
+    else:
+        q = np.stack([b & 15, b >> 4], -1).reshape(b.shape[:3] + (32,))
+    want = (d[..., None] * (q - 8)).reshape(e_, n_, k_)
+    w = cri.ExpertWeights("q4_0", torch.from_numpy(blocks.reshape(-1)).cuda(), e_, n_, k_)
+    groups = cri.ExpertGroups(k_, e_, e_)
+    cri.group_experts(torch.arange(e_, dtype=torch.int32, device="cuda").repeat(k_, 1).contiguous(), groups)
+    out = torch.empty(k_ * e_, n_, device="cuda")
+    cri.expert_matmul(w, groups, torch.eye(k_, device="cuda"), out)
+    assert np.array_equal(ref.f64(out).reshape(e_, k_, n_), want.transpose(0, 2, 1))
 
 
 # ---- the C++ reader ------------------------------------------------------------------------------------------------------------
