@@ -185,7 +185,8 @@ struct Plan {
 enum class Use { kMatmul, kSwiglu, kCombine };
 
 // The one that a rough model of both gives the least time, in us; it knows only host numbers, so rows are taken to be spread
-// over the experts.  All read the weights of the experts that have rows at 5.5 TB/s at best.  few_kernel: 8 us, 0.6 ns for each
+// over the experts.  All read the weights of the experts that have rows at 5.5 TB/s at best (as counted here: the calls that this
+// was fitted to named some experts more than others, 48 tokens, 4 of 60, 38 and not 58).  few_kernel: 8 us, 0.6 ns for each
 // unit that a tile meets (that often as a 256th of the GPU) and 0.1 ns for each row of it.  rows_kernel: 8.8 us with the planes'
 // pass, then stages of 64 k at 0.42, 0.52 or 0.88 us (16, 32, 64 rows) while a CU has one workgroup or less, 0.47, 0.52 or 0.96 us
 // for each beyond, some of a last round that is not full; an expert's further tiles read its weights again at 0.28 of the
