@@ -78,7 +78,7 @@ class ExpertWeights:
 
 class ExpertGroups:
     """The pairs (token, choice) grouped by expert: int32 offsets [n_experts + 1], rows and slots
-    [n_tokens * top_k] (allocated when None)."""
+    [n_tokens * top_k] (when None allocated and zeroed on the current stream, which another one has to wait for)."""
 
     def __init__(self, n_tokens, top_k, n_experts, offsets=None, rows=None, slots=None):
         _torch()

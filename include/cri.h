@@ -522,8 +522,8 @@ long long cri_expert_group_workspace_bytes(const cri_expert_groups* groups);
 /* out[r, :] = x[row(r), :] W[e]^T for the grouped rows r of every expert e; row(r) is rows[r] / top_k (x: [n_tokens, K], a row
  * per token) or, with grouped, r (x: [n_tokens * top_k, K] in grouped order).  out [n_tokens * top_k, N]; its rows from
  * offsets[n_experts] on stay as they were.  Rows ldx and ldo floats apart, 4-byte aligned.  fp32 results: weights are exact,
- * activations have 22 bits of their row's (256 values' of their row's) largest magnitude; a row that is not finite makes its
- * own results not finite.  FP16 weights below 2^-14 (its subnormals) lose bits in the matrix units: a matrix of nothing else is
+ * activations have 22 bits of their row's (256 values' of their row's) largest magnitude, whatever that is (below 2^-126 results
+ * have fp32's own step of 2^-149); a row that is not finite makes its own results not finite.  FP16 weights below 2^-14 (its subnormals) lose bits in the matrix units: a matrix of nothing else is
  * good to 1e-6 at weights of 2^-19, to 1e-5 at 2^-23.  out and the workspace (16-byte aligned) overlap no other buffer. */
 int cri_expert_matmul(const cri_expert_weights* w, const cri_expert_groups* groups, const float* x, int ldx, int grouped,
                       float* out, int ldo, void* workspace, long long workspace_bytes, hipStream_t stream);
